@@ -319,6 +319,30 @@ int samhip_layer_norm(samhip_context* ctx, const float* x, float* y, int64_t row
 int samhip_flash_attn(samhip_context* ctx, const float* q, const float* k, const float* v, int64_t ld, float* out,
                       int64_t batches, int64_t n, int32_t heads, int32_t head_dim, float scale);
 
+/* Activation after a normalization. */
+enum samhip_activation {
+    SAMHIP_ACT_NONE = 0,
+    SAMHIP_ACT_RELU = 1,
+    SAMHIP_ACT_SILU = 2,
+    SAMHIP_ACT_GELU_ERF = 3 /* ggml_gelu_erf */
+};
+
+/* Group norm of channels-last maps with an activation (no reference
+ * counterpart: ggml_group_norm takes channel planes; the neck's levels and
+ * the feature cache hold pixel rows):
+ *   y = act((x - mean) / sqrt(var + eps) * w[c] + b[c])
+ * x and y are F32 or F16 (each its own), ne = {channels, pixels, images, 1},
+ * nb[0] the element size, pixel and image strides any multiples of it;
+ * mean and biased variance over the channels / groups neighbouring channels
+ * of a group in every pixel of one image (sums in F64).  w, b: device F32
+ * [channels], each may be NULL.  channels a multiple of groups, at most 4096;
+ * images at most 65535.  y may be x itself (same type and strides).  A
+ * non-finite value makes its group's outputs non-finite.  May be captured. */
+int samhip_supports_group_norm(const samhip_tensor* x, const samhip_tensor* y, int32_t groups, const float* w,
+                               const float* b, float eps, int32_t activation);   /* 1 if group_norm takes these, else 0 */
+int samhip_group_norm(samhip_context* ctx, const samhip_tensor* x, const samhip_tensor* y, int32_t groups,
+                      const float* w, const float* b, float eps, int32_t activation);
+
 /* --- diagnostics ------------------------------------------------------------ */
 int samhip_query(samhip_context* ctx, samhip_exec_info* info);
 
@@ -350,8 +374,9 @@ int samhip_trace_pause(samhip_context* ctx, int paused);
  * at M = 32): the calls between capture_begin and capture_end are recorded
  * into a HIP graph instead of running, and graph_launch replays them on the
  * context's stream with one host call.  Only samhip_mul_mat,
- * samhip_quantize_rows and samhip_dequantize_rows may be captured; every
- * other entry point fails with INVALID_ARGUMENT while a capture is open.  A
+ * samhip_quantize_rows, samhip_dequantize_rows and samhip_group_norm may be
+ * captured; every other entry point fails with INVALID_ARGUMENT while a
+ * capture is open.  A
  * captured call must fit the context's current staging (run the same
  * product once before capturing); staging that has to grow later is
  * reallocated without freeing the buffer that live graphs use.  Replays

@@ -313,6 +313,46 @@ const char* mul_mat_problem(const samhip_tensor* w, const samhip_tensor* x, cons
     return nullptr;
 }
 
+// Why `t` is no F32 or F16 tensor of up to `dims` dimensions with contiguous
+// innermost rows, or nullptr.  Empty ones (ne 0) need no data.
+const char* strided_problem(const samhip_tensor& t, int dims) {
+    if (t.type != T_F32 && t.type != T_F16) return "type must be F32 or F16";
+    const size_t e = size_t(block_bytes(t.type));
+    bool empty = false;
+    for (int i = 0; i < 4; ++i) {
+        if (t.ne[i] < 0 || t.ne[i] > (int64_t(1) << 40)) return "bad dimension";
+        if (i >= dims && t.ne[i] != 1) return "too many dimensions";
+        empty = empty || t.ne[i] == 0;
+    }
+    if (empty) return nullptr;
+    if (t.nb[0] != e) return "innermost rows must be contiguous";
+    for (int i = 1; i < dims; ++i) {
+        if (t.nb[i] % e) return "strides must be multiples of the element size";
+        if (t.nb[i] > (size_t(1) << 48)) return "stride too large";
+        if (t.ne[i] > 1 && t.nb[i] < t.nb[i - 1] * size_t(t.ne[i - 1])) return "rows overlap";
+    }
+    if (!t.data) return "null data pointer";
+    if (reinterpret_cast<uintptr_t>(t.data) % e) return "data must be aligned to the element size";
+    return nullptr;
+}
+
+const char* group_norm_problem(const samhip_tensor* x, const samhip_tensor* y, int32_t groups, const float* w, const float* b,
+                               float eps, int32_t activation) {
+    if (!x || !y) return "null tensor descriptor";
+    if (const char* why = strided_problem(*x, 3)) return why;
+    if (const char* why = strided_problem(*y, 3)) return why;
+    for (int i = 0; i < 3; ++i) {
+        if (x->ne[i] != y->ne[i]) return "y must have the shape of x";
+        if (x->ne[i] <= 0) return "empty operand";
+    }
+    if (x->ne[0] > kGroupNormMaxChannels || x->ne[1] > (int64_t(1) << 30) || x->ne[2] > 65535) return "dimension too large";
+    if (groups <= 0 || x->ne[0] % groups) return "channels must be a multiple of groups";
+    if (activation < SAMHIP_ACT_NONE || activation > SAMHIP_ACT_GELU_ERF) return "unknown activation";
+    if (!(eps >= 0.f) || std::isinf(eps)) return "eps must be nonnegative and finite";
+    if (reinterpret_cast<uintptr_t>(w) % 4 || reinterpret_cast<uintptr_t>(b) % 4) return "w and b must be 4-byte aligned";
+    return nullptr;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1130,6 +1170,29 @@ int samhip_flash_attn(samhip_context* ctx, const float* q, const float* k, const
                               att_bytes, ctx->cus, ctx->stream))
             return fail(SAMHIP_ERR_UNSUPPORTED, "flash_attn: no attention launch for this grid");
         HIP_TRY(hipGetLastError(), "attention launch");
+        return SAMHIP_OK;
+    });
+}
+
+int samhip_supports_group_norm(const samhip_tensor* x, const samhip_tensor* y, int32_t groups, const float* w,
+                               const float* b, float eps, int32_t activation) {
+    return group_norm_problem(x, y, groups, w, b, eps, activation) == nullptr ? 1 : 0;
+}
+
+int samhip_group_norm(samhip_context* ctx, const samhip_tensor* x, const samhip_tensor* y, int32_t groups,
+                      const float* w, const float* b, float eps, int32_t activation) {
+    if (!ctx) return fail(SAMHIP_ERR_INVALID_ARGUMENT, "null context");
+    if (const char* why = group_norm_problem(x, y, groups, w, b, eps, activation))
+        return fail(SAMHIP_ERR_INVALID_ARGUMENT, "group_norm: %s", why);
+    const int xb = block_bytes(x->type), yb = block_bytes(y->type);
+    const GroupNormShape s{int(x->ne[2]), int(x->ne[1]), int(x->ne[0]), groups, int64_t(x->nb[1] / xb), int64_t(x->nb[2] / xb),
+                           int64_t(y->nb[1] / yb), int64_t(y->nb[2] / yb)};
+    if (int rc = set_device(ctx)) return rc;
+    const int vec = group_norm_vec(s, x->data, xb, y->data, yb);
+    if (int rc = ensure_staging(ctx, group_norm_scratch_bytes(s, vec))) return rc;
+    return traced(ctx, "group_norm", x->type, int64_t(s.images) * s.pixels, s.channels, groups, [&]() -> int {
+        launch_group_norm(x->data, x->type, y->data, y->type, s, vec, w, b, eps, activation, ctx->staging, ctx->stream);
+        HIP_TRY(hipGetLastError(), "group_norm launch");
         return SAMHIP_OK;
     });
 }

@@ -18,6 +18,7 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "samhip.h")
 ABI_VERSION = 1
 F32, F16, Q8_0, Q8_1, Q4_K, Q5_K, Q6_K, Q8_K, I32 = 0, 1, 8, 9, 12, 13, 14, 15, 26
 COMPUTE_Q8_NATIVE, COMPUTE_F16 = 0, 1
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU_ERF = 0, 1, 2, 3
 ROUND_X86, ROUND_REF = 0, 1
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_DEVICE, ERR_OUT_OF_MEMORY = 0, -1, -2, -3, -4
 BLOCK_ELEMS = {F32: 1, F16: 1, Q8_0: 32, Q8_1: 32, Q4_K: 256, Q5_K: 256, Q6_K: 256, Q8_K: 256, I32: 1}
@@ -121,6 +122,8 @@ SIGNATURES = {
     "samhip_vit_neck": ([_P, ctypes.POINTER(VitNeckDesc), _P, _P, _P, _P, _P], _I),
     "samhip_layer_norm": ([_P, _P, _P, _I64, _I64, _P, _P, ctypes.c_float], _I),
     "samhip_flash_attn": ([_P, _P, _P, _P, _I64, _P, _I64, _I64, _I32, _I32, ctypes.c_float], _I),
+    "samhip_supports_group_norm": ([ctypes.POINTER(Tensor), ctypes.POINTER(Tensor), _I32, _P, _P, ctypes.c_float, _I32], _I),
+    "samhip_group_norm": ([_P, ctypes.POINTER(Tensor), ctypes.POINTER(Tensor), _I32, _P, _P, ctypes.c_float, _I32], _I),
 }
 
 _lib = None
@@ -187,6 +190,17 @@ def tensor(qtype, ne0, ne1, data, nb1=None):
     t.nb[1] = rb if nb1 is None else nb1
     t.nb[2] = t.nb[1] * ne1
     t.nb[3] = t.nb[2]
+    t.data = data
+    return t
+
+
+def tensor_nd(qtype, ne, nb, data):
+    """A ggml descriptor from up to four dimensions and byte strides, innermost first."""
+    t = Tensor()
+    t.type = qtype
+    for i in range(4):
+        t.ne[i] = ne[i] if i < len(ne) else 1
+        t.nb[i] = nb[i] if i < len(nb) else t.nb[i - 1] * t.ne[i - 1]
     t.data = data
     return t
 
@@ -284,6 +298,10 @@ class Context:
 
     def dequantize_rows(self, qtype, src_ptr, src_stride, dst_ptr, rows, k):
         check(lib().samhip_dequantize_rows(self.handle, qtype, src_ptr, src_stride, dst_ptr, rows, k))
+
+    def group_norm(self, x, y, groups, w_ptr, b_ptr, eps, activation=ACT_NONE):
+        """samhip_group_norm on channels-last descriptors {channels, pixels, images}."""
+        check(lib().samhip_group_norm(self.handle, ctypes.byref(x), ctypes.byref(y), groups, w_ptr, b_ptr, eps, activation))
 
     def query(self):
         info = ExecInfo()
