@@ -177,6 +177,31 @@ int samhip_mul_mat(samhip_context* ctx, const samhip_tensor* w, const samhip_ten
 int samhip_mul_mat_noalloc(samhip_context* ctx, const samhip_tensor* w, const samhip_tensor* x,
                            const samhip_tensor* y);
 
+/* Low-rank adapters of many requests beside a shared projection (no
+ * reference counterpart; for programs that serve one packed checkpoint with
+ * an adapter per request):
+ *   y[m] = base[m] + scale[s] * B[s] (A[s] x[m]),  s = ids[m]
+ * with base the shared product, e.g. of samhip_mul_mat.  The adapters stand
+ * in banks of equal slots, a (F32 or F16, ne = {K, R, slots, 1}) and b (the
+ * same type, ne = {R, N, slots, 1}), with any row and slot strides. */
+typedef struct samhip_lora_bank {
+    int32_t version;        /* SAMHIP_ABI_VERSION */
+    samhip_tensor a, b;     /* R at most 256 */
+    const int32_t* ranks;   /* device I32 [slots]: ranks in use, the rest of a slot is not read; NULL: R */
+    const float* scales;    /* device F32 [slots]; NULL: 1 */
+} samhip_lora_bank;
+
+/* x: F32 {K, M}; ids: device I32 {M}, in any order; base: F32 {N, M}, NULL
+ * for zeros, may be y itself (same data and row stride); y: F32 {N, M}.  A
+ * row whose id is not in [0, slots) gets base alone; ranks are cut to
+ * [0, R].  Products and sums in F32.  ids, ranks, scales and the banks are
+ * read on the device, at every replay of a captured call too, so slots can be
+ * refilled and requests moved between replays.  May be captured. */
+int samhip_supports_lora_add(const samhip_lora_bank* bank, const samhip_tensor* x, const samhip_tensor* ids,
+                             const samhip_tensor* base, const samhip_tensor* y);
+int samhip_lora_add(samhip_context* ctx, const samhip_lora_bank* bank, const samhip_tensor* x, const samhip_tensor* ids,
+                    const samhip_tensor* base, const samhip_tensor* y);
+
 /* GGML_OP_GET_ROWS: dst row i = to_float(src row ids[i]) (ggml_get_rows,
  * src/models/sam3/text_encoder.hpp:158).  src type F32/F16/Q8_0/Q4_K/Q5_K/
  * Q6_K, ids I32, dst F32.  Out-of-range ids fail with INVALID_ARGUMENT. */
@@ -374,8 +399,8 @@ int samhip_trace_pause(samhip_context* ctx, int paused);
  * at M = 32): the calls between capture_begin and capture_end are recorded
  * into a HIP graph instead of running, and graph_launch replays them on the
  * context's stream with one host call.  Only samhip_mul_mat,
- * samhip_quantize_rows, samhip_dequantize_rows and samhip_group_norm may be
- * captured; every other entry point fails with INVALID_ARGUMENT while a
+ * samhip_quantize_rows, samhip_dequantize_rows, samhip_lora_add and
+ * samhip_group_norm may be captured; every other entry point fails with INVALID_ARGUMENT while a
  * capture is open.  A
  * captured call must fit the context's current staging (run the same
  * product once before capturing); staging that has to grow later is

@@ -336,6 +336,34 @@ const char* strided_problem(const samhip_tensor& t, int dims) {
     return nullptr;
 }
 
+const char* lora_problem(const samhip_lora_bank* bank, const samhip_tensor* x, const samhip_tensor* ids,
+                         const samhip_tensor* base, const samhip_tensor* y) {
+    if (!bank || !x || !ids || !y) return "null argument";
+    if (bank->version != SAMHIP_ABI_VERSION) return "unsupported bank version";
+    if (const char* why = strided_problem(bank->a, 3)) return why;
+    if (const char* why = strided_problem(bank->b, 3)) return why;
+    for (const samhip_tensor* t : {x, base, y}) {
+        if (!t) continue;
+        if (t->type != T_F32) return "x, base and y must be F32";
+        if (const char* why = strided_problem(*t, 2)) return why;
+    }
+    if (bank->a.type != bank->b.type) return "a and b must be of one type";
+    const int64_t K = bank->a.ne[0], R = bank->a.ne[1], slots = bank->a.ne[2], N = y->ne[0], M = y->ne[1];
+    if (K <= 0 || R <= 0 || slots <= 0 || N <= 0 || M <= 0) return "empty operand";
+    if (bank->b.ne[0] != R || bank->b.ne[1] != N || bank->b.ne[2] != slots) return "b must be [R, N, slots]";
+    if (x->ne[0] != K || x->ne[1] != M) return "x must be [K, M]";
+    if (base && (base->ne[0] != N || base->ne[1] != M)) return "base must be [N, M]";
+    if (ids->type != T_I32 || ids->ne[0] != M || ids->ne[1] != 1 || ids->ne[2] != 1 || ids->ne[3] != 1 || ids->nb[0] != 4 ||
+        !ids->data || reinterpret_cast<uintptr_t>(ids->data) % 4)
+        return "ids must be M contiguous I32";
+    if (R > kLoraMaxRank) return "rank too large";
+    if (K > (int64_t(1) << 24) || N > (int64_t(1) << 23) || M > (int64_t(1) << 27) || slots > (int64_t(1) << 20))
+        return "dimension too large";
+    if (reinterpret_cast<uintptr_t>(bank->ranks) % 4 || reinterpret_cast<uintptr_t>(bank->scales) % 4)
+        return "ranks and scales must be 4-byte aligned";
+    return nullptr;
+}
+
 const char* group_norm_problem(const samhip_tensor* x, const samhip_tensor* y, int32_t groups, const float* w, const float* b,
                                float eps, int32_t activation) {
     if (!x || !y) return "null tensor descriptor";
@@ -861,6 +889,48 @@ int samhip_mul_mat(samhip_context* ctx, const samhip_tensor* w, const samhip_ten
     ctx->info.activation_payload_peak_bytes = std::max<uint64_t>(ctx->info.activation_payload_peak_bytes, a_bytes);
     std::snprintf(ctx->info.kernel_variant, sizeof(ctx->info.kernel_variant), "%s", variant);
     return SAMHIP_OK;
+}
+
+int samhip_supports_lora_add(const samhip_lora_bank* bank, const samhip_tensor* x, const samhip_tensor* ids,
+                             const samhip_tensor* base, const samhip_tensor* y) {
+    return lora_problem(bank, x, ids, base, y) == nullptr ? 1 : 0;
+}
+
+int samhip_lora_add(samhip_context* ctx, const samhip_lora_bank* bank, const samhip_tensor* x, const samhip_tensor* ids,
+                    const samhip_tensor* base, const samhip_tensor* y) {
+    if (!ctx) return fail(SAMHIP_ERR_INVALID_ARGUMENT, "null context");
+    if (const char* why = lora_problem(bank, x, ids, base, y)) return fail(SAMHIP_ERR_INVALID_ARGUMENT, "lora_add: %s", why);
+    const size_t e = size_t(block_bytes(bank->a.type));
+    LoraArgs a{};
+    a.x = static_cast<const float*>(x->data);
+    a.ldx = int64_t(x->nb[1] / 4);
+    a.ids = static_cast<const int32_t*>(ids->data);
+    a.base = base ? static_cast<const float*>(base->data) : nullptr;
+    a.ldbase = base ? int64_t(base->nb[1] / 4) : 0;
+    a.y = static_cast<float*>(y->data);
+    a.ldy = int64_t(y->nb[1] / 4);
+    a.a = bank->a.data;
+    a.b = bank->b.data;
+    a.a_row = int64_t(bank->a.nb[1] / e);
+    a.a_slot = int64_t(bank->a.nb[2] / e);
+    a.b_row = int64_t(bank->b.nb[1] / e);
+    a.b_slot = int64_t(bank->b.nb[2] / e);
+    a.ranks = bank->ranks;
+    a.scales = bank->scales;
+    a.m = x->ne[1];
+    a.k = int(bank->a.ne[0]);
+    a.n = int(y->ne[0]);
+    a.rank = int(bank->a.ne[1]);
+    a.slots = int(bank->a.ne[2]);
+    if (int rc = set_device(ctx)) return rc;
+    a.splits = lora_splits(a.m, a.k, ctx->cus);
+    if (int rc = ensure_staging(ctx, lora_part_bytes(a.m, a.rank, a.splits))) return rc;
+    a.part = static_cast<float*>(ctx->staging);
+    return traced(ctx, "lora_add", bank->a.type, a.m, a.n, a.k, [&]() -> int {
+        launch_lora(a, bank->a.type, ctx->cus, ctx->stream);
+        HIP_TRY(hipGetLastError(), "lora_add launch");
+        return SAMHIP_OK;
+    });
 }
 
 int samhip_get_rows(samhip_context* ctx, const samhip_tensor* src, const samhip_tensor* ids, const samhip_tensor* dst) {

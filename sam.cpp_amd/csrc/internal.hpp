@@ -434,4 +434,29 @@ size_t group_norm_scratch_bytes(const GroupNormShape& s, int vec);
 void launch_group_norm(const void* x, int x_type, void* y, int y_type, const GroupNormShape& s, int vec, const float* w,
                        const float* b, float eps, int act, void* scratch, hipStream_t stream);
 
+// Low-rank adapters beside a shared projection (lora.hip): strides in
+// elements; `part` holds lora_part_bytes, `splits` is lora_splits'.
+constexpr int kLoraMaxRank = 256;
+struct LoraArgs {
+    const float* x;
+    int64_t ldx;
+    const int32_t* ids;
+    const float* base;   // nullable; may be y
+    int64_t ldbase;
+    float* y;
+    int64_t ldy;
+    const void *a, *b;   // banks: A[slot][rank][k], B[slot][n][rank]
+    int64_t a_row, a_slot, b_row, b_slot;
+    const int32_t* ranks;   // nullable
+    const float* scales;    // nullable
+    int64_t m;
+    int k, n, rank, slots;
+    int splits;
+    float* part;
+    int k_len, part_ld;   // set by launch_lora
+};
+int lora_splits(int64_t m, int k, int cus);
+size_t lora_part_bytes(int64_t m, int rank, int splits);
+void launch_lora(LoraArgs a, int type, int cus, hipStream_t stream);
+
 }  // namespace samhip

@@ -87,6 +87,12 @@ class VitPrefixDesc(ctypes.Structure):
                [(n, ctypes.c_void_p) for n in ("patch_w", "pos_embed", "ln_pre_w", "ln_pre_b")]
 
 
+class LoraBank(ctypes.Structure):
+    """samhip_lora_bank."""
+    _fields_ = [("version", ctypes.c_int32), ("a", Tensor), ("b", Tensor), ("ranks", ctypes.c_void_p),
+                ("scales", ctypes.c_void_p)]
+
+
 SIGNATURES = {
     "samhip_abi_version": ([], _I),
     "samhip_device_count": ([_P], _I),
@@ -122,6 +128,8 @@ SIGNATURES = {
     "samhip_vit_neck": ([_P, ctypes.POINTER(VitNeckDesc), _P, _P, _P, _P, _P], _I),
     "samhip_layer_norm": ([_P, _P, _P, _I64, _I64, _P, _P, ctypes.c_float], _I),
     "samhip_flash_attn": ([_P, _P, _P, _P, _I64, _P, _I64, _I64, _I32, _I32, ctypes.c_float], _I),
+    "samhip_supports_lora_add": ([ctypes.POINTER(LoraBank)] + [ctypes.POINTER(Tensor)] * 4, _I),
+    "samhip_lora_add": ([_P, ctypes.POINTER(LoraBank)] + [ctypes.POINTER(Tensor)] * 4, _I),
     "samhip_supports_group_norm": ([ctypes.POINTER(Tensor), ctypes.POINTER(Tensor), _I32, _P, _P, ctypes.c_float, _I32], _I),
     "samhip_group_norm": ([_P, ctypes.POINTER(Tensor), ctypes.POINTER(Tensor), _I32, _P, _P, ctypes.c_float, _I32], _I),
 }
@@ -203,6 +211,11 @@ def tensor_nd(qtype, ne, nb, data):
         t.nb[i] = nb[i] if i < len(nb) else t.nb[i - 1] * t.ne[i - 1]
     t.data = data
     return t
+
+
+def lora_bank(a, b, ranks_ptr=None, scales_ptr=None):
+    """A samhip_lora_bank over device banks a {K, R, slots} and b {R, N, slots}."""
+    return LoraBank(ABI_VERSION, a, b, ranks_ptr, scales_ptr)
 
 
 def validate_quantized_payload(qtype, ne0, rows, payload):
@@ -298,6 +311,11 @@ class Context:
 
     def dequantize_rows(self, qtype, src_ptr, src_stride, dst_ptr, rows, k):
         check(lib().samhip_dequantize_rows(self.handle, qtype, src_ptr, src_stride, dst_ptr, rows, k))
+
+    def lora_add(self, bank, x, ids, base, y):
+        """samhip_lora_add; base is a descriptor or None."""
+        check(lib().samhip_lora_add(self.handle, ctypes.byref(bank), ctypes.byref(x), ctypes.byref(ids),
+                                    None if base is None else ctypes.byref(base), ctypes.byref(y)))
 
     def group_norm(self, x, y, groups, w_ptr, b_ptr, eps, activation=ACT_NONE):
         """samhip_group_norm on channels-last descriptors {channels, pixels, images}."""
