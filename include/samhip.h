@@ -344,6 +344,42 @@ int samhip_layer_norm(samhip_context* ctx, const float* x, float* y, int64_t row
 int samhip_flash_attn(samhip_context* ctx, const float* q, const float* k, const float* v, int64_t ld, float* out,
                       int64_t batches, int64_t n, int32_t heads, int32_t head_dim, float scale);
 
+/* Attention of a batch of requests (prompts) that share a prefix of keys (an
+ * image's tokens), each with further keys of its own; no reference
+ * counterpart.  For every query row and head
+ *   out = softmax(scale * q K^T) V,  K, V = [prefix ; the request's own rows]
+ * F32-accurate as samhip_flash_attn.  Grouped heads: head h reads kv head
+ * h / (heads / kv_heads), at columns (kv head) * head_dim.  Row strides are
+ * free; the prefix and the own rows may be empty (ne[1] = 0).  The queries
+ * of request r are rows [q_start[r], q_start[r + 1]), its own keys rows
+ * [own_start[r], own_start[r] + own_len[r]) of own_k and own_v, so a request
+ * may keep its rows packed or in a slot of a cache.  With `causal`, query i
+ * of a request's n sees its first own_len - n + i + 1 own keys (and all of the
+ * prefix).  A query without any key gets zeros; rows of out outside
+ * [q_start[0], q_start[requests]) are left as they were.  Rows behind own_len
+ * are not read; the rows that are read must be finite, masked ones too.
+ * The three tables are read on the device (at every replay of a captured
+ * call) and cut to what exists: query rows to [0, rows), lengths to
+ * [0, own_max] and the rows of own_k; an own_start outside them means no
+ * keys.  q_start must not decrease. */
+typedef struct samhip_prefix_attn_desc {
+    int32_t version;                  /* SAMHIP_ABI_VERSION */
+    int32_t heads, kv_heads;          /* heads a multiple of kv_heads */
+    int32_t head_dim;                 /* 32, 64 or 128 */
+    float scale;
+    int32_t causal;
+    int32_t requests;
+    int32_t own_max;                  /* no own_len counts beyond it; 0: no own keys */
+    samhip_tensor q, out;             /* F32 {heads * head_dim, rows} */
+    samhip_tensor prefix_k, prefix_v; /* F16 or F32 {kv_heads * head_dim, keys} */
+    samhip_tensor own_k, own_v;       /* the same type {kv_heads * head_dim, rows of all requests} */
+    const int32_t* q_start;           /* device I32 [requests + 1] */
+    const int32_t *own_start, *own_len;   /* device I32 [requests]; not read with own_max 0 */
+} samhip_prefix_attn_desc;
+int samhip_supports_prefix_attn(const samhip_prefix_attn_desc* desc);
+/* May be captured. */
+int samhip_prefix_attn(samhip_context* ctx, const samhip_prefix_attn_desc* desc);
+
 /* Activation after a normalization. */
 enum samhip_activation {
     SAMHIP_ACT_NONE = 0,
@@ -399,8 +435,8 @@ int samhip_trace_pause(samhip_context* ctx, int paused);
  * at M = 32): the calls between capture_begin and capture_end are recorded
  * into a HIP graph instead of running, and graph_launch replays them on the
  * context's stream with one host call.  Only samhip_mul_mat,
- * samhip_quantize_rows, samhip_dequantize_rows, samhip_lora_add and
- * samhip_group_norm may be captured; every other entry point fails with INVALID_ARGUMENT while a
+ * samhip_quantize_rows, samhip_dequantize_rows, samhip_lora_add, samhip_prefix_attn
+ * and samhip_group_norm may be captured; every other entry point fails with INVALID_ARGUMENT while a
  * capture is open.  A
  * captured call must fit the context's current staging (run the same
  * product once before capturing); staging that has to grow later is

@@ -364,6 +364,32 @@ const char* lora_problem(const samhip_lora_bank* bank, const samhip_tensor* x, c
     return nullptr;
 }
 
+const char* prefix_attn_problem(const samhip_prefix_attn_desc* d) {
+    if (!d) return "null descriptor";
+    if (d->version != SAMHIP_ABI_VERSION) return "unsupported descriptor version";
+    for (const samhip_tensor* t : {&d->q, &d->out, &d->prefix_k, &d->prefix_v, &d->own_k, &d->own_v})
+        if (const char* why = strided_problem(*t, 2)) return why;
+    if (d->q.type != T_F32 || d->out.type != T_F32) return "q and out must be F32";
+    const int type = d->prefix_k.type;
+    if (d->prefix_v.type != type || d->own_k.type != type || d->own_v.type != type) return "keys and values must be of one type";
+    if (d->heads <= 0 || d->kv_heads <= 0 || d->heads > 4096 || d->heads % d->kv_heads) return "heads must be a multiple of kv_heads";
+    if (d->head_dim != 32 && d->head_dim != 64 && d->head_dim != 128) return "head_dim must be 32, 64 or 128";
+    const int64_t width = int64_t(d->heads) * d->head_dim, kv_width = int64_t(d->kv_heads) * d->head_dim, rows = d->q.ne[1];
+    if (d->q.ne[0] != width || d->out.ne[0] != width || d->out.ne[1] != rows) return "q and out must be [heads * head_dim, rows]";
+    if (rows <= 0 || d->requests <= 0 || d->own_max < 0) return "empty operand";
+    for (const samhip_tensor* t : {&d->prefix_k, &d->prefix_v, &d->own_k, &d->own_v})
+        if (t->ne[0] != kv_width) return "keys and values must be kv_heads * head_dim wide";
+    if (d->prefix_k.ne[1] != d->prefix_v.ne[1] || d->own_k.ne[1] != d->own_v.ne[1]) return "keys and values differ in rows";
+    if (!std::isfinite(d->scale)) return "scale must be finite";
+    if (!d->q_start || (d->own_max > 0 && (!d->own_start || !d->own_len))) return "null table";
+    for (const int32_t* t : {d->q_start, d->own_start, d->own_len})
+        if (reinterpret_cast<uintptr_t>(t) % 4) return "tables must be 4-byte aligned";
+    if (rows * d->heads > (int64_t(1) << 26) || d->prefix_k.ne[1] > (int64_t(1) << 30) || d->own_max > (1 << 30) ||
+        d->requests > (1 << 20))
+        return "dimension too large";
+    return nullptr;
+}
+
 const char* group_norm_problem(const samhip_tensor* x, const samhip_tensor* y, int32_t groups, const float* w, const float* b,
                                float eps, int32_t activation) {
     if (!x || !y) return "null tensor descriptor";
@@ -1240,6 +1266,47 @@ int samhip_flash_attn(samhip_context* ctx, const float* q, const float* k, const
                               att_bytes, ctx->cus, ctx->stream))
             return fail(SAMHIP_ERR_UNSUPPORTED, "flash_attn: no attention launch for this grid");
         HIP_TRY(hipGetLastError(), "attention launch");
+        return SAMHIP_OK;
+    });
+}
+
+int samhip_supports_prefix_attn(const samhip_prefix_attn_desc* desc) { return prefix_attn_problem(desc) == nullptr ? 1 : 0; }
+
+int samhip_prefix_attn(samhip_context* ctx, const samhip_prefix_attn_desc* d) {
+    if (!ctx) return fail(SAMHIP_ERR_INVALID_ARGUMENT, "null context");
+    if (const char* why = prefix_attn_problem(d)) return fail(SAMHIP_ERR_INVALID_ARGUMENT, "prefix_attn: %s", why);
+    const size_t e = size_t(block_bytes(d->prefix_k.type));
+    PrefixAttnArgs a{};
+    a.q = static_cast<const float*>(d->q.data);
+    a.ldq = int64_t(d->q.nb[1] / 4);
+    a.out = static_cast<float*>(d->out.data);
+    a.ldo = int64_t(d->out.nb[1] / 4);
+    a.prefix_k = d->prefix_k.data;
+    a.prefix_v = d->prefix_v.data;
+    a.own_k = d->own_k.data;
+    a.own_v = d->own_v.data;
+    a.ld_prefix_k = int64_t(d->prefix_k.nb[1] / e);
+    a.ld_prefix_v = int64_t(d->prefix_v.nb[1] / e);
+    a.ld_own_k = int64_t(d->own_k.nb[1] / e);
+    a.ld_own_v = int64_t(d->own_v.nb[1] / e);
+    a.own_rows = d->own_k.ne[1];
+    a.q_start = d->q_start;
+    a.own_start = d->own_start;
+    a.own_len = d->own_len;
+    a.prefix = int(d->prefix_k.ne[1]);
+    a.own_max = int(std::min<int64_t>(d->own_max, a.own_rows));
+    a.requests = d->requests;
+    a.rows = int(d->q.ne[1]);
+    a.heads = d->heads;
+    a.kv_heads = d->kv_heads;
+    a.scale = d->scale;
+    a.causal = d->causal != 0;
+    if (int rc = set_device(ctx)) return rc;
+    prefix_attn_plan(a, ctx->cus);
+    if (int rc = ensure_staging(ctx, prefix_attn_scratch_bytes(a, d->head_dim))) return rc;
+    return traced(ctx, "prefix_attn", d->prefix_k.type, a.rows, int64_t(a.heads) * d->head_dim, a.prefix, [&]() -> int {
+        launch_prefix_attn(a, d->prefix_k.type, d->head_dim, ctx->staging, ctx->stream);
+        HIP_TRY(hipGetLastError(), "prefix_attn launch");
         return SAMHIP_OK;
     });
 }

@@ -459,4 +459,29 @@ int lora_splits(int64_t m, int k, int cus);
 size_t lora_part_bytes(int64_t m, int rank, int splits);
 void launch_lora(LoraArgs a, int type, int cus, hipStream_t stream);
 
+// Attention of requests that share a prefix (prefix_attn.hip); strides in
+// elements.  prefix_attn_plan sets the fields behind `causal` but the two
+// scratch pointers, which launch_prefix_attn sets.
+struct PrefixAttnArgs {
+    const float* q;
+    int64_t ldq;
+    float* out;
+    int64_t ldo;
+    const void *prefix_k, *prefix_v, *own_k, *own_v;
+    int64_t ld_prefix_k, ld_prefix_v, ld_own_k, ld_own_v;
+    int64_t own_rows;
+    const int32_t *q_start, *own_start, *own_len;
+    int prefix, own_max, requests, rows, heads, kv_heads;
+    float scale;
+    bool causal;
+    int group;
+    int prefix_tiles, prefix_splits, prefix_chunk;   // workgroups per kv head, and keys of a split
+    int own_tiles, own_splits, own_chunk;
+    int parts;
+    float *part_o, *part_ml;
+};
+void prefix_attn_plan(PrefixAttnArgs& a, int cus);
+size_t prefix_attn_scratch_bytes(const PrefixAttnArgs& a, int head_dim);
+void launch_prefix_attn(PrefixAttnArgs a, int type, int head_dim, void* scratch, hipStream_t stream);
+
 }  // namespace samhip

@@ -93,6 +93,15 @@ class LoraBank(ctypes.Structure):
                 ("scales", ctypes.c_void_p)]
 
 
+class PrefixAttnDesc(ctypes.Structure):
+    """samhip_prefix_attn_desc."""
+    _fields_ = [("version", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("scale", ctypes.c_float), ("causal", ctypes.c_int32),
+                ("requests", ctypes.c_int32), ("own_max", ctypes.c_int32)] + \
+               [(n, Tensor) for n in ("q", "out", "prefix_k", "prefix_v", "own_k", "own_v")] + \
+               [(n, ctypes.c_void_p) for n in ("q_start", "own_start", "own_len")]
+
+
 SIGNATURES = {
     "samhip_abi_version": ([], _I),
     "samhip_device_count": ([_P], _I),
@@ -130,6 +139,8 @@ SIGNATURES = {
     "samhip_flash_attn": ([_P, _P, _P, _P, _I64, _P, _I64, _I64, _I32, _I32, ctypes.c_float], _I),
     "samhip_supports_lora_add": ([ctypes.POINTER(LoraBank)] + [ctypes.POINTER(Tensor)] * 4, _I),
     "samhip_lora_add": ([_P, ctypes.POINTER(LoraBank)] + [ctypes.POINTER(Tensor)] * 4, _I),
+    "samhip_supports_prefix_attn": ([ctypes.POINTER(PrefixAttnDesc)], _I),
+    "samhip_prefix_attn": ([_P, ctypes.POINTER(PrefixAttnDesc)], _I),
     "samhip_supports_group_norm": ([ctypes.POINTER(Tensor), ctypes.POINTER(Tensor), _I32, _P, _P, ctypes.c_float, _I32], _I),
     "samhip_group_norm": ([_P, ctypes.POINTER(Tensor), ctypes.POINTER(Tensor), _I32, _P, _P, ctypes.c_float, _I32], _I),
 }
@@ -216,6 +227,13 @@ def tensor_nd(qtype, ne, nb, data):
 def lora_bank(a, b, ranks_ptr=None, scales_ptr=None):
     """A samhip_lora_bank over device banks a {K, R, slots} and b {R, N, slots}."""
     return LoraBank(ABI_VERSION, a, b, ranks_ptr, scales_ptr)
+
+
+def prefix_attn_desc(heads, kv_heads, head_dim, scale, q, out, prefix_k, prefix_v, own_k, own_v, requests, q_start_ptr,
+                     own_start_ptr=None, own_len_ptr=None, own_max=0, causal=False):
+    """A samhip_prefix_attn_desc; the tables are device addresses of I32."""
+    return PrefixAttnDesc(ABI_VERSION, heads, kv_heads, head_dim, scale, 1 if causal else 0, requests, own_max, q, out,
+                          prefix_k, prefix_v, own_k, own_v, q_start_ptr, own_start_ptr, own_len_ptr)
 
 
 def validate_quantized_payload(qtype, ne0, rows, payload):
@@ -316,6 +334,10 @@ class Context:
         """samhip_lora_add; base is a descriptor or None."""
         check(lib().samhip_lora_add(self.handle, ctypes.byref(bank), ctypes.byref(x), ctypes.byref(ids),
                                     None if base is None else ctypes.byref(base), ctypes.byref(y)))
+
+    def prefix_attn(self, desc):
+        """samhip_prefix_attn."""
+        check(lib().samhip_prefix_attn(self.handle, ctypes.byref(desc)))
 
     def group_norm(self, x, y, groups, w_ptr, b_ptr, eps, activation=ACT_NONE):
         """samhip_group_norm on channels-last descriptors {channels, pixels, images}."""
