@@ -1325,10 +1325,9 @@ int samhip_group_norm(samhip_context* ctx, const samhip_tensor* x, const samhip_
     const GroupNormShape s{int(x->ne[2]), int(x->ne[1]), int(x->ne[0]), groups, int64_t(x->nb[1] / xb), int64_t(x->nb[2] / xb),
                            int64_t(y->nb[1] / yb), int64_t(y->nb[2] / yb)};
     if (int rc = set_device(ctx)) return rc;
-    const int vec = group_norm_vec(s, x->data, xb, y->data, yb);
-    if (int rc = ensure_staging(ctx, group_norm_scratch_bytes(s, vec))) return rc;
+    if (int rc = ensure_staging(ctx, group_norm_scratch_bytes(s, group_norm_vec(x->type)))) return rc;
     return traced(ctx, "group_norm", x->type, int64_t(s.images) * s.pixels, s.channels, groups, [&]() -> int {
-        launch_group_norm(x->data, x->type, y->data, y->type, s, vec, w, b, eps, activation, ctx->staging, ctx->stream);
+        launch_group_norm(x->data, x->type, y->data, y->type, s, w, b, eps, activation, ctx->staging, ctx->stream);
         HIP_TRY(hipGetLastError(), "group_norm launch");
         return SAMHIP_OK;
     });

@@ -18,56 +18,90 @@ namespace samhip {
 
 namespace {
 
-template <class T, int VEC>
-struct Vec {
-    typedef T type __attribute__((ext_vector_type(VEC)));
+// Channels of one load: 16 bytes.  Rows need no alignment beyond their
+// element's; the last vector of a row that holds fewer channels is read and
+// written one by one.
+template <class T>
+constexpr int kVec = 16 / sizeof(T);
+
+template <class T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Packed {
+    typedef T type __attribute__((ext_vector_type(N)));
+    type v;
 };
 template <class T>
-struct Vec<T, 1> {
-    typedef T type;
+using Vector = typename Packed<T, kVec<T>>::type;
+
+// n channels at p
+template <class T>
+__device__ __forceinline__ Vector<T> load(const T* p, int n) {
+    if (n == kVec<T>) return reinterpret_cast<const Packed<T, kVec<T>>*>(p)->v;
+    Vector<T> v;
+#pragma unroll
+    for (int e = 0; e < kVec<T>; ++e) v[e] = p[min(e, n - 1)];
+    return v;
+}
+template <class T, int VEC>
+__device__ __forceinline__ void store(T* p, int n, const float (&v)[VEC]) {
+    if (n == VEC) {
+        Packed<T, VEC> r;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) r.v[e] = (T)v[e];   // F16: round to nearest even
+        *reinterpret_cast<Packed<T, VEC>*>(p) = r;
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (e < n) p[e] = (T)v[e];
+    }
+}
+
+// Sums of x and x^2: F32 runs of x - shift, with a value of the run itself as
+// the shift, so that a mean far above the deviation cancels exactly; what a
+// run leaves goes to F64.
+struct Run {
+    float shift, s1 = 0.f, s2 = 0.f;
+    __device__ __forceinline__ void add(float x) {
+        const float d = x - shift;
+        s1 += d;
+        s2 = __builtin_fmaf(d, d, s2);
+    }
+    __device__ __forceinline__ void into(float n, double& sum, double& sq) const {
+        const double a = shift, s = s1;
+        sum += __builtin_fma((double)n, a, s);
+        sq += __builtin_fma(a, __builtin_fma((double)n, a, 2.0 * s), (double)s2);
+    }
 };
 
-template <class T, int VEC>
-__device__ __forceinline__ void load(const T* p, float (&v)[VEC]) {
-    const auto r = *reinterpret_cast<const typename Vec<T, VEC>::type*>(p);
-    if constexpr (VEC == 1) v[0] = (float)r;
-    else
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = (float)r[e];
-}
-
-template <class T, int VEC>
-__device__ __forceinline__ void store(T* p, const float (&v)[VEC]) {
-    typename Vec<T, VEC>::type r;
-    if constexpr (VEC == 1) r = (T)v[0];
-    else
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) r[e] = (T)v[e];   // F16: round to nearest even
-    *reinterpret_cast<typename Vec<T, VEC>::type*>(p) = r;
-}
-
-// one row swap or rotation of a double's two halves
-template <int STEP>
-__device__ __forceinline__ double partner(double v) {
+template <int CTRL>
+__device__ __forceinline__ double dpp_double(double v) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    uint32_t lo = uint32_t(u), hi = uint32_t(u >> 32);
-    lo = uint32_t(__shfl_xor(int(lo), STEP, 64));
-    hi = uint32_t(__shfl_xor(int(hi), STEP, 64));
-    return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+    return __builtin_bit_cast(double, uint64_t(uint32_t(samhip::dpp<CTRL>(int(u >> 32)))) << 32 | uint32_t(samhip::dpp<CTRL>(int(uint32_t(u)))));
 }
-__device__ __forceinline__ double wave_sum(double v) {
-    v += partner<32>(v);
-    v += partner<16>(v);
-    v += partner<8>(v);
-    v += partner<4>(v);
-    v += partner<2>(v);
-    return v + partner<1>(v);
+// Sum over aligned runs of `lanes` (a power of two): each step adds the other
+// half's sum, which a mirror reaches as well as an xor once halves agree.
+__device__ __forceinline__ double lane_sum(double v, int lanes) {
+    constexpr int HALF_MIRROR = 0x141, MIRROR = 0x140;
+    if (lanes >= 2) v += dpp_double<DPP_XOR1>(v);
+    if (lanes >= 4) v += dpp_double<DPP_XOR2>(v);
+    if (lanes >= 8) v += dpp_double<HALF_MIRROR>(v);
+    if (lanes >= 16) v += dpp_double<MIRROR>(v);
+    const auto swapped = [&](auto swap) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const auto lo = swap(uint32_t(u)), hi = swap(uint32_t(u >> 32));
+        return __builtin_bit_cast(double, uint64_t(hi[0]) << 32 | lo[0]) + __builtin_bit_cast(double, uint64_t(hi[1]) << 32 | lo[1]);
+    };
+    if (lanes >= 32) v = swapped([](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
+    if (lanes >= 64) v = swapped([](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
+    return v;
 }
+__device__ __forceinline__ double wave_sum(double v) { return lane_sum(v, 64); }
 
 // A group's statistics as the apply step uses them: mean = hi + lo.
 struct Moments {
     float hi, lo, rstd;
 };
+
+constexpr int kGroupNormInline = 2048;   // partial sums that every workgroup of the last launch adds up itself
 
 __device__ __forceinline__ Moments moments(double sum, double sq, double n, float eps) {
     const double mean = sum / n;
@@ -80,53 +114,47 @@ __device__ __forceinline__ Moments moments(double sum, double sq, double n, floa
     return m;
 }
 
-template <int ACT>
-__device__ __forceinline__ float activate(float v) {
-    if (ACT == ACT_RELU) return v > 0.f || v != v ? v : 0.f;
-    if (ACT == ACT_SILU) return v / (1.f + __expf(-v));
-    if (ACT == ACT_GELU_ERF) return gelu_erf(v);
+__device__ __forceinline__ float activate(int act, float v) {   // act is uniform
+    if (act == ACT_RELU) return v > 0.f || v != v ? v : 0.f;
+    // reciprocal and exponential within an ulp each
+    if (act == ACT_SILU) return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+    if (act == ACT_GELU_ERF) return gelu_erf(v);
     return v;
 }
-__device__ __forceinline__ float activate(int act, float v) {
-    switch (act) {   // uniform
-        case ACT_RELU: return activate<ACT_RELU>(v);
-        case ACT_SILU: return activate<ACT_SILU>(v);
-        case ACT_GELU_ERF: return activate<ACT_GELU_ERF>(v);
-        default: return v;
-    }
-}
 
-__device__ __forceinline__ float normalize(float x, const Moments& m) { return ((x - m.hi) - m.lo) * m.rstd; }
-
-template <class TI, class TO, int VEC, int NV>
+// One workgroup per (image, group).  A thread keeps to one vector of the
+// group's channels and takes every rows-th pixel.
+template <class TI, class TO, int NV>
 __global__ __launch_bounds__(1024) void group_norm_block_kernel(const TI* x, TO* y, GroupNormShape s, const float* __restrict__ w,
                                                                 const float* __restrict__ b, float eps, int act) {
+    constexpr int VEC = kVec<TI>;
     __shared__ double part[16][2];
     const int g = blockIdx.x, image = blockIdx.y, tid = threadIdx.x;
-    const int size = s.channels / s.groups, cols = size / VEC, total = s.pixels * cols;
-    const TI* xg = x + image * s.x_image + g * size;
-    TO* yg = y + image * s.y_image + g * size;
-    float v[NV][VEC];
-    double sum = 0.0, sq = 0.0;
+    const int size = s.channels / s.groups, cols = (size + VEC - 1) / VEC, rows = blockDim.x / cols;
+    const int row = tid / cols, c = (tid - row * cols) * VEC, n = min(size - c, VEC);
+    const int count = row < rows && row < s.pixels ? (s.pixels - 1 - row) / rows + 1 : 0;   // at most NV
+    const int64_t first = min(row, s.pixels - 1), x_step = rows * s.x_pixel, y_step = rows * s.y_pixel;
+    const TI* xg = x + image * s.x_image + g * size + c + first * s.x_pixel;
+    TO* yg = y + image * s.y_image + g * size + c + first * s.y_pixel;
+    Vector<TI> v[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int at = tid + i * 1024;
-        if (at < total) {
-            const int p = at / cols, c = at - p * cols;
-            load<TI, VEC>(xg + p * s.x_pixel + c * VEC, v[i]);
-        } else {
+    for (int i = 0; i < NV; ++i) v[i] = load<TI>(xg + max(min(i, count - 1), 0) * x_step, n);
+    float ww[VEC], bb[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[i][e] = 0.f;
-        }
+    for (int e = 0; e < VEC; ++e) {
+        const int ch = g * size + min(c + e, size - 1);
+        ww[e] = w ? w[ch] : 1.f;
+        bb[e] = b ? b[ch] : 0.f;
     }
+    double sum = 0.0, sq = 0.0;
+    {
+        Run run{(float)v[0][0]};
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const double d = (double)v[i][e];
-            sum += d;
-            sq = __builtin_fma(d, d, sq);
-        }
+            for (int e = 0; e < VEC; ++e) run.add(i < count && e < n ? (float)v[i][e] : run.shift);
+        if (count) run.into((float)(count * n), sum, sq);
+    }
     sum = wave_sum(sum);
     sq = wave_sum(sq);
     if ((tid & 63) == 0) {
@@ -135,75 +163,92 @@ __global__ __launch_bounds__(1024) void group_norm_block_kernel(const TI* x, TO*
     }
     __syncthreads();
     sum = sq = 0.0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < int(blockDim.x) / 64; ++i) {
         sum += part[i][0];
         sq += part[i][1];
     }
     const Moments m = moments(sum, sq, double(s.pixels) * size, eps);
 #pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        ww[e] = ww[e] * m.rstd;
+        bb[e] = bb[e] - m.lo * ww[e];
+    }
+#pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int at = tid + i * 1024;
-        if (at >= total) break;
-        const int p = at / cols, c = at - p * cols, ch = g * size + c * VEC;
+        if (i >= count) break;
         float o[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            o[e] = normalize(v[i][e], m);
-            if (w) o[e] = o[e] * w[ch + e];
-            if (b) o[e] = o[e] + b[ch + e];
-            o[e] = activate(act, o[e]);
-        }
-        store<TO, VEC>(yg + p * s.y_pixel + c * VEC, o);
+        for (int e = 0; e < VEC; ++e) o[e] = activate(act, __builtin_fmaf((float)v[i][e] - m.hi, ww[e], bb[e]));
+        store<TO, VEC>(yg + i * y_step, n, o);
     }
 }
 
-// Thread t of 256 owns the VEC channels of column t % cols (pass j: column
-// t % cols + 256 j) and every rows-th pixel of the chunk.
-template <class TI, int VEC>
+constexpr int FLIGHT = 8;   // pixels that a thread has in flight
+constexpr int RUN = 8;      // of which batches one F32 run
+
+// Thread t of 256 owns the channels of vector t % cols (pass j: of vector
+// t % cols + 256 j) and every rows-th pixel of the chunk.  SAME: the channels
+// of a vector are of one group, and one run takes them all.
+template <class TI, bool SAME>
 __global__ __launch_bounds__(256) void group_norm_stats_kernel(const TI* __restrict__ x, GroupNormShape s, int chunk,
                                                                double* __restrict__ partial) {
-    extern __shared__ double sums[][2];   // [rows][channels]
-    const int tid = threadIdx.x, cols = s.channels / VEC;
-    const int width = min(cols, 256), rows = 256 / width, col0 = tid % width, row = tid / width;
-    const int p0 = blockIdx.x * chunk, p1 = min(p0 + chunk, s.pixels);
-    const TI* xi = x + blockIdx.y * s.x_image;
+    constexpr int VEC = kVec<TI>, RUNS = SAME ? 1 : VEC;
+    extern __shared__ double sums[];   // [sum, sum of squares][rows][RUNS][cols]: lanes write neighbouring places
+    const int tid = threadIdx.x, cols = (s.channels + VEC - 1) / VEC;
+    const int width = min(cols, 256), rows = 256 / width, row = tid / width, col0 = tid - row * width;
+    const int p0 = blockIdx.x * chunk + row, p1 = min((blockIdx.x + 1) * chunk, s.pixels);
+    const int plane = rows * RUNS * cols;
     if (row < rows) {
         for (int col = col0; col < cols; col += width) {
-            double sum[VEC], sq[VEC];
+            double sum[RUNS], sq[RUNS];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) sum[e] = sq[e] = 0.0;
-            const TI* xc = xi + col * VEC;
-#pragma unroll 4
-            for (int p = p0 + row; p < p1; p += rows) {
-                float v[VEC];
-                load<TI, VEC>(xc + p * s.x_pixel, v);
+            for (int e = 0; e < RUNS; ++e) sum[e] = sq[e] = 0.0;
+            const TI* xc = x + blockIdx.y * s.x_image + col * VEC;
+            const int n = min(s.channels - col * VEC, VEC);
+            for (int p = p0; p < p1;) {
+                const int q = p;
+                Run run[RUNS];
+                for (int k = 0; k < RUN && p < p1; ++k, p += FLIGHT * rows) {
+                    Vector<TI> v[FLIGHT];   // the last pixel again where there are no more
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const double d = (double)v[e];
-                    sum[e] += d;
-                    sq[e] = __builtin_fma(d, d, sq[e]);
+                    for (int u = 0; u < FLIGHT; ++u) v[u] = load<TI>(xc + min(p + u * rows, p1 - 1) * s.x_pixel, n);
+                    if (k == 0)
+#pragma unroll
+                        for (int e = 0; e < RUNS; ++e) run[e].shift = (float)v[0][e];
+#pragma unroll
+                    for (int u = 0; u < FLIGHT; ++u)
+                        if (p + u * rows < p1)
+#pragma unroll
+                            for (int e = 0; e < VEC; ++e) run[SAME ? 0 : e].add((float)v[u][e]);
                 }
+                const float count = (float)((min(p, p1) - q + rows - 1) / rows * (SAME ? VEC : 1));
+#pragma unroll
+                for (int e = 0; e < RUNS; ++e) run[e].into(count, sum[e], sq[e]);
             }
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                sums[row * s.channels + col * VEC + e][0] = sum[e];
-                sums[row * s.channels + col * VEC + e][1] = sq[e];
+            for (int e = 0; e < RUNS; ++e) {
+                sums[(row * RUNS + e) * cols + col] = sum[e];
+                sums[plane + (row * RUNS + e) * cols + col] = sq[e];
             }
         }
     }
     __syncthreads();
-    const int size = s.channels / s.groups, members = size * rows, lane = tid & 63;
-    for (int g = tid >> 6; g < s.groups; g += 4) {
+    const int size = s.channels / s.groups;
+    const int members = SAME ? size / VEC : size, all = rows * members;
+    // as many lanes per group as leave a place for every group, 64 at most
+    int lanes = 64;
+    while (lanes > 1 && lanes * s.groups > 256) lanes >>= 1;
+    for (int g = tid / lanes; g < s.groups; g += 256 / lanes) {
         double sum = 0.0, sq = 0.0;
-        for (int i = lane; i < members; i += 64) {
-            const int r = i / size, at = r * s.channels + g * size + (i - r * size);
-            sum += sums[at][0];
-            sq += sums[at][1];
+        for (int i = tid & (lanes - 1); i < all; i += lanes) {
+            const int r = i / members, ch = g * members + i - r * members;
+            const int at = SAME ? r * cols + ch : (r * RUNS + ch % VEC) * cols + ch / VEC;
+            sum += sums[at];
+            sq += sums[plane + at];
         }
-        sum = wave_sum(sum);
-        sq = wave_sum(sq);
-        if (lane == 0) {
+        sum = lane_sum(sum, lanes);
+        sq = lane_sum(sq, lanes);
+        if ((tid & (lanes - 1)) == 0) {
             double* out = partial + ((int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * s.groups + g) * 2;
             out[0] = sum;
             out[1] = sq;
@@ -211,111 +256,166 @@ __global__ __launch_bounds__(256) void group_norm_stats_kernel(const TI* __restr
     }
 }
 
-__global__ __launch_bounds__(64) void group_norm_finish_kernel(const double* __restrict__ partial, int chunks, int groups,
-                                                               double n, float eps, Moments* __restrict__ out) {
-    const int g = blockIdx.x, image = blockIdx.y;
-    double sum = 0.0, sq = 0.0;
-    for (int i = threadIdx.x; i < chunks; i += 64) {
-        const double* p = partial + ((int64_t(image) * chunks + i) * groups + g) * 2;
-        sum += p[0];
-        sq += p[1];
+// An image's partial sums over its chunks, by 256 threads: thread t adds
+// every (256 / groups)-th chunk's of group t % groups, neighbours reading
+// neighbouring places.  `out` has a place for each group.
+__device__ __forceinline__ void finish(const double* __restrict__ partial, int chunks, int groups, double n, float eps,
+                                       double (*lds)[2], Moments* out) {
+    typedef double double2_t __attribute__((ext_vector_type(2)));
+    const int tid = threadIdx.x;
+    for (int g0 = 0; g0 < groups; g0 += 256) {
+        const int here = min(groups - g0, 256), step = 256 / here, c0 = tid / here, g = tid - c0 * here;
+        double sum = 0.0, sq = 0.0;
+        if (c0 < step) {
+#pragma unroll 8
+            for (int c = c0; c < chunks; c += step) {
+                const double2_t p = *reinterpret_cast<const double2_t*>(partial + (int64_t(c) * groups + g0 + g) * 2);
+                sum += p[0];
+                sq += p[1];
+            }
+        }
+        lds[tid][0] = sum;
+        lds[tid][1] = sq;
+        __syncthreads();
+        if (tid < here) {
+#pragma unroll 8
+            for (int i = 1; i < step; ++i) {
+                sum += lds[tid + i * here][0];
+                sq += lds[tid + i * here][1];
+            }
+            out[g0 + tid] = moments(sum, sq, n, eps);
+        }
+        __syncthreads();
     }
-    sum = wave_sum(sum);
-    sq = wave_sum(sq);
-    if (threadIdx.x == 0) out[image * groups + g] = moments(sum, sq, n, eps);
 }
 
-template <class TI, class TO, int VEC>
+__global__ __launch_bounds__(256) void group_norm_finish_kernel(const double* __restrict__ partial, int chunks, int groups, double n,
+                                                                float eps, Moments* __restrict__ out) {
+    __shared__ double lds[256][2];
+    finish(partial + int64_t(blockIdx.x) * chunks * groups * 2, chunks, groups, n, eps, lds, out + int64_t(blockIdx.x) * groups);
+}
+
+// `stats` is null where the workgroups finish the partial sums themselves.
+// The chunks in the other order: the last ones read are still in L2.
+template <class TI, class TO, bool SAME>
 __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* y, GroupNormShape s, int chunk,
-                                                               const Moments* __restrict__ stats, const float* __restrict__ w,
-                                                               const float* __restrict__ b, int act) {
-    const int tid = threadIdx.x, cols = s.channels / VEC, size = s.channels / s.groups;
-    const int width = min(cols, 256), rows = 256 / width, col0 = tid % width, row = tid / width;
-    if (row >= rows) return;
-    const int p0 = blockIdx.x * chunk, p1 = min(p0 + chunk, s.pixels);
+                                                               const double* __restrict__ partial, const Moments* __restrict__ stats,
+                                                               const float* __restrict__ w, const float* __restrict__ b, float eps,
+                                                               int act) {
+    constexpr int VEC = kVec<TI>;
+    __shared__ Moments shared[kGroupNormInline];
+    __shared__ double lds[256][2];
+    const int tid = threadIdx.x, cols = (s.channels + VEC - 1) / VEC, size = s.channels / s.groups;
+    const int width = min(cols, 256), rows = 256 / width, row = tid / width, col0 = tid - row * width;
+    const int at = gridDim.x - 1 - blockIdx.x;
+    const int p0 = at * chunk + row, p1 = min((at + 1) * chunk, s.pixels);
+    const bool some = row < rows && p0 < p1;
     const TI* xi = x + blockIdx.y * s.x_image;
     TO* yi = y + blockIdx.y * s.y_image;
+    constexpr int U = FLIGHT / 2;   // a batch is under way while the one before it is computed
+    Vector<TI> v[U], next[U];
+    auto fetch = [&](int col, int p, Vector<TI>(&v)[U]) {
+        const int n = min(s.channels - col * VEC, VEC);
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = load<TI>(xi + col * VEC + min(p + u * rows, p1 - 1) * s.x_pixel, n);
+    };
+    if (some) fetch(col0, p0, v);   // under way while the sums are finished
+    const Moments* moments_of = stats + int64_t(blockIdx.y) * s.groups;
+    if (!stats) {
+        finish(partial + int64_t(blockIdx.y) * gridDim.x * s.groups * 2, gridDim.x, s.groups, double(s.pixels) * size, eps, lds, shared);
+        moments_of = shared;
+    }
+    if (!some) return;
     for (int col = col0; col < cols; col += width) {
-        Moments m[VEC];
-        float ww[VEC], bb[VEC];
+        float hi[SAME ? 1 : VEC], ww[VEC], bb[VEC];
+        const int n = min(s.channels - col * VEC, VEC);
+        Moments m;
+        if (SAME) {
+            m = moments_of[col * VEC / size];
+            hi[0] = m.hi;
+        }
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            const int c = col * VEC + e;
-            m[e] = stats[blockIdx.y * s.groups + c / size];
-            ww[e] = w ? w[c] : 1.f;
-            bb[e] = b ? b[c] : 0.f;
+            const int c = min(col * VEC + e, s.channels - 1);
+            if (!SAME) {
+                m = moments_of[c / size];
+                hi[e] = m.hi;
+            }
+            ww[e] = w ? w[c] * m.rstd : m.rstd;
+            bb[e] = (b ? b[c] : 0.f) - m.lo * ww[e];
         }
-        const TI* xc = xi + col * VEC;
-        TO* yc = yi + col * VEC;
-#pragma unroll 4
-        for (int p = p0 + row; p < p1; p += rows) {
-            float v[VEC];
-            load<TI, VEC>(xc + p * s.x_pixel, v);
+        if (col != col0) fetch(col, p0, v);
+        for (int p = p0; p < p1; p += U * rows) {
+            const bool more = p + U * rows < p1;
+            if (more) fetch(col, p + U * rows, next);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] = activate(act, normalize(v[e], m[e]) * ww[e] + bb[e]);
-            store<TO, VEC>(yc + p * s.y_pixel, v);
+            for (int u = 0; u < U; ++u) {
+                const int q = p + u * rows;
+                if (q < p1) {
+                    float o[VEC];
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        o[e] = activate(act, __builtin_fmaf((float)v[u][e] - hi[SAME ? 0 : e], ww[e], bb[e]));
+                    store<TO, VEC>(yi + col * VEC + q * s.y_pixel, n, o);
+                }
+            }
+            if (more)
+#pragma unroll
+                for (int u = 0; u < U; ++u) v[u] = next[u];
         }
     }
 }
 
-struct Launch {
-    const GroupNormShape& s;
-    const float *w, *b;
-    float eps;
-    int act;
-    void* scratch;
-    hipStream_t stream;
-};
-
-template <class TI, class TO, int VEC>
-void launch_typed(const TI* x, TO* y, const Launch& l) {
-    const GroupNormShape& s = l.s;
-    const int64_t vectors = int64_t(s.pixels) * (s.channels / s.groups) / VEC;
+template <class TI, class TO>
+void launch_typed(const TI* x, TO* y, const GroupNormShape& s, const float* w, const float* b, float eps, int act, void* scratch,
+                  hipStream_t stream) {
+    constexpr int VEC = kVec<TI>;
+    const int size = s.channels / s.groups;
     if (group_norm_one_launch(s, VEC)) {
+        const int cols = (size + VEC - 1) / VEC;
         const dim3 grid(s.groups, s.images);
-#define SAMHIP_GN_BLOCK(NV) \
-    group_norm_block_kernel<TI, TO, VEC, NV><<<grid, 1024, 0, l.stream>>>(x, y, s, l.w, l.b, l.eps, l.act)
-        if (vectors <= 1024) SAMHIP_GN_BLOCK(1);
-        else if (vectors <= 4096) SAMHIP_GN_BLOCK(4);
-        else SAMHIP_GN_BLOCK(16);
+        const unsigned threads = unsigned(std::min<int64_t>((int64_t(s.pixels) * cols + 63) / 64 * 64, 1024));
+        const int rows = int(threads) / cols, most = (s.pixels + rows - 1) / rows;   // vectors of a thread
+#define SAMHIP_GN_BLOCK(NV) group_norm_block_kernel<TI, TO, NV><<<grid, threads, 0, stream>>>(x, y, s, w, b, eps, act)
+        if (most <= 1) SAMHIP_GN_BLOCK(1);
+        else if (most <= 4) SAMHIP_GN_BLOCK(4);
+        else SAMHIP_GN_BLOCK(8);
 #undef SAMHIP_GN_BLOCK
         return;
     }
     const int chunk = group_norm_chunk(s, VEC), chunks = (s.pixels + chunk - 1) / chunk;
     const dim3 grid(chunks, s.images);
-    double* partial = static_cast<double*>(l.scratch);
-    Moments* stats = reinterpret_cast<Moments*>(partial + int64_t(s.images) * chunks * s.groups * 2);
-    const int cols = s.channels / VEC, rows = 256 / std::min(cols, 256);
-    group_norm_stats_kernel<TI, VEC><<<grid, 256, size_t(rows) * s.channels * 16, l.stream>>>(x, s, chunk, partial);
-    group_norm_finish_kernel<<<dim3(s.groups, s.images), 64, 0, l.stream>>>(
-        partial, chunks, s.groups, double(s.pixels) * (s.channels / s.groups), l.eps, stats);
-    group_norm_apply_kernel<TI, TO, VEC><<<grid, 256, 0, l.stream>>>(x, y, s, chunk, stats, l.w, l.b, l.act);
-}
-
-template <class TI, class TO>
-void launch_vec(const void* x, void* y, int vec, const Launch& l) {
-    if (vec == 4) launch_typed<TI, TO, 4>(static_cast<const TI*>(x), static_cast<TO*>(y), l);
-    else launch_typed<TI, TO, 1>(static_cast<const TI*>(x), static_cast<TO*>(y), l);
+    double* partial = static_cast<double*>(scratch);
+    const int cols = (s.channels + VEC - 1) / VEC, rows = 256 / std::min(cols, 256);
+    const bool same = size % VEC == 0;
+    const size_t lds = size_t(rows) * cols * 16;
+    if (same) group_norm_stats_kernel<TI, true><<<grid, 256, lds, stream>>>(x, s, chunk, partial);
+    else group_norm_stats_kernel<TI, false><<<grid, 256, lds * VEC, stream>>>(x, s, chunk, partial);
+    Moments* stats = nullptr;
+    if (int64_t(chunks) * s.groups > kGroupNormInline) {
+        stats = reinterpret_cast<Moments*>(partial + int64_t(s.images) * chunks * s.groups * 2);
+        group_norm_finish_kernel<<<s.images, 256, 0, stream>>>(partial, chunks, s.groups, double(s.pixels) * size, eps, stats);
+    }
+    if (same) group_norm_apply_kernel<TI, TO, true><<<grid, 256, 0, stream>>>(x, y, s, chunk, partial, stats, w, b, eps, act);
+    else group_norm_apply_kernel<TI, TO, false><<<grid, 256, 0, stream>>>(x, y, s, chunk, partial, stats, w, b, eps, act);
 }
 
 }  // namespace
 
-int group_norm_vec(const GroupNormShape& s, const void* x, int x_bytes, const void* y, int y_bytes) {
-    const auto aligned = [](const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (4 * size_t(bytes)) == 0; };
-    const bool four = (s.channels / s.groups) % 4 == 0 && s.x_pixel % 4 == 0 && s.x_image % 4 == 0 && s.y_pixel % 4 == 0 &&
-                      s.y_image % 4 == 0 && aligned(x, x_bytes) && aligned(y, y_bytes);
-    return four ? 4 : 1;
-}
+int group_norm_vec(int x_type) { return x_type == T_F16 ? kVec<_Float16> : kVec<float>; }
 
+// Eight vectors of each of 1024 threads are what a workgroup holds; past 8192
+// channels of pixels a CU's arithmetic takes longer than another launch,
+// unless there are groups for most CUs.
 bool group_norm_one_launch(const GroupNormShape& s, int vec) {
-    return int64_t(s.pixels) * (s.channels / s.groups) / vec <= 16 * 1024;
+    const int size = s.channels / s.groups, cols = (size + vec - 1) / vec, rows = 1024 / cols;
+    return (s.pixels + rows - 1) / rows <= 8 && (int64_t(s.pixels) * size <= 8192 || int64_t(s.groups) * s.images >= 192);
 }
 
 int group_norm_chunk(const GroupNormShape& s, int vec) {
-    const int cols = s.channels / vec, rows = 256 / std::min(cols, 256);
-    const int most = std::max(1, 2048 / s.images);
-    const int least = 8 * rows;
-    return std::max(least, (s.pixels + most - 1) / most);
+    const int rows = 256 / std::min((s.channels + vec - 1) / vec, 256);
+    const int most = std::max(1, 1024 / s.images);
+    return std::max(4 * rows, (s.pixels + most - 1) / most);
 }
 
 size_t group_norm_scratch_bytes(const GroupNormShape& s, int vec) {
@@ -324,13 +424,17 @@ size_t group_norm_scratch_bytes(const GroupNormShape& s, int vec) {
     return (size_t(chunks) * 16 + sizeof(Moments)) * s.images * s.groups;
 }
 
-void launch_group_norm(const void* x, int x_type, void* y, int y_type, const GroupNormShape& s, int vec, const float* w,
-                       const float* b, float eps, int act, void* scratch, hipStream_t stream) {
-    const Launch l{s, w, b, eps, act, scratch, stream};
-    if (x_type == T_F32 && y_type == T_F32) launch_vec<float, float>(x, y, vec, l);
-    else if (x_type == T_F32) launch_vec<float, _Float16>(x, y, vec, l);
-    else if (y_type == T_F32) launch_vec<_Float16, float>(x, y, vec, l);
-    else launch_vec<_Float16, _Float16>(x, y, vec, l);
+void launch_group_norm(const void* x, int x_type, void* y, int y_type, const GroupNormShape& s, const float* w, const float* b,
+                       float eps, int act, void* scratch, hipStream_t stream) {
+    const auto run = [&](auto* xp, auto* yp) { launch_typed(xp, yp, s, w, b, eps, act, scratch, stream); };
+    const float* xf = static_cast<const float*>(x);
+    const _Float16* xh = static_cast<const _Float16*>(x);
+    float* yf = static_cast<float*>(y);
+    _Float16* yh = static_cast<_Float16*>(y);
+    if (x_type == T_F32 && y_type == T_F32) run(xf, yf);
+    else if (x_type == T_F32) run(xf, yh);
+    else if (y_type == T_F32) run(xh, yf);
+    else run(xh, yh);
 }
 
 }  // namespace samhip

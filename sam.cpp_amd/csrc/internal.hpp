@@ -418,21 +418,21 @@ const char* launch_strip_skinny(int wtype, bool f16, const float* x, int64_t ldx
                                 float* y, int64_t ldy, float* part, int M, int N, int K, int x86, hipStream_t stream);
 
 // Group norm with an activation on channels-last maps (group_norm.hip).
-// Strides in elements; the launch takes `vec` (group_norm_vec: channels per
-// load) and group_norm_scratch_bytes of scratch, 16-byte aligned.
+// Strides in elements; `vec` is group_norm_vec (channels per load), `scratch`
+// holds group_norm_scratch_bytes.
 constexpr int ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU_ERF = 3;
 constexpr int kGroupNormMaxChannels = 4096;
 struct GroupNormShape {
     int images, pixels, channels, groups;
     int64_t x_pixel, x_image, y_pixel, y_image;
 };
-int group_norm_vec(const GroupNormShape& s, const void* x, int x_bytes, const void* y, int y_bytes);
+int group_norm_vec(int x_type);
 // one workgroup per (image, group), its values in registers
 bool group_norm_one_launch(const GroupNormShape& s, int vec);
 int group_norm_chunk(const GroupNormShape& s, int vec);   // pixels per workgroup otherwise
 size_t group_norm_scratch_bytes(const GroupNormShape& s, int vec);
-void launch_group_norm(const void* x, int x_type, void* y, int y_type, const GroupNormShape& s, int vec, const float* w,
-                       const float* b, float eps, int act, void* scratch, hipStream_t stream);
+void launch_group_norm(const void* x, int x_type, void* y, int y_type, const GroupNormShape& s, const float* w, const float* b,
+                       float eps, int act, void* scratch, hipStream_t stream);
 
 // Low-rank adapters beside a shared projection (lora.hip): strides in
 // elements; `part` holds lora_part_bytes, `splits` is lora_splits'.
