@@ -32,10 +32,11 @@ struct __attribute__((packed, aligned(sizeof(T)))) Packed {
 template <class T>
 using Vector = typename Packed<T, kVec<T>>::type;
 
-// n channels at p
+// n channels at p.  `whole`: the memory behind them is the tensor's too (its
+// next pixel), so the whole vector may be read.
 template <class T>
-__device__ __forceinline__ Vector<T> load(const T* p, int n) {
-    if (n == kVec<T>) return reinterpret_cast<const Packed<T, kVec<T>>*>(p)->v;
+__device__ __forceinline__ Vector<T> load(const T* p, int n, bool whole) {
+    if (n == kVec<T> || whole) return reinterpret_cast<const Packed<T, kVec<T>>*>(p)->v;
     Vector<T> v;
 #pragma unroll
     for (int e = 0; e < kVec<T>; ++e) v[e] = p[min(e, n - 1)];
@@ -48,11 +49,28 @@ __device__ __forceinline__ void store(T* p, int n, const float (&v)[VEC]) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) r.v[e] = (T)v[e];   // F16: round to nearest even
         *reinterpret_cast<Packed<T, VEC>*>(p) = r;
-    } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-            if (e < n) p[e] = (T)v[e];
+        return;
     }
+    // in pieces of 4, 2 and 1
+    int at = 0;
+    float a = v[0], b = v[1], c = v[2];
+    if constexpr (VEC == 8) {
+        if (n & 4) {
+            Packed<T, 4> r;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.v[e] = (T)v[e];
+            *reinterpret_cast<Packed<T, 4>*>(p) = r;
+            at = 4, a = v[4], b = v[5], c = v[6];
+        }
+    }
+    if (n & 2) {
+        Packed<T, 2> r;
+        r.v[0] = (T)a;
+        r.v[1] = (T)b;
+        *reinterpret_cast<Packed<T, 2>*>(p + at) = r;
+        at += 2, a = c;
+    }
+    if (n & 1) p[at] = (T)a;
 }
 
 // Sums of x and x^2: F32 runs of x - shift, with a value of the run itself as
@@ -136,9 +154,10 @@ __global__ __launch_bounds__(1024) void group_norm_block_kernel(const TI* x, TO*
     const int64_t first = min(row, s.pixels - 1), x_step = rows * s.x_pixel, y_step = rows * s.y_pixel;
     const TI* xg = x + image * s.x_image + g * size + c + first * s.x_pixel;
     TO* yg = y + image * s.y_image + g * size + c + first * s.y_pixel;
+    const bool whole = s.x_pixel >= VEC && row + (count - 1) * rows < s.pixels - 1 && count;
     Vector<TI> v[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = load<TI>(xg + max(min(i, count - 1), 0) * x_step, n);
+    for (int i = 0; i < NV; ++i) v[i] = load<TI>(xg + max(min(i, count - 1), 0) * x_step, n, whole);
     float ww[VEC], bb[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
@@ -198,20 +217,21 @@ __global__ __launch_bounds__(256) void group_norm_stats_kernel(const TI* __restr
     const int width = min(cols, 256), rows = 256 / width, row = tid / width, col0 = tid - row * width;
     const int p0 = blockIdx.x * chunk + row, p1 = min((blockIdx.x + 1) * chunk, s.pixels);
     const int plane = rows * RUNS * cols;
+    const bool whole = s.x_pixel >= VEC && p1 < s.pixels;
     if (row < rows) {
         for (int col = col0; col < cols; col += width) {
             double sum[RUNS], sq[RUNS];
 #pragma unroll
             for (int e = 0; e < RUNS; ++e) sum[e] = sq[e] = 0.0;
             const TI* xc = x + blockIdx.y * s.x_image + col * VEC;
-            const int n = min(s.channels - col * VEC, VEC);
+            const int n = SAME ? VEC : min(s.channels - col * VEC, VEC);
             for (int p = p0; p < p1;) {
                 const int q = p;
                 Run run[RUNS];
                 for (int k = 0; k < RUN && p < p1; ++k, p += FLIGHT * rows) {
                     Vector<TI> v[FLIGHT];   // the last pixel again where there are no more
 #pragma unroll
-                    for (int u = 0; u < FLIGHT; ++u) v[u] = load<TI>(xc + min(p + u * rows, p1 - 1) * s.x_pixel, n);
+                    for (int u = 0; u < FLIGHT; ++u) v[u] = load<TI>(xc + min(p + u * rows, p1 - 1) * s.x_pixel, n, whole);
                     if (k == 0)
 #pragma unroll
                         for (int e = 0; e < RUNS; ++e) run[e].shift = (float)v[0][e];
@@ -309,15 +329,15 @@ __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* 
     const int width = min(cols, 256), rows = 256 / width, row = tid / width, col0 = tid - row * width;
     const int at = gridDim.x - 1 - blockIdx.x;
     const int p0 = at * chunk + row, p1 = min((at + 1) * chunk, s.pixels);
-    const bool some = row < rows && p0 < p1;
+    const bool some = row < rows && p0 < p1, whole = s.x_pixel >= VEC && p1 < s.pixels;
     const TI* xi = x + blockIdx.y * s.x_image;
     TO* yi = y + blockIdx.y * s.y_image;
     constexpr int U = FLIGHT / 2;   // a batch is under way while the one before it is computed
     Vector<TI> v[U], next[U];
     auto fetch = [&](int col, int p, Vector<TI>(&v)[U]) {
-        const int n = min(s.channels - col * VEC, VEC);
+        const int n = SAME ? VEC : min(s.channels - col * VEC, VEC);
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = load<TI>(xi + col * VEC + min(p + u * rows, p1 - 1) * s.x_pixel, n);
+        for (int u = 0; u < U; ++u) v[u] = load<TI>(xi + col * VEC + min(p + u * rows, p1 - 1) * s.x_pixel, n, whole);
     };
     if (some) fetch(col0, p0, v);   // under way while the sums are finished
     const Moments* moments_of = stats + int64_t(blockIdx.y) * s.groups;
@@ -328,7 +348,7 @@ __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* 
     if (!some) return;
     for (int col = col0; col < cols; col += width) {
         float hi[SAME ? 1 : VEC], ww[VEC], bb[VEC];
-        const int n = min(s.channels - col * VEC, VEC);
+        const int n = SAME ? VEC : min(s.channels - col * VEC, VEC);
         Moments m;
         if (SAME) {
             m = moments_of[col * VEC / size];
