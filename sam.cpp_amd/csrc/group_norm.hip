@@ -319,7 +319,7 @@ __global__ __launch_bounds__(256) void group_norm_finish_kernel(const double* __
 // The chunks in the other order: the last ones read are still in L2.
 template <class TI, class TO, bool SAME>
 __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* y, GroupNormShape s, int chunk,
-                                                               const double* __restrict__ partial, const Moments* __restrict__ stats,
+                                                               const double* __restrict__ partial, int chunks, const Moments* __restrict__ stats,
                                                                const float* __restrict__ w, const float* __restrict__ b, float eps,
                                                                int act) {
     constexpr int VEC = kVec<TI>;
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* 
     if (some) fetch(col0, p0, v);   // under way while the sums are finished
     const Moments* moments_of = stats + int64_t(blockIdx.y) * s.groups;
     if (!stats) {
-        finish(partial + int64_t(blockIdx.y) * gridDim.x * s.groups * 2, gridDim.x, s.groups, double(s.pixels) * size, eps, lds, shared);
+        finish(partial + int64_t(blockIdx.y) * chunks * s.groups * 2, chunks, s.groups, double(s.pixels) * size, eps, lds, shared);
         moments_of = shared;
     }
     if (!some) return;
@@ -386,6 +386,8 @@ __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* 
     }
 }
 
+int chunk_of(const GroupNormShape& s, int vec, int most);
+
 template <class TI, class TO>
 void launch_typed(const TI* x, TO* y, const GroupNormShape& s, const float* w, const float* b, float eps, int act, void* scratch,
                   hipStream_t stream) {
@@ -403,8 +405,10 @@ void launch_typed(const TI* x, TO* y, const GroupNormShape& s, const float* w, c
 #undef SAMHIP_GN_BLOCK
         return;
     }
-    const int chunk = group_norm_chunk(s, VEC), chunks = (s.pixels + chunk - 1) / chunk;
+    const int chunk = group_norm_stats_chunk(s, VEC), chunks = (s.pixels + chunk - 1) / chunk;
     const dim3 grid(chunks, s.images);
+    const int apply_chunk = chunk_of(s, VEC, 1024 / s.images);
+    const dim3 apply_grid((s.pixels + apply_chunk - 1) / apply_chunk, s.images);
     double* partial = static_cast<double*>(scratch);
     const int cols = (s.channels + VEC - 1) / VEC, rows = 256 / std::min(cols, 256);
     const bool same = size % VEC == 0;
@@ -416,8 +420,8 @@ void launch_typed(const TI* x, TO* y, const GroupNormShape& s, const float* w, c
         stats = reinterpret_cast<Moments*>(partial + int64_t(s.images) * chunks * s.groups * 2);
         group_norm_finish_kernel<<<s.images, 256, 0, stream>>>(partial, chunks, s.groups, double(s.pixels) * size, eps, stats);
     }
-    if (same) group_norm_apply_kernel<TI, TO, true><<<grid, 256, 0, stream>>>(x, y, s, chunk, partial, stats, w, b, eps, act);
-    else group_norm_apply_kernel<TI, TO, false><<<grid, 256, 0, stream>>>(x, y, s, chunk, partial, stats, w, b, eps, act);
+    if (same) group_norm_apply_kernel<TI, TO, true><<<apply_grid, 256, 0, stream>>>(x, y, s, apply_chunk, partial, chunks, stats, w, b, eps, act);
+    else group_norm_apply_kernel<TI, TO, false><<<apply_grid, 256, 0, stream>>>(x, y, s, apply_chunk, partial, chunks, stats, w, b, eps, act);
 }
 
 }  // namespace
@@ -432,15 +436,23 @@ bool group_norm_one_launch(const GroupNormShape& s, int vec) {
     return (s.pixels + rows - 1) / rows <= 8 && (int64_t(s.pixels) * size <= 8192 || int64_t(s.groups) * s.images >= 192);
 }
 
-int group_norm_chunk(const GroupNormShape& s, int vec) {
+namespace {
+// Pixels of a workgroup's chunk for at most `most` chunks an image.
+int chunk_of(const GroupNormShape& s, int vec, int most) {
     const int rows = 256 / std::min((s.channels + vec - 1) / vec, 256);
-    const int most = std::max(1, 1024 / s.images);
-    return std::max(4 * rows, (s.pixels + most - 1) / most);
+    return std::max(4 * rows, (s.pixels + std::max(most, 1) - 1) / std::max(most, 1));
+}
+}  // namespace
+
+// 1024 workgroups in all, or fewer where their partial sums then are so few
+// that the last launch adds them up, but a workgroup for every CU.
+int group_norm_stats_chunk(const GroupNormShape& s, int vec) {
+    return chunk_of(s, vec, std::min(1024 / s.images, std::max(kGroupNormInline / s.groups, 256 / s.images)));
 }
 
 size_t group_norm_scratch_bytes(const GroupNormShape& s, int vec) {
     if (group_norm_one_launch(s, vec)) return 0;
-    const int chunk = group_norm_chunk(s, vec), chunks = (s.pixels + chunk - 1) / chunk;
+    const int chunk = group_norm_stats_chunk(s, vec), chunks = (s.pixels + chunk - 1) / chunk;
     return (size_t(chunks) * 16 + sizeof(Moments)) * s.images * s.groups;
 }
 

@@ -429,7 +429,7 @@ struct GroupNormShape {
 int group_norm_vec(int x_type);
 // one workgroup per (image, group), its values in registers
 bool group_norm_one_launch(const GroupNormShape& s, int vec);
-int group_norm_chunk(const GroupNormShape& s, int vec);   // pixels per workgroup otherwise
+int group_norm_stats_chunk(const GroupNormShape& s, int vec);   // pixels per partial sum otherwise
 size_t group_norm_scratch_bytes(const GroupNormShape& s, int vec);
 void launch_group_norm(const void* x, int x_type, void* y, int y_type, const GroupNormShape& s, const float* w, const float* b,
                        float eps, int act, void* scratch, hipStream_t stream);
