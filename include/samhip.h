@@ -183,7 +183,8 @@ int samhip_mul_mat_noalloc(samhip_context* ctx, const samhip_tensor* w, const sa
  *   y[m] = base[m] + scale[s] * B[s] (A[s] x[m]),  s = ids[m]
  * with base the shared product, e.g. of samhip_mul_mat.  The adapters stand
  * in banks of equal slots, a (F32 or F16, ne = {K, R, slots, 1}) and b (the
- * same type, ne = {R, N, slots, 1}), with any row and slot strides. */
+ * same type, ne = {R, N, slots, 1}), with any row and slot strides; at most
+ * 4096 slots. */
 typedef struct samhip_lora_bank {
     int32_t version;        /* SAMHIP_ABI_VERSION */
     samhip_tensor a, b;     /* R at most 256 */

@@ -357,8 +357,8 @@ const char* lora_problem(const samhip_lora_bank* bank, const samhip_tensor* x, c
         !ids->data || reinterpret_cast<uintptr_t>(ids->data) % 4)
         return "ids must be M contiguous I32";
     if (R > kLoraMaxRank) return "rank too large";
-    if (K > (int64_t(1) << 24) || N > (int64_t(1) << 23) || M > (int64_t(1) << 27) || slots > (int64_t(1) << 20))
-        return "dimension too large";
+    if (slots > kLoraMaxSlots) return "too many slots";
+    if (K > (int64_t(1) << 24) || N > (int64_t(1) << 23) || M > (int64_t(1) << 23)) return "dimension too large";
     if (reinterpret_cast<uintptr_t>(bank->ranks) % 4 || reinterpret_cast<uintptr_t>(bank->scales) % 4)
         return "ranks and scales must be 4-byte aligned";
     return nullptr;
@@ -949,11 +949,10 @@ int samhip_lora_add(samhip_context* ctx, const samhip_lora_bank* bank, const sam
     a.rank = int(bank->a.ne[1]);
     a.slots = int(bank->a.ne[2]);
     if (int rc = set_device(ctx)) return rc;
-    a.splits = lora_splits(a.m, a.k, ctx->cus);
-    if (int rc = ensure_staging(ctx, lora_part_bytes(a.m, a.rank, a.splits))) return rc;
-    a.part = static_cast<float*>(ctx->staging);
+    lora_plan(a, ctx->cus);
+    if (int rc = ensure_staging(ctx, lora_scratch_bytes(a))) return rc;
     return traced(ctx, "lora_add", bank->a.type, a.m, a.n, a.k, [&]() -> int {
-        launch_lora(a, bank->a.type, ctx->cus, ctx->stream);
+        launch_lora(a, bank->a.type, ctx->staging, ctx->stream);
         HIP_TRY(hipGetLastError(), "lora_add launch");
         return SAMHIP_OK;
     });

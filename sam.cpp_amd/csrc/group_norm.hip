@@ -43,12 +43,14 @@ __device__ __forceinline__ Vector<T> load(const T* p, int n, bool whole) {
     return v;
 }
 template <class T, int VEC>
-__device__ __forceinline__ void store(T* p, int n, const float (&v)[VEC]) {
+__device__ __forceinline__ void store(T* p, int n, const float (&v)[VEC], bool past_cache = false) {
     if (n == VEC) {
         Packed<T, VEC> r;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) r.v[e] = (T)v[e];   // F16: round to nearest even
-        *reinterpret_cast<Packed<T, VEC>*>(p) = r;
+        typedef T raw __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
+        if (past_cache) __builtin_nontemporal_store(r.v, reinterpret_cast<raw*>(p));
+        else *reinterpret_cast<raw*>(p) = r.v;
         return;
     }
     // in pieces of 4, 2 and 1
@@ -321,7 +323,7 @@ template <class TI, class TO, bool SAME>
 __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* y, GroupNormShape s, int chunk,
                                                                const double* __restrict__ partial, int chunks, const Moments* __restrict__ stats,
                                                                const float* __restrict__ w, const float* __restrict__ b, float eps,
-                                                               int act) {
+                                                               int act, bool past_cache) {
     constexpr int VEC = kVec<TI>;
     __shared__ Moments shared[kGroupNormInline];
     __shared__ double lds[256][2];
@@ -376,7 +378,7 @@ __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* 
 #pragma unroll
                     for (int e = 0; e < VEC; ++e)
                         o[e] = activate(act, __builtin_fmaf((float)v[u][e] - hi[SAME ? 0 : e], ww[e], bb[e]));
-                    store<TO, VEC>(yi + col * VEC + q * s.y_pixel, n, o);
+                    store<TO, VEC>(yi + col * VEC + q * s.y_pixel, n, o, past_cache);
                 }
             }
             if (more)
@@ -407,6 +409,9 @@ void launch_typed(const TI* x, TO* y, const GroupNormShape& s, const float* w, c
     }
     const int chunk = group_norm_stats_chunk(s, VEC), chunks = (s.pixels + chunk - 1) / chunk;
     const dim3 grid(chunks, s.images);
+    // A map that no L2 would hold is written past the caches: 288 x 288 x 256
+    // F32 57.2 -> 45.3 us (no write-back of the L2s at the launch's end)
+    const bool past_cache = int64_t(s.images) * s.pixels * s.channels * int64_t(sizeof(TO)) > (int64_t(32) << 20);
     const int apply_chunk = chunk_of(s, VEC, 1024 / s.images);
     const dim3 apply_grid((s.pixels + apply_chunk - 1) / apply_chunk, s.images);
     double* partial = static_cast<double*>(scratch);
@@ -420,8 +425,8 @@ void launch_typed(const TI* x, TO* y, const GroupNormShape& s, const float* w, c
         stats = reinterpret_cast<Moments*>(partial + int64_t(s.images) * chunks * s.groups * 2);
         group_norm_finish_kernel<<<s.images, 256, 0, stream>>>(partial, chunks, s.groups, double(s.pixels) * size, eps, stats);
     }
-    if (same) group_norm_apply_kernel<TI, TO, true><<<apply_grid, 256, 0, stream>>>(x, y, s, apply_chunk, partial, chunks, stats, w, b, eps, act);
-    else group_norm_apply_kernel<TI, TO, false><<<apply_grid, 256, 0, stream>>>(x, y, s, apply_chunk, partial, chunks, stats, w, b, eps, act);
+    if (same) group_norm_apply_kernel<TI, TO, true><<<apply_grid, 256, 0, stream>>>(x, y, s, apply_chunk, partial, chunks, stats, w, b, eps, act, past_cache);
+    else group_norm_apply_kernel<TI, TO, false><<<apply_grid, 256, 0, stream>>>(x, y, s, apply_chunk, partial, chunks, stats, w, b, eps, act, past_cache);
 }
 
 }  // namespace

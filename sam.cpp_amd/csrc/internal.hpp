@@ -435,8 +435,9 @@ void launch_group_norm(const void* x, int x_type, void* y, int y_type, const Gro
                        float eps, int act, void* scratch, hipStream_t stream);
 
 // Low-rank adapters beside a shared projection (lora.hip): strides in
-// elements; `part` holds lora_part_bytes, `splits` is lora_splits'.
-constexpr int kLoraMaxRank = 256;
+// elements.  lora_plan sets the fields behind `slots` but the two scratch
+// pointers, which launch_lora sets.
+constexpr int kLoraMaxRank = 256, kLoraMaxSlots = 4096, kLoraBlockRows = 4096;
 struct LoraArgs {
     const float* x;
     int64_t ldx;
@@ -451,13 +452,15 @@ struct LoraArgs {
     const float* scales;    // nullable
     int64_t m;
     int k, n, rank, slots;
-    int splits;
+    bool copy_bare, past_cache, fused;
+    int tile_rows, block_rows, block_tiles, tile_count;   // tiles of one slot's rows within a block of rows
+    int splits, k_len, n_len, part_ld;
     float* part;
-    int k_len, part_ld;   // set by launch_lora
+    int* tiles;
 };
-int lora_splits(int64_t m, int k, int cus);
-size_t lora_part_bytes(int64_t m, int rank, int splits);
-void launch_lora(LoraArgs a, int type, int cus, hipStream_t stream);
+void lora_plan(LoraArgs& a, int cus);
+size_t lora_scratch_bytes(const LoraArgs& a);
+void launch_lora(LoraArgs a, int type, void* scratch, hipStream_t stream);
 
 // Attention of requests that share a prefix (prefix_attn.hip); strides in
 // elements.  prefix_attn_plan sets the fields behind `causal` but the two

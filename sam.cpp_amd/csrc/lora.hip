@@ -1,12 +1,17 @@
 // Low-rank adapters of many requests beside a shared projection:
 //   y[m] = base[m] + scale[s] * B[s] (A[s] x[m]),  s = ids[m]
 // A and B of all adapters stand in banks of equal slots; a row whose id is
-// no slot gets base alone.  Rows come in any order: a workgroup takes 16
-// neighbouring rows and goes through the distinct slots among them (one for
-// a request's run of tokens), each product on all 16 rows with the other
-// slots' rows left out, so there is no sorting and no host copy of the ids.
-//   lora_down_kernel : t = A x, the K range split over workgroups
-//   lora_up_kernel   : y = base + scale * B t
+// no slot gets base alone.  Rows come in any order and the ids stay on the
+// device: a workgroup counts the ids of its block of rows per slot, which
+// numbers the block's tiles of 16 or 64 rows of one slot, and picks its own
+// tile's rows in row order, so that scattered rows cost no more products
+// than sorted ones (777 rows of 24 slots in no order, K = 1001, N = 1359,
+// ranks to 40: 54 us with tiles of neighbouring rows that went through
+// their slots one by one).  Rows without a slot form tiles of their own
+// that only copy base.
+//   lora_fused_kernel : few tiles; t = A x and its share of B t in one launch
+//   lora_down_kernel  : t = A x, the K range split over workgroups
+//   lora_up_kernel    : y = base + scale * B t
 // Products on the F32 matrix instruction: F32 products and sums throughout.
 #include <algorithm>
 
@@ -18,210 +23,522 @@ namespace samhip {
 
 namespace {
 
-constexpr int ROWS = 16;   // rows of a workgroup
+typedef float float4_at __attribute__((ext_vector_type(4), aligned(4)));
 
-__device__ __forceinline__ floatx4 ld4(const float* p) {   // 4-byte aligned
-    struct __attribute__((packed, aligned(4))) unaligned4 {
-        floatx4 v;
-    };
-    return reinterpret_cast<const unaligned4*>(p)->v;
-}
-__device__ __forceinline__ void st4(float* p, floatx4 v) {
-    struct __attribute__((packed, aligned(4))) unaligned4 {
-        floatx4 v;
-    };
-    reinterpret_cast<unaligned4*>(p)->v = v;
+__device__ __forceinline__ floatx4 ld4(const float* p) { return *reinterpret_cast<const float4_at*>(p); }
+__device__ __forceinline__ void st4(float* p, floatx4 v, bool past_cache) {
+    if (past_cache) __builtin_nontemporal_store(v, reinterpret_cast<float4_at*>(p));
+    else *reinterpret_cast<float4_at*>(p) = v;
 }
 
-// N values p[0 .. N) as floats, those at or behind `left` zero and not read.
-template <int N>
-__device__ __forceinline__ void take(const float* p, int64_t left, float (&v)[N]) {
-    if (left >= N) {
+// p[0 .. 4) as floats, those at or behind `left` zero and not read.
+__device__ __forceinline__ floatx4 take4(const float* p, int left) {
+    if (left >= 4) return ld4(p);
+    floatx4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < N; j += 4) {
-            const floatx4 f = ld4(p + j);
-            v[j] = f[0], v[j + 1] = f[1], v[j + 2] = f[2], v[j + 3] = f[3];
+    for (int j = 0; j < 3; ++j)
+        if (j < left) v[j] = p[j];
+    return v;
+}
+__device__ __forceinline__ floatx4 take4(const _Float16* p, int left) {
+    typedef _Float16 half4_at __attribute__((ext_vector_type(4), aligned(2)));
+    floatx4 v{0.f, 0.f, 0.f, 0.f};
+    if (left >= 4) {
+        const half4_at h = *reinterpret_cast<const half4_at*>(p);
+        return floatx4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+        if (j < left) v[j] = (float)p[j];
+    return v;
+}
+
+__device__ __forceinline__ floatx4 mfma(float a, float b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// Inclusive sums over the wave's lanes: within rows of 16 by shifts, then the
+// last lane of each row (15, 31 of the half) onto the rows behind it.
+__device__ __forceinline__ int prefix_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);    // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast:15 onto rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // row_bcast:31 onto rows 2 and 3
+    return v;
+}
+
+// The rows of one tile: offsets from the block's first row, -1 where the
+// tile has fewer.
+template <int TR>
+struct Tile {
+    int rows[TR];
+    int counts[64];   // matches per wave and pass
+};
+
+// The p-th tile of a block of `n` rows (at most 4096): its slot (a.slots: rows
+// without one), or -1 past the last tile.  hist: slots + 1 counters.
+template <int TR>
+__device__ __forceinline__ int find_tile(const LoraArgs& a, const int32_t* ids, int n, int p, int* hist, Tile<TR>& tile) {
+    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
+    const int passes = (n + threads - 1) / threads;
+    const int first_id = ids[min(tid, n - 1)];   // the only one where a pass takes all rows
+    const auto slot_of = [&](int pass, int row) {
+        const int id = pass == 0 ? first_id : ids[min(row, n - 1)];
+        return row >= n ? -1 : id >= 0 && id < a.slots ? id : a.copy_bare ? a.slots : -1;
+    };
+    for (int s = tid; s <= a.slots; s += threads) hist[s] = 0;
+    if (tid < TR) tile.rows[tid] = -1;
+    __syncthreads();
+    for (int i = 0; i < passes; ++i) {
+        const int s = slot_of(i, i * threads + tid);
+        // one request's rows in a run: one addition for the wave
+        const int s0 = __builtin_amdgcn_readfirstlane(s);
+        if (__all(s == s0)) {
+            if (s0 >= 0 && lane == 0) atomicAdd(&hist[s0], 64);
+        } else if (s >= 0) {
+            atomicAdd(&hist[s], 1);
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = j < left ? p[j] : 0.f;
     }
-}
-template <int N>
-__device__ __forceinline__ void take(const _Float16* p, int64_t left, float (&v)[N]) {
-    typedef _Float16 halves __attribute__((ext_vector_type(N)));
-    struct __attribute__((packed, aligned(2))) unaligned {
-        halves v;
-    };
-    if (left >= N) {
-        const halves h = reinterpret_cast<const unaligned*>(p)->v;
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = (float)h[j];
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = j < left ? (float)p[j] : 0.f;
+    __syncthreads();
+    int slot = -1, skip = 0, before = 0;
+    for (int s0 = 0; s0 <= a.slots && slot < 0; s0 += 64) {
+        const int tiles = s0 + lane <= a.slots ? (hist[s0 + lane] + TR - 1) / TR : 0;
+        const int sum = prefix_sum(tiles);
+        const uint64_t past = __ballot(before + sum > p);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            slot = s0 + at;
+            skip = (p - before - __builtin_amdgcn_readlane(sum - tiles, at)) * TR;
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
     }
-}
-
-// The distinct slots of a tile's rows: body(slot, mask of its rows), the
-// z-th of every Z.  Every wave sees the same ids and takes the same path.
-template <class Body>
-__device__ __forceinline__ void for_slots(const LoraArgs& a, int64_t row0, int z, int Z, Body body) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = row0 + lane;
-    const int id = lane < ROWS && row < a.m ? a.ids[row] : -1;
-    uint32_t left = uint32_t(__ballot(id >= 0 && id < a.slots));
-    for (int i = 0; left; ++i) {
-        const int slot = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
-        const uint32_t mask = uint32_t(__ballot(id == slot)) & left;
-        left &= ~mask;
-        if (i % Z == z) body(slot, mask);
+    slot = __builtin_amdgcn_readfirstlane(slot);
+    if (slot < 0) return -1;
+    for (int i = 0; i < passes; ++i) {
+        const uint64_t same = __ballot(slot_of(i, i * threads + tid) == slot);
+        if (lane == 0) tile.counts[i * waves + wave] = __builtin_popcountll(same);
     }
+    __syncthreads();
+    const int count = lane < passes * waves ? tile.counts[lane] : 0, first = prefix_sum(count) - count;
+    for (int i = 0; i < passes; ++i) {
+        const int row = i * threads + tid, at = i * waves + wave;
+        const bool here = slot_of(i, row) == slot;
+        const uint64_t same = __ballot(here);
+        const int ahead = __builtin_amdgcn_readlane(first, at) + __builtin_popcountll(same & ((uint64_t(1) << lane) - 1)) - skip;
+        if (here && ahead >= 0 && ahead < TR) tile.rows[ahead] = row;
+    }
+    __syncthreads();
+    return slot;
 }
 
 __device__ __forceinline__ int slot_rank(const LoraArgs& a, int slot) {
     return a.ranks ? min(max(a.ranks[slot], 0), a.rank) : a.rank;
 }
 
-// Grid: row tiles x K splits x slot lanes.  The 4 waves share the split's K
-// range in steps of 32 values; lane (r, g) of a step holds row r's values
-// 8g .. 8g + 7 of both operands, the K order of either being the same.
-template <class T, int RT>
-__global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
-    __shared__ floatx4 red[3][RT][64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
-    const int64_t row0 = int64_t(blockIdx.x) * ROWS;
-    const int k0 = blockIdx.y * a.k_len, k1 = min(a.k, k0 + a.k_len);
-    for_slots(a, row0, blockIdx.z, gridDim.z, [&](int slot, uint32_t mask) {
-        const int rank = slot_rank(a, slot), tiles = (rank + 15) / 16;
-        const bool mine = (mask >> r) & 1;
-        const float* x = a.x + (row0 + r) * a.ldx;
-        const T* w = static_cast<const T*>(a.a) + slot * a.a_slot;
-        floatx4 acc[RT];
+// Operands of t = A x through LDS, KC values of K at a time: lanes of the
+// matrix instruction's operands stand for rows, so reading them straight
+// from memory takes a cache line per lane; here neighbouring lanes read
+// neighbouring 16 bytes of a row, and a chunk is under way during the
+// products of the one before.
+template <class T, int THREADS, int TR, int RT, int KC>
+struct Stage {
+    static constexpr int VA = 16 / sizeof(T), XC = KC / 4, AC = KC / VA;                   // 16-byte pieces of a row
+    static constexpr int XN = (TR * XC + THREADS - 1) / THREADS, AN = (16 * RT * AC + THREADS - 1) / THREADS;   // of a thread
+    typedef T vec __attribute__((ext_vector_type(VA)));
+    typedef T vec_at __attribute__((ext_vector_type(VA), aligned(sizeof(T))));
+    struct Lds {
+        __attribute__((aligned(16))) float x[TR][KC + 4];
+        __attribute__((aligned(16))) T a[16 * RT][KC + VA];
+    };
+    floatx4 x[XN];
+    vec w[AN];
+
+    // values [k, k + KC) of the tile's rows (block0 + rows[]) and of A's first
+    // `rank` rows; zeros at or behind k1, for absent rows and behind the rank
+    __device__ __forceinline__ void load(const LoraArgs& a, int64_t block0, const int* rows, const T* A, int rank, int k, int k1) {
 #pragma unroll
-        for (int t = 0; t < RT; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-        for (int k = k0 + 32 * wave + 8 * g; k < k1 + 8 * g; k += 128) {
-            float xv[8], av[8];
-            take<8>(x + k, mine ? k1 - k : 0, xv);
+        for (int i = 0; i < XN; ++i) {
+            const int f = threadIdx.x + i * THREADS, row = f / XC < TR ? rows[f / XC] : -1, at = k + f % XC * 4;
+            x[i] = take4(a.x + (block0 + max(row, 0)) * a.ldx + at, row >= 0 ? k1 - at : 0);
+        }
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                if (t < tiles) {
-                    const int q = 16 * t + r;
-                    take<8>(w + q * a.a_row + k, q < rank ? k1 - k : 0, av);
+        for (int i = 0; i < AN; ++i) {
+            const int f = threadIdx.x + i * THREADS, q = f / AC, at = k + f % AC * VA, left = q < rank ? k1 - at : 0;
+            const T* p = A + q * a.a_row + at;
+            if (left >= VA) {
+                w[i] = *reinterpret_cast<const vec_at*>(p);
+            } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[j], xv[j], acc[t], 0, 0, 0);
-                }
+                for (int j = 0; j < VA; ++j) w[i][j] = j < left ? p[j] : (T)0;
             }
         }
-        // lane (r, g) holds row r's ranks 16t + 4g .. + 3
-        if (wave) {
+    }
+    __device__ __forceinline__ void store(Lds& l) const {
+#pragma unroll
+        for (int i = 0; i < XN; ++i) {
+            const int f = threadIdx.x + i * THREADS;
+            if (TR * XC % THREADS == 0 || f < TR * XC) *reinterpret_cast<floatx4*>(&l.x[f / XC][f % XC * 4]) = x[i];
+        }
+#pragma unroll
+        for (int i = 0; i < AN; ++i) {
+            const int f = threadIdx.x + i * THREADS;
+            if (16 * RT * AC % THREADS == 0 || f < 16 * RT * AC) *reinterpret_cast<vec*>(&l.a[f / AC][f % AC * VA]) = w[i];
+        }
+    }
+};
+
+// acc[i] += A x of subtile `sub` over the chunk's units first, first + step, ..
+// of 16 values: lane (r, g) holds values 4g .. 4g + 3 of row r of both operands
+// and ends with row r's ranks 16i + 4g .. + 3.
+template <int RT, int UNITS, class Lds>
+__device__ __forceinline__ void multiply(const Lds& l, int sub, int first, int step, int tiles, floatx4 (&acc)[RT]) {
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+#pragma unroll RT <= 4 ? UNITS : 1
+    for (int n = 0; n < UNITS; ++n) {
+        const int at = 16 * (first + n * step) + 4 * g;
+        const floatx4 x = *reinterpret_cast<const floatx4*>(&l.x[16 * sub + r][at]);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+            if (i < tiles) {
+                const auto* p = &l.a[16 * i + r][at];
+                const floatx4 w{(float)p[0], (float)p[1], (float)p[2], (float)p[3]};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i] = mfma(w[j], x[j], acc[i]);
+            }
+    }
+}
+
+// Over [k0, k1), every chunk
+template <class T, int THREADS, int TR, int RT, int KC, int UNITS>
+__device__ __forceinline__ void down(const LoraArgs& a, typename Stage<T, THREADS, TR, RT, KC>::Lds& lds, int64_t block0, const int* rows, const T* A,
+                                     int rank, int k0, int k1, int sub, int first, int step, floatx4 (&acc)[RT]) {
+    Stage<T, THREADS, TR, RT, KC> stage;
+    const int tiles = (rank + 15) / 16;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    stage.load(a, block0, rows, A, rank, k0, k1);
+    for (int k = k0; k < k1; k += KC) {
+        if (k != k0) __syncthreads();   // the last chunk is read
+        stage.store(lds);
+        __syncthreads();
+        if (k + KC < k1) stage.load(a, block0, rows, A, rank, k + KC, k1);
+        multiply<RT, UNITS>(lds, sub, first, step, tiles, acc);
+    }
+}
+
+// One tile's t for the lane's rows: zero behind the rank, times the scale.
+template <int RT>
+__device__ __forceinline__ void finish_t(const LoraArgs& a, int slot, int rank, floatx4 (&t)[RT]) {
+    const int g = (threadIdx.x & 63) >> 4;
+    const float scale = a.scales ? a.scales[slot] : 1.f;
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[i][j] = 16 * i + 4 * g + j < rank ? t[i][j] * scale : 0.f;
+}
+
+// B's rows n .. n + 15, and their products with t: lane (r, g) ends with row
+// r's columns n + 4g .. + 3.
+template <class T, int RT>
+__device__ __forceinline__ void take_b(const LoraArgs& a, const T* w, int n, int rank, floatx4 (&b)[RT]) {
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const T* row = w + min(n + r, a.n - 1) * a.b_row + 4 * g;
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+        if (16 * i < rank) b[i] = take4(row + 16 * i, rank - (16 * i + 4 * g));
+}
+template <int RT, int SUB>
+__device__ __forceinline__ void up(int rank, const floatx4 (&b)[RT], const floatx4 (&t)[SUB][RT], floatx4 (&acc)[SUB]) {
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) acc[s] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+        if (16 * i < rank)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int s = 0; s < SUB; ++s) acc[s] = mfma(b[i][j], t[s][i][j], acc[s]);
+}
+
+__device__ __forceinline__ floatx4 base4(const LoraArgs& a, int64_t row, int n) {
+    return a.base ? take4(a.base + row * a.ldbase + n, a.n - n) : floatx4{0.f, 0.f, 0.f, 0.f};
+}
+__device__ __forceinline__ void put4(const LoraArgs& a, int64_t row, int n, floatx4 v) {
+    float* y = a.y + row * a.ldy + n;
+    if (n + 4 <= a.n) {
+        st4(y, v, a.past_cache);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (n + j < a.n) y[j] = v[j];
+    }
+}
+
+// Grid: tiles x blocks of 256 columns.  The 8 waves share each chunk of K,
+// then take 32 columns each.
+template <class T, int RT>
+__global__ __launch_bounds__(512) void lora_fused_kernel(LoraArgs a) {
+    constexpr int KC = 512 / RT;
+    extern __shared__ int hist[];
+    __shared__ Tile<16> tile;
+    __shared__ typename Stage<T, 512, 16, RT, KC>::Lds lds;
+    __shared__ floatx4 red[8][RT][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
+    const int slot = find_tile<16>(a, a.ids, int(a.m), blockIdx.x, hist, tile);
+    if (slot < 0) return;
+    const int row = tile.rows[r], n0 = blockIdx.y * 256 + wave * 32;
+    const bool mine = row >= 0;
+    const int64_t at = max(row, 0);
+    floatx4 base[2];   // under way during the products
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+        if (mine) base[c] = base4(a, at, n0 + 16 * c + 4 * g);
+    if (slot < a.slots) {
+        const int rank = slot_rank(a, slot);
+        floatx4 t[1][RT], b[2][RT];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) take_b<T, RT>(a, static_cast<const T*>(a.b) + slot * a.b_slot, n0 + 16 * c, rank, b[c]);
+        down<T, 512, 16, RT, KC, KC / 128>(a, lds, 0, tile.rows, static_cast<const T*>(a.a) + slot * a.a_slot, rank, 0, a.k, 0, wave, 8, t[0]);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) red[wave][i][lane] = t[0][i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            t[0][i] = red[0][i][lane];
+#pragma unroll
+            for (int w = 1; w < 8; ++w) t[0][i] += red[w][i][lane];
+        }
+        finish_t(a, slot, rank, t[0]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            floatx4 acc[1];
+            up<RT, 1>(rank, b[c], t, acc);
+            if (mine) base[c] += acc[0];
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+        if (mine) put4(a, at, n0 + 16 * c + 4 * g, base[c]);
+}
+
+// Grid: a block's tiles x blocks of rows x K splits.  A wave takes 16 of 64
+// rows; with 16 the four waves share each chunk of K.  The first split writes
+// the tile's slot and rows down for lora_up_kernel.
+template <class T, int RT, int SUB>
+__global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
+    constexpr int TR = 16 * SUB, KC = SUB == 4 ? (RT <= 2 ? 128 : 64) : 512 / (RT < 2 ? 2 : RT), UNITS = SUB == 4 || KC < 64 ? KC / 16 : KC / 64;
+    extern __shared__ int hist[];
+    __shared__ Tile<TR> tile;
+    __shared__ typename Stage<T, 256, TR, RT, KC>::Lds lds;
+    __shared__ floatx4 red[SUB == 4 ? 1 : 3][RT][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
+    const int64_t block0 = int64_t(blockIdx.y) * a.block_rows;
+    const int slot = find_tile<TR>(a, a.ids + block0, int(min(int64_t(a.block_rows), a.m - block0)), blockIdx.x, hist, tile);
+    if (blockIdx.z == 0) {
+        int* out = a.tiles + (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * (TR + 1);
+        if (tid == 0) out[TR] = slot;
+        if (tid < TR && slot >= 0) out[tid] = tile.rows[tid];
+    }
+    if (slot < 0 || slot == a.slots) return;
+    const int rank = slot_rank(a, slot), tiles = (rank + 15) / 16;
+    const int k0 = blockIdx.z * a.k_len, k1 = min(a.k, k0 + a.k_len);
+    floatx4 acc[RT];
+    const T* A = static_cast<const T*>(a.a) + slot * a.a_slot;
+    // chunks of 32 values hold two units: the first two waves take one each
+    if constexpr (SUB == 4) down<T, 256, TR, RT, KC, UNITS>(a, lds, block0, tile.rows, A, rank, k0, k1, wave, 0, 1, acc);
+    else if constexpr (KC >= 64) down<T, 256, TR, RT, KC, UNITS>(a, lds, block0, tile.rows, A, rank, k0, k1, 0, wave, 4, acc);
+    else down<T, 256, TR, RT, KC, 1>(a, lds, block0, tile.rows, A, rank, k0, k1, 0, wave & 1, 1, acc);
+    if constexpr (SUB == 1) {
+        constexpr int SHARE = KC >= 64 ? 4 : 2;   // waves with a part of the sum
+        if (wave && wave < SHARE) {
 #pragma unroll
             for (int t = 0; t < RT; ++t)
                 if (t < tiles) red[wave - 1][t][lane] = acc[t];
         }
         __syncthreads();
-        if (wave == 0 && mine) {
-            float* out = a.part + ((blockIdx.y * a.m + row0 + r) * a.part_ld + 4 * g);
+        if (wave) return;
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
-                if (t < tiles) *reinterpret_cast<floatx4*>(out + 16 * t) = acc[t] + red[0][t][lane] + red[1][t][lane] + red[2][t][lane];
-        }
-        __syncthreads();
-    });
+        for (int t = 0; t < RT; ++t)
+            if (t < tiles)
+#pragma unroll
+                for (int w = 1; w < SHARE; ++w) acc[t] += red[w - 1][t][lane];
+    }
+    const int row = tile.rows[(SUB == 4 ? 16 * wave : 0) + r];
+    if (row < 0) return;
+    float* out = a.part + (blockIdx.z * a.m + block0 + row) * a.part_ld + 4 * g;
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+        if (t < tiles) *reinterpret_cast<floatx4*>(out + 16 * t) = acc[t];
 }
 
-// Grid: row tiles x blocks of 256 columns x slot lanes; 64 columns a wave.
-template <class T, int RT>
+// Grid: column splits x parts of a block's tiles x blocks of rows.  A workgroup goes
+// through its split in blocks of 256 columns, 64 to a wave; the sums pass
+// through LDS, so that base and y move in whole KB of a row, and the next
+// block's base is under way as soon as this one's is used.
+template <class T, int RT, int SUB, int TILE>
 __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
+    constexpr int TR = 16 * SUB, PARTS = TILE / TR, PITCH = 256 + 4, OWN = TR / 4;   // rows that a wave moves
+    __shared__ __attribute__((aligned(16))) float sums[TR][PITCH];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
-    const int64_t row0 = int64_t(blockIdx.x) * ROWS, row = row0 + r;
-    const int n0 = blockIdx.y * 256 + wave * 64;
-    // base and y of this lane's row, columns n .. n + 3
-    auto put = [&](int n, floatx4 v) {
-        if (n + 4 <= a.n) {
-            if (a.base) v += ld4(a.base + row * a.ldbase + n);
-            st4(a.y + row * a.ldy + n, v);
-        } else {
+    const int* tile = a.tiles + (int64_t(blockIdx.z) * a.block_tiles + blockIdx.y / PARTS) * (TILE + 1);
+    const int slot = tile[TILE];
+    if (slot < 0) return;
+    tile += blockIdx.y % PARTS * TR;
+    const int64_t block0 = int64_t(blockIdx.z) * a.block_rows;
+    const int n0 = blockIdx.x * a.n_len, n1 = min(a.n, n0 + a.n_len);
+    floatx4 base[OWN];
+    int row[OWN];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (n + j < a.n) a.y[row * a.ldy + n + j] = a.base ? v[j] + a.base[row * a.ldbase + n + j] : v[j];
-        }
+    for (int i = 0; i < OWN; ++i) row[i] = __builtin_amdgcn_readfirstlane(tile[OWN * wave + i]);
+    const bool whole = row[OWN - 1] >= 0;   // rows fill from the front
+    const auto fetch = [&](int i, int n) {
+        base[i] = row[i] >= 0 && n < n1 ? base4(a, block0 + row[i], n) : floatx4{0.f, 0.f, 0.f, 0.f};
     };
-    for_slots(a, row0, blockIdx.z, gridDim.z, [&](int slot, uint32_t mask) {
-        const int rank = slot_rank(a, slot), tiles = (rank + 15) / 16;
-        const float scale = a.scales ? a.scales[slot] : 1.f;
-        const bool mine = (mask >> r) & 1;
-        floatx4 t[RT];
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            t[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-            if (i < tiles && mine) {
-                for (int s = 0; s < a.splits; ++s)
-                    t[i] += *reinterpret_cast<const floatx4*>(a.part + (s * a.m + row) * a.part_ld + 16 * i + 4 * g);
+    for (int i = 0; i < OWN; ++i) fetch(i, n0 + 4 * lane);
+    const bool product = slot < a.slots;
+    const int rank = product ? slot_rank(a, slot) : 0;
+    const T* B = static_cast<const T*>(a.b) + (product ? slot : 0) * a.b_slot;
+    // B of a whole block is under way before the stores of the one before: a
+    // wait for any load is one for every store that was issued ahead of it
+    constexpr int AHEAD = RT <= 2 ? 4 : 1;
+    floatx4 t[SUB][RT], b[AHEAD][RT];
+    const auto fetch_b = [&](int nb) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) t[i][j] = 16 * i + 4 * g + j < rank ? t[i][j] * scale : 0.f;
-            }
-        }
-        const T* w = static_cast<const T*>(a.b) + slot * a.b_slot;
+        for (int c = 0; c < AHEAD; ++c) take_b<T, RT>(a, B, nb + 64 * wave + 16 * c, rank, b[c]);
+    };
+    if (product) {
+        fetch_b(n0);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const int n = n0 + 16 * c;
-            if (n >= a.n) break;
-            floatx4 acc{0.f, 0.f, 0.f, 0.f};
-            const T* wr = w + min(n + r, a.n - 1) * a.b_row + 4 * g;
+        for (int s = 0; s < SUB; ++s) {
+            const int at = tile[16 * s + r];
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
-                if (i < tiles) {
-                    float bv[4];
-                    take<4>(wr + 16 * i, rank - (16 * i + 4 * g), bv);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[j], t[i][j], acc, 0, 0, 0);
+                t[s][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+                if (16 * i < rank && at >= 0) {
+                    const float* p = a.part + (block0 + at) * a.part_ld + 16 * i + 4 * g;
+                    const int64_t step = a.m * a.part_ld;
+#pragma unroll 4
+                    for (int k = 0; k < a.splits; ++k) t[s][i] += *reinterpret_cast<const floatx4*>(p + k * step);
                 }
             }
-            if (mine) put(n + 4 * g, acc);
+            finish_t(a, slot, rank, t[s]);
         }
-    });
-    if (blockIdx.z == 0 && row < a.m && (a.base != a.y || a.ldbase != a.ldy)) {   // rows without an adapter
-        const int id = a.ids[row];
-        if (id < 0 || id >= a.slots)
+    }
+    for (int nb = n0; nb < n1; nb += 256) {
+        if (product) {
+            if (nb != n0) __syncthreads();   // the last block's sums are read
 #pragma unroll
-            for (int c = 0; c < 4; ++c) put(n0 + 16 * c + 4 * g, floatx4{0.f, 0.f, 0.f, 0.f});
+            for (int c = 0; c < 4; ++c) {
+                floatx4 acc[SUB], now[RT];
+#pragma unroll
+                for (int i = 0; i < RT; ++i) now[i] = b[c % AHEAD][i];
+                if (AHEAD == 1 && c < 3) take_b<T, RT>(a, B, nb + 64 * wave + 16 * (c + 1), rank, b[0]);
+                up<RT, SUB>(rank, now, t, acc);
+#pragma unroll
+                for (int s = 0; s < SUB; ++s) *reinterpret_cast<floatx4*>(&sums[16 * s + r][64 * wave + 16 * c + 4 * g]) = acc[s];
+            }
+            if (nb + 256 < n1) fetch_b(nb + 256);
+            __syncthreads();
+        }
+        const int n = nb + 4 * lane;
+        const auto sum_of = [&](int i) {
+            return product ? base[i] + *reinterpret_cast<const floatx4*>(&sums[OWN * wave + i][4 * lane]) : base[i];
+        };
+        if (whole && nb + 512 <= n1) {   // without a branch, behind which every wait would be for all
+#pragma unroll
+            for (int i0 = 0; i0 < OWN; i0 += 4) {
+                floatx4 v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[i] = sum_of(i0 + i);
+                    if (a.base) base[i0 + i] = ld4(a.base + (block0 + row[i0 + i]) * a.ldbase + n + 256);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) st4(a.y + (block0 + row[i0 + i]) * a.ldy + n, v[i], a.past_cache);
+            }
+        } else {
+#pragma unroll
+            for (int i0 = 0; i0 < OWN; i0 += 4) {
+                floatx4 v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[i] = sum_of(i0 + i);
+                    fetch(i0 + i, n + 256);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (row[i0 + i] >= 0 && n < n1) put4(a, block0 + row[i0 + i], n, v[i]);
+            }
+        }
     }
 }
 
 template <class T, int RT>
-void launch_ranks(const LoraArgs& a, int slot_lanes, hipStream_t stream) {
-    const unsigned tiles = unsigned((a.m + ROWS - 1) / ROWS);
-    lora_down_kernel<T, RT><<<dim3(tiles, a.splits, slot_lanes), 256, 0, stream>>>(a);
-    lora_up_kernel<T, RT><<<dim3(tiles, (a.n + 255) / 256, slot_lanes), 256, 0, stream>>>(a);
+void launch_ranks(const LoraArgs& a, hipStream_t stream) {
+    const unsigned columns = (a.n + 255) / 256;
+    const size_t lds = size_t(a.slots + 1) * 4;
+    if constexpr (RT <= 4)
+        if (a.fused) {
+            lora_fused_kernel<T, RT><<<dim3(a.block_tiles, columns), 512, lds, stream>>>(a);
+            return;
+        }
+    const unsigned blocks = a.tile_count / a.block_tiles;
+    const dim3 grid(a.block_tiles, blocks, a.splits), up_grid((a.n + a.n_len - 1) / a.n_len, a.block_tiles * (a.tile_rows == 64 ? 2 : 1), blocks);
+    if constexpr (RT <= 8)
+        if (a.tile_rows == 64) {
+            lora_down_kernel<T, RT, 4><<<grid, 256, lds, stream>>>(a);
+            lora_up_kernel<T, RT, 2, 64><<<up_grid, 256, 0, stream>>>(a);
+            return;
+        }
+    lora_down_kernel<T, RT, 1><<<grid, 256, lds, stream>>>(a);
+    lora_up_kernel<T, RT, 1, 16><<<up_grid, 256, 0, stream>>>(a);
 }
 
 template <class T>
-void launch_typed(const LoraArgs& a, int slot_lanes, hipStream_t stream) {
-    if (a.rank <= 16) launch_ranks<T, 1>(a, slot_lanes, stream);
-    else if (a.rank <= 32) launch_ranks<T, 2>(a, slot_lanes, stream);
-    else if (a.rank <= 64) launch_ranks<T, 4>(a, slot_lanes, stream);
-    else if (a.rank <= 128) launch_ranks<T, 8>(a, slot_lanes, stream);
-    else launch_ranks<T, 16>(a, slot_lanes, stream);
+void launch_typed(const LoraArgs& a, hipStream_t stream) {
+    if (a.rank <= 16) launch_ranks<T, 1>(a, stream);
+    else if (a.rank <= 32) launch_ranks<T, 2>(a, stream);
+    else if (a.rank <= 64) launch_ranks<T, 4>(a, stream);
+    else if (a.rank <= 128) launch_ranks<T, 8>(a, stream);
+    else launch_ranks<T, 16>(a, stream);
 }
 
 }  // namespace
 
-// About two workgroups per CU from splits of at least 256 values of K.
-int lora_splits(int64_t m, int k, int cus) {
-    const int64_t tiles = (m + ROWS - 1) / ROWS;
-    return int(std::max<int64_t>(1, std::min<int64_t>((2 * cus + tiles - 1) / tiles, (k + 255) / 256)));
+void lora_plan(LoraArgs& a, int cus) {
+    a.copy_bare = a.base != a.y || a.ldbase != a.ldy;
+    a.past_cache = a.m * a.n * 4 > (int64_t(32) << 20);   // an output that no L2 would hold
+    a.part_ld = (a.rank + 15) / 16 * 16;
+    const int columns = (a.n + 255) / 256;
+    // tiles of a block of `rows` rows: whole ones, and one begun per slot
+    const auto tiles_of = [&](int64_t rows, int tile) { return int(std::min<int64_t>(rows, rows / tile + a.slots + 1)); };
+    const int64_t few = std::min<int64_t>(a.m, kLoraBlockRows);
+    a.fused = a.rank <= 64 && a.m <= kLoraBlockRows && int64_t(tiles_of(few, 16)) * columns <= 2 * cus;
+    a.tile_rows = !a.fused && a.rank <= 128 && a.m >= 64 * cus / 4 ? 64 : 16;
+    a.block_rows = int(few);
+    a.block_tiles = tiles_of(few, a.tile_rows);
+    a.tile_count = int((a.m + a.block_rows - 1) / a.block_rows) * a.block_tiles;
+    // about two workgroups per CU from splits of at least 256 values of K
+    const int64_t full = (a.m + a.tile_rows - 1) / a.tile_rows;
+    a.splits = int(std::max<int64_t>(1, std::min<int64_t>((2 * cus + full - 1) / full, (a.k + 255) / 256)));
+    a.k_len = ((a.k + a.splits - 1) / a.splits + 127) / 128 * 128;
+    a.splits = (a.k + a.k_len - 1) / a.k_len;
+    const int column_splits = int(std::min<int64_t>(columns, (3 * cus + full - 1) / full));
+    a.n_len = (columns + column_splits - 1) / column_splits * 256;
 }
 
-size_t lora_part_bytes(int64_t m, int rank, int splits) { return size_t(splits) * size_t(m) * ((rank + 15) / 16 * 16) * 4; }
+static size_t part_bytes(const LoraArgs& a) { return size_t(a.splits) * a.m * a.part_ld * 4; }
 
-void launch_lora(LoraArgs a, int type, int cus, hipStream_t stream) {
-    const int64_t tiles = (a.m + ROWS - 1) / ROWS;
-    a.k_len = ((a.k + a.splits - 1) / a.splits + 127) / 128 * 128;
-    a.part_ld = (a.rank + 15) / 16 * 16;
-    const int slot_lanes = int(std::max<int64_t>(1, std::min<int64_t>({2 * cus / tiles, ROWS, a.slots})));
-    if (type == T_F16) launch_typed<_Float16>(a, slot_lanes, stream);
-    else launch_typed<float>(a, slot_lanes, stream);
+size_t lora_scratch_bytes(const LoraArgs& a) {
+    return a.fused ? 0 : part_bytes(a) + size_t(a.tile_count) * (a.tile_rows + 1) * 4;
+}
+
+void launch_lora(LoraArgs a, int type, void* scratch, hipStream_t stream) {
+    a.part = static_cast<float*>(scratch);
+    a.tiles = a.fused ? nullptr : reinterpret_cast<int*>(static_cast<char*>(scratch) + part_bytes(a));
+    if (type == T_F16) launch_typed<_Float16>(a, stream);
+    else launch_typed<float>(a, stream);
 }
 
 }  // namespace samhip
