@@ -188,7 +188,7 @@ int samhip_mul_mat_noalloc(samhip_context* ctx, const samhip_tensor* w, const sa
 typedef struct samhip_lora_bank {
     int32_t version;        /* SAMHIP_ABI_VERSION */
     samhip_tensor a, b;     /* R at most 256 */
-    const int32_t* ranks;   /* device I32 [slots]: ranks in use, the rest of a slot is not read; NULL: R */
+    const int32_t* ranks;   /* device I32 [slots]: ranks in use, whatever a slot holds behind them; NULL: R */
     const float* scales;    /* device F32 [slots]; NULL: 1 */
 } samhip_lora_bank;
 

@@ -3,7 +3,7 @@
 // A and B of all adapters stand in banks of equal slots; a row whose id is
 // no slot gets base alone.  Rows come in any order and the ids stay on the
 // device: a workgroup counts the ids of its block of rows per slot, which
-// numbers the block's tiles of 16 or 64 rows of one slot, and picks its own
+// numbers the block's tiles of 16 or 32 rows of one slot, and picks its own
 // tile's rows in row order, so that scattered rows cost no more products
 // than sorted ones (777 rows of 24 slots in no order, K = 1001, N = 1359,
 // ranks to 40: 54 us with tiles of neighbouring rows that went through
@@ -31,22 +31,17 @@ __device__ __forceinline__ void st4(float* p, floatx4 v, bool past_cache) {
     else *reinterpret_cast<float4_at*>(p) = v;
 }
 
-// p[0 .. 4) as floats, those at or behind `left` zero and not read.
-__device__ __forceinline__ floatx4 take4(const float* p, int left) {
-    if (left >= 4) return ld4(p);
-    floatx4 v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 3; ++j)
-        if (j < left) v[j] = p[j];
-    return v;
+// p[0 .. 4) as floats; with `left`, those at or behind it zero and not read
+typedef _Float16 half4_at __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ floatx4 take4(const float* p) { return ld4(p); }
+__device__ __forceinline__ floatx4 take4(const _Float16* p) {
+    const half4_at h = *reinterpret_cast<const half4_at*>(p);
+    return floatx4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
 }
-__device__ __forceinline__ floatx4 take4(const _Float16* p, int left) {
-    typedef _Float16 half4_at __attribute__((ext_vector_type(4), aligned(2)));
+template <class T>
+__device__ __forceinline__ floatx4 take4(const T* p, int left) {
     floatx4 v{0.f, 0.f, 0.f, 0.f};
-    if (left >= 4) {
-        const half4_at h = *reinterpret_cast<const half4_at*>(p);
-        return floatx4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
-    }
+    if (left >= 4) return take4(p);
 #pragma unroll
     for (int j = 0; j < 3; ++j)
         if (j < left) v[j] = (float)p[j];
@@ -77,20 +72,20 @@ struct Tile {
 
 // The p-th tile of a block of `n` rows (at most 4096): its slot (a.slots: rows
 // without one), or -1 past the last tile.  hist: slots + 1 counters.
-template <int TR>
+template <int TR, int THREADS, int PASSES>
 __device__ __forceinline__ int find_tile(const LoraArgs& a, const int32_t* ids, int n, int p, int* hist, Tile<TR>& tile) {
-    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
-    const int passes = (n + threads - 1) / threads;
-    const int first_id = ids[min(tid, n - 1)];   // the only one where a pass takes all rows
-    const auto slot_of = [&](int pass, int row) {
-        const int id = pass == 0 ? first_id : ids[min(row, n - 1)];
-        return row >= n ? -1 : id >= 0 && id < a.slots ? id : a.copy_bare ? a.slots : -1;
-    };
-    for (int s = tid; s <= a.slots; s += threads) hist[s] = 0;
+    constexpr int WAVES = THREADS / 64;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int key[PASSES];   // slots of rows tid, tid + THREADS, ..; -1 where none is to be moved
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) key[i] = ids[min(i * THREADS + tid, n - 1)];
+    for (int s = tid; s <= a.slots; s += THREADS) hist[s] = 0;
     if (tid < TR) tile.rows[tid] = -1;
     __syncthreads();
-    for (int i = 0; i < passes; ++i) {
-        const int s = slot_of(i, i * threads + tid);
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const int id = key[i], s = i * THREADS + tid >= n ? -1 : id >= 0 && id < a.slots ? id : a.copy_bare ? a.slots : -1;
+        key[i] = s;
         // one request's rows in a run: one addition for the wave
         const int s0 = __builtin_amdgcn_readfirstlane(s);
         if (__all(s == s0)) {
@@ -114,21 +109,28 @@ __device__ __forceinline__ int find_tile(const LoraArgs& a, const int32_t* ids, 
     }
     slot = __builtin_amdgcn_readfirstlane(slot);
     if (slot < 0) return -1;
-    for (int i = 0; i < passes; ++i) {
-        const uint64_t same = __ballot(slot_of(i, i * threads + tid) == slot);
-        if (lane == 0) tile.counts[i * waves + wave] = __builtin_popcountll(same);
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const uint64_t same = __ballot(key[i] == slot);
+        if (lane == 0) tile.counts[i * WAVES + wave] = __builtin_popcountll(same);
     }
     __syncthreads();
-    const int count = lane < passes * waves ? tile.counts[lane] : 0, first = prefix_sum(count) - count;
-    for (int i = 0; i < passes; ++i) {
-        const int row = i * threads + tid, at = i * waves + wave;
-        const bool here = slot_of(i, row) == slot;
-        const uint64_t same = __ballot(here);
-        const int ahead = __builtin_amdgcn_readlane(first, at) + __builtin_popcountll(same & ((uint64_t(1) << lane) - 1)) - skip;
-        if (here && ahead >= 0 && ahead < TR) tile.rows[ahead] = row;
+    const int count = lane < PASSES * WAVES ? tile.counts[lane] : 0, first = prefix_sum(count) - count;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const uint64_t same = __ballot(key[i] == slot);
+        const int ahead = __builtin_amdgcn_readlane(first, i * WAVES + wave) + __builtin_popcountll(same & ((uint64_t(1) << lane) - 1)) - skip;
+        if (key[i] == slot && ahead >= 0 && ahead < TR) tile.rows[ahead] = i * THREADS + tid;
     }
     __syncthreads();
     return slot;
+}
+
+template <int TR, int THREADS>
+__device__ __forceinline__ int find_tile(const LoraArgs& a, const int32_t* ids, int n, int p, int* hist, Tile<TR>& tile) {
+    if (n <= THREADS) return find_tile<TR, THREADS, 1>(a, ids, n, p, hist, tile);
+    if (n <= 4 * THREADS) return find_tile<TR, THREADS, 4>(a, ids, n, p, hist, tile);
+    return find_tile<TR, THREADS, kLoraBlockRows / THREADS>(a, ids, n, p, hist, tile);
 }
 
 __device__ __forceinline__ int slot_rank(const LoraArgs& a, int slot) {
@@ -153,23 +155,39 @@ struct Stage {
     floatx4 x[XN];
     vec w[AN];
 
-    // values [k, k + KC) of the tile's rows (block0 + rows[]) and of A's first
-    // `rank` rows; zeros at or behind k1, for absent rows and behind the rank
+    // Values [k, k + KC) of the tile's rows (block0 + rows[]) and of A's first
+    // `rank` rows, zeros at or behind k1.  An absent row's place gets the
+    // tile's first row, places behind the rank its last one: what becomes of
+    // them is left out of t.  No branch lies between the loads of a whole
+    // chunk, which the compiler would have wait for each other there.
     __device__ __forceinline__ void load(const LoraArgs& a, int64_t block0, const int* rows, const T* A, int rank, int k, int k1) {
+        const int first = rows[0], last = max(rank - 1, 0);
+        const auto x_at = [&](int f) {
+            const int row = rows[min(f / XC, TR - 1)];
+            return a.x + (block0 + (row < 0 ? first : row)) * a.ldx + k + f % XC * 4;
+        };
+        const auto a_at = [&](int f) { return A + min(f / AC, last) * a.a_row + k + f % AC * VA; };
+        if (k + KC <= k1) {
 #pragma unroll
-        for (int i = 0; i < XN; ++i) {
-            const int f = threadIdx.x + i * THREADS, row = f / XC < TR ? rows[f / XC] : -1, at = k + f % XC * 4;
-            x[i] = take4(a.x + (block0 + max(row, 0)) * a.ldx + at, row >= 0 ? k1 - at : 0);
-        }
+            for (int i = 0; i < XN; ++i) x[i] = ld4(x_at(threadIdx.x + i * THREADS));
 #pragma unroll
-        for (int i = 0; i < AN; ++i) {
-            const int f = threadIdx.x + i * THREADS, q = f / AC, at = k + f % AC * VA, left = q < rank ? k1 - at : 0;
-            const T* p = A + q * a.a_row + at;
-            if (left >= VA) {
-                w[i] = *reinterpret_cast<const vec_at*>(p);
-            } else {
+            for (int i = 0; i < AN; ++i) w[i] = *reinterpret_cast<const vec_at*>(a_at(threadIdx.x + i * THREADS));
+        } else {
 #pragma unroll
-                for (int j = 0; j < VA; ++j) w[i][j] = j < left ? p[j] : (T)0;
+            for (int i = 0; i < XN; ++i) {
+                const int f = threadIdx.x + i * THREADS;
+                x[i] = take4(x_at(f), k1 - (k + f % XC * 4));
+            }
+#pragma unroll
+            for (int i = 0; i < AN; ++i) {
+                const int f = threadIdx.x + i * THREADS, left = k1 - (k + f % AC * VA);
+                const T* p = a_at(f);
+                if (left >= VA) {
+                    w[i] = *reinterpret_cast<const vec_at*>(p);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VA; ++j) w[i][j] = j < left ? p[j] : (T)0;
+                }
             }
         }
     }
@@ -211,17 +229,22 @@ __device__ __forceinline__ void multiply(const Lds& l, int sub, int first, int s
 // Over [k0, k1), every chunk
 template <class T, int THREADS, int TR, int RT, int KC, int UNITS>
 __device__ __forceinline__ void down(const LoraArgs& a, typename Stage<T, THREADS, TR, RT, KC>::Lds& lds, int64_t block0, const int* rows, const T* A,
-                                     int rank, int k0, int k1, int sub, int first, int step, floatx4 (&acc)[RT]) {
+                                     int rank, int k0, int k1, int turn, int sub, int first, int step, floatx4 (&acc)[RT]) {
     Stage<T, THREADS, TR, RT, KC> stage;
     const int tiles = (rank + 15) / 16;
 #pragma unroll
     for (int i = 0; i < RT; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-    stage.load(a, block0, rows, A, rank, k0, k1);
-    for (int k = k0; k < k1; k += KC) {
-        if (k != k0) __syncthreads();   // the last chunk is read
+    // `turn`: the chunk to begin with.  Rows of a power of two apart would have
+    // all workgroups at the same few memory channels, chunk after chunk.
+    const int chunks = max((k1 - k0 + KC - 1) / KC, 0);
+    int c = chunks ? turn % chunks : 0;
+    if (chunks) stage.load(a, block0, rows, A, rank, k0 + c * KC, k1);
+    for (int i = 0; i < chunks; ++i) {
+        if (i) __syncthreads();   // the last chunk is read
         stage.store(lds);
         __syncthreads();
-        if (k + KC < k1) stage.load(a, block0, rows, A, rank, k + KC, k1);
+        c = c + 1 < chunks ? c + 1 : 0;
+        if (i + 1 < chunks) stage.load(a, block0, rows, A, rank, k0 + c * KC, k1);
         multiply<RT, UNITS>(lds, sub, first, step, tiles, acc);
     }
 }
@@ -242,10 +265,19 @@ __device__ __forceinline__ void finish_t(const LoraArgs& a, int slot, int rank, 
 template <class T, int RT>
 __device__ __forceinline__ void take_b(const LoraArgs& a, const T* w, int n, int rank, floatx4 (&b)[RT]) {
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const T* row = w + min(n + r, a.n - 1) * a.b_row + 4 * g;
+    const T* row = w + min(n + r, a.n - 1) * a.b_row;
+    if (a.rank % 4 == 0) {   // whole vectors of the bank's row
+#pragma unroll
+        for (int i = 0; i < RT; ++i) b[i] = take4(row + min(16 * i + 4 * g, a.rank - 4));
+    } else {
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+            if (16 * i < rank) b[i] = take4(row + 16 * i + 4 * g, rank - (16 * i + 4 * g));
+    }
 #pragma unroll
     for (int i = 0; i < RT; ++i)
-        if (16 * i < rank) b[i] = take4(row + 16 * i, rank - (16 * i + 4 * g));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[i][j] = 16 * i + 4 * g + j < rank ? b[i][j] : 0.f;   // what stands there does not count
 }
 template <int RT, int SUB>
 __device__ __forceinline__ void up(int rank, const floatx4 (&b)[RT], const floatx4 (&t)[SUB][RT], floatx4 (&acc)[SUB]) {
@@ -284,21 +316,26 @@ __global__ __launch_bounds__(512) void lora_fused_kernel(LoraArgs a) {
     __shared__ typename Stage<T, 512, 16, RT, KC>::Lds lds;
     __shared__ floatx4 red[8][RT][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
-    const int slot = find_tile<16>(a, a.ids, int(a.m), blockIdx.x, hist, tile);
+    const int slot = find_tile<16, 512>(a, a.ids, int(a.m), blockIdx.x, hist, tile);
     if (slot < 0) return;
     const int row = tile.rows[r], n0 = blockIdx.y * 256 + wave * 32;
     const bool mine = row >= 0;
     const int64_t at = max(row, 0);
     floatx4 base[2];   // under way during the products
+    const int64_t any = mine ? at : tile.rows[0];
+    const bool whole = n0 + 32 <= a.n;
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-        if (mine) base[c] = base4(a, at, n0 + 16 * c + 4 * g);
+    for (int c = 0; c < 2; ++c) {
+        const int n = n0 + 16 * c + 4 * g;
+        if (whole && a.base) base[c] = ld4(a.base + any * a.ldbase + n);
+        else base[c] = base4(a, any, n);
+    }
     if (slot < a.slots) {
         const int rank = slot_rank(a, slot);
         floatx4 t[1][RT], b[2][RT];
 #pragma unroll
         for (int c = 0; c < 2; ++c) take_b<T, RT>(a, static_cast<const T*>(a.b) + slot * a.b_slot, n0 + 16 * c, rank, b[c]);
-        down<T, 512, 16, RT, KC, KC / 128>(a, lds, 0, tile.rows, static_cast<const T*>(a.a) + slot * a.a_slot, rank, 0, a.k, 0, wave, 8, t[0]);
+        down<T, 512, 16, RT, KC, KC / 128>(a, lds, 0, tile.rows, static_cast<const T*>(a.a) + slot * a.a_slot, rank, 0, a.k, 0, 0, wave, 8, t[0]);
 #pragma unroll
         for (int i = 0; i < RT; ++i) red[wave][i][lane] = t[0][i];
         __syncthreads();
@@ -321,19 +358,21 @@ __global__ __launch_bounds__(512) void lora_fused_kernel(LoraArgs a) {
         if (mine) put4(a, at, n0 + 16 * c + 4 * g, base[c]);
 }
 
-// Grid: a block's tiles x blocks of rows x K splits.  A wave takes 16 of 64
-// rows; with 16 the four waves share each chunk of K.  The first split writes
-// the tile's slot and rows down for lora_up_kernel.
+// Grid: a block's tiles x blocks of rows x K splits.  The waves of a
+// workgroup take a subtile of 16 rows each, and share the chunks of K where
+// they are more.  The first split writes the tile's slot and rows down for
+// lora_up_kernel.
 template <class T, int RT, int SUB>
 __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
-    constexpr int TR = 16 * SUB, KC = SUB == 4 ? (RT <= 2 ? 128 : 64) : 512 / (RT < 2 ? 2 : RT), UNITS = SUB == 4 || KC < 64 ? KC / 16 : KC / 64;
+    constexpr int TR = 16 * SUB, KC = 512 / (RT < 2 ? 2 : RT);
+    constexpr int SHARE = KC / 16 < 4 / SUB ? KC / 16 : 4 / SUB, UNITS = KC / 16 / SHARE;   // waves of a subtile, and their units of a chunk
     extern __shared__ int hist[];
     __shared__ Tile<TR> tile;
     __shared__ typename Stage<T, 256, TR, RT, KC>::Lds lds;
-    __shared__ floatx4 red[SUB == 4 ? 1 : 3][RT][64];
+    __shared__ floatx4 red[SHARE - 1][SUB][RT][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
     const int64_t block0 = int64_t(blockIdx.y) * a.block_rows;
-    const int slot = find_tile<TR>(a, a.ids + block0, int(min(int64_t(a.block_rows), a.m - block0)), blockIdx.x, hist, tile);
+    const int slot = find_tile<TR, 256>(a, a.ids + block0, int(min(int64_t(a.block_rows), a.m - block0)), blockIdx.x, hist, tile);
     if (blockIdx.z == 0) {
         int* out = a.tiles + (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * (TR + 1);
         if (tid == 0) out[TR] = slot;
@@ -342,48 +381,40 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
     if (slot < 0 || slot == a.slots) return;
     const int rank = slot_rank(a, slot), tiles = (rank + 15) / 16;
     const int k0 = blockIdx.z * a.k_len, k1 = min(a.k, k0 + a.k_len);
+    const int sub = wave % SUB, part = wave / SUB;   // a part past SHARE does another's work again, unused
     floatx4 acc[RT];
-    const T* A = static_cast<const T*>(a.a) + slot * a.a_slot;
-    // chunks of 32 values hold two units: the first two waves take one each
-    if constexpr (SUB == 4) down<T, 256, TR, RT, KC, UNITS>(a, lds, block0, tile.rows, A, rank, k0, k1, wave, 0, 1, acc);
-    else if constexpr (KC >= 64) down<T, 256, TR, RT, KC, UNITS>(a, lds, block0, tile.rows, A, rank, k0, k1, 0, wave, 4, acc);
-    else down<T, 256, TR, RT, KC, 1>(a, lds, block0, tile.rows, A, rank, k0, k1, 0, wave & 1, 1, acc);
-    if constexpr (SUB == 1) {
-        constexpr int SHARE = KC >= 64 ? 4 : 2;   // waves with a part of the sum
-        if (wave && wave < SHARE) {
-#pragma unroll
-            for (int t = 0; t < RT; ++t)
-                if (t < tiles) red[wave - 1][t][lane] = acc[t];
-        }
-        __syncthreads();
-        if (wave) return;
+    down<T, 256, TR, RT, KC, UNITS>(a, lds, block0, tile.rows, static_cast<const T*>(a.a) + slot * a.a_slot, rank, k0, k1, blockIdx.x, sub,
+                                    part % SHARE, SHARE, acc);
+    if (part && part < SHARE) {
 #pragma unroll
         for (int t = 0; t < RT; ++t)
-            if (t < tiles)
-#pragma unroll
-                for (int w = 1; w < SHARE; ++w) acc[t] += red[w - 1][t][lane];
+            if (t < tiles) red[part - 1][sub][t][lane] = acc[t];
     }
-    const int row = tile.rows[(SUB == 4 ? 16 * wave : 0) + r];
-    if (row < 0) return;
+    __syncthreads();
+    const int row = tile.rows[16 * sub + r];
+    if (part || row < 0) return;
     float* out = a.part + (blockIdx.z * a.m + block0 + row) * a.part_ld + 4 * g;
 #pragma unroll
     for (int t = 0; t < RT; ++t)
-        if (t < tiles) *reinterpret_cast<floatx4*>(out + 16 * t) = acc[t];
+        if (t < tiles) {
+#pragma unroll
+            for (int p = 1; p < SHARE; ++p) acc[t] += red[p - 1][sub][t][lane];
+            *reinterpret_cast<floatx4*>(out + 16 * t) = acc[t];
+        }
 }
 
-// Grid: column splits x parts of a block's tiles x blocks of rows.  A workgroup goes
+// Grid: column splits x a block's tiles x blocks of rows.  A workgroup goes
 // through its split in blocks of 256 columns, 64 to a wave; the sums pass
 // through LDS, so that base and y move in whole KB of a row, and the next
 // block's base is under way as soon as this one's is used.
-template <class T, int RT, int SUB, int TILE>
+template <class T, int RT, int SUB>
 __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
-    constexpr int TR = 16 * SUB, PARTS = TILE / TR, PITCH = 256 + 4, OWN = TR / 4;   // rows that a wave moves
+    constexpr int TR = 16 * SUB, PITCH = 256 + 4, OWN = TR / 4;   // rows that a wave moves
     __shared__ __attribute__((aligned(16))) float sums[TR][PITCH];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
-    const int* tile = a.tiles + (int64_t(blockIdx.z) * a.block_tiles + blockIdx.y / PARTS) * (TILE + 1);
-    const int slot = tile[TILE];
+    const int* tile = a.tiles + (int64_t(blockIdx.z) * gridDim.y + blockIdx.y) * (TR + 1);
+    const int slot = tile[TR];
     if (slot < 0) return;
-    tile += blockIdx.y % PARTS * TR;
     const int64_t block0 = int64_t(blockIdx.z) * a.block_rows;
     const int n0 = blockIdx.x * a.n_len, n1 = min(a.n, n0 + a.n_len);
     floatx4 base[OWN];
@@ -484,15 +515,15 @@ void launch_ranks(const LoraArgs& a, hipStream_t stream) {
             return;
         }
     const unsigned blocks = a.tile_count / a.block_tiles;
-    const dim3 grid(a.block_tiles, blocks, a.splits), up_grid((a.n + a.n_len - 1) / a.n_len, a.block_tiles * (a.tile_rows == 64 ? 2 : 1), blocks);
+    const dim3 grid(a.block_tiles, blocks, a.splits), up_grid((a.n + a.n_len - 1) / a.n_len, a.block_tiles, blocks);
     if constexpr (RT <= 8)
-        if (a.tile_rows == 64) {
-            lora_down_kernel<T, RT, 4><<<grid, 256, lds, stream>>>(a);
-            lora_up_kernel<T, RT, 2, 64><<<up_grid, 256, 0, stream>>>(a);
+        if (a.tile_rows == 32) {
+            lora_down_kernel<T, RT, 2><<<grid, 256, lds, stream>>>(a);
+            lora_up_kernel<T, RT, 2><<<up_grid, 256, 0, stream>>>(a);
             return;
         }
     lora_down_kernel<T, RT, 1><<<grid, 256, lds, stream>>>(a);
-    lora_up_kernel<T, RT, 1, 16><<<up_grid, 256, 0, stream>>>(a);
+    lora_up_kernel<T, RT, 1><<<up_grid, 256, 0, stream>>>(a);
 }
 
 template <class T>
@@ -513,9 +544,10 @@ void lora_plan(LoraArgs& a, int cus) {
     const int columns = (a.n + 255) / 256;
     // tiles of a block of `rows` rows: whole ones, and one begun per slot
     const auto tiles_of = [&](int64_t rows, int tile) { return int(std::min<int64_t>(rows, rows / tile + a.slots + 1)); };
-    const int64_t few = std::min<int64_t>(a.m, kLoraBlockRows);
+    // past one block's rows, blocks of a quarter: a tile is found sooner
+    const int64_t few = a.m > kLoraBlockRows ? kLoraBlockRows / 4 : a.m;
     a.fused = a.rank <= 64 && a.m <= kLoraBlockRows && int64_t(tiles_of(few, 16)) * columns <= 2 * cus;
-    a.tile_rows = !a.fused && a.rank <= 128 && a.m >= 64 * cus / 4 ? 64 : 16;
+    a.tile_rows = !a.fused && a.rank <= 128 && a.m >= 16 * cus ? 32 : 16;
     a.block_rows = int(few);
     a.block_tiles = tiles_of(few, a.tile_rows);
     a.tile_count = int((a.m + a.block_rows - 1) / a.block_rows) * a.block_tiles;
