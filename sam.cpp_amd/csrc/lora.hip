@@ -154,39 +154,45 @@ struct Stage {
     };
     floatx4 x[XN];
     vec w[AN];
+    const float* xp[XN];   // this thread's pieces at k = 0
+    const T* wp[AN];
 
-    // Values [k, k + KC) of the tile's rows (block0 + rows[]) and of A's first
-    // `rank` rows, zeros at or behind k1.  An absent row's place gets the
-    // tile's first row, places behind the rank its last one: what becomes of
-    // them is left out of t.  No branch lies between the loads of a whole
-    // chunk, which the compiler would have wait for each other there.
-    __device__ __forceinline__ void load(const LoraArgs& a, int64_t block0, const int* rows, const T* A, int rank, int k, int k1) {
+    // The tile's rows (block0 + rows[]) and A's first `rank` rows.  An absent
+    // row's place gets the tile's first row, places behind the rank its last
+    // one: what becomes of them is left out of t.
+    __device__ __forceinline__ Stage(const LoraArgs& a, int64_t block0, const int* rows, const T* A, int rank) {
         const int first = rows[0], last = max(rank - 1, 0);
-        const auto x_at = [&](int f) {
-            const int row = rows[min(f / XC, TR - 1)];
-            return a.x + (block0 + (row < 0 ? first : row)) * a.ldx + k + f % XC * 4;
-        };
-        const auto a_at = [&](int f) { return A + min(f / AC, last) * a.a_row + k + f % AC * VA; };
+#pragma unroll
+        for (int i = 0; i < XN; ++i) {
+            const int f = threadIdx.x + i * THREADS, row = rows[min(f / XC, TR - 1)];
+            xp[i] = a.x + (block0 + (row < 0 ? first : row)) * a.ldx + f % XC * 4;
+        }
+#pragma unroll
+        for (int i = 0; i < AN; ++i) {
+            const int f = threadIdx.x + i * THREADS;
+            wp[i] = A + min(f / AC, last) * a.a_row + f % AC * VA;
+        }
+    }
+    // Values [k, k + KC), zeros at or behind k1.  No branch lies between the
+    // loads of a whole chunk, which the compiler would have wait for each
+    // other there.
+    __device__ __forceinline__ void load(int k, int k1) {
         if (k + KC <= k1) {
 #pragma unroll
-            for (int i = 0; i < XN; ++i) x[i] = ld4(x_at(threadIdx.x + i * THREADS));
+            for (int i = 0; i < XN; ++i) x[i] = ld4(xp[i] + k);
 #pragma unroll
-            for (int i = 0; i < AN; ++i) w[i] = *reinterpret_cast<const vec_at*>(a_at(threadIdx.x + i * THREADS));
+            for (int i = 0; i < AN; ++i) w[i] = *reinterpret_cast<const vec_at*>(wp[i] + k);
         } else {
 #pragma unroll
-            for (int i = 0; i < XN; ++i) {
-                const int f = threadIdx.x + i * THREADS;
-                x[i] = take4(x_at(f), k1 - (k + f % XC * 4));
-            }
+            for (int i = 0; i < XN; ++i) x[i] = take4(xp[i] + k, k1 - (k + (threadIdx.x + i * THREADS) % XC * 4));
 #pragma unroll
             for (int i = 0; i < AN; ++i) {
-                const int f = threadIdx.x + i * THREADS, left = k1 - (k + f % AC * VA);
-                const T* p = a_at(f);
+                const int left = k1 - (k + (threadIdx.x + i * THREADS) % AC * VA);
                 if (left >= VA) {
-                    w[i] = *reinterpret_cast<const vec_at*>(p);
+                    w[i] = *reinterpret_cast<const vec_at*>(wp[i] + k);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < VA; ++j) w[i][j] = j < left ? p[j] : (T)0;
+                    for (int j = 0; j < VA; ++j) w[i][j] = j < left ? wp[i][k + j] : (T)0;
                 }
             }
         }
@@ -230,7 +236,7 @@ __device__ __forceinline__ void multiply(const Lds& l, int sub, int first, int s
 template <class T, int THREADS, int TR, int RT, int KC, int UNITS>
 __device__ __forceinline__ void down(const LoraArgs& a, typename Stage<T, THREADS, TR, RT, KC>::Lds& lds, int64_t block0, const int* rows, const T* A,
                                      int rank, int k0, int k1, int turn, int sub, int first, int step, floatx4 (&acc)[RT]) {
-    Stage<T, THREADS, TR, RT, KC> stage;
+    Stage<T, THREADS, TR, RT, KC> stage(a, block0, rows, A, rank);
     const int tiles = (rank + 15) / 16;
 #pragma unroll
     for (int i = 0; i < RT; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -238,13 +244,13 @@ __device__ __forceinline__ void down(const LoraArgs& a, typename Stage<T, THREAD
     // all workgroups at the same few memory channels, chunk after chunk.
     const int chunks = max((k1 - k0 + KC - 1) / KC, 0);
     int c = chunks ? turn % chunks : 0;
-    if (chunks) stage.load(a, block0, rows, A, rank, k0 + c * KC, k1);
+    if (chunks) stage.load(k0 + c * KC, k1);
     for (int i = 0; i < chunks; ++i) {
         if (i) __syncthreads();   // the last chunk is read
         stage.store(lds);
         __syncthreads();
         c = c + 1 < chunks ? c + 1 : 0;
-        if (i + 1 < chunks) stage.load(a, block0, rows, A, rank, k0 + c * KC, k1);
+        if (i + 1 < chunks) stage.load(k0 + c * KC, k1);
         multiply<RT, UNITS>(lds, sub, first, step, tiles, acc);
     }
 }
@@ -364,7 +370,7 @@ __global__ __launch_bounds__(512) void lora_fused_kernel(LoraArgs a) {
 // lora_up_kernel.
 template <class T, int RT, int SUB>
 __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
-    constexpr int TR = 16 * SUB, KC = 512 / (RT < 2 ? 2 : RT);
+    constexpr int TR = 16 * SUB, KC = RT == 1 ? 256 : RT <= 4 ? 128 : 512 / RT;
     constexpr int SHARE = KC / 16 < 4 / SUB ? KC / 16 : 4 / SUB, UNITS = KC / 16 / SHARE;   // waves of a subtile, and their units of a chunk
     extern __shared__ int hist[];
     __shared__ Tile<TR> tile;
