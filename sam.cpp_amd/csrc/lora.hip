@@ -552,7 +552,7 @@ void lora_plan(LoraArgs& a, int cus) {
     const auto tiles_of = [&](int64_t rows, int tile) { return int(std::min<int64_t>(rows, rows / tile + a.slots + 1)); };
     // past one block's rows, blocks of a quarter: a tile is found sooner
     const int64_t few = a.m > kLoraBlockRows ? kLoraBlockRows / 4 : a.m;
-    a.fused = a.rank <= 64 && a.m <= kLoraBlockRows && int64_t(tiles_of(few, 16)) * columns <= 2 * cus;
+    a.fused = a.rank <= 32 && a.m <= kLoraBlockRows && int64_t(tiles_of(few, 16)) * columns <= cus;
     a.tile_rows = !a.fused && a.rank <= 128 && a.m >= 16 * cus ? 32 : 16;
     a.block_rows = int(few);
     a.block_tiles = tiles_of(few, a.tile_rows);
