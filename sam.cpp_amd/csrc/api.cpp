@@ -384,7 +384,7 @@ const char* prefix_attn_problem(const samhip_prefix_attn_desc* d) {
     if (!d->q_start || (d->own_max > 0 && (!d->own_start || !d->own_len))) return "null table";
     for (const int32_t* t : {d->q_start, d->own_start, d->own_len})
         if (reinterpret_cast<uintptr_t>(t) % 4) return "tables must be 4-byte aligned";
-    if (rows * d->heads > (int64_t(1) << 26) || d->prefix_k.ne[1] > (int64_t(1) << 30) || d->own_max > (1 << 30) ||
+    if (rows * d->heads > (int64_t(1) << 23) || d->prefix_k.ne[1] > (int64_t(1) << 30) || d->own_max > (1 << 30) ||
         d->requests > (1 << 20))
         return "dimension too large";
     return nullptr;

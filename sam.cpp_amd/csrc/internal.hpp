@@ -478,7 +478,9 @@ struct PrefixAttnArgs {
     float scale;
     bool causal;
     int group;
-    int prefix_tiles, prefix_splits, prefix_chunk;   // workgroups per kv head, and keys of a split
+    bool wide;
+    int prefix_groups;   // workgroups of the prefix part
+    int prefix_tiles, prefix_splits, prefix_chunk;   // tiles of query places per kv head, and keys of a split
     int own_tiles, own_splits, own_chunk;
     int parts;
     float *part_o, *part_ml;

@@ -15,6 +15,7 @@
 // scaled by powers of two so that the largest magnitude lies in [2^14, 2^15)
 // and any F32 range keeps ~22 bits.  F16 keys and values enter as they are.
 #include <algorithm>
+#include <type_traits>
 
 #include "internal.hpp"
 #include "q8stage.hpp"
@@ -43,33 +44,25 @@ constexpr int WAVES = 4;
 #endif
 }
 
-struct __attribute__((packed, aligned(2))) Half8At {
-    half8 v;
-};
-struct __attribute__((packed, aligned(4))) Float4At {
-    floatx4 v;
-};
+typedef _Float16 half8_at __attribute__((ext_vector_type(8), aligned(2)));
+typedef float float4_at __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
 
-// Eight neighbouring values as loaded, zeros where the row is not to be read.
+// Eight neighbouring values as loaded.
 template <class T>
 struct Raw8;
 template <>
 struct Raw8<_Float16> {
     half8 v;
-    __device__ __forceinline__ void load(const _Float16* p, bool real) {
-        v = half8{0, 0, 0, 0, 0, 0, 0, 0};
-        if (real) v = reinterpret_cast<const Half8At*>(p)->v;
-    }
+    __device__ __forceinline__ void load(const _Float16* p) { v = *reinterpret_cast<const half8_at*>(p); }
 };
 template <>
 struct Raw8<float> {
     floatx4 a, b;
-    __device__ __forceinline__ void load(const float* p, bool real) {
-        a = b = floatx4{0.f, 0.f, 0.f, 0.f};
-        if (real) {
-            a = reinterpret_cast<const Float4At*>(p)->v;
-            b = reinterpret_cast<const Float4At*>(p + 4)->v;
-        }
+    __device__ __forceinline__ void load(const float* p) {
+        a = *reinterpret_cast<const float4_at*>(p);
+        b = *reinterpret_cast<const float4_at*>(p + 4);
     }
     __device__ __forceinline__ uint32_t magnitude() const {
         uint32_t m = 0;
@@ -94,14 +87,16 @@ struct Raw8<float> {
 
 // Biased exponent of the largest magnitude, kept where both powers below are
 // normal floats.
-__device__ __forceinline__ int exponent_of(uint32_t magnitude_bits) { return min(max(int(magnitude_bits >> 23), 20), 254); }
+__device__ __forceinline__ int exponent_of(uint32_t magnitude_bits) {
+    return magnitude_bits ? min(max(int(magnitude_bits >> 23), 20), 254) : 141;
+}
 __device__ __forceinline__ float down(int e) { return __uint_as_float(uint32_t(268 - e) << 23); }   // 2^(141 - e)
 __device__ __forceinline__ float up(int e) { return __uint_as_float(uint32_t(e - 14) << 23); }      // 2^(e - 141)
 
 __device__ __forceinline__ uint32_t wave_umax(uint32_t v) { return umax_xor32(umax_xor16(umax_row(umax_quad(v)))); }
 
 // What a workgroup reads: keys [k0, k1) of one kv head, for query rows
-// [q0, q0 + n) in the tile's 32 flattened (row, head in group) places.
+// [q0, q0 + n) in flattened (row, head in group) places.
 template <class T>
 struct Span {
     const T *k, *v;       // row 0, this kv head
@@ -112,227 +107,402 @@ struct Span {
     bool causal;
 };
 
+// One wave's 32 query places: lane (li, hh) holds place li's values
+// 16t + 8hh .. + 7 as hi + lo, and c, which takes a product of the scaled
+// operands to a score in units of log 2 (the sign of a negative scale is the
+// query's; factor() keeps it positive, for a masked product is -inf).
+template <int HD>
+struct Queries {
+    half8 hi[HD / 16], lo[HD / 16];
+    float c;
+    int row, head, limit;
+    bool mine;
+
+    __device__ __forceinline__ float factor(float of_keys) const { return fmaxf(c * of_keys, 0x1p-120f); }
+
+    template <class T>
+    __device__ __forceinline__ Queries(const PrefixAttnArgs& a, const Span<T>& s, int kvh, int place) {
+        const int hh = (threadIdx.x & 63) >> 5, i = place / a.group;
+        mine = i < s.n;
+        row = s.q0 + (mine ? i : 0);
+        head = kvh * a.group + place - i * a.group;
+        limit = s.causal ? min(s.k1, s.limit0 + i) : s.k1;
+        Raw8<float> raw[HD / 16];
+        uint32_t m = 0;
+#pragma unroll
+        for (int t = 0; t < HD / 16; ++t) raw[t].load(a.q + row * a.ldq + head * HD + 16 * t + 8 * hh);
+#pragma unroll
+        for (int t = 0; t < HD / 16; ++t) m = umax(m, raw[t].magnitude());
+        const int e = exponent_of(umax_xor32(m));
+        const float f = a.scale < 0.f ? -down(e) : down(e);
+#pragma unroll
+        for (int t = 0; t < HD / 16; ++t) raw[t].split(f, hi[t], lo[t]);
+        c = fabsf(a.scale) * LOG2E * up(e);
+    }
+};
+
+// Running maximum (in units of log 2), sum of weights and weighted sums of
+// values of a wave's places: o[d] holds, transposed, lane (li, hh)'s
+// dimensions 32d + 8 (r / 4) + 4hh + r % 4 of place li.
+template <int HD>
+struct Sums {
+    floatx16 o[HD / 32];
+    float m = -__builtin_inff(), l = 0.f;
+
+    __device__ __forceinline__ Sums() { scale(0.f, true); }
+    __device__ __forceinline__ void scale(float f, bool clear = false) {
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = clear ? 0.f : o[d][r] * f;
+    }
+
+    // Weights of N blocks of 32 keys from key `k` on: sc[n] holds products with
+    // keys 32n + 8 (r / 4) + 4hh + r % 4, c takes them to scores; hi + lo of the
+    // weights leave in the order the value operand is read in.
+    template <int N>
+    __device__ __forceinline__ void weigh(floatx16 (&sc)[N], float c, int k, int limit, half8 (&hi)[2 * N], half8 (&lo)[2 * N]) {
+        const int hh = (threadIdx.x & 63) >> 5;
+        if (__any(k + 32 * N > limit)) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (k + 32 * n + 8 * (r >> 2) + 4 * hh + (r & 3) >= limit) sc[n][r] = -__builtin_inff();
+        }
+        // IEEE maximum: a NaN score gives a NaN row either way, and fmaxf
+        // would first quiet every product
+        float mx = sc[0][0];
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = __builtin_elementwise_maximum(mx, sc[n][r]);
+        const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+        mx = c * __builtin_elementwise_maximum(__uint_as_float(other[0]), __uint_as_float(other[1]));
+        // the exponent base moves only when a score passes it by 8, so that
+        // weights stay below 2^8 and most steps skip the rescaling
+        if (__any(mx > m + 8.0f)) {
+            const float mnew = fmaxf(m, mx);
+            const float alpha = mnew == m ? 1.f : __builtin_amdgcn_exp2f(m - mnew);
+            m = mnew;
+            l = l * alpha;
+            scale(alpha);
+        }
+        const float mb = m == -__builtin_inff() ? 0.f : m;   // nothing seen yet: weights 0
+        float ps = 0.f;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                sc[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][r], c, -mb));
+                ps += sc[n][r];
+            }
+        l = l + ps;
+        // hi two at a time; lo = fp16(p - hi) by a mixed-precision fma, whose
+        // factor one is kept from the compiler, which would fold it away
+        float one = 1.0f;
+        asm("" : "+s"(one));
+#pragma unroll
+        for (int u = 0; u < 2 * N; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const float2_t p{sc[u / 2][8 * (u % 2) + j], sc[u / 2][8 * (u % 2) + j + 1]};
+                const half2_t h = __builtin_convertvector(p, half2_t);
+                const float2_t hf = __builtin_convertvector(h, float2_t);
+                hi[u][j] = h[0];
+                hi[u][j + 1] = h[1];
+                lo[u][j] = (_Float16)__builtin_fmaf(p[0], one, -hf[0]);
+                lo[u][j + 1] = (_Float16)__builtin_fmaf(p[1], one, -hf[1]);
+            }
+    }
+};
+
+// A tile of KEYS keys or values of HD as fp16 rows in LDS, F32 ones as hi
+// and, behind them, lo; 16 bytes of padding a row spread the rows' reads over
+// the banks.
+template <class T, int HD, int KEYS>
+struct TileRows {
+    static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, STRIDE = HD * 2 + 16, BYTES = KEYS * STRIDE * PARTS;
+    // piece f (8 values) of the tile
+    static __device__ __forceinline__ void put(uint8_t* tile, int f, const Raw8<T>& raw, float factor) {
+        half8* to = reinterpret_cast<half8*>(tile + f / (HD / 8) * STRIDE + f % (HD / 8) * 16);
+        if constexpr (sizeof(T) == 4) {
+            half8 hi, lo;
+            raw.split(factor, hi, lo);
+            *to = hi;
+            to[KEYS * STRIDE / 16] = lo;
+        } else {
+            *to = raw.v;
+        }
+    }
+};
+
+// sc[n] += K Q^T of keys 32n .. + 31 of a tile of keys in LDS
+template <class T, int HD, int N>
+__device__ __forceinline__ void scores(const uint8_t* kt, const Queries<HD>& q, floatx16 (&sc)[N]) {
+    typedef TileRows<T, HD, 32 * N> R;
+    const int lane = threadIdx.x & 63, li = lane & 31, hh = lane >> 5;
+    const uint8_t* at = kt + li * R::STRIDE + 16 * hh;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[n][r] = 0.f;
+#pragma unroll
+    for (int t = 0; t < HD / 16; ++t)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const half8 kh = *reinterpret_cast<const half8*>(at + 32 * n * R::STRIDE + 32 * t);
+            sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.hi[t], sc[n], 0, 0, 0);
+            sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.lo[t], sc[n], 0, 0, 0);
+            if constexpr (R::PARTS == 2) {
+                const half8 kl = *reinterpret_cast<const half8*>(at + (32 * N + 32 * n) * R::STRIDE + 32 * t);
+                sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, q.hi[t], sc[n], 0, 0, 0);
+            }
+        }
+}
+
+// O^T += V^T P^T with a tile of values in LDS: of 16 keys, lane (li, hh) holds
+// keys 4hh .. + 3 and 8 + 4hh .. + 3 of both operands, V^T read transposed.
+template <class T, int HD, int N>
+__device__ __forceinline__ void values(const uint8_t* vt, const half8 (&hi)[2 * N], const half8 (&lo)[2 * N], Sums<HD>& sums) {
+    typedef TileRows<T, HD, 32 * N> R;
+    const int lane = threadIdx.x & 63, hh = lane >> 5;
+    const uint8_t* at = vt + (4 * hh + ((lane & 15) >> 2)) * R::STRIDE + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+#pragma unroll
+    for (int u = 0; u < 2 * N; ++u)
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) {
+            const uint8_t* p = at + 16 * u * R::STRIDE + 64 * d;
+            const half8 vh = __builtin_shufflevector(ds_read_tr(p), ds_read_tr(p + 8 * R::STRIDE), 0, 1, 2, 3, 4, 5, 6, 7);
+            sums.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, hi[u], sums.o[d], 0, 0, 0);
+            sums.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, lo[u], sums.o[d], 0, 0, 0);
+            if constexpr (R::PARTS == 2) {
+                const uint8_t* q = p + 32 * N * R::STRIDE;
+                const half8 vl = __builtin_shufflevector(ds_read_tr(q), ds_read_tr(q + 8 * R::STRIDE), 0, 1, 2, 3, 4, 5, 6, 7);
+                sums.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, hi[u], sums.o[d], 0, 0, 0);
+            }
+        }
+}
+
+// the sum of weights, of both lanes of a place
+__device__ __forceinline__ float pair_sum(float l) {
+    const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    return __uint_as_float(other[0]) + __uint_as_float(other[1]);
+}
+
+// Few query places: all four waves have the same 32, and each takes tiles of
+// 32 keys of its own, keys straight from memory, values through LDS that no
+// other wave touches.
 template <class T, int HD>
-struct Shared {
-    static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
-    static constexpr int STRIDE = HD * 2 + 16;                  // bytes of a key's values
-    static constexpr int VBYTES = TILE * STRIDE * PARTS;        // one wave's tile
-    static constexpr int OBYTES = TILE * (HD + 4) * 4;          // one wave's sums, at the end
-    static constexpr int BYTES = WAVES * (VBYTES > OBYTES ? VBYTES : OBYTES);
+struct Narrow {
+    static constexpr int VBYTES = TileRows<T, HD, 32>::BYTES, OBYTES = TILE * (HD + 4) * 4;   // a wave's tile, and its sums at the end
+    uint8_t __attribute__((aligned(16))) lds[WAVES * (VBYTES > OBYTES ? VBYTES : OBYTES)];
+    float m[WAVES][TILE], l[WAVES][TILE], total[TILE];
 };
 
 template <class T, int HD>
-__device__ __forceinline__ void attend(const PrefixAttnArgs& a, const Span<T>& s, int kvh, int part, uint8_t* lds, float (*wave_m)[TILE],
-                                       float (*wave_l)[TILE], float* total) {
-    constexpr int STEPS = HD / 16, DB = HD / 32;
-    constexpr bool F32 = sizeof(T) == 4;
-    typedef Shared<T, HD> S;
+__device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Span<T>& s, int kvh, int part, Narrow<T, HD>& sh) {
+    constexpr int STEPS = HD / 16;
+    constexpr bool F32 = sizeof(T) == 4, AHEAD = HD * sizeof(T) <= 256;   // registers for the next tile
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hh = lane >> 5;
-    const int place = s.first + li, i = place / a.group;
-    const bool mine = i < s.n;
-    const int row = s.q0 + i, head = kvh * a.group + place - i * a.group;
-    const int limit = s.causal ? min(s.k1, s.limit0 + i) : s.k1;
-
-    // the query row as hi + lo, scaled by its own power of two
-    half8 qh[STEPS], ql[STEPS];
-    float c;
-    {
-        Raw8<float> raw[STEPS];
-        uint32_t m = 0;
-#pragma unroll
-        for (int t = 0; t < STEPS; ++t) {
-            raw[t].load(a.q + row * a.ldq + head * HD + 16 * t + 8 * hh, mine);
-            m = umax(m, raw[t].magnitude());
-        }
-        const int e = exponent_of(umax_xor32(m));
-#pragma unroll
-        for (int t = 0; t < STEPS; ++t) raw[t].split(down(e), qh[t], ql[t]);
-        c = a.scale * LOG2E * up(e);   // scores in units of log 2
-    }
-
-    floatx16 o[DB];
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-    float mrun = -__builtin_inff(), lsum = 0.f;
+    const Queries<HD> q(a, s, kvh, s.first + li);
+    Sums<HD> sums;
     int ev = 20;   // F32 values: the exponent that the sums are scaled by
-    uint8_t* vt = lds + wave * S::VBYTES;
-
-    for (int k = s.k0 + TILE * wave; k < s.k1; k += TILE * WAVES) {
-        Raw8<T> kr[STEPS], vr[STEPS];
+    uint8_t* vt = sh.lds + wave * Narrow<T, HD>::VBYTES;
+    Raw8<T> kr[STEPS], vr[STEPS];
+    const auto load = [&](int k) {   // behind the last key the last one again: its weight is zero there
+        const T* kp = s.k + min(k + li, s.k1 - 1) * s.ldk + 8 * hh;
 #pragma unroll
-        for (int t = 0; t < STEPS; ++t) kr[t].load(s.k + (k + li) * s.ldk + 16 * t + 8 * hh, k + li < s.k1);
+        for (int t = 0; t < STEPS; ++t) kr[t].load(kp + 16 * t);
 #pragma unroll
         for (int t = 0; t < STEPS; ++t) {
-            const int at = t * 64 + lane, key = at / (HD / 8), col = at % (HD / 8);
-            vr[t].load(s.v + (k + key) * s.ldv + 8 * col, k + key < s.k1);
+            const int f = t * 64 + lane;
+            vr[t].load(s.v + min(k + f / (HD / 8), s.k1 - 1) * s.ldv + 8 * (f % (HD / 8)));
         }
-        floatx16 sc;
+    };
+    const int step = TILE * WAVES, kw = s.k0 + TILE * wave;
+    if (AHEAD && kw < s.k1) load(kw);
+    for (int k = kw; k < s.k1; k += step) {
+        if (!AHEAD) load(k);
+        floatx16 sc[1];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sc[r] = 0.f;
-        float ck = c;
+        for (int r = 0; r < 16; ++r) sc[0][r] = 0.f;
+        float c = q.factor(1.f);
         if constexpr (F32) {
-            uint32_t m = 0;
+            uint32_t m = 0, mv = 0;
 #pragma unroll
-            for (int t = 0; t < STEPS; ++t) m = umax(m, kr[t].magnitude());
+            for (int t = 0; t < STEPS; ++t) m = umax(m, kr[t].magnitude()), mv = umax(mv, vr[t].magnitude());
             const int e = exponent_of(__builtin_amdgcn_readfirstlane(wave_umax(m)));
-            ck = c * up(e);
+            const int en = exponent_of(__builtin_amdgcn_readfirstlane(wave_umax(mv)));
+            c = q.factor(up(e));
 #pragma unroll
             for (int t = 0; t < STEPS; ++t) {
                 half8 kh, kl;
                 kr[t].split(down(e), kh, kl);
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[t], sc, 0, 0, 0);
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[t], sc, 0, 0, 0);
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[t], sc, 0, 0, 0);
+                sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.hi[t], sc[0], 0, 0, 0);
+                sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, q.hi[t], sc[0], 0, 0, 0);
+                sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.lo[t], sc[0], 0, 0, 0);
+            }
+            if (en > ev) {
+                sums.scale(__builtin_ldexpf(1.f, ev - en));
+                ev = en;
             }
         } else {
 #pragma unroll
             for (int t = 0; t < STEPS; ++t) {
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kr[t].v, qh[t], sc, 0, 0, 0);
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kr[t].v, ql[t], sc, 0, 0, 0);
+                sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kr[t].v, q.hi[t], sc[0], 0, 0, 0);
+                sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kr[t].v, q.lo[t], sc[0], 0, 0, 0);
             }
         }
-        // values to LDS, one row per key
         wave_lds_handoff();   // the last tile's reads came first
-        if constexpr (F32) {
-            uint32_t m = 0;
 #pragma unroll
-            for (int t = 0; t < STEPS; ++t) m = umax(m, vr[t].magnitude());
-            const int e = exponent_of(__builtin_amdgcn_readfirstlane(wave_umax(m)));
-            if (e > ev) {
-                const float f = __builtin_ldexpf(1.f, ev - e);
-                ev = e;
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * f;
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < STEPS; ++t) {
-            const int at = t * 64 + lane, key = at / (HD / 8), col = at % (HD / 8);
-            half8* to = reinterpret_cast<half8*>(vt + key * S::STRIDE + col * 16);
-            if constexpr (F32) {
-                half8 vh, vl;
-                vr[t].split(down(ev), vh, vl);
-                *to = vh;
-                to[TILE * S::STRIDE / 16] = vl;
-            } else {
-                *to = vr[t].v;
-            }
-        }
+        for (int t = 0; t < STEPS; ++t) TileRows<T, HD, 32>::put(vt, t * 64 + lane, vr[t], down(ev));
         wave_lds_handoff();
-        // softmax: lane (li, hh) holds place li's scores of keys
-        // 8 (r / 4) + 4 hh + r % 4
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sc[r] = sc[r] * ck;
-        if (__any(k + TILE > limit)) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (k + 8 * (r >> 2) + 4 * hh + (r & 3) >= limit) sc[r] = -__builtin_inff();
-        }
-        float mx = sc[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx = __builtin_elementwise_maximum(mx, sc[r]);
-        const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = __builtin_elementwise_maximum(__uint_as_float(other[0]), __uint_as_float(other[1]));
-        // the exponent base moves only when a score passes it by 8, so that
-        // weights stay below 2^8 and most steps skip the rescaling
-        if (__any(mx > mrun + 8.0f)) {
-            const float mnew = fmaxf(mrun, mx);
-            const float alpha = mnew == mrun ? 1.f : __builtin_amdgcn_exp2f(mrun - mnew);
-            mrun = mnew;
-            lsum = lsum * alpha;
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * alpha;
-        }
-        const float mb = mrun == -__builtin_inff() ? 0.f : mrun;   // nothing seen yet: weights 0
-        float ps = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            sc[r] = __builtin_amdgcn_exp2f(sc[r] - mb);
-            ps += sc[r];
-        }
-        lsum = lsum + ps;
+        if (AHEAD && k + step < s.k1) load(k + step);
         half8 ph[2], pl[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float p = sc[8 * u + j];
-                const _Float16 h = (_Float16)p;
-                ph[u][j] = h;
-                pl[u][j] = (_Float16)(p - (float)h);
-            }
-        // O^T += V^T P^T: keys 16u + 4hh .. + 3 and 16u + 8 + 4hh .. + 3
-        const uint8_t* at = vt + (4 * hh + ((lane & 15) >> 2)) * S::STRIDE + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const uint8_t* p = at + 16 * u * S::STRIDE + 64 * d;
-                const half8 vh = __builtin_shufflevector(ds_read_tr(p), ds_read_tr(p + 8 * S::STRIDE), 0, 1, 2, 3, 4, 5, 6, 7);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[u], o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[u], o[d], 0, 0, 0);
-                if constexpr (F32) {
-                    const uint8_t* q = p + TILE * S::STRIDE;
-                    const half8 vl = __builtin_shufflevector(ds_read_tr(q), ds_read_tr(q + 8 * S::STRIDE), 0, 1, 2, 3, 4, 5, 6, 7);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[u], o[d], 0, 0, 0);
-                }
-            }
+        sums.weigh(sc, c, k, q.limit, ph, pl);
+        values<T, HD, 1>(vt, ph, pl, sums);
     }
     // the four waves' sums, joined through LDS
-    const auto lother = __builtin_amdgcn_permlane32_swap(__float_as_uint(lsum), __float_as_uint(lsum), false, false);
-    lsum = __uint_as_float(lother[0]) + __uint_as_float(lother[1]);
+    sums.l = pair_sum(sums.l);
     if (hh == 0) {
-        wave_m[wave][li] = mrun;
-        wave_l[wave][li] = lsum;
+        sh.m[wave][li] = sums.m;
+        sh.l[wave][li] = sums.l;
     }
     __syncthreads();   // also: every wave is past its value tiles
     float m = -__builtin_inff(), l = 0.f;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, wave_m[w][li]);
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, sh.m[w][li]);
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-        const float lw = wave_l[w][li];
-        if (lw != 0.f) l += lw * __builtin_amdgcn_exp2f(wave_m[w][li] - m);   // a NaN sum stays one
+        const float lw = sh.l[w][li];
+        if (lw != 0.f) l += lw * __builtin_amdgcn_exp2f(sh.m[w][li] - m);   // a NaN sum stays one
     }
-    float f = lsum != 0.f ? __builtin_amdgcn_exp2f(mrun - m) : 0.f;
+    float f = sums.l != 0.f ? __builtin_amdgcn_exp2f(sums.m - m) : 0.f;
     if constexpr (F32) f = f * up(ev);
-    float* sums = reinterpret_cast<float*>(lds);
+    float* all = reinterpret_cast<float*>(sh.lds);
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+    for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            float* to = sums + (wave * TILE + li) * (HD + 4) + 32 * d + 2 * r + 4 * hh;
-            *reinterpret_cast<floatx4*>(to) = floatx4{o[d][r] * f, o[d][r + 1] * f, o[d][r + 2] * f, o[d][r + 3] * f};
+        for (int r = 0; r < 16; r += 4)
+            *reinterpret_cast<floatx4*>(all + (wave * TILE + li) * (HD + 4) + 32 * d + 2 * r + 4 * hh) =
+                floatx4{sums.o[d][r] * f, sums.o[d][r + 1] * f, sums.o[d][r + 2] * f, sums.o[d][r + 3] * f};
+    if (wave == 0 && hh == 0) {
+        sh.total[li] = l;
+        if (part >= 0 && q.mine) {
+            float* ml = a.part_ml + (int64_t(part) * a.rows * a.heads + int64_t(q.row) * a.heads + q.head) * 2;
+            ml[0] = m;
+            ml[1] = l;
         }
-    if (part >= 0 && wave == 0 && hh == 0 && mine) {
-        float* ml = a.part_ml + (int64_t(part) * a.rows * a.heads + int64_t(row) * a.heads + head) * 2;
-        ml[0] = m;
-        ml[1] = l;
     }
-    if (wave == 0 && hh == 0) total[li] = l;
     __syncthreads();
     constexpr int QUADS = HD / 4;
     for (int t = tid; t < TILE * QUADS; t += 64 * WAVES) {
-        const int p = t / QUADS, d = 4 * (t % QUADS), pl = s.first + p, pi = pl / a.group;
-        if (pi >= s.n) continue;
+        const int p = t / QUADS, d = 4 * (t % QUADS), place = s.first + p, i = place / a.group;
+        if (i >= s.n) continue;
         floatx4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) v += *reinterpret_cast<const floatx4*>(sums + (w * TILE + p) * (HD + 4) + d);
-        const int64_t r = s.q0 + pi, h = kvh * a.group + pl - pi * a.group;
+        for (int w = 0; w < WAVES; ++w) v += *reinterpret_cast<const floatx4*>(all + (w * TILE + p) * (HD + 4) + d);
+        const int64_t r = s.q0 + i, h = kvh * a.group + place - i * a.group;
         if (part < 0) {
-            const float lt = total[p];
-            const float inv = lt == 0.f ? 0.f : 1.f / lt;
-            reinterpret_cast<Float4At*>(a.out + r * a.ldo + h * HD + d)->v = v * inv;
+            const float lt = sh.total[p], inv = lt == 0.f ? 0.f : 1.f / lt;
+            *reinterpret_cast<float4_at*>(a.out + r * a.ldo + h * HD + d) = v * inv;
         } else {
             *reinterpret_cast<floatx4*>(a.part_o + ((int64_t(part) * a.rows + r) * a.heads + h) * HD + d) = v;
         }
     }
+}
+
+// Many query places: 32 to a wave, and tiles of 64 keys and values that the
+// four waves share in LDS; the next tile is on its way to registers during a
+// tile's products.
+template <class T, int HD>
+struct Wide {
+    uint8_t __attribute__((aligned(16))) k[TileRows<T, HD, 64>::BYTES];
+    uint8_t __attribute__((aligned(16))) v[TileRows<T, HD, 64>::BYTES];
+    uint32_t largest[WAVES][2];
+};
+
+template <class T, int HD>
+__device__ __forceinline__ void attend_wide(const PrefixAttnArgs& a, const Span<T>& s, int kvh, int part, Wide<T, HD>& sh) {
+    constexpr int PIECES = HD / 32;   // of 8 values, a thread's part of a tile
+    constexpr bool F32 = sizeof(T) == 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hh = lane >> 5;
+    const int first = s.first + TILE * wave;
+    const bool any = first < s.n * a.group;
+    const Queries<HD> q(a, s, kvh, first + li);
+    Sums<HD> sums;
+    int ev = 20;
+    Raw8<T> kr[PIECES], vr[PIECES];
+    const auto load = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int f = tid + 256 * i;
+            const int64_t key = min(k + f / (HD / 8), s.k1 - 1), col = 8 * (f % (HD / 8));
+            kr[i].load(s.k + key * s.ldk + col);
+            vr[i].load(s.v + key * s.ldv + col);
+        }
+    };
+    load(s.k0);
+    for (int k = s.k0; k < s.k1; k += 64) {
+        float c = q.factor(1.f), fk = 1.f;
+        if constexpr (F32) {
+            uint32_t mk = 0, mv = 0;
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) mk = umax(mk, kr[i].magnitude()), mv = umax(mv, vr[i].magnitude());
+            mk = wave_umax(mk);
+            mv = wave_umax(mv);
+            if (lane == 0) sh.largest[wave][0] = mk, sh.largest[wave][1] = mv;
+        }
+        __syncthreads();   // the last tile is read, the largest magnitudes are written
+        if constexpr (F32) {
+            uint32_t mk = 0, mv = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) mk = umax(mk, sh.largest[w][0]), mv = umax(mv, sh.largest[w][1]);
+            const int e = exponent_of(__builtin_amdgcn_readfirstlane(mk)), en = exponent_of(__builtin_amdgcn_readfirstlane(mv));
+            c = q.factor(up(e));
+            fk = down(e);
+            if (en > ev) {
+                sums.scale(__builtin_ldexpf(1.f, ev - en));
+                ev = en;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            TileRows<T, HD, 64>::put(sh.k, tid + 256 * i, kr[i], fk);
+            TileRows<T, HD, 64>::put(sh.v, tid + 256 * i, vr[i], down(ev));
+        }
+        __syncthreads();
+        if (k + 64 < s.k1) load(k + 64);
+        if (any) {
+            floatx16 sc[2];
+            half8 ph[4], pl[4];
+            scores<T, HD, 2>(sh.k, q, sc);
+            sums.weigh(sc, c, k, q.limit, ph, pl);
+            values<T, HD, 2>(sh.v, ph, pl, sums);
+        }
+    }
+    const float l = pair_sum(sums.l);
+    if (!q.mine) return;
+    float f = F32 ? up(ev) : 1.f;
+    float* to;
+    if (part < 0) {
+        f = l == 0.f ? 0.f : f / l;
+        to = a.out + q.row * a.ldo + q.head * HD;
+    } else {
+        const int64_t at = int64_t(part) * a.rows * a.heads + int64_t(q.row) * a.heads + q.head;
+        to = a.part_o + at * HD;
+        if (hh == 0) {
+            a.part_ml[2 * at] = sums.m;
+            a.part_ml[2 * at + 1] = l;
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+            *reinterpret_cast<float4_at*>(to + 32 * d + 2 * r + 4 * hh) =
+                floatx4{sums.o[d][r] * f, sums.o[d][r + 1] * f, sums.o[d][r + 2] * f, sums.o[d][r + 3] * f};
 }
 
 // Query rows [from, from + n) of request r, cut to the rows that exist.
@@ -368,21 +538,26 @@ __device__ __forceinline__ bool find_tile(const PrefixAttnArgs& a, int t, int& r
     return false;
 }
 
-// Grid: the prefix part's workgroups (tiles x splits), then the own parts',
-// times kv heads.
-template <class T, int HD>
+// Grid: the prefix part's workgroups, then the own parts'.  Workgroups are
+// dispatched round-robin over the 8 XCDs: the prefix part's are numbered so
+// that the query tiles that read the same keys run one behind the other on
+// one XCD and share its L2.
+template <class T, int HD, bool WIDE>
 __global__ __launch_bounds__(64 * WAVES) void prefix_attn_kernel(PrefixAttnArgs a) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[Shared<T, HD>::BYTES];
-    __shared__ float wave_m[WAVES][TILE], wave_l[WAVES][TILE], total[TILE];
-    const int kvh = blockIdx.y;
+    union Shared {
+        Narrow<T, HD> narrow;
+        Wide<T, HD> wide;
+    };
+    __shared__ typename std::conditional<WIDE, Shared, Narrow<T, HD>>::type sh;
     int w = blockIdx.x;
     Span<T> s;
-    int part;
-    if (w < a.prefix_tiles * a.prefix_splits) {
-        const int split = w / a.prefix_tiles;
+    if (w < a.prefix_groups) {
+        const int order = w >> 3, set = (w & 7) + 8 * (order / a.prefix_tiles);   // of kv head and split
+        const int kvh = set / a.prefix_splits, split = set - kvh * a.prefix_splits;
+        if (kvh >= a.kv_heads) return;
         s.q0 = min(max(a.q_start[0], 0), a.rows);
         s.n = min(max(a.q_start[a.requests], 0), a.rows) - s.q0;
-        s.first = (w - split * a.prefix_tiles) * TILE;
+        s.first = order % a.prefix_tiles * (WIDE ? TILE * WAVES : TILE);
         if (s.first >= s.n * a.group) return;
         s.k = static_cast<const T*>(a.prefix_k) + kvh * HD;
         s.v = static_cast<const T*>(a.prefix_v) + kvh * HD;
@@ -392,68 +567,96 @@ __global__ __launch_bounds__(64 * WAVES) void prefix_attn_kernel(PrefixAttnArgs 
         s.k1 = min(s.k0 + a.prefix_chunk, a.prefix);
         s.causal = false;
         s.limit0 = 0;
-        part = split;
-    } else {
-        w -= a.prefix_tiles * a.prefix_splits;
-        const int split = w / a.own_tiles;
-        int request, tile;
-        if (!find_tile(a, w - split * a.own_tiles, request, tile)) return;
-        s.n = rows_of(a, request, s.q0);
-        s.first = tile * TILE;
-        int64_t start = 0;
-        int len = 0;
-        if (a.own_max > 0) {
-            start = a.own_start[request];
-            len = min(max(a.own_len[request], 0), a.own_max);
-            if (start < 0 || start > a.own_rows) start = len = 0;
-            len = int(min(int64_t(len), a.own_rows - start));
-        }
-        s.k = static_cast<const T*>(a.own_k) + start * a.ld_own_k + kvh * HD;
-        s.v = static_cast<const T*>(a.own_v) + start * a.ld_own_v + kvh * HD;
-        s.ldk = a.ld_own_k;
-        s.ldv = a.ld_own_v;
-        s.causal = a.causal;
-        s.limit0 = len - s.n + 1;
-        s.k0 = split * a.own_chunk;
-        s.k1 = min(s.k0 + a.own_chunk, len);
-        if (s.causal) s.k1 = min(s.k1, s.limit0 + min(s.n - 1, (s.first + TILE - 1) / a.group));
-        part = a.prefix_splits + split;
+        const int part = a.parts > 1 ? split : -1;
+        if constexpr (WIDE) attend_wide<T, HD>(a, s, kvh, part, sh.wide);
+        else attend_narrow<T, HD>(a, s, kvh, part, sh);
+        return;
     }
-    attend<T, HD>(a, s, kvh, a.parts > 1 ? part : -1, lds, wave_m, wave_l, total);
+    w -= a.prefix_groups;
+    const int per_head = a.own_tiles * a.own_splits, kvh = w / per_head, split = (w - kvh * per_head) / a.own_tiles;
+    int request, tile;
+    if (!find_tile(a, w - kvh * per_head - split * a.own_tiles, request, tile)) return;
+    s.n = rows_of(a, request, s.q0);
+    s.first = tile * TILE;
+    int64_t start = 0;
+    int len = 0;
+    if (a.own_max > 0) {
+        start = a.own_start[request];
+        len = min(max(a.own_len[request], 0), a.own_max);
+        if (start < 0 || start > a.own_rows) start = len = 0;
+        len = int(min(int64_t(len), a.own_rows - start));
+    }
+    s.k = static_cast<const T*>(a.own_k) + start * a.ld_own_k + kvh * HD;
+    s.v = static_cast<const T*>(a.own_v) + start * a.ld_own_v + kvh * HD;
+    s.ldk = a.ld_own_k;
+    s.ldv = a.ld_own_v;
+    s.causal = a.causal;
+    s.limit0 = len - s.n + 1;
+    s.k0 = split * a.own_chunk;
+    s.k1 = min(s.k0 + a.own_chunk, len);
+    if (s.causal) s.k1 = min(s.k1, s.limit0 + min(s.n - 1, (s.first + TILE - 1) / a.group));
+    const int part = a.parts > 1 ? a.prefix_splits + split : -1;
+    if constexpr (WIDE) attend_narrow<T, HD>(a, s, kvh, part, sh.narrow);
+    else attend_narrow<T, HD>(a, s, kvh, part, sh);
 }
 
-// One (row, head) per HD / 4 lanes.
+// A wave per (row, head): the parts' maxima and sums one to a lane, then
+// HD / 4 lanes to a part's values.
 template <int HD>
 __global__ __launch_bounds__(256) void attn_merge_kernel(PrefixAttnArgs a) {
-    constexpr int QUADS = HD / 4;
-    const int64_t item = (int64_t(blockIdx.x) * 256 + threadIdx.x) / QUADS, items = int64_t(a.rows) * a.heads;
-    const int d = 4 * (threadIdx.x % QUADS);
+    constexpr int QUADS = HD / 4, AT_ONCE = 64 / QUADS;
+    const int lane = threadIdx.x & 63;
+    const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6), items = int64_t(a.rows) * a.heads;
     if (item >= items) return;
     const int64_t row = item / a.heads, h = item - row * a.heads;
     if (row < min(max(a.q_start[0], 0), a.rows) || row >= min(max(a.q_start[a.requests], 0), a.rows)) return;
-    float m = -__builtin_inff();
-    for (int p = 0; p < a.parts; ++p) m = fmaxf(m, a.part_ml[(p * items + item) * 2]);
-    float l = 0.f;
+    const int d = 4 * (lane % QUADS), slot = lane / QUADS;
+    float m = -__builtin_inff(), l = 0.f;
     floatx4 v{0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < a.parts; ++p) {
-        const float lp = a.part_ml[(p * items + item) * 2 + 1];
-        if (lp == 0.f) continue;   // no key in this part
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[(p * items + item) * 2] - m);
-        l += lp * f;
-        v += *reinterpret_cast<const floatx4*>(a.part_o + (p * items + item) * HD + d) * f;
+    for (int p0 = 0; p0 < a.parts; p0 += 64) {
+        float mp = -__builtin_inff(), lp = 0.f;
+        if (p0 + lane < a.parts) {
+            const float* ml = a.part_ml + ((p0 + lane) * items + item) * 2;
+            mp = ml[0];
+            lp = ml[1];
+        }
+        const float mnew = fmaxf(m, wave_max(lp != 0.f ? mp : -__builtin_inff()));
+        const float old = m == mnew ? 1.f : __builtin_amdgcn_exp2f(m - mnew);
+        const float f = lp != 0.f ? __builtin_amdgcn_exp2f(mp - mnew) : 0.f;   // 0: no key in this part
+        m = mnew;
+        l = l * old + wave_sum(lp * f);
+        v = v * old;
+        const int here = min(a.parts - p0, 64);
+        for (int p1 = 0; p1 < here; p1 += 4 * AT_ONCE) {
+            floatx4 o[4];
+            float fp[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int p = p1 + u * AT_ONCE + slot, at = min(p, here - 1);
+                o[u] = *reinterpret_cast<const floatx4*>(a.part_o + ((p0 + at) * items + item) * HD + d);
+                fp[u] = __shfl(f, at, 64);
+                if (p >= here) fp[u] = 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += fp[u] != 0.f ? o[u][j] * fp[u] : 0.f;   // without keys its sums may never have been written
+        }
     }
+#pragma unroll
+    for (int off = QUADS; off < 64; off <<= 1)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += __shfl_xor(v[j], off, 64);
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    reinterpret_cast<Float4At*>(a.out + row * a.ldo + h * HD + d)->v = v * inv;
+    if (slot == 0) *reinterpret_cast<float4_at*>(a.out + row * a.ldo + h * HD + d) = v * inv;
 }
 
 template <class T, int HD>
 void launch_typed(const PrefixAttnArgs& a, hipStream_t stream) {
-    const unsigned groups = unsigned(a.prefix_tiles) * a.prefix_splits + unsigned(a.own_tiles) * a.own_splits;
-    prefix_attn_kernel<T, HD><<<dim3(groups, a.kv_heads), 64 * WAVES, 0, stream>>>(a);
-    if (a.parts > 1) {
-        const int64_t threads = int64_t(a.rows) * a.heads * (HD / 4);
-        attn_merge_kernel<HD><<<unsigned((threads + 255) / 256), 256, 0, stream>>>(a);
-    }
+    const unsigned groups = unsigned(a.prefix_groups) + unsigned(a.own_tiles) * a.own_splits * a.kv_heads;
+    if (a.wide) prefix_attn_kernel<T, HD, true><<<groups, 64 * WAVES, 0, stream>>>(a);
+    else prefix_attn_kernel<T, HD, false><<<groups, 64 * WAVES, 0, stream>>>(a);
+    if (a.parts > 1) attn_merge_kernel<HD><<<unsigned((int64_t(a.rows) * a.heads + 3) / 4), 256, 0, stream>>>(a);
 }
 
 }  // namespace
@@ -466,11 +669,15 @@ void prefix_attn_plan(PrefixAttnArgs& a, int cus) {
     const auto chunk = [](int64_t keys, int n) { return int(((keys + n - 1) / n + TILE * WAVES - 1) / (TILE * WAVES) * (TILE * WAVES)); };
     a.group = a.heads / a.kv_heads;
     const int64_t places = int64_t(a.rows) * a.group;
-    a.prefix_tiles = a.prefix ? int((places + TILE - 1) / TILE) : 0;
+    a.wide = a.prefix && places > 2 * TILE;
+    const int tile = a.wide ? TILE * WAVES : TILE;
+    a.prefix_tiles = a.prefix ? int((places + tile - 1) / tile) : 0;
     a.prefix_splits = a.prefix ? splits(int64_t(a.prefix_tiles) * a.kv_heads, a.prefix) : 0;
+    a.prefix_groups = 0;
     if (a.prefix) {
         a.prefix_chunk = chunk(a.prefix, a.prefix_splits);
         a.prefix_splits = (a.prefix + a.prefix_chunk - 1) / a.prefix_chunk;
+        a.prefix_groups = (a.prefix_splits * a.kv_heads + 7) / 8 * 8 * a.prefix_tiles;
     }
     // without a prefix the own parts write every row, an empty one as zeros
     const bool own = a.own_max > 0 || !a.prefix;
