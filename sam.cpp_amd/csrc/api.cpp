@@ -1301,7 +1301,7 @@ int samhip_prefix_attn(samhip_context* ctx, const samhip_prefix_attn_desc* d) {
     a.scale = d->scale;
     a.causal = d->causal != 0;
     if (int rc = set_device(ctx)) return rc;
-    prefix_attn_plan(a, ctx->cus);
+    prefix_attn_plan(a, d->head_dim, ctx->cus);
     if (int rc = ensure_staging(ctx, prefix_attn_scratch_bytes(a, d->head_dim))) return rc;
     return traced(ctx, "prefix_attn", d->prefix_k.type, a.rows, int64_t(a.heads) * d->head_dim, a.prefix, [&]() -> int {
         launch_prefix_attn(a, d->prefix_k.type, d->head_dim, ctx->staging, ctx->stream);

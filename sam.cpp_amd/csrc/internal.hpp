@@ -485,7 +485,7 @@ struct PrefixAttnArgs {
     int parts;
     float *part_o, *part_ml;
 };
-void prefix_attn_plan(PrefixAttnArgs& a, int cus);
+void prefix_attn_plan(PrefixAttnArgs& a, int head_dim, int cus);
 size_t prefix_attn_scratch_bytes(const PrefixAttnArgs& a, int head_dim);
 void launch_prefix_attn(PrefixAttnArgs a, int type, int head_dim, void* scratch, hipStream_t stream);
 

@@ -49,6 +49,22 @@ typedef float float4_at __attribute__((ext_vector_type(4), aligned(4)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef float float2_t __attribute__((ext_vector_type(2)));
 
+// Values j and j + 1 as hi + lo: hi two at a time; lo = fp16(x - hi) by a
+// mixed-precision fma, whose factor one is kept from the compiler, which
+// would fold it away.
+__device__ __forceinline__ void split_pair(float2_t x, half8& hi, half8& lo, int j) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    float one = 1.0f;
+    asm("" : "+s"(one));
+    const half2_t h = __builtin_convertvector(x, half2_t);
+    const float2_t hf = __builtin_convertvector(h, float2_t);
+    hi[j] = h[0];
+    hi[j + 1] = h[1];
+    lo[j] = (_Float16)__builtin_fmaf(x[0], one, -hf[0]);
+    lo[j + 1] = (_Float16)__builtin_fmaf(x[1], one, -hf[1]);
+#endif
+}
+
 // Eight neighbouring values as loaded.
 template <class T>
 struct Raw8;
@@ -76,11 +92,9 @@ struct Raw8<float> {
     // values * factor as hi + lo
     __device__ __forceinline__ void split(float factor, half8& hi, half8& lo) const {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float x = (j < 4 ? a[j & 3] : b[j & 3]) * factor;
-            const _Float16 h = (_Float16)x;
-            hi[j] = h;
-            lo[j] = (_Float16)(x - (float)h);
+        for (int j = 0; j < 8; j += 2) {
+            const float2_t x{(j < 4 ? a[j & 3] : b[j & 3]) * factor, (j < 4 ? a[(j & 3) + 1] : b[(j & 3) + 1]) * factor};
+            split_pair(x, hi, lo, j);
         }
     }
 };
@@ -198,22 +212,11 @@ struct Sums {
                 ps += sc[n][r];
             }
         l = l + ps;
-        // hi two at a time; lo = fp16(p - hi) by a mixed-precision fma, whose
-        // factor one is kept from the compiler, which would fold it away
-        float one = 1.0f;
-        asm("" : "+s"(one));
 #pragma unroll
         for (int u = 0; u < 2 * N; ++u)
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                const float2_t p{sc[u / 2][8 * (u % 2) + j], sc[u / 2][8 * (u % 2) + j + 1]};
-                const half2_t h = __builtin_convertvector(p, half2_t);
-                const float2_t hf = __builtin_convertvector(h, float2_t);
-                hi[u][j] = h[0];
-                hi[u][j + 1] = h[1];
-                lo[u][j] = (_Float16)__builtin_fmaf(p[0], one, -hf[0]);
-                lo[u][j + 1] = (_Float16)__builtin_fmaf(p[1], one, -hf[1]);
-            }
+            for (int j = 0; j < 8; j += 2)
+                split_pair(float2_t{sc[u / 2][8 * (u % 2) + j], sc[u / 2][8 * (u % 2) + j + 1]}, hi[u], lo[u], j);
     }
 };
 
@@ -268,20 +271,25 @@ __device__ __forceinline__ void values(const uint8_t* vt, const half8 (&hi)[2 * 
     typedef TileRows<T, HD, 32 * N> R;
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     const uint8_t* at = vt + (4 * hh + ((lane & 15) >> 2)) * R::STRIDE + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    constexpr int DB = HD / 32, COUNT = 2 * N * DB, AHEAD = HD < 128 ? 1 : 0;   // 128: no registers left
+    half8 v[2][R::PARTS];   // the next one is under way during a product
+    const auto fetch = [&](int i) {
+        const uint8_t* p = at + 16 * (i / DB) * R::STRIDE + 64 * (i % DB);
 #pragma unroll
-    for (int u = 0; u < 2 * N; ++u)
-#pragma unroll
-        for (int d = 0; d < HD / 32; ++d) {
-            const uint8_t* p = at + 16 * u * R::STRIDE + 64 * d;
-            const half8 vh = __builtin_shufflevector(ds_read_tr(p), ds_read_tr(p + 8 * R::STRIDE), 0, 1, 2, 3, 4, 5, 6, 7);
-            sums.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, hi[u], sums.o[d], 0, 0, 0);
-            sums.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, lo[u], sums.o[d], 0, 0, 0);
-            if constexpr (R::PARTS == 2) {
-                const uint8_t* q = p + 32 * N * R::STRIDE;
-                const half8 vl = __builtin_shufflevector(ds_read_tr(q), ds_read_tr(q + 8 * R::STRIDE), 0, 1, 2, 3, 4, 5, 6, 7);
-                sums.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, hi[u], sums.o[d], 0, 0, 0);
-            }
+        for (int part = 0; part < R::PARTS; ++part) {
+            const uint8_t* q = p + part * 32 * N * R::STRIDE;
+            v[i & 1][part] = __builtin_shufflevector(ds_read_tr(q), ds_read_tr(q + 8 * R::STRIDE), 0, 1, 2, 3, 4, 5, 6, 7);
         }
+    };
+    if (AHEAD) fetch(0);
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+        const int u = i / DB, d = i % DB;
+        if (i + AHEAD < COUNT) fetch(i + AHEAD);
+        sums.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 1][0], hi[u], sums.o[d], 0, 0, 0);
+        sums.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 1][0], lo[u], sums.o[d], 0, 0, 0);
+        if constexpr (R::PARTS == 2) sums.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 1][R::PARTS - 1], hi[u], sums.o[d], 0, 0, 0);
+    }
 }
 
 // the sum of weights, of both lanes of a place
@@ -303,24 +311,32 @@ struct Narrow {
 template <class T, int HD>
 __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Span<T>& s, int kvh, int part, Narrow<T, HD>& sh) {
     constexpr int STEPS = HD / 16;
-    constexpr bool F32 = sizeof(T) == 4, AHEAD = HD * sizeof(T) <= 256;   // registers for the next tile
+    constexpr bool F32 = sizeof(T) == 4, AHEAD = HD * sizeof(T) <= 128;   // registers for the next tile
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hh = lane >> 5;
     const Queries<HD> q(a, s, kvh, s.first + li);
     Sums<HD> sums;
     int ev = 20;   // F32 values: the exponent that the sums are scaled by
     uint8_t* vt = sh.lds + wave * Narrow<T, HD>::VBYTES;
     Raw8<T> kr[STEPS], vr[STEPS];
-    const auto load = [&](int k) {   // behind the last key the last one again: its weight is zero there
-        const T* kp = s.k + min(k + li, s.k1 - 1) * s.ldk + 8 * hh;
+    const int step = TILE * WAVES, kw = s.k0 + TILE * wave;
+    const int key = lane / (HD / 8), col = 8 * (lane % (HD / 8));   // of the first 64 pieces of values
+    const T *kp = s.k + (kw + li) * s.ldk + 8 * hh, *vp = s.v + (kw + key) * s.ldv + col;
+    const auto load = [&](int k) {
+        if (k + TILE <= s.k1) {
 #pragma unroll
-        for (int t = 0; t < STEPS; ++t) kr[t].load(kp + 16 * t);
+            for (int t = 0; t < STEPS; ++t) kr[t].load(kp + 16 * t);
 #pragma unroll
-        for (int t = 0; t < STEPS; ++t) {
-            const int f = t * 64 + lane;
-            vr[t].load(s.v + min(k + f / (HD / 8), s.k1 - 1) * s.ldv + 8 * (f % (HD / 8)));
+            for (int t = 0; t < STEPS; ++t) vr[t].load(vp + t * (512 / HD) * s.ldv);
+            kp += step * s.ldk;
+            vp += step * s.ldv;
+        } else {   // behind the last key the last one again: its weight is zero there
+            const T* last = s.k + min(k + li, s.k1 - 1) * s.ldk + 8 * hh;
+#pragma unroll
+            for (int t = 0; t < STEPS; ++t) kr[t].load(last + 16 * t);
+#pragma unroll
+            for (int t = 0; t < STEPS; ++t) vr[t].load(s.v + min(k + key + t * (512 / HD), s.k1 - 1) * s.ldv + col);
         }
     };
-    const int step = TILE * WAVES, kw = s.k0 + TILE * wave;
     if (AHEAD && kw < s.k1) load(kw);
     for (int k = kw; k < s.k1; k += step) {
         if (!AHEAD) load(k);
@@ -434,13 +450,25 @@ __device__ __forceinline__ void attend_wide(const PrefixAttnArgs& a, const Span<
     Sums<HD> sums;
     int ev = 20;
     Raw8<T> kr[PIECES], vr[PIECES];
+    // this thread's piece of the first 256; the others are whole rows of keys on
+    const int key = tid / (HD / 8), col = 8 * (tid % (HD / 8));
+    const T *kp = s.k + (s.k0 + key) * s.ldk + col, *vp = s.v + (s.k0 + key) * s.ldv + col;
     const auto load = [&](int k) {
+        if (k + 64 <= s.k1) {
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int f = tid + 256 * i;
-            const int64_t key = min(k + f / (HD / 8), s.k1 - 1), col = 8 * (f % (HD / 8));
-            kr[i].load(s.k + key * s.ldk + col);
-            vr[i].load(s.v + key * s.ldv + col);
+            for (int i = 0; i < PIECES; ++i) {
+                kr[i].load(kp + i * (2048 / HD) * s.ldk);
+                vr[i].load(vp + i * (2048 / HD) * s.ldv);
+            }
+            kp += 64 * s.ldk;
+            vp += 64 * s.ldv;
+        } else {   // behind the last key the last one again: its weight is zero there
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int64_t at = min(k + key + i * (2048 / HD), s.k1 - 1);
+                kr[i].load(s.k + at * s.ldk + col);
+                vr[i].load(s.v + at * s.ldv + col);
+            }
         }
     };
     load(s.k0);
@@ -538,17 +566,20 @@ __device__ __forceinline__ bool find_tile(const PrefixAttnArgs& a, int t, int& r
     return false;
 }
 
-// Grid: the prefix part's workgroups, then the own parts'.  Workgroups are
+// Grid: the prefix part's workgroups and the own parts'.  Workgroups are
 // dispatched round-robin over the 8 XCDs: the prefix part's are numbered so
 // that the query tiles that read the same keys run one behind the other on
 // one XCD and share its L2.
 template <class T, int HD, bool WIDE>
-__global__ __launch_bounds__(64 * WAVES) void prefix_attn_kernel(PrefixAttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, 2) void prefix_attn_kernel(PrefixAttnArgs a) {
     union Shared {
         Narrow<T, HD> narrow;
         Wide<T, HD> wide;
     };
     __shared__ typename std::conditional<WIDE, Shared, Narrow<T, HD>>::type sh;
+    // The prefix part first: behind its products the own parts fill the CUs
+    // that end early (in turn with them 60 us against 50 for 8 prompts of 201
+    // queries on 5184 keys, 44 against 33 for ragged causal requests).
     int w = blockIdx.x;
     Span<T> s;
     if (w < a.prefix_groups) {
@@ -661,18 +692,32 @@ void launch_typed(const PrefixAttnArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-// Two workgroups per CU where the keys allow splits of 256.
-void prefix_attn_plan(PrefixAttnArgs& a, int cus) {
-    const auto splits = [&](int64_t groups, int64_t keys) {
-        return int(std::max<int64_t>(1, std::min<int64_t>((2 * cus + groups - 1) / groups, (keys + 255) / 256)));
+void prefix_attn_plan(PrefixAttnArgs& a, int head_dim, int cus) {
+    // The number of key splits for `groups` workgroups a split.  A CU takes
+    // ceil(workgroups / CUs) of them, each with its tiles of `step` keys and about
+    // three tiles' time to begin and end; one alone reaches some 60 % of
+    // what three together do, two 85 %.  A split costs its partial sums' way
+    // to memory and back, 3 TB/s, where a tile takes 0.5 us + 6 ns a dimension.
+    const auto splits = [&](int64_t groups, int64_t keys, int step) {
+        const int most = int(std::max<int64_t>(1, std::min<int64_t>((keys + 255) / 256, (4 * cus + groups - 1) / groups)));
+        const double tile_us = 0.5 + 0.006 * head_dim, split_us = double(a.rows) * a.heads * head_dim * 8 / 3e6;
+        int best = 1;
+        double least = 0;
+        for (int n = 1; n <= most; ++n) {
+            const int64_t per_cu = (groups * n + cus - 1) / cus, tiles = (keys + int64_t(n) * step - 1) / (int64_t(n) * step);
+            const double rate = per_cu == 1 ? 0.6 : per_cu == 2 ? 0.85 : 1.0;
+            const double us = per_cu * (tiles + 3) / rate * tile_us + (n > 1 ? n * split_us : 0.0);
+            if (n == 1 || us < least) best = n, least = us;
+        }
+        return best;
     };
-    const auto chunk = [](int64_t keys, int n) { return int(((keys + n - 1) / n + TILE * WAVES - 1) / (TILE * WAVES) * (TILE * WAVES)); };
+    const auto chunk = [](int64_t keys, int n) { return int(((keys + n - 1) / n + 63) / 64 * 64); };
     a.group = a.heads / a.kv_heads;
     const int64_t places = int64_t(a.rows) * a.group;
     a.wide = a.prefix && places > 2 * TILE;
-    const int tile = a.wide ? TILE * WAVES : TILE;
+    const int tile = a.wide ? TILE * WAVES : TILE, step = a.wide ? 64 : TILE * WAVES;
     a.prefix_tiles = a.prefix ? int((places + tile - 1) / tile) : 0;
-    a.prefix_splits = a.prefix ? splits(int64_t(a.prefix_tiles) * a.kv_heads, a.prefix) : 0;
+    a.prefix_splits = a.prefix ? splits(int64_t(a.prefix_tiles) * a.kv_heads, a.prefix, step) : 0;
     a.prefix_groups = 0;
     if (a.prefix) {
         a.prefix_chunk = chunk(a.prefix, a.prefix_splits);
@@ -682,7 +727,7 @@ void prefix_attn_plan(PrefixAttnArgs& a, int cus) {
     // without a prefix the own parts write every row, an empty one as zeros
     const bool own = a.own_max > 0 || !a.prefix;
     a.own_tiles = own ? int(places / TILE + std::min<int64_t>(a.requests, a.rows)) : 0;
-    a.own_splits = own ? splits(int64_t(a.own_tiles) * a.kv_heads, a.own_max) : 0;
+    a.own_splits = own ? splits(int64_t(a.own_tiles) * a.kv_heads, a.own_max, TILE * WAVES) : 0;
     if (own) {
         a.own_chunk = std::max(chunk(a.own_max, a.own_splits), TILE);
         a.own_splits = std::max(1, (a.own_max + a.own_chunk - 1) / a.own_chunk);
