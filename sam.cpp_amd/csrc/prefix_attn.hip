@@ -221,11 +221,13 @@ struct Sums {
 };
 
 // A tile of KEYS keys or values of HD as fp16 rows in LDS, F32 ones as hi
-// and, behind them, lo; 16 bytes of padding a row spread the rows' reads over
-// the banks.
-template <class T, int HD, int KEYS>
+// and, behind them, lo.  Keys are read 16 bytes a row from 16 rows at once,
+// values (V) 64 bytes a row from 4: the rows' padding spreads either over the
+// 64 banks.
+template <class T, int HD, int KEYS, bool V>
 struct TileRows {
-    static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, STRIDE = HD * 2 + 16, BYTES = KEYS * STRIDE * PARTS;
+    static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, STRIDE = !V ? HD * 2 + 16 : HD == 32 ? 64 : HD * 2 + 64;
+    static constexpr int BYTES = KEYS * STRIDE * PARTS;
     // piece f (8 values) of the tile
     static __device__ __forceinline__ void put(uint8_t* tile, int f, const Raw8<T>& raw, float factor) {
         half8* to = reinterpret_cast<half8*>(tile + f / (HD / 8) * STRIDE + f % (HD / 8) * 16);
@@ -243,7 +245,7 @@ struct TileRows {
 // sc[n] += K Q^T of keys 32n .. + 31 of a tile of keys in LDS
 template <class T, int HD, int N>
 __device__ __forceinline__ void scores(const uint8_t* kt, const Queries<HD>& q, floatx16 (&sc)[N]) {
-    typedef TileRows<T, HD, 32 * N> R;
+    typedef TileRows<T, HD, 32 * N, false> R;
     const int lane = threadIdx.x & 63, li = lane & 31, hh = lane >> 5;
     const uint8_t* at = kt + li * R::STRIDE + 16 * hh;
 #pragma unroll
@@ -268,7 +270,7 @@ __device__ __forceinline__ void scores(const uint8_t* kt, const Queries<HD>& q, 
 // keys 4hh .. + 3 and 8 + 4hh .. + 3 of both operands, V^T read transposed.
 template <class T, int HD, int N>
 __device__ __forceinline__ void values(const uint8_t* vt, const half8 (&hi)[2 * N], const half8 (&lo)[2 * N], Sums<HD>& sums) {
-    typedef TileRows<T, HD, 32 * N> R;
+    typedef TileRows<T, HD, 32 * N, true> R;
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     const uint8_t* at = vt + (4 * hh + ((lane & 15) >> 2)) * R::STRIDE + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
     constexpr int DB = HD / 32, COUNT = 2 * N * DB, AHEAD = HD < 128 ? 1 : 0;   // 128: no registers left
@@ -303,7 +305,7 @@ __device__ __forceinline__ float pair_sum(float l) {
 // other wave touches.
 template <class T, int HD>
 struct Narrow {
-    static constexpr int VBYTES = TileRows<T, HD, 32>::BYTES, OBYTES = TILE * (HD + 4) * 4;   // a wave's tile, and its sums at the end
+    static constexpr int VBYTES = TileRows<T, HD, 32, true>::BYTES, OBYTES = TILE * (HD + 4) * 4;   // a wave's tile, and its sums at the end
     uint8_t __attribute__((aligned(16))) lds[WAVES * (VBYTES > OBYTES ? VBYTES : OBYTES)];
     float m[WAVES][TILE], l[WAVES][TILE], total[TILE];
 };
@@ -372,7 +374,7 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
         }
         wave_lds_handoff();   // the last tile's reads came first
 #pragma unroll
-        for (int t = 0; t < STEPS; ++t) TileRows<T, HD, 32>::put(vt, t * 64 + lane, vr[t], down(ev));
+        for (int t = 0; t < STEPS; ++t) TileRows<T, HD, 32, true>::put(vt, t * 64 + lane, vr[t], down(ev));
         wave_lds_handoff();
         if (AHEAD && k + step < s.k1) load(k + step);
         half8 ph[2], pl[2];
@@ -406,7 +408,7 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
     if (wave == 0 && hh == 0) {
         sh.total[li] = l;
         if (part >= 0 && q.mine) {
-            float* ml = a.part_ml + (int64_t(part) * a.rows * a.heads + int64_t(q.row) * a.heads + q.head) * 2;
+            float* ml = a.part_ml + ((int64_t(q.row) * a.heads + q.head) * a.parts + part) * 2;
             ml[0] = m;
             ml[1] = l;
         }
@@ -424,7 +426,7 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
             const float lt = sh.total[p], inv = lt == 0.f ? 0.f : 1.f / lt;
             *reinterpret_cast<float4_at*>(a.out + r * a.ldo + h * HD + d) = v * inv;
         } else {
-            *reinterpret_cast<floatx4*>(a.part_o + ((int64_t(part) * a.rows + r) * a.heads + h) * HD + d) = v;
+            *reinterpret_cast<floatx4*>(a.part_o + ((r * a.heads + h) * a.parts + part) * HD + d) = v;
         }
     }
 }
@@ -434,8 +436,8 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
 // tile's products.
 template <class T, int HD>
 struct Wide {
-    uint8_t __attribute__((aligned(16))) k[TileRows<T, HD, 64>::BYTES];
-    uint8_t __attribute__((aligned(16))) v[TileRows<T, HD, 64>::BYTES];
+    uint8_t __attribute__((aligned(16))) k[TileRows<T, HD, 64, false>::BYTES];
+    uint8_t __attribute__((aligned(16))) v[TileRows<T, HD, 64, true>::BYTES];
     uint32_t largest[WAVES][2];
 };
 
@@ -497,8 +499,8 @@ __device__ __forceinline__ void attend_wide(const PrefixAttnArgs& a, const Span<
         }
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            TileRows<T, HD, 64>::put(sh.k, tid + 256 * i, kr[i], fk);
-            TileRows<T, HD, 64>::put(sh.v, tid + 256 * i, vr[i], down(ev));
+            TileRows<T, HD, 64, false>::put(sh.k, tid + 256 * i, kr[i], fk);
+            TileRows<T, HD, 64, true>::put(sh.v, tid + 256 * i, vr[i], down(ev));
         }
         __syncthreads();
         if (k + 64 < s.k1) load(k + 64);
@@ -518,7 +520,7 @@ __device__ __forceinline__ void attend_wide(const PrefixAttnArgs& a, const Span<
         f = l == 0.f ? 0.f : f / l;
         to = a.out + q.row * a.ldo + q.head * HD;
     } else {
-        const int64_t at = int64_t(part) * a.rows * a.heads + int64_t(q.row) * a.heads + q.head;
+        const int64_t at = (int64_t(q.row) * a.heads + q.head) * a.parts + part;
         to = a.part_o + at * HD;
         if (hh == 0) {
             a.part_ml[2 * at] = sums.m;
@@ -647,7 +649,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(PrefixAttnArgs a) {
     for (int p0 = 0; p0 < a.parts; p0 += 64) {
         float mp = -__builtin_inff(), lp = 0.f;
         if (p0 + lane < a.parts) {
-            const float* ml = a.part_ml + ((p0 + lane) * items + item) * 2;
+            const float* ml = a.part_ml + (item * a.parts + p0 + lane) * 2;
             mp = ml[0];
             lp = ml[1];
         }
@@ -658,21 +660,26 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(PrefixAttnArgs a) {
         l = l * old + wave_sum(lp * f);
         v = v * old;
         const int here = min(a.parts - p0, 64);
-        for (int p1 = 0; p1 < here; p1 += 4 * AT_ONCE) {
-            floatx4 o[4];
-            float fp[4];
+        const float* parts = a.part_o + (item * a.parts + p0) * HD + d;
+        const auto add = [&](auto count, int p1) {   // parts p1 + slot, p1 + slot + AT_ONCE, ..
+            constexpr int U = decltype(count)::value;
+            floatx4 o[U];
+            float fp[U];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < U; ++u) {
                 const int p = p1 + u * AT_ONCE + slot, at = min(p, here - 1);
-                o[u] = *reinterpret_cast<const floatx4*>(a.part_o + ((p0 + at) * items + item) * HD + d);
+                o[u] = *reinterpret_cast<const floatx4*>(parts + at * HD);
                 fp[u] = __shfl(f, at, 64);
                 if (p >= here) fp[u] = 0.f;
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[j] += fp[u] != 0.f ? o[u][j] * fp[u] : 0.f;   // without keys its sums may never have been written
-        }
+        };
+        int p1 = 0;
+        for (; p1 + 3 * AT_ONCE < here; p1 += 4 * AT_ONCE) add(std::integral_constant<int, 4>{}, p1);
+        for (; p1 < here; p1 += AT_ONCE) add(std::integral_constant<int, 1>{}, p1);
     }
 #pragma unroll
     for (int off = QUADS; off < 64; off <<= 1)
