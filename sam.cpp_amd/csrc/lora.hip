@@ -31,21 +31,50 @@ __device__ __forceinline__ void st4(float* p, floatx4 v, bool past_cache) {
     else *reinterpret_cast<float4_at*>(p) = v;
 }
 
-// p[0 .. 4) as floats; with `left`, those at or behind it zero and not read
 typedef _Float16 half4_at __attribute__((ext_vector_type(4), aligned(2)));
 __device__ __forceinline__ floatx4 take4(const float* p) { return ld4(p); }
 __device__ __forceinline__ floatx4 take4(const _Float16* p) {
     const half4_at h = *reinterpret_cast<const half4_at*>(p);
     return floatx4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
 }
-template <class T>
-__device__ __forceinline__ floatx4 take4(const T* p, int left) {
+// v[off ..], zeros behind
+template <int N, class V>
+__device__ __forceinline__ V shift_down(V v, int off) {
+#pragma unroll
+    for (int s = 1; s < N; s *= 2)
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = off & s ? (j + s < N ? v[j + s] : 0) : v[j];
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = off >= N ? 0 : v[j];
+    return v;
+}
+// row[n .. n + 4) as floats, those at or behind `end` zero and not read.  A
+// branch around a load has it waited for at once, so how a group of loads is
+// done is chosen outside of it: WHOLE reads them as they are, SHIFTED (end at
+// least 4) the last whole vector again, shifted, GUARDED one by one.
+enum class Edge { WHOLE, SHIFTED, GUARDED };
+template <Edge E, class T>
+__device__ __forceinline__ floatx4 take4(const T* row, int n, int end) {
+    if constexpr (E == Edge::WHOLE) return take4(row + n);
+    if constexpr (E == Edge::SHIFTED) {
+        const int at = min(n, end - 4);
+        return shift_down<4>(take4(row + at), n - at);
+    }
     floatx4 v{0.f, 0.f, 0.f, 0.f};
-    if (left >= 4) return take4(p);
 #pragma unroll
     for (int j = 0; j < 3; ++j)
-        if (j < left) v[j] = (float)p[j];
+        if (n + j < end) v[j] = (float)row[n + j];
     return v;
+}
+template <Edge E>
+struct EdgeTag {
+    static constexpr Edge value = E;
+};
+template <class Body>
+__device__ __forceinline__ void with_edge(bool whole, int end, Body body) {   // uniform
+    if (whole) body(EdgeTag<Edge::WHOLE>{});
+    else if (end >= 4) body(EdgeTag<Edge::SHIFTED>{});
+    else body(EdgeTag<Edge::GUARDED>{});
 }
 
 __device__ __forceinline__ floatx4 mfma(float a, float b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
@@ -182,19 +211,26 @@ struct Stage {
             for (int i = 0; i < XN; ++i) x[i] = ld4(xp[i] + k);
 #pragma unroll
             for (int i = 0; i < AN; ++i) w[i] = *reinterpret_cast<const vec_at*>(wp[i] + k);
-        } else {
+        } else if (k1 >= VA) {   // the last whole vector again, shifted
 #pragma unroll
-            for (int i = 0; i < XN; ++i) x[i] = take4(xp[i] + k, k1 - (k + (threadIdx.x + i * THREADS) % XC * 4));
+            for (int i = 0; i < XN; ++i) {
+                const int over = max(k + int(threadIdx.x + i * THREADS) % XC * 4 + 4 - k1, 0);
+                x[i] = shift_down<4>(ld4(xp[i] + k - over), over);
+            }
 #pragma unroll
             for (int i = 0; i < AN; ++i) {
-                const int left = k1 - (k + (threadIdx.x + i * THREADS) % AC * VA);
-                if (left >= VA) {
-                    w[i] = *reinterpret_cast<const vec_at*>(wp[i] + k);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VA; ++j) w[i][j] = j < left ? wp[i][k + j] : (T)0;
-                }
+                const int over = max(k + int(threadIdx.x + i * THREADS) % AC * VA + VA - k1, 0);
+                w[i] = shift_down<VA>(*reinterpret_cast<const vec_at*>(wp[i] + k - over), over);
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < XN; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[i][j] = k + int(threadIdx.x + i * THREADS) % XC * 4 + j < k1 ? xp[i][k + j] : 0.f;
+#pragma unroll
+            for (int i = 0; i < AN; ++i)
+#pragma unroll
+                for (int j = 0; j < VA; ++j) w[i][j] = k + int(threadIdx.x + i * THREADS) % AC * VA + j < k1 ? wp[i][k + j] : (T)0;
         }
     }
     __device__ __forceinline__ void store(Lds& l) const {
@@ -272,14 +308,14 @@ template <class T, int RT>
 __device__ __forceinline__ void take_b(const LoraArgs& a, const T* w, int n, int rank, floatx4 (&b)[RT]) {
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const T* row = w + min(n + r, a.n - 1) * a.b_row;
-    if (a.rank % 4 == 0) {   // whole vectors of the bank's row
+    with_edge(a.rank % 4 == 0, a.rank, [&](auto edge) {
+        constexpr Edge E = decltype(edge)::value;
 #pragma unroll
-        for (int i = 0; i < RT; ++i) b[i] = take4(row + min(16 * i + 4 * g, a.rank - 4));
-    } else {
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-            if (16 * i < rank) b[i] = take4(row + 16 * i + 4 * g, rank - (16 * i + 4 * g));
-    }
+        for (int i = 0; i < RT; ++i) {
+            const int at = 16 * i + 4 * g;
+            b[i] = take4<E>(row, E == Edge::WHOLE ? min(at, a.rank - 4) : at, a.rank);
+        }
+    });
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -298,9 +334,6 @@ __device__ __forceinline__ void up(int rank, const floatx4 (&b)[RT], const float
                 for (int s = 0; s < SUB; ++s) acc[s] = mfma(b[i][j], t[s][i][j], acc[s]);
 }
 
-__device__ __forceinline__ floatx4 base4(const LoraArgs& a, int64_t row, int n) {
-    return a.base ? take4(a.base + row * a.ldbase + n, a.n - n) : floatx4{0.f, 0.f, 0.f, 0.f};
-}
 __device__ __forceinline__ void put4(const LoraArgs& a, int64_t row, int n, floatx4 v) {
     float* y = a.y + row * a.ldy + n;
     if (n + 4 <= a.n) {
@@ -328,13 +361,14 @@ __global__ __launch_bounds__(512) void lora_fused_kernel(LoraArgs a) {
     const bool mine = row >= 0;
     const int64_t at = max(row, 0);
     floatx4 base[2];   // under way during the products
-    const int64_t any = mine ? at : tile.rows[0];
-    const bool whole = n0 + 32 <= a.n;
+    if (a.base) {
+        const float* from = a.base + (mine ? at : tile.rows[0]) * a.ldbase;
+        with_edge(n0 + 32 <= a.n, a.n, [&](auto edge) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        const int n = n0 + 16 * c + 4 * g;
-        if (whole && a.base) base[c] = ld4(a.base + any * a.ldbase + n);
-        else base[c] = base4(a, any, n);
+            for (int c = 0; c < 2; ++c) base[c] = take4<decltype(edge)::value>(from, n0 + 16 * c + 4 * g, a.n);
+        });
+    } else {
+        base[0] = base[1] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
     if (slot < a.slots) {
         const int rank = slot_rank(a, slot);
@@ -414,7 +448,7 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
 // through LDS, so that base and y move in whole KB of a row, and the next
 // block's base is under way as soon as this one's is used.
 template <class T, int RT, int SUB>
-__global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
+__global__ __launch_bounds__(256, RT <= 2 ? 3 : RT <= 4 ? 2 : 1) void lora_up_kernel(LoraArgs a) {
     constexpr int TR = 16 * SUB, PITCH = 256 + 4, OWN = TR / 4;   // rows that a wave moves
     __shared__ __attribute__((aligned(16))) float sums[TR][PITCH];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
@@ -428,11 +462,17 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
 #pragma unroll
     for (int i = 0; i < OWN; ++i) row[i] = __builtin_amdgcn_readfirstlane(tile[OWN * wave + i]);
     const bool whole = row[OWN - 1] >= 0;   // rows fill from the front
-    const auto fetch = [&](int i, int n) {
-        base[i] = row[i] >= 0 && n < n1 ? base4(a, block0 + row[i], n) : floatx4{0.f, 0.f, 0.f, 0.f};
-    };
 #pragma unroll
-    for (int i = 0; i < OWN; ++i) fetch(i, n0 + 4 * lane);
+    for (int i = 0; i < OWN; ++i) base[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    const auto fetch = [&](int nb) {   // an absent row's place gets the block's first
+        if (a.base)
+            with_edge(nb + 256 <= a.n, a.n, [&](auto edge) {
+#pragma unroll
+                for (int i = 0; i < OWN; ++i)
+                    base[i] = take4<decltype(edge)::value>(a.base + (block0 + max(row[i], 0)) * a.ldbase, nb + 4 * lane, a.n);
+            });
+    };
+    fetch(n0);
     const bool product = slot < a.slots;
     const int rank = product ? slot_rank(a, slot) : 0;
     const T* B = static_cast<const T*>(a.b) + (product ? slot : 0) * a.b_slot;
@@ -495,18 +535,13 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
                 for (int i = 0; i < 4; ++i) st4(a.y + (block0 + row[i0 + i]) * a.ldy + n, v[i], a.past_cache);
             }
         } else {
+            floatx4 v[OWN];
 #pragma unroll
-            for (int i0 = 0; i0 < OWN; i0 += 4) {
-                floatx4 v[4];
+            for (int i = 0; i < OWN; ++i) v[i] = sum_of(i);
+            if (nb + 256 < n1) fetch(nb + 256);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[i] = sum_of(i0 + i);
-                    fetch(i0 + i, n + 256);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (row[i0 + i] >= 0 && n < n1) put4(a, block0 + row[i0 + i], n, v[i]);
-            }
+            for (int i = 0; i < OWN; ++i)
+                if (row[i] >= 0 && n < n1) put4(a, block0 + row[i], n, v[i]);
         }
     }
 }
@@ -552,7 +587,13 @@ void lora_plan(LoraArgs& a, int cus) {
     const auto tiles_of = [&](int64_t rows, int tile) { return int(std::min<int64_t>(rows, rows / tile + a.slots + 1)); };
     // past one block's rows, blocks of a quarter: a tile is found sooner
     const int64_t few = a.m > kLoraBlockRows ? kLoraBlockRows / 4 : a.m;
-    a.fused = a.rank <= 32 && a.m <= kLoraBlockRows && int64_t(tiles_of(few, 16)) * columns <= cus;
+    // One launch where a workgroup for every tile and block of columns fits a
+    // CU and K takes at most four chunks, so that a second launch costs more
+    // than doing A x again for each block: 16 tokens 1024 -> 1024 10.4 -> 6.4
+    // us; 777 rows 1001 -> 1359 of rank 40 (438 workgroups of eight chunks)
+    // 28.3 fused, 18.7 in two.
+    const int rank_tiles = a.rank <= 16 ? 1 : a.rank <= 32 ? 2 : 4;
+    a.fused = a.rank <= 64 && a.m <= kLoraBlockRows && int64_t(tiles_of(few, 16)) * columns <= cus && a.k <= 2048 / rank_tiles;
     a.tile_rows = !a.fused && a.rank <= 128 && a.m >= 16 * cus ? 32 : 16;
     a.block_rows = int(few);
     a.block_tiles = tiles_of(few, a.tile_rows);

@@ -251,6 +251,19 @@ public:
         check_status(samhip_get_rows(ctx_, &src, &ids, &dst));
     }
 
+    // The operators of a batch of requests on one image (no ggml nodes):
+    // adapters added to a product, attention to a shared prefix, group norm
+    // of channels-last maps.
+    void lora_add(const samhip_lora_bank& bank, const samhip_tensor& x, const samhip_tensor& ids, const samhip_tensor* base,
+                  const samhip_tensor& y) {
+        check_status(samhip_lora_add(ctx_, &bank, &x, &ids, base, &y));
+    }
+    void prefix_attn(const samhip_prefix_attn_desc& desc) { check_status(samhip_prefix_attn(ctx_, &desc)); }
+    void group_norm(const samhip_tensor& x, const samhip_tensor& y, int32_t groups, const float* w, const float* b, float eps,
+                    samhip_activation activation = SAMHIP_ACT_NONE) {
+        check_status(samhip_group_norm(ctx_, &x, &y, groups, w, b, eps, activation));
+    }
+
 private:
     HipBackend(samhip_context* ctx, int device, HipComputeMode compute) : ctx_(ctx), device_(device), compute_(compute) {}
     void reset() {
