@@ -195,7 +195,7 @@ typedef struct samhip_lora_bank {
 /* x: F32 {K, M}; ids: device I32 {M}, in any order; base: F32 {N, M}, NULL
  * for zeros, may be y itself (same data and row stride); y: F32 {N, M}.  A
  * row whose id is not in [0, slots) gets base alone; ranks are cut to
- * [0, R].  Products and sums in F32.  ids, ranks, scales and the banks are
+ * [0, R].  y overlaps no other operand.  Products and sums in F32.  ids, ranks, scales and the banks are
  * read on the device, at every replay of a captured call too, so slots can be
  * refilled and requests moved between replays.  May be captured. */
 int samhip_supports_lora_add(const samhip_lora_bank* bank, const samhip_tensor* x, const samhip_tensor* ids,
@@ -362,7 +362,7 @@ int samhip_flash_attn(samhip_context* ctx, const float* q, const float* k, const
  * The three tables are read on the device (at every replay of a captured
  * call) and cut to what exists: query rows to [0, rows), lengths to
  * [0, own_max] and the rows of own_k; an own_start outside them means no
- * keys.  q_start must not decrease. */
+ * keys.  q_start must not decrease.  out overlaps no other operand. */
 typedef struct samhip_prefix_attn_desc {
     int32_t version;                  /* SAMHIP_ABI_VERSION */
     int32_t heads, kv_heads;          /* heads a multiple of kv_heads */
@@ -398,8 +398,9 @@ enum samhip_activation {
  * mean and biased variance over the channels / groups neighbouring channels
  * of a group in every pixel of one image (sums in F64).  w, b: device F32
  * [channels], each may be NULL.  channels a multiple of groups, at most 4096;
- * images at most 65535.  y may be x itself (same type and strides).  A
- * non-finite value makes its group's outputs non-finite.  May be captured. */
+ * images at most 65535.  y may be x itself (same type and strides), and
+ * overlaps nothing else.  A non-finite value makes its group's outputs
+ * non-finite.  May be captured. */
 int samhip_supports_group_norm(const samhip_tensor* x, const samhip_tensor* y, int32_t groups, const float* w,
                                const float* b, float eps, int32_t activation);   /* 1 if group_norm takes these, else 0 */
 int samhip_group_norm(samhip_context* ctx, const samhip_tensor* x, const samhip_tensor* y, int32_t groups,

@@ -271,22 +271,17 @@ __device__ __forceinline__ void multiply(const Lds& l, int sub, int first, int s
 // Over [k0, k1), every chunk
 template <class T, int THREADS, int TR, int RT, int KC, int UNITS>
 __device__ __forceinline__ void down(const LoraArgs& a, typename Stage<T, THREADS, TR, RT, KC>::Lds& lds, int64_t block0, const int* rows, const T* A,
-                                     int rank, int k0, int k1, int turn, int sub, int first, int step, floatx4 (&acc)[RT]) {
+                                     int rank, int k0, int k1, int sub, int first, int step, floatx4 (&acc)[RT]) {
     Stage<T, THREADS, TR, RT, KC> stage(a, block0, rows, A, rank);
     const int tiles = (rank + 15) / 16;
 #pragma unroll
     for (int i = 0; i < RT; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-    // `turn`: the chunk to begin with.  Rows of a power of two apart would have
-    // all workgroups at the same few memory channels, chunk after chunk.
-    const int chunks = max((k1 - k0 + KC - 1) / KC, 0);
-    int c = chunks ? turn % chunks : 0;
-    if (chunks) stage.load(k0 + c * KC, k1);
-    for (int i = 0; i < chunks; ++i) {
-        if (i) __syncthreads();   // the last chunk is read
+    if (k0 < k1) stage.load(k0, k1);
+    for (int k = k0; k < k1; k += KC) {
+        if (k != k0) __syncthreads();   // the last chunk is read
         stage.store(lds);
         __syncthreads();
-        c = c + 1 < chunks ? c + 1 : 0;
-        if (i + 1 < chunks) stage.load(k0 + c * KC, k1);
+        if (k + KC < k1) stage.load(k + KC, k1);
         multiply<RT, UNITS>(lds, sub, first, step, tiles, acc);
     }
 }
@@ -375,7 +370,7 @@ __global__ __launch_bounds__(512) void lora_fused_kernel(LoraArgs a) {
         floatx4 t[1][RT], b[2][RT];
 #pragma unroll
         for (int c = 0; c < 2; ++c) take_b<T, RT>(a, static_cast<const T*>(a.b) + slot * a.b_slot, n0 + 16 * c, rank, b[c]);
-        down<T, 512, 16, RT, KC, KC / 128>(a, lds, 0, tile.rows, static_cast<const T*>(a.a) + slot * a.a_slot, rank, 0, a.k, 0, 0, wave, 8, t[0]);
+        down<T, 512, 16, RT, KC, KC / 128>(a, lds, 0, tile.rows, static_cast<const T*>(a.a) + slot * a.a_slot, rank, 0, a.k, 0, wave, 8, t[0]);
 #pragma unroll
         for (int i = 0; i < RT; ++i) red[wave][i][lane] = t[0][i];
         __syncthreads();
@@ -423,7 +418,7 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
     const int k0 = blockIdx.z * a.k_len, k1 = min(a.k, k0 + a.k_len);
     const int sub = wave % SUB, part = wave / SUB;   // a part past SHARE does another's work again, unused
     floatx4 acc[RT];
-    down<T, 256, TR, RT, KC, UNITS>(a, lds, block0, tile.rows, static_cast<const T*>(a.a) + slot * a.a_slot, rank, k0, k1, blockIdx.x, sub,
+    down<T, 256, TR, RT, KC, UNITS>(a, lds, block0, tile.rows, static_cast<const T*>(a.a) + slot * a.a_slot, rank, k0, k1, sub,
                                     part % SHARE, SHARE, acc);
     if (part && part < SHARE) {
 #pragma unroll

@@ -710,12 +710,16 @@ void prefix_attn_plan(PrefixAttnArgs& a, int head_dim, int cus) {
         const double tile_us = 0.5 + 0.006 * head_dim, split_us = double(a.rows) * a.heads * head_dim * 8 / 3e6;
         int best = 1;
         double least = 0;
-        for (int n = 1; n <= most; ++n) {
+        const auto consider = [&](int64_t candidate) {
+            const int n = int(std::max<int64_t>(1, std::min<int64_t>(candidate, most)));
             const int64_t per_cu = (groups * n + cus - 1) / cus, tiles = (keys + int64_t(n) * step - 1) / (int64_t(n) * step);
             const double rate = per_cu == 1 ? 0.6 : per_cu == 2 ? 0.85 : 1.0;
             const double us = per_cu * (tiles + 3) / rate * tile_us + (n > 1 ? n * split_us : 0.0);
-            if (n == 1 || us < least) best = n, least = us;
-        }
+            if (least == 0 || us < least) best = n, least = us;
+        };
+        for (int per_cu = 4; per_cu >= 1; --per_cu) consider(int64_t(per_cu) * cus / groups);   // the most that a level takes
+        for (int64_t n = cus / groups / 2; n >= 1; n /= 2) consider(n);
+        consider(1);
         return best;
     };
     const auto chunk = [](int64_t keys, int n) { return int(((keys + n - 1) / n + 63) / 64 * 64); };

@@ -64,7 +64,7 @@ def call(samhip, ctx, x, y, groups, w, b, eps, act):
 # loads of 1 or 4 channels per group), odd sizes, groups of one channel, one
 # group of all, more columns than a workgroup has threads
 SHAPES = [(1, 1, 1, 1), (1, 1, 8, 8), (2, 3, 6, 3), (1, 1296, 256, 8), (3, 1961, 345, 15), (1, 16385, 4, 4), (2, 16385, 5, 5), (1, 5184, 256, 8),
-          (2, 5000, 96, 1), (1, 300, 4096, 2), (3, 900, 1023, 3), (1, 4096, 2052, 9), (5, 777, 260, 65), (1, 65536, 1, 1)]
+          (2, 5000, 96, 1), (1, 300, 4096, 2), (3, 900, 1023, 3), (1, 4096, 2052, 9), (5, 777, 260, 65), (1, 65536, 1, 1), (2, 700, 4095, 7), (1500, 9, 24, 8), (1100, 3000, 6, 2)]
 
 
 @pytest.mark.gpu

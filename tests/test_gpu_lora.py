@@ -73,7 +73,7 @@ def ids_of(order, m, slots, g):
 
 CASES = [(1, 32, 32, 1, 1), (1, 1, 1, 1, 1), (3, 7, 5, 3, 2), (16, 1024, 1024, 16, 40), (17, 257, 65, 17, 3), (256, 1024, 4096, 16, 8),
          (201, 256, 2048, 33, 5), (777, 1001, 1359, 40, 24), (50, 4736, 1024, 128, 4), (33, 500, 258, 129, 2), (31, 96, 127, 256, 3),
-         (5184, 1024, 1024, 64, 2), (1500, 64, 4736, 8, 64)]
+         (5184, 1024, 1024, 64, 2), (1500, 64, 4736, 8, 64), (4100, 130, 259, 130, 3), (6000, 36, 50, 4, 3000), (4097, 66, 300, 2, 4096)]
 
 
 @pytest.mark.gpu
