@@ -42,14 +42,16 @@ __device__ __forceinline__ Vector<T> load(const T* p, int n, bool whole) {
     for (int e = 0; e < kVec<T>; ++e) v[e] = p[min(e, n - 1)];
     return v;
 }
-template <class T, int VEC>
-__device__ __forceinline__ void store(T* p, int n, const float (&v)[VEC], bool past_cache = false) {
+// PAST: past the caches (a template's argument: of two stores in the branches
+// of a condition the compiler makes an ordinary one).
+template <bool PAST, class T, int VEC>
+__device__ __forceinline__ void store(T* p, int n, const float (&v)[VEC]) {
     if (n == VEC) {
         Packed<T, VEC> r;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) r.v[e] = (T)v[e];   // F16: round to nearest even
         typedef T raw __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
-        if (past_cache) __builtin_nontemporal_store(r.v, reinterpret_cast<raw*>(p));
+        if constexpr (PAST) __builtin_nontemporal_store(r.v, reinterpret_cast<raw*>(p));
         else *reinterpret_cast<raw*>(p) = r.v;
         return;
     }
@@ -142,6 +144,20 @@ __device__ __forceinline__ float activate(int act, float v) {   // act is unifor
     return v;
 }
 
+// Gain and bias of channels c .. (`last` at most), all loads at once: a test
+// for null around each would have it waited for there.
+template <int VEC>
+__device__ __forceinline__ void gain_and_bias(const float* w, const float* b, int c, int last, float (&ww)[VEC], float (&bb)[VEC]) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) ww[e] = 1.f, bb[e] = 0.f;
+    if (w)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) ww[e] = w[min(c + e, last)];
+    if (b)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) bb[e] = b[min(c + e, last)];
+}
+
 // One workgroup per (image, group).  A thread keeps to one vector of the
 // group's channels and takes every rows-th pixel.
 template <class TI, class TO, int NV>
@@ -161,12 +177,7 @@ __global__ __launch_bounds__(1024) void group_norm_block_kernel(const TI* x, TO*
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] = load<TI>(xg + max(min(i, count - 1), 0) * x_step, n, whole);
     float ww[VEC], bb[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        const int ch = g * size + min(c + e, size - 1);
-        ww[e] = w ? w[ch] : 1.f;
-        bb[e] = b ? b[ch] : 0.f;
-    }
+    gain_and_bias<VEC>(w, b, g * size + c, g * size + size - 1, ww, bb);
     double sum = 0.0, sq = 0.0;
     {
         Run run{(float)v[0][0]};
@@ -200,7 +211,7 @@ __global__ __launch_bounds__(1024) void group_norm_block_kernel(const TI* x, TO*
         float o[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) o[e] = activate(act, __builtin_fmaf((float)v[i][e] - m.hi, ww[e], bb[e]));
-        store<TO, VEC>(yg + i * y_step, n, o);
+        store<false>(yg + i * y_step, n, o);
     }
 }
 
@@ -319,11 +330,11 @@ __global__ __launch_bounds__(256) void group_norm_finish_kernel(const double* __
 
 // `stats` is null where the workgroups finish the partial sums themselves.
 // The chunks in the other order: the last ones read are still in L2.
-template <class TI, class TO, bool SAME>
+template <class TI, class TO, bool SAME, bool PAST>
 __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* y, GroupNormShape s, int chunk,
                                                                const double* __restrict__ partial, int chunks, const Moments* __restrict__ stats,
                                                                const float* __restrict__ w, const float* __restrict__ b, float eps,
-                                                               int act, bool past_cache) {
+                                                               int act) {
     constexpr int VEC = kVec<TI>;
     __shared__ Moments shared[kGroupNormInline];
     __shared__ double lds[256][2];
@@ -341,7 +352,11 @@ __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* 
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = load<TI>(xi + col * VEC + min(p + u * rows, p1 - 1) * s.x_pixel, n, whole);
     };
-    if (some) fetch(col0, p0, v);   // under way while the sums are finished
+    float ww[VEC], bb[VEC];
+    if (some) {   // under way while the sums are finished
+        fetch(col0, p0, v);
+        gain_and_bias<VEC>(w, b, col0 * VEC, s.channels - 1, ww, bb);
+    }
     const Moments* moments_of = stats + int64_t(blockIdx.y) * s.groups;
     if (!stats) {
         finish(partial + int64_t(blockIdx.y) * chunks * s.groups * 2, chunks, s.groups, double(s.pixels) * size, eps, lds, shared);
@@ -349,7 +364,8 @@ __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* 
     }
     if (!some) return;
     for (int col = col0; col < cols; col += width) {
-        float hi[SAME ? 1 : VEC], ww[VEC], bb[VEC];
+        float hi[SAME ? 1 : VEC];
+        if (col != col0) gain_and_bias<VEC>(w, b, col * VEC, s.channels - 1, ww, bb);
         const int n = SAME ? VEC : min(s.channels - col * VEC, VEC);
         Moments m;
         if (SAME) {
@@ -358,13 +374,12 @@ __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* 
         }
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            const int c = min(col * VEC + e, s.channels - 1);
             if (!SAME) {
-                m = moments_of[c / size];
+                m = moments_of[min(col * VEC + e, s.channels - 1) / size];
                 hi[e] = m.hi;
             }
-            ww[e] = w ? w[c] * m.rstd : m.rstd;
-            bb[e] = (b ? b[c] : 0.f) - m.lo * ww[e];
+            ww[e] = ww[e] * m.rstd;
+            bb[e] = bb[e] - m.lo * ww[e];
         }
         if (col != col0) fetch(col, p0, v);
         for (int p = p0; p < p1; p += U * rows) {
@@ -378,7 +393,7 @@ __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* 
 #pragma unroll
                     for (int e = 0; e < VEC; ++e)
                         o[e] = activate(act, __builtin_fmaf((float)v[u][e] - hi[SAME ? 0 : e], ww[e], bb[e]));
-                    store<TO, VEC>(yi + col * VEC + q * s.y_pixel, n, o, past_cache);
+                    store<PAST>(yi + col * VEC + q * s.y_pixel, n, o);
                 }
             }
             if (more)
@@ -425,8 +440,13 @@ void launch_typed(const TI* x, TO* y, const GroupNormShape& s, const float* w, c
         stats = reinterpret_cast<Moments*>(partial + int64_t(s.images) * chunks * s.groups * 2);
         group_norm_finish_kernel<<<s.images, 256, 0, stream>>>(partial, chunks, s.groups, double(s.pixels) * size, eps, stats);
     }
-    if (same) group_norm_apply_kernel<TI, TO, true><<<apply_grid, 256, 0, stream>>>(x, y, s, apply_chunk, partial, chunks, stats, w, b, eps, act, past_cache);
-    else group_norm_apply_kernel<TI, TO, false><<<apply_grid, 256, 0, stream>>>(x, y, s, apply_chunk, partial, chunks, stats, w, b, eps, act, past_cache);
+#define SAMHIP_GN_APPLY(SAME, PAST) \
+    group_norm_apply_kernel<TI, TO, SAME, PAST><<<apply_grid, 256, 0, stream>>>(x, y, s, apply_chunk, partial, chunks, stats, w, b, eps, act)
+    if (same && past_cache) SAMHIP_GN_APPLY(true, true);
+    else if (same) SAMHIP_GN_APPLY(true, false);
+    else if (past_cache) SAMHIP_GN_APPLY(false, true);
+    else SAMHIP_GN_APPLY(false, false);
+#undef SAMHIP_GN_APPLY
 }
 
 }  // namespace

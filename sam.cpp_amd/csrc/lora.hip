@@ -26,8 +26,11 @@ namespace {
 typedef float float4_at __attribute__((ext_vector_type(4), aligned(4)));
 
 __device__ __forceinline__ floatx4 ld4(const float* p) { return *reinterpret_cast<const float4_at*>(p); }
-__device__ __forceinline__ void st4(float* p, floatx4 v, bool past_cache) {
-    if (past_cache) __builtin_nontemporal_store(v, reinterpret_cast<float4_at*>(p));
+// PAST: past the caches (a template's argument: of two stores in the branches
+// of a condition the compiler makes an ordinary one)
+template <bool PAST>
+__device__ __forceinline__ void st4(float* p, floatx4 v) {
+    if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<float4_at*>(p));
     else *reinterpret_cast<float4_at*>(p) = v;
 }
 
@@ -329,10 +332,11 @@ __device__ __forceinline__ void up(int rank, const floatx4 (&b)[RT], const float
                 for (int s = 0; s < SUB; ++s) acc[s] = mfma(b[i][j], t[s][i][j], acc[s]);
 }
 
+template <bool PAST>
 __device__ __forceinline__ void put4(const LoraArgs& a, int64_t row, int n, floatx4 v) {
     float* y = a.y + row * a.ldy + n;
     if (n + 4 <= a.n) {
-        st4(y, v, a.past_cache);
+        st4<PAST>(y, v);
     } else {
 #pragma unroll
         for (int j = 0; j < 3; ++j)
@@ -390,7 +394,7 @@ __global__ __launch_bounds__(512) void lora_fused_kernel(LoraArgs a) {
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c)
-        if (mine) put4(a, at, n0 + 16 * c + 4 * g, base[c]);
+        if (mine) put4<false>(a, at, n0 + 16 * c + 4 * g, base[c]);
 }
 
 // Grid: a block's tiles x blocks of rows x K splits.  The waves of a
@@ -442,7 +446,7 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
 // through its split in blocks of 256 columns, 64 to a wave; the sums pass
 // through LDS, so that base and y move in whole KB of a row, and the next
 // block's base is under way as soon as this one's is used.
-template <class T, int RT, int SUB>
+template <class T, int RT, int SUB, bool PAST>
 __global__ __launch_bounds__(256, RT <= 2 ? 3 : RT <= 4 ? 2 : 1) void lora_up_kernel(LoraArgs a) {
     constexpr int TR = 16 * SUB, PITCH = 256 + 4, OWN = TR / 4;   // rows that a wave moves
     __shared__ __attribute__((aligned(16))) float sums[TR][PITCH];
@@ -527,7 +531,7 @@ __global__ __launch_bounds__(256, RT <= 2 ? 3 : RT <= 4 ? 2 : 1) void lora_up_ke
                     if (a.base) base[i0 + i] = ld4(a.base + (block0 + row[i0 + i]) * a.ldbase + n + 256);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) st4(a.y + (block0 + row[i0 + i]) * a.ldy + n, v[i], a.past_cache);
+                for (int i = 0; i < 4; ++i) st4<PAST>(a.y + (block0 + row[i0 + i]) * a.ldy + n, v[i]);
             }
         } else {
             floatx4 v[OWN];
@@ -536,7 +540,7 @@ __global__ __launch_bounds__(256, RT <= 2 ? 3 : RT <= 4 ? 2 : 1) void lora_up_ke
             if (nb + 256 < n1) fetch(nb + 256);
 #pragma unroll
             for (int i = 0; i < OWN; ++i)
-                if (row[i] >= 0 && n < n1) put4(a, block0 + row[i], n, v[i]);
+                if (row[i] >= 0 && n < n1) put4<PAST>(a, block0 + row[i], n, v[i]);
         }
     }
 }
@@ -555,11 +559,12 @@ void launch_ranks(const LoraArgs& a, hipStream_t stream) {
     if constexpr (RT <= 8)
         if (a.tile_rows == 32) {
             lora_down_kernel<T, RT, 2><<<grid, 256, lds, stream>>>(a);
-            lora_up_kernel<T, RT, 2><<<up_grid, 256, 0, stream>>>(a);
+            if (a.past_cache) lora_up_kernel<T, RT, 2, true><<<up_grid, 256, 0, stream>>>(a);
+            else lora_up_kernel<T, RT, 2, false><<<up_grid, 256, 0, stream>>>(a);
             return;
         }
     lora_down_kernel<T, RT, 1><<<grid, 256, lds, stream>>>(a);
-    lora_up_kernel<T, RT, 1><<<up_grid, 256, 0, stream>>>(a);
+    lora_up_kernel<T, RT, 1, false><<<up_grid, 256, 0, stream>>>(a);
 }
 
 template <class T>
