@@ -19,8 +19,7 @@ namespace samhip {
 namespace {
 
 // Channels of one load: 16 bytes.  Rows need no alignment beyond their
-// element's; the last vector of a row that holds fewer channels is read and
-// written one by one.
+// element's.
 template <class T>
 constexpr int kVec = 16 / sizeof(T);
 
@@ -32,16 +31,45 @@ struct __attribute__((packed, aligned(sizeof(T)))) Packed {
 template <class T>
 using Vector = typename Packed<T, kVec<T>>::type;
 
-// n channels at p.  `whole`: the memory behind them is the tensor's too (its
-// next pixel), so the whole vector may be read.
-template <class T>
-__device__ __forceinline__ Vector<T> load(const T* p, int n, bool whole) {
-    if (n == kVec<T> || whole) return reinterpret_cast<const Packed<T, kVec<T>>*>(p)->v;
-    Vector<T> v;
+// Channels ch .. of a pixel's row; those at or behind `channels` are whatever
+// comes, and not read.  A branch around a load has it waited for at once, so
+// how a group of loads is done is chosen outside of it: WHOLE reads them as
+// they are, SHIFTED (a row holds a vector) the row's last vector again,
+// shifted, GUARDED one by one.
+enum class Edge { WHOLE, SHIFTED, GUARDED };
+template <Edge E, class T>
+__device__ __forceinline__ Vector<T> load(const T* row, int ch, int channels) {
+    constexpr int VEC = kVec<T>;
+    if constexpr (E == Edge::GUARDED) {
+        Vector<T> v;
 #pragma unroll
-    for (int e = 0; e < kVec<T>; ++e) v[e] = p[min(e, n - 1)];
+        for (int e = 0; e < VEC; ++e) v[e] = row[min(ch + e, channels - 1)];
+        return v;
+    }
+    const int at = E == Edge::WHOLE ? ch : min(ch, channels - VEC);
+    Vector<T> v = reinterpret_cast<const Packed<T, VEC>*>(row + at)->v;
+    if constexpr (E == Edge::SHIFTED)
+#pragma unroll
+        for (int s = 1; s < VEC; s *= 2)
+#pragma unroll
+            for (int e = 0; e + s < VEC; ++e) v[e] = (ch - at) & s ? v[e + s] : v[e];
     return v;
 }
+template <Edge E>
+struct EdgeTag {
+    static constexpr Edge value = E;
+};
+template <bool SAME, class T, class Body>
+__device__ __forceinline__ void with_edge(int channels, Body body) {   // uniform
+    if constexpr (SAME) {
+        body(EdgeTag<Edge::WHOLE>{});
+    } else {
+        if (channels % kVec<T> == 0) body(EdgeTag<Edge::WHOLE>{});
+        else if (channels >= kVec<T>) body(EdgeTag<Edge::SHIFTED>{});
+        else body(EdgeTag<Edge::GUARDED>{});
+    }
+}
+
 // PAST: past the caches (a template's argument: of two stores in the branches
 // of a condition the compiler makes an ordinary one).
 template <bool PAST, class T, int VEC>
@@ -136,12 +164,26 @@ __device__ __forceinline__ Moments moments(double sum, double sq, double n, floa
     return m;
 }
 
-__device__ __forceinline__ float activate(int act, float v) {   // act is uniform
-    if (act == ACT_RELU) return v > 0.f || v != v ? v : 0.f;
+template <int ACT>
+__device__ __forceinline__ float activate(float v) {
+    if constexpr (ACT == ACT_RELU) return v > 0.f || v != v ? v : 0.f;
     // reciprocal and exponential within an ulp each
-    if (act == ACT_SILU) return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
-    if (act == ACT_GELU_ERF) return gelu_erf(v);
-    return v;
+    else if constexpr (ACT == ACT_SILU) return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+    else if constexpr (ACT == ACT_GELU_ERF) return gelu_erf(v);
+    else return v;
+}
+template <int ACT>
+struct ActTag {
+    static constexpr int value = ACT;
+};
+template <class Body>
+__device__ __forceinline__ void with_activation(int act, Body body) {   // uniform: once per pass, not per value
+    switch (act) {
+        case ACT_RELU: body(ActTag<ACT_RELU>{}); break;
+        case ACT_SILU: body(ActTag<ACT_SILU>{}); break;
+        case ACT_GELU_ERF: body(ActTag<ACT_GELU_ERF>{}); break;
+        default: body(ActTag<ACT_NONE>{});
+    }
 }
 
 // Gain and bias of channels c .. (`last` at most), all loads at once: a test
@@ -170,12 +212,17 @@ __global__ __launch_bounds__(1024) void group_norm_block_kernel(const TI* x, TO*
     const int row = tid / cols, c = (tid - row * cols) * VEC, n = min(size - c, VEC);
     const int count = row < rows && row < s.pixels ? (s.pixels - 1 - row) / rows + 1 : 0;   // at most NV
     const int64_t first = min(row, s.pixels - 1), x_step = rows * s.x_pixel, y_step = rows * s.y_pixel;
-    const TI* xg = x + image * s.x_image + g * size + c + first * s.x_pixel;
+    const TI* xg = x + image * s.x_image + first * s.x_pixel;
     TO* yg = y + image * s.y_image + g * size + c + first * s.y_pixel;
-    const bool whole = s.x_pixel >= VEC && row + (count - 1) * rows < s.pixels - 1 && count;
     Vector<TI> v[NV];
+    const auto fetch = [&](auto edge) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = load<TI>(xg + max(min(i, count - 1), 0) * x_step, n, whole);
+        for (int i = 0; i < NV; ++i)
+            v[i] = load<decltype(edge)::value>(xg + max(min(i, count - 1), 0) * x_step, g * size + c, s.channels);
+    };
+    if (size % VEC == 0) fetch(EdgeTag<Edge::WHOLE>{});
+    else if (s.channels >= VEC) fetch(EdgeTag<Edge::SHIFTED>{});
+    else fetch(EdgeTag<Edge::GUARDED>{});
     float ww[VEC], bb[VEC];
     gain_and_bias<VEC>(w, b, g * size + c, g * size + size - 1, ww, bb);
     double sum = 0.0, sq = 0.0;
@@ -205,14 +252,16 @@ __global__ __launch_bounds__(1024) void group_norm_block_kernel(const TI* x, TO*
         ww[e] = ww[e] * m.rstd;
         bb[e] = bb[e] - m.lo * ww[e];
     }
+    with_activation(act, [&](auto tag) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        if (i >= count) break;
-        float o[VEC];
+        for (int i = 0; i < NV; ++i) {
+            if (i >= count) continue;
+            float o[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) o[e] = activate(act, __builtin_fmaf((float)v[i][e] - m.hi, ww[e], bb[e]));
-        store<false>(yg + i * y_step, n, o);
-    }
+            for (int e = 0; e < VEC; ++e) o[e] = activate<decltype(tag)::value>(__builtin_fmaf((float)v[i][e] - m.hi, ww[e], bb[e]));
+            store<false>(yg + i * y_step, n, o);
+        }
+    });
 }
 
 constexpr int FLIGHT = 8;   // pixels that a thread has in flight
@@ -230,21 +279,22 @@ __global__ __launch_bounds__(256) void group_norm_stats_kernel(const TI* __restr
     const int width = min(cols, 256), rows = 256 / width, row = tid / width, col0 = tid - row * width;
     const int p0 = blockIdx.x * chunk + row, p1 = min((blockIdx.x + 1) * chunk, s.pixels);
     const int plane = rows * RUNS * cols;
-    const bool whole = s.x_pixel >= VEC && p1 < s.pixels;
     if (row < rows) {
         for (int col = col0; col < cols; col += width) {
             double sum[RUNS], sq[RUNS];
 #pragma unroll
             for (int e = 0; e < RUNS; ++e) sum[e] = sq[e] = 0.0;
-            const TI* xc = x + blockIdx.y * s.x_image + col * VEC;
-            const int n = SAME ? VEC : min(s.channels - col * VEC, VEC);
+            const TI* xi = x + blockIdx.y * s.x_image;
             for (int p = p0; p < p1;) {
                 const int q = p;
                 Run run[RUNS];
                 for (int k = 0; k < RUN && p < p1; ++k, p += FLIGHT * rows) {
                     Vector<TI> v[FLIGHT];   // the last pixel again where there are no more
+                    with_edge<SAME, TI>(s.channels, [&](auto edge) {
 #pragma unroll
-                    for (int u = 0; u < FLIGHT; ++u) v[u] = load<TI>(xc + min(p + u * rows, p1 - 1) * s.x_pixel, n, whole);
+                        for (int u = 0; u < FLIGHT; ++u)
+                            v[u] = load<decltype(edge)::value>(xi + min(p + u * rows, p1 - 1) * s.x_pixel, col * VEC, s.channels);
+                    });
                     if (k == 0)
 #pragma unroll
                         for (int e = 0; e < RUNS; ++e) run[e].shift = (float)v[0][e];
@@ -328,40 +378,45 @@ __global__ __launch_bounds__(256) void group_norm_finish_kernel(const double* __
     finish(partial + int64_t(blockIdx.x) * chunks * groups * 2, chunks, groups, n, eps, lds, out + int64_t(blockIdx.x) * groups);
 }
 
-// `stats` is null where the workgroups finish the partial sums themselves.
+// FINISH: the workgroups add up the partial sums themselves.
 // The chunks in the other order: the last ones read are still in L2.
-template <class TI, class TO, bool SAME, bool PAST>
+template <class TI, class TO, bool SAME, bool PAST, bool FINISH>
 __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* y, GroupNormShape s, int chunk,
                                                                const double* __restrict__ partial, int chunks, const Moments* __restrict__ stats,
                                                                const float* __restrict__ w, const float* __restrict__ b, float eps,
                                                                int act) {
     constexpr int VEC = kVec<TI>;
-    __shared__ Moments shared[kGroupNormInline];
-    __shared__ double lds[256][2];
+    __shared__ Moments shared[FINISH ? kGroupNormInline : 1];
+    __shared__ double lds[FINISH ? 256 : 1][2];
     const int tid = threadIdx.x, cols = (s.channels + VEC - 1) / VEC, size = s.channels / s.groups;
     const int width = min(cols, 256), rows = 256 / width, row = tid / width, col0 = tid - row * width;
     const int at = gridDim.x - 1 - blockIdx.x;
     const int p0 = at * chunk + row, p1 = min((at + 1) * chunk, s.pixels);
-    const bool some = row < rows && p0 < p1, whole = s.x_pixel >= VEC && p1 < s.pixels;
+    const bool some = row < rows && p0 < p1;
     const TI* xi = x + blockIdx.y * s.x_image;
     TO* yi = y + blockIdx.y * s.y_image;
     constexpr int U = FLIGHT / 2;   // a batch is under way while the one before it is computed
     Vector<TI> v[U], next[U];
     auto fetch = [&](int col, int p, Vector<TI>(&v)[U]) {
-        const int n = SAME ? VEC : min(s.channels - col * VEC, VEC);
+        with_edge<SAME, TI>(s.channels, [&](auto edge) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = load<TI>(xi + col * VEC + min(p + u * rows, p1 - 1) * s.x_pixel, n, whole);
+            for (int u = 0; u < U; ++u)
+                v[u] = load<decltype(edge)::value>(xi + min(p + u * rows, p1 - 1) * s.x_pixel, col * VEC, s.channels);
+        });
     };
     float ww[VEC], bb[VEC];
     if (some) {   // under way while the sums are finished
         fetch(col0, p0, v);
         gain_and_bias<VEC>(w, b, col0 * VEC, s.channels - 1, ww, bb);
     }
-    const Moments* moments_of = stats + int64_t(blockIdx.y) * s.groups;
-    if (!stats) {
+    if constexpr (FINISH) {
         finish(partial + int64_t(blockIdx.y) * chunks * s.groups * 2, chunks, s.groups, double(s.pixels) * size, eps, lds, shared);
-        moments_of = shared;
+        __syncthreads();
     }
+    const auto moments_of = [&](int g) -> Moments {   // from LDS or from memory, never from either by one pointer
+        if constexpr (FINISH) return shared[g];
+        else return stats[int64_t(blockIdx.y) * s.groups + g];
+    };
     if (!some) return;
     for (int col = col0; col < cols; col += width) {
         float hi[SAME ? 1 : VEC];
@@ -369,37 +424,39 @@ __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* 
         const int n = SAME ? VEC : min(s.channels - col * VEC, VEC);
         Moments m;
         if (SAME) {
-            m = moments_of[col * VEC / size];
+            m = moments_of(col * VEC / size);
             hi[0] = m.hi;
         }
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             if (!SAME) {
-                m = moments_of[min(col * VEC + e, s.channels - 1) / size];
+                m = moments_of(min(col * VEC + e, s.channels - 1) / size);
                 hi[e] = m.hi;
             }
             ww[e] = ww[e] * m.rstd;
             bb[e] = bb[e] - m.lo * ww[e];
         }
         if (col != col0) fetch(col, p0, v);
-        for (int p = p0; p < p1; p += U * rows) {
-            const bool more = p + U * rows < p1;
-            if (more) fetch(col, p + U * rows, next);
+        with_activation(act, [&](auto tag) {
+            for (int p = p0; p < p1; p += U * rows) {
+                const bool more = p + U * rows < p1;
+                if (more) fetch(col, p + U * rows, next);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int q = p + u * rows;
-                if (q < p1) {
-                    float o[VEC];
+                for (int u = 0; u < U; ++u) {
+                    const int q = p + u * rows;
+                    if (q < p1) {
+                        float o[VEC];
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e)
-                        o[e] = activate(act, __builtin_fmaf((float)v[u][e] - hi[SAME ? 0 : e], ww[e], bb[e]));
-                    store<PAST>(yi + col * VEC + q * s.y_pixel, n, o);
+                        for (int e = 0; e < VEC; ++e)
+                            o[e] = activate<decltype(tag)::value>(__builtin_fmaf((float)v[u][e] - hi[SAME ? 0 : e], ww[e], bb[e]));
+                        store<PAST>(yi + col * VEC + q * s.y_pixel, n, o);
+                    }
                 }
-            }
-            if (more)
+                if (more)
 #pragma unroll
-                for (int u = 0; u < U; ++u) v[u] = next[u];
-        }
+                    for (int u = 0; u < U; ++u) v[u] = next[u];
+            }
+        });
     }
 }
 
@@ -441,11 +498,17 @@ void launch_typed(const TI* x, TO* y, const GroupNormShape& s, const float* w, c
         group_norm_finish_kernel<<<s.images, 256, 0, stream>>>(partial, chunks, s.groups, double(s.pixels) * size, eps, stats);
     }
 #define SAMHIP_GN_APPLY(SAME, PAST) \
-    group_norm_apply_kernel<TI, TO, SAME, PAST><<<apply_grid, 256, 0, stream>>>(x, y, s, apply_chunk, partial, chunks, stats, w, b, eps, act)
-    if (same && past_cache) SAMHIP_GN_APPLY(true, true);
-    else if (same) SAMHIP_GN_APPLY(true, false);
-    else if (past_cache) SAMHIP_GN_APPLY(false, true);
-    else SAMHIP_GN_APPLY(false, false);
+    if (stats) group_norm_apply_kernel<TI, TO, SAME, PAST, false><<<apply_grid, 256, 0, stream>>>(x, y, s, apply_chunk, partial, chunks, stats, w, b, eps, act); \
+    else group_norm_apply_kernel<TI, TO, SAME, PAST, true><<<apply_grid, 256, 0, stream>>>(x, y, s, apply_chunk, partial, chunks, stats, w, b, eps, act)
+    if (same && past_cache) {
+        SAMHIP_GN_APPLY(true, true);
+    } else if (same) {
+        SAMHIP_GN_APPLY(true, false);
+    } else if (past_cache) {
+        SAMHIP_GN_APPLY(false, true);
+    } else {
+        SAMHIP_GN_APPLY(false, false);
+    }
 #undef SAMHIP_GN_APPLY
 }
 
