@@ -183,8 +183,8 @@ int samhip_mul_mat_noalloc(samhip_context* ctx, const samhip_tensor* w, const sa
  *   y[m] = base[m] + scale[s] * B[s] (A[s] x[m]),  s = ids[m]
  * with base the shared product, e.g. of samhip_mul_mat.  The adapters stand
  * in banks of equal slots, a (F32 or F16, ne = {K, R, slots, 1}) and b (the
- * same type, ne = {R, N, slots, 1}), with any row and slot strides; at most
- * 4096 slots. */
+ * same type, ne = {R, N, slots, 1}), with any row and slot strides that leave
+ * rows and slots apart; at most 4096 slots. */
 typedef struct samhip_lora_bank {
     int32_t version;        /* SAMHIP_ABI_VERSION */
     samhip_tensor a, b;     /* R at most 256 */
@@ -195,9 +195,10 @@ typedef struct samhip_lora_bank {
 /* x: F32 {K, M}; ids: device I32 {M}, in any order; base: F32 {N, M}, NULL
  * for zeros, may be y itself (same data and row stride); y: F32 {N, M}.  A
  * row whose id is not in [0, slots) gets base alone; ranks are cut to
- * [0, R].  y overlaps no other operand.  Products and sums in F32.  ids, ranks, scales and the banks are
- * read on the device, at every replay of a captured call too, so slots can be
- * refilled and requests moved between replays.  May be captured. */
+ * [0, R].  y overlaps no other operand.  Products and sums in F32.  ids, ranks,
+ * scales and the banks are read on the device, at every replay of a captured
+ * call too, so slots can be refilled and requests moved between replays.  May
+ * be captured. */
 int samhip_supports_lora_add(const samhip_lora_bank* bank, const samhip_tensor* x, const samhip_tensor* ids,
                              const samhip_tensor* base, const samhip_tensor* y);
 int samhip_lora_add(samhip_context* ctx, const samhip_lora_bank* bank, const samhip_tensor* x, const samhip_tensor* ids,
@@ -358,7 +359,9 @@ int samhip_flash_attn(samhip_context* ctx, const float* q, const float* k, const
  * of a request's n sees its first own_len - n + i + 1 own keys (and all of the
  * prefix).  A query without any key gets zeros; rows of out outside
  * [q_start[0], q_start[requests]) are left as they were.  Rows behind own_len
- * are not read; the rows that are read must be finite, masked ones too.
+ * are not read, and a row that is not finite reaches only the queries that see
+ * it.  F32 keys, and values, of 64 neighbouring rows share a scale: one 2^18
+ * times below the largest of them begins to lose digits.
  * The three tables are read on the device (at every replay of a captured
  * call) and cut to what exists: query rows to [0, rows), lengths to
  * [0, own_max] and the rows of own_k; an own_start outside them means no
@@ -394,9 +397,12 @@ enum samhip_activation {
  * the feature cache hold pixel rows):
  *   y = act((x - mean) / sqrt(var + eps) * w[c] + b[c])
  * x and y are F32 or F16 (each its own), ne = {channels, pixels, images, 1},
- * nb[0] the element size, pixel and image strides any multiples of it;
+ * nb[0] the element size, pixel and image strides any multiples of it that
+ * leave rows and images apart;
  * mean and biased variance over the channels / groups neighbouring channels
- * of a group in every pixel of one image (sums in F64).  w, b: device F32
+ * of a group in every pixel of one image (F32 runs of up to 512 values'
+ * differences from one of them, joined in F64; deviations within 1e-18 ..
+ * 1e18).  w, b: device F32
  * [channels], each may be NULL.  channels a multiple of groups, at most 4096;
  * images at most 65535.  y may be x itself (same type and strides), and
  * overlaps nothing else.  A non-finite value makes its group's outputs
@@ -437,9 +443,9 @@ int samhip_trace_pause(samhip_context* ctx, int paused);
  * at M = 32): the calls between capture_begin and capture_end are recorded
  * into a HIP graph instead of running, and graph_launch replays them on the
  * context's stream with one host call.  Only samhip_mul_mat,
- * samhip_quantize_rows, samhip_dequantize_rows, samhip_lora_add, samhip_prefix_attn
- * and samhip_group_norm may be captured; every other entry point fails with INVALID_ARGUMENT while a
- * capture is open.  A
+ * samhip_quantize_rows, samhip_dequantize_rows, samhip_lora_add,
+ * samhip_prefix_attn and samhip_group_norm may be captured; every other entry
+ * point fails with INVALID_ARGUMENT while a capture is open.  A
  * captured call must fit the context's current staging (run the same
  * product once before capturing); staging that has to grow later is
  * reallocated without freeing the buffer that live graphs use.  Replays

@@ -72,6 +72,16 @@ template <>
 struct Raw8<_Float16> {
     half8 v;
     __device__ __forceinline__ void load(const _Float16* p) { v = *reinterpret_cast<const half8_at*>(p); }
+    // zeros for values of which one is not finite; whether that was so
+    __device__ __forceinline__ bool clear_non_finite() {
+        typedef uint16_t ushort8 __attribute__((ext_vector_type(8)));
+        const ushort8 bits = __builtin_bit_cast(ushort8, v);
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) bad = bad || (bits[j] & 0x7c00) == 0x7c00;
+        if (bad) v = half8{};
+        return bad;
+    }
 };
 template <>
 struct Raw8<float> {
@@ -88,6 +98,11 @@ struct Raw8<float> {
             m = umax(m, __float_as_uint(b[j]) & 0x7fffffffu);
         }
         return m;
+    }
+    __device__ __forceinline__ bool clear_non_finite() {
+        const bool bad = magnitude() >= 0x7f800000u;
+        if (bad) a = b = floatx4{};
+        return bad;
     }
     // values * factor as hi + lo
     __device__ __forceinline__ void split(float factor, half8& hi, half8& lo) const {
@@ -339,9 +354,26 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
             for (int t = 0; t < STEPS; ++t) vr[t].load(s.v + min(k + key + t * (512 / HD), s.k1 - 1) * s.ldv + col);
         }
     };
+    // Keys below this one are seen by every place.  In a tile that reaches
+    // further a weight of zero keeps no infinity or NaN out, so such keys and
+    // values are replaced by zeros and the places that see them get a NaN sum.
+    const int seen_by_all = s.causal ? s.limit0 + s.first / a.group : s.k1 + TILE;
     if (AHEAD && kw < s.k1) load(kw);
     for (int k = kw; k < s.k1; k += step) {
         if (!AHEAD) load(k);
+        uint32_t bad = 0;   // keys k + n of the tile
+        if (k + TILE > seen_by_all) {
+#pragma unroll
+            for (int t = 0; t < STEPS; ++t) {
+                bad |= kr[t].clear_non_finite() ? 1u << li : 0u;
+                bad |= vr[t].clear_non_finite() ? 1u << (key + t * (512 / HD)) : 0u;
+            }
+            if (__any(bad != 0)) {
+                uint32_t all = 0;
+                for (int n = 0; n < TILE; ++n) all |= __any(bad >> n & 1) ? 1u << n : 0u;
+                bad = all;
+            }
+        }
         floatx16 sc[1];
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[0][r] = 0.f;
@@ -379,6 +411,7 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
         if (AHEAD && k + step < s.k1) load(k + step);
         half8 ph[2], pl[2];
         sums.weigh(sc, c, k, q.limit, ph, pl);
+        if (bad && q.limit > k && bad << max(k + TILE - q.limit, 0)) sums.l = __builtin_nanf("");
         values<T, HD, 1>(vt, ph, pl, sums);
     }
     // the four waves' sums, joined through LDS

@@ -168,6 +168,31 @@ def test_zero_keys_values_and_queries(samhip, gpu_ctx):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("prefix", [0, 200])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_non_finite_keys_reach_only_queries_that_see_them(samhip, gpu_ctx, dtype, hd, prefix):
+    """Query i of 40 sees own keys up to i + 30 of 70: key 50 holds a NaN in kv
+    head 0, value 61 an infinity in kv head 1, value 69 both."""
+    b = Batch([40, 3], prefix, [70, 3], 4, 2, hd, dtype, causal=True, seed=13)
+    ref, bound = b.reference()
+    b.ok[50, 5] = float("nan")
+    b.ov[61, hd + 7] = float("inf")
+    b.ov[69, hd - 1] = float("-inf")
+    b.ov[69, hd] = float("nan")
+    torch.cuda.synchronize()
+    gpu_ctx.prefix_attn(b.desc(samhip))
+    gpu_ctx.synchronize()
+    sees = torch.zeros(43, 4, dtype=torch.bool, device="cuda")   # by query and head
+    sees[20:40, :2] = True
+    sees[31:40, 2:] = True
+    out = b.out.view(43, 4, hd)
+    err, most = (out.double() - ref.view(43, 4, hd)).abs(), bound.view(43, 4, hd)
+    assert (err[~sees] <= most[~sees]).all(), (err[~sees] / most[~sees]).max().item()
+    assert not out[sees].isfinite().all(-1).any()
+
+
+@pytest.mark.gpu
 def test_tables_out_of_range_are_cut(samhip, gpu_ctx):
     """Lengths and starts beyond the buffers: nothing outside them is read."""
     b = Batch([4, 4, 4, 4], 50, [10, 10, 10, 10], 2, 2, 32, "f16", seed=9, gap=0)
