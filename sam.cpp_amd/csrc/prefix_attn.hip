@@ -14,6 +14,11 @@
 // hi*hi + hi*lo + lo*hi; queries (by row), keys and values (by tile) are
 // scaled by powers of two so that the largest magnitude lies in [2^14, 2^15)
 // and any F32 range keeps ~22 bits.  F16 keys and values enter as they are.
+// Bound by the vector instructions of softmax and splitting beside the matrix
+// instructions (8 prompts of 201 queries on 5184 + 33 F32 keys, 8 heads of 32:
+// 48 us, 550 TFLOP/s of hi + lo products; 64 queries of 16 heads of 128 on
+// 65536 F16 keys: 76 us, 905 TFLOP/s, and 103 with up to 1024 own keys each),
+// by two launches' latency for few queries (8 on 5184: 9 us).
 #include <algorithm>
 #include <type_traits>
 
