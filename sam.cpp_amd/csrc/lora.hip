@@ -14,9 +14,9 @@
 //   lora_up_kernel    : y = base + scale * B t
 // Products on the F32 matrix instruction: F32 products and sums throughout.
 // Bound by HBM with many rows (41472 x 1024 -> 4736, rank 32, 8 slots: 421 us,
-// 4.1 TB/s, of it 390 for base and y; a copy of the bytes takes 364), by one or
-// two launches' latency with few (16 rows 1024 -> 1024, rank 16: 6.3 us; 256
-// rows 1024 -> 4096: 10.1).
+// 4.1 TB/s, most of it the second launch, from base to y; a copy of the bytes
+// takes 364), by one or two launches' latency with few (16 rows 1024 -> 1024,
+// rank 16: 6.3 us; 256 rows 1024 -> 4096: 10.1).
 #include <algorithm>
 
 #include "internal.hpp"
@@ -310,7 +310,7 @@ template <class T, int RT>
 __device__ __forceinline__ void take_b(const LoraArgs& a, const T* w, int n, int rank, floatx4 (&b)[RT]) {
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const T* row = w + min(n + r, a.n - 1) * a.b_row;
-    with_edge(a.rank % 4 == 0, a.rank, [&](auto edge) {
+    with_edge(a.rank % 4 == 0, RT > 2 ? 4 : a.rank, [&](auto edge) {
         constexpr Edge E = decltype(edge)::value;
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
@@ -465,6 +465,7 @@ __global__ __launch_bounds__(256, RT <= 2 ? 3 : RT <= 4 ? 2 : 1) void lora_up_ke
 #pragma unroll
     for (int i = 0; i < OWN; ++i) row[i] = __builtin_amdgcn_readfirstlane(tile[OWN * wave + i]);
     const bool whole = row[OWN - 1] >= 0;   // rows fill from the front
+    const int row0 = tile[0];
 #pragma unroll
     for (int i = 0; i < OWN; ++i) base[i] = floatx4{0.f, 0.f, 0.f, 0.f};
     const auto fetch = [&](int nb) {   // an absent row's place gets the block's first
@@ -489,26 +490,30 @@ __global__ __launch_bounds__(256, RT <= 2 ? 3 : RT <= 4 ? 2 : 1) void lora_up_ke
     };
     if (product) {
         fetch_b(n0);
+        // t of a subtile: no branch between a split's loads, an absent row's
+        // or rank tile's place reads the first row's or last tile's
+        const int last = max((rank + 15) / 16 - 1, 0);
+        const int64_t step = a.m * a.part_ld;
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
             const int at = tile[16 * s + r];
+            const float* p = a.part + (block0 + (at < 0 ? row0 : at)) * a.part_ld + 4 * g;
 #pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                t[s][i] = floatx4{0.f, 0.f, 0.f, 0.f};
-                if (16 * i < rank && at >= 0) {
-                    const float* p = a.part + (block0 + at) * a.part_ld + 16 * i + 4 * g;
-                    const int64_t step = a.m * a.part_ld;
-#pragma unroll 4
-                    for (int k = 0; k < a.splits; ++k) t[s][i] += *reinterpret_cast<const floatx4*>(p + k * step);
-                }
-            }
+            for (int i = 0; i < RT; ++i) t[s][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll RT <= 2 ? 4 : 2
+            for (int k = 0; k < a.splits; ++k, p += step)
+#pragma unroll
+                for (int i = 0; i < RT; ++i) t[s][i] += *reinterpret_cast<const floatx4*>(p + 16 * min(i, last));
             finish_t(a, slot, rank, t[s]);
         }
     }
     for (int nb = n0; nb < n1; nb += 256) {
         if (product) {
             if (nb != n0) __syncthreads();   // the last block's sums are read
-#pragma unroll
+            // a loop where the ranks make it long: the way of 20 KB more code to
+            // the CU takes longer than its steps (38 rows 1623 -> 266 of rank 110
+            // 18.9 us unrolled, 13.8 so; rank 40, 777 rows 1001 -> 1359, 9.8 and 10.9)
+#pragma unroll RT <= 4 ? 4 : 1
             for (int c = 0; c < 4; ++c) {
                 floatx4 acc[SUB], now[RT];
 #pragma unroll
