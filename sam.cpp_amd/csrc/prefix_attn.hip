@@ -388,7 +388,8 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
 #pragma unroll
             for (int t = 0; t < STEPS; ++t) m = umax(m, kr[t].magnitude()), mv = umax(mv, vr[t].magnitude());
             const int e = exponent_of(__builtin_amdgcn_readfirstlane(wave_umax(m)));
-            const int en = exponent_of(__builtin_amdgcn_readfirstlane(wave_umax(mv)));
+            mv = __builtin_amdgcn_readfirstlane(wave_umax(mv));
+            const int en = mv ? exponent_of(mv) : ev;   // values that are all zero ask for nothing
             c = q.factor(up(e));
 #pragma unroll
             for (int t = 0; t < STEPS; ++t) {
@@ -527,7 +528,8 @@ __device__ __forceinline__ void attend_wide(const PrefixAttnArgs& a, const Span<
             uint32_t mk = 0, mv = 0;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) mk = umax(mk, sh.largest[w][0]), mv = umax(mv, sh.largest[w][1]);
-            const int e = exponent_of(__builtin_amdgcn_readfirstlane(mk)), en = exponent_of(__builtin_amdgcn_readfirstlane(mv));
+            mv = __builtin_amdgcn_readfirstlane(mv);
+            const int e = exponent_of(__builtin_amdgcn_readfirstlane(mk)), en = mv ? exponent_of(mv) : ev;   // all zero: as narrow
             c = q.factor(up(e));
             fk = down(e);
             if (en > ev) {

@@ -238,6 +238,33 @@ def test_captured_replays_follow_the_tables(samhip, gpu_ctx):
     graph.destroy()
 
 
+# The two forms of the prefix part, few query places and many, with own keys;
+# then calls of one part, which writes the output itself, in either form.
+FORMS = [([3], 3000, [40]), ([100, 30], 3000, [200, 3]), ([3], 200, [0]), ([100], 200, [0])]
+
+
+def change_values(b, change):
+    """`change` on the values of the prefix and of each request's own rows."""
+    change(b.pv)
+    for r, n in enumerate(b.own_len):
+        change(b.ov[r * b.slot:r * b.slot + n])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", range(len(FORMS)))
+@pytest.mark.parametrize("exponent", [-30, -60])
+@pytest.mark.parametrize("place", [0, 2])
+def test_zero_value_rows_beside_small_values(samhip, gpu_ctx, form, exponent, place):
+    """64 of every 256 value rows are zero, as padded tokens' are: the others keep their digits."""
+    b = Batch(*FORMS[form], 4, 4, 64, "f32", seed=20)
+
+    def change(v):
+        v.mul_(2.0 ** exponent)
+        v[torch.arange(v.shape[0], device="cuda") // 64 % 4 == place] = 0.0
+    change_values(b, change)
+    b.check(samhip, gpu_ctx)
+
+
 def test_refusals(samhip):
     L = samhip.lib()
 
