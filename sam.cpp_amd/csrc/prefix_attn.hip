@@ -4,8 +4,9 @@
 // The prefix part does not depend on the request, so it is computed for
 // tiles of query rows of all requests; the own part for tiles of one
 // request's rows.  Either part's keys may be split over workgroups.  Each
-// leaves a maximum, a sum of weights and a weighted sum of values, which
-// attn_merge_kernel joins (a part that is alone writes the output itself).
+// leaves a maximum, a sum of weights and a weighted mean of values (a mean fits
+// F32 wherever the values do), which attn_merge_kernel joins (a part that is
+// alone writes the output itself).
 // Grouped heads: the queries that share a kv head are neighbouring rows of a
 // tile (row index = query row * group + head in group).
 //
@@ -190,6 +191,12 @@ struct Sums {
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[d][r] = clear ? 0.f : o[d][r] * f;
     }
+    __device__ __forceinline__ void shift(int by) {   // times 2^by
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = __builtin_ldexpf(o[d][r], by);
+    }
 
     // Weights of N blocks of 32 keys from key `k` on: sc[n] holds products with
     // keys 32n + 8 (r / 4) + 4hh + r % 4, c takes them to scores; hi + lo of the
@@ -327,7 +334,7 @@ template <class T, int HD>
 struct Narrow {
     static constexpr int VBYTES = TileRows<T, HD, 32, true>::BYTES, OBYTES = TILE * (HD + 4) * 4;   // a wave's tile, and its sums at the end
     uint8_t __attribute__((aligned(16))) lds[WAVES * (VBYTES > OBYTES ? VBYTES : OBYTES)];
-    float m[WAVES][TILE], l[WAVES][TILE], total[TILE];
+    float m[WAVES][TILE], l[WAVES][TILE];
 };
 
 template <class T, int HD>
@@ -435,22 +442,20 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
         const float lw = sh.l[w][li];
         if (lw != 0.f) l += lw * __builtin_amdgcn_exp2f(sh.m[w][li] - m);   // a NaN sum stays one
     }
-    float f = sums.l != 0.f ? __builtin_amdgcn_exp2f(sums.m - m) : 0.f;
-    if constexpr (F32) f = f * up(ev);
+    const float f = sums.l != 0.f ? __builtin_amdgcn_exp2f(sums.m - m) / l : 0.f;
+    sums.scale(f);
+    if constexpr (F32) sums.shift(ev - 141);
     float* all = reinterpret_cast<float*>(sh.lds);
 #pragma unroll
     for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; r += 4)
             *reinterpret_cast<floatx4*>(all + (wave * TILE + li) * (HD + 4) + 32 * d + 2 * r + 4 * hh) =
-                floatx4{sums.o[d][r] * f, sums.o[d][r + 1] * f, sums.o[d][r + 2] * f, sums.o[d][r + 3] * f};
-    if (wave == 0 && hh == 0) {
-        sh.total[li] = l;
-        if (part >= 0 && q.mine) {
-            float* ml = a.part_ml + ((int64_t(q.row) * a.heads + q.head) * a.parts + part) * 2;
-            ml[0] = m;
-            ml[1] = l;
-        }
+                floatx4{sums.o[d][r], sums.o[d][r + 1], sums.o[d][r + 2], sums.o[d][r + 3]};
+    if (part >= 0 && wave == 0 && hh == 0 && q.mine) {
+        float* ml = a.part_ml + ((int64_t(q.row) * a.heads + q.head) * a.parts + part) * 2;
+        ml[0] = m;
+        ml[1] = l;
     }
     __syncthreads();
     constexpr int QUADS = HD / 4;
@@ -461,12 +466,8 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) v += *reinterpret_cast<const floatx4*>(all + (w * TILE + p) * (HD + 4) + d);
         const int64_t r = s.q0 + i, h = kvh * a.group + place - i * a.group;
-        if (part < 0) {
-            const float lt = sh.total[p], inv = lt == 0.f ? 0.f : 1.f / lt;
-            *reinterpret_cast<float4_at*>(a.out + r * a.ldo + h * HD + d) = v * inv;
-        } else {
-            *reinterpret_cast<floatx4*>(a.part_o + ((r * a.heads + h) * a.parts + part) * HD + d) = v;
-        }
+        float* to = part < 0 ? a.out + r * a.ldo + h * HD : a.part_o + ((r * a.heads + h) * a.parts + part) * HD;
+        *reinterpret_cast<float4_at*>(to + d) = v;
     }
 }
 
@@ -554,10 +555,10 @@ __device__ __forceinline__ void attend_wide(const PrefixAttnArgs& a, const Span<
     }
     const float l = pair_sum(sums.l);
     if (!q.mine) return;
-    float f = F32 ? up(ev) : 1.f;
+    sums.scale(l == 0.f ? 0.f : 1.f / l);
+    if constexpr (F32) sums.shift(ev - 141);
     float* to;
     if (part < 0) {
-        f = l == 0.f ? 0.f : f / l;
         to = a.out + q.row * a.ldo + q.head * HD;
     } else {
         const int64_t at = (int64_t(q.row) * a.heads + q.head) * a.parts + part;
@@ -572,7 +573,7 @@ __device__ __forceinline__ void attend_wide(const PrefixAttnArgs& a, const Span<
 #pragma unroll
         for (int r = 0; r < 16; r += 4)
             *reinterpret_cast<float4_at*>(to + 32 * d + 2 * r + 4 * hh) =
-                floatx4{sums.o[d][r] * f, sums.o[d][r + 1] * f, sums.o[d][r + 2] * f, sums.o[d][r + 3] * f};
+                floatx4{sums.o[d][r], sums.o[d][r + 1], sums.o[d][r + 2], sums.o[d][r + 3]};
 }
 
 // Query rows [from, from + n) of request r, cut to the rows that exist.
@@ -674,7 +675,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prefix_attn_kernel(PrefixAttnAr
 }
 
 // A wave per (row, head): the parts' maxima and sums one to a lane, then
-// HD / 4 lanes to a part's values.
+// HD / 4 lanes to a part's mean.
 template <int HD>
 __global__ __launch_bounds__(256) void attn_merge_kernel(PrefixAttnArgs a) {
     constexpr int QUADS = HD / 4, AT_ONCE = 64 / QUADS;
@@ -695,10 +696,13 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(PrefixAttnArgs a) {
         }
         const float mnew = fmaxf(m, wave_max(lp != 0.f ? mp : -__builtin_inff()));
         const float old = m == mnew ? 1.f : __builtin_amdgcn_exp2f(m - mnew);
-        const float f = lp != 0.f ? __builtin_amdgcn_exp2f(mp - mnew) : 0.f;   // 0: no key in this part
+        float f = lp != 0.f ? lp * __builtin_amdgcn_exp2f(mp - mnew) : 0.f;   // 0: no key in this part
+        const float before = l * old;
         m = mnew;
-        l = l * old + wave_sum(lp * f);
-        v = v * old;
+        l = before + wave_sum(f);
+        const float inv = l == 0.f ? 0.f : 1.f / l;   // v stays a mean
+        f = f * inv;
+        v = v * (before * inv);
         const int here = min(a.parts - p0, 64);
         const float* parts = a.part_o + (item * a.parts + p0) * HD + d;
         const auto add = [&](auto count, int p1) {   // parts p1 + slot, p1 + slot + AT_ONCE, ..
@@ -725,8 +729,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(PrefixAttnArgs a) {
     for (int off = QUADS; off < 64; off <<= 1)
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] += __shfl_xor(v[j], off, 64);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (slot == 0) *reinterpret_cast<float4_at*>(a.out + row * a.ldo + h * HD + d) = v * inv;
+    if (slot == 0) *reinterpret_cast<float4_at*>(a.out + row * a.ldo + h * HD + d) = v;
 }
 
 template <class T, int HD>

@@ -265,6 +265,16 @@ def test_zero_value_rows_beside_small_values(samhip, gpu_ctx, form, exponent, pl
     b.check(samhip, gpu_ctx)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", range(len(FORMS)))
+@pytest.mark.parametrize("exponent", [112, 124])
+def test_f32_values_near_the_largest(samhip, gpu_ctx, form, exponent):
+    """Values to 5 * 2^exponent: their weighted mean fits, whatever their sum does."""
+    b = Batch(*FORMS[form], 4, 2, 32, "f32", seed=24)
+    change_values(b, lambda v: v.mul_(2.0 ** exponent))
+    b.check(samhip, gpu_ctx)
+
+
 def test_refusals(samhip):
     L = samhip.lib()
 
