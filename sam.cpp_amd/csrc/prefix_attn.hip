@@ -176,9 +176,10 @@ struct Queries {
     }
 };
 
-// Running maximum (in units of log 2), sum of weights and weighted sums of
-// values of a wave's places: o[d] holds, transposed, lane (li, hh)'s
-// dimensions 32d + 8 (r / 4) + 4hh + r % 4 of place li.
+// The base of the weights 2^(score - m), below the running maximum (in units of
+// log 2), their sum, and the weighted sums of values of a wave's places: o[d]
+// holds, transposed, lane (li, hh)'s dimensions 32d + 8 (r / 4) + 4hh + r % 4 of
+// place li.
 template <int HD>
 struct Sums {
     floatx16 o[HD / 32];
@@ -219,11 +220,13 @@ struct Sums {
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = __builtin_elementwise_maximum(mx, sc[n][r]);
         const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = c * __builtin_elementwise_maximum(__uint_as_float(other[0]), __uint_as_float(other[1]));
-        // the exponent base moves only when a score passes it by 8, so that
-        // weights stay below 2^8 and most steps skip the rescaling
-        if (__any(mx > m + 8.0f)) {
-            const float mnew = fmaxf(m, mx);
+        mx = __builtin_elementwise_maximum(__uint_as_float(other[0]), __uint_as_float(other[1]));
+        // The largest weight so far lies in [2^11, 2^15): the base moves only
+        // when a score passes it by 15, so that most steps skip the rescaling,
+        // and as fp16 halves a weight keeps 22 bits down to 2^-14 of the
+        // largest and is off by 2^-36 of it at most.
+        if (__any(__builtin_fmaf(mx, c, -m) > 15.0f)) {
+            const float mnew = fmaxf(m, __builtin_fmaf(mx, c, -11.0f));
             const float alpha = mnew == m ? 1.f : __builtin_amdgcn_exp2f(m - mnew);
             m = mnew;
             l = l * alpha;

@@ -275,6 +275,30 @@ def test_f32_values_near_the_largest(samhip, gpu_ctx, form, exponent):
     b.check(samhip, gpu_ctx)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,prefix", [(1, 65536), (40, 1024), (4096, 5184)])
+@pytest.mark.parametrize("below", [16.75, 17.5, 18.5])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_many_small_weights_behind_a_large_one(samhip, gpu_ctx, dtype, rows, prefix, below):
+    """The first key's score is `below` nats above all others', and all values
+    are one: the output is one.  Scores are exact (queries 1, keys a multiple of
+    2^-14), numerator and denominator have the same weights, so what counts is
+    the split of the weights (2^-22 of each, 2^-36 of the largest at least) and
+    the F32 sums: 2^-19 + prefix 2^-36 + (prefix / 16 + 48) 2^-24."""
+    heads, hd = 8, 32
+    b = Batch([rows], prefix, [0], heads, heads, hd, dtype, seed=25)
+    b.scale = 0.125
+    b.q.fill_(1.0)
+    b.pk.zero_()
+    b.pk[0] = below / (hd * b.scale)
+    b.pv.fill_(1.0)
+    torch.cuda.synchronize()
+    gpu_ctx.prefix_attn(b.desc(samhip))
+    gpu_ctx.synchronize()
+    err = (b.out.double() - 1).abs().max().item()
+    assert err <= 2.0 ** -19 + prefix * 2.0 ** -36 + (prefix / 16 + 48) * 2.0 ** -24, err
+
+
 def test_refusals(samhip):
     L = samhip.lib()
 
