@@ -360,8 +360,10 @@ int samhip_flash_attn(samhip_context* ctx, const float* q, const float* k, const
  * prefix).  A query without any key gets zeros; rows of out outside
  * [q_start[0], q_start[requests]) are left as they were.  Rows behind own_len
  * are not read, and a row that is not finite reaches only the queries that see
- * it.  F32 keys, and values, of 64 neighbouring rows share a scale: one 2^18
- * times below the largest of them begins to lose digits.
+ * it.  Digits begin to be lost of F32 keys, and values, 2^18 times below the
+ * largest of 64 neighbouring rows, which share a scale; of weights 2^12 times
+ * below the largest of their query (2^-34 of it at most); and of a row of
+ * values 2^75 times below what others have come to.
  * The three tables are read on the device (at every replay of a captured
  * call) and cut to what exists: query rows to [0, rows), lengths to
  * [0, own_max] and the rows of own_k; an own_start outside them means no

@@ -13,8 +13,9 @@
 // F32-accurate: queries, weights P and F32 keys and values enter the fp16
 // matrix instructions as hi + lo (lo = fp16(v - hi)), with the products
 // hi*hi + hi*lo + lo*hi; queries (by row), keys and values (by tile) are
-// scaled by powers of two so that the largest magnitude lies in [2^14, 2^15)
-// and any F32 range keeps ~22 bits.  F16 keys and values enter as they are.
+// scaled by powers of two so that the largest magnitude lies in [2^14, 2^15),
+// which leaves ~22 bits to those no more than 2^18 times smaller.  F16 keys and
+// values enter as they are.
 // Bound by the vector instructions of softmax and splitting beside the matrix
 // instructions (8 prompts of 201 queries on 5184 + 33 F32 keys, 8 heads of 32:
 // 48 us, 550 TFLOP/s of hi + lo products; 64 queries of 16 heads of 128 on
@@ -179,11 +180,14 @@ struct Queries {
 // The base of the weights 2^(score - m), below the running maximum (in units of
 // log 2), their sum, and the weighted sums of values of a wave's places: o[d]
 // holds, transposed, lane (li, hh)'s dimensions 32d + 8 (r / 4) + 4hh + r % 4 of
-// place li.
+// place li, F32 values in units of 2^(e - 141), one e for the wave (NONE: no
+// value but zeros yet).
 template <int HD>
 struct Sums {
+    static constexpr int NONE = 0, SLACK = 2;
     floatx16 o[HD / 32];
     float m = -__builtin_inff(), l = 0.f;
+    int e = NONE;
 
     __device__ __forceinline__ Sums() { scale(0.f, true); }
     __device__ __forceinline__ void scale(float f, bool clear = false) {
@@ -199,11 +203,39 @@ struct Sums {
             for (int r = 0; r < 16; ++r) o[d][r] = __builtin_ldexpf(o[d][r], by);
     }
 
+    // F32 values of one tile, whose largest has exponent `to` (0: all zero), come
+    // in units of 2^(to - 141).  The sums follow it, down where they leave room:
+    // values 2^75 apart keep their digits beside each other.  Returns how many
+    // powers of two the weights have to be lowered by, SLACK at most where there
+    // is room, so that most steps change nothing.
+    __device__ __forceinline__ int follow(int to) {
+        if (to == 0) return 0;
+        if (e == NONE) e = to;
+        if (to > e) {
+            shift(e - to);
+            e = to;
+        } else if (to < e - SLACK) {
+            uint32_t most = 0;   // of the finite sums
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const uint32_t b = __float_as_uint(o[d][r]) & 0x7fffffffu;
+                    most = umax(most, b < 0x7f800000u ? b : 0u);
+                }
+            const int room = 251 - int(__builtin_amdgcn_readfirstlane(wave_umax(most)) >> 23);   // they stay below 2^125
+            const int by = min(e - to, max(room, 0));
+            shift(by);
+            e -= by;
+        }
+        return min(e - to, 100);   // past 40 no weight is left as fp16, but in l
+    }
+
     // Weights of N blocks of 32 keys from key `k` on: sc[n] holds products with
     // keys 32n + 8 (r / 4) + 4hh + r % 4, c takes them to scores; hi + lo of the
-    // weights leave in the order the value operand is read in.
+    // weights, lowered by 2^-low, leave in the order the value operand is read in.
     template <int N>
-    __device__ __forceinline__ void weigh(floatx16 (&sc)[N], float c, int k, int limit, half8 (&hi)[2 * N], half8 (&lo)[2 * N]) {
+    __device__ __forceinline__ void weigh(floatx16 (&sc)[N], float c, int k, int limit, int low, half8 (&hi)[2 * N], half8 (&lo)[2 * N]) {
         const int hh = (threadIdx.x & 63) >> 5;
         if (__any(k + 32 * N > limit)) {
 #pragma unroll
@@ -223,8 +255,8 @@ struct Sums {
         mx = __builtin_elementwise_maximum(__uint_as_float(other[0]), __uint_as_float(other[1]));
         // The largest weight so far lies in [2^11, 2^15): the base moves only
         // when a score passes it by 15, so that most steps skip the rescaling,
-        // and as fp16 halves a weight keeps 22 bits down to 2^-14 of the
-        // largest and is off by 2^-36 of it at most.
+        // and as fp16 halves a weight keeps 22 bits down to 2^(low - 14) of the
+        // largest and is off by 2^(low - 36) of it at most.
         if (__any(__builtin_fmaf(mx, c, -m) > 15.0f)) {
             const float mnew = fmaxf(m, __builtin_fmaf(mx, c, -11.0f));
             const float alpha = mnew == m ? 1.f : __builtin_amdgcn_exp2f(m - mnew);
@@ -232,7 +264,7 @@ struct Sums {
             l = l * alpha;
             scale(alpha);
         }
-        const float mb = m == -__builtin_inff() ? 0.f : m;   // nothing seen yet: weights 0
+        const float mb = (m == -__builtin_inff() ? 0.f : m) + float(low);   // nothing seen yet: weights 0
         float ps = 0.f;
 #pragma unroll
         for (int n = 0; n < N; ++n)
@@ -241,7 +273,7 @@ struct Sums {
                 sc[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][r], c, -mb));
                 ps += sc[n][r];
             }
-        l = l + ps;
+        l = l + ps * __builtin_ldexpf(1.f, low);
 #pragma unroll
         for (int u = 0; u < 2 * N; ++u)
 #pragma unroll
@@ -347,7 +379,6 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hh = lane >> 5;
     const Queries<HD> q(a, s, kvh, s.first + li);
     Sums<HD> sums;
-    int ev = 20;   // F32 values: the exponent that the sums are scaled by
     uint8_t* vt = sh.lds + wave * Narrow<T, HD>::VBYTES;
     Raw8<T> kr[STEPS], vr[STEPS];
     const int step = TILE * WAVES, kw = s.k0 + TILE * wave;
@@ -392,14 +423,15 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
         floatx16 sc[1];
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[0][r] = 0.f;
-        float c = q.factor(1.f);
+        float c = q.factor(1.f), fv = 1.f;
+        int low = 0;
         if constexpr (F32) {
             uint32_t m = 0, mv = 0;
 #pragma unroll
             for (int t = 0; t < STEPS; ++t) m = umax(m, kr[t].magnitude()), mv = umax(mv, vr[t].magnitude());
             const int e = exponent_of(__builtin_amdgcn_readfirstlane(wave_umax(m)));
             mv = __builtin_amdgcn_readfirstlane(wave_umax(mv));
-            const int en = mv ? exponent_of(mv) : ev;   // values that are all zero ask for nothing
+            fv = down(exponent_of(mv));
             c = q.factor(up(e));
 #pragma unroll
             for (int t = 0; t < STEPS; ++t) {
@@ -409,10 +441,7 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
                 sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, q.hi[t], sc[0], 0, 0, 0);
                 sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.lo[t], sc[0], 0, 0, 0);
             }
-            if (en > ev) {
-                sums.scale(__builtin_ldexpf(1.f, ev - en));
-                ev = en;
-            }
+            low = sums.follow(mv ? exponent_of(mv) : 0);
         } else {
 #pragma unroll
             for (int t = 0; t < STEPS; ++t) {
@@ -422,11 +451,11 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
         }
         wave_lds_handoff();   // the last tile's reads came first
 #pragma unroll
-        for (int t = 0; t < STEPS; ++t) TileRows<T, HD, 32, true>::put(vt, t * 64 + lane, vr[t], down(ev));
+        for (int t = 0; t < STEPS; ++t) TileRows<T, HD, 32, true>::put(vt, t * 64 + lane, vr[t], fv);
         wave_lds_handoff();
         if (AHEAD && k + step < s.k1) load(k + step);
         half8 ph[2], pl[2];
-        sums.weigh(sc, c, k, q.limit, ph, pl);
+        sums.weigh(sc, c, k, q.limit, low, ph, pl);
         if (bad && q.limit > k && bad << max(k + TILE - q.limit, 0)) sums.l = __builtin_nanf("");
         values<T, HD, 1>(vt, ph, pl, sums);
     }
@@ -447,7 +476,7 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
     }
     const float f = sums.l != 0.f ? __builtin_amdgcn_exp2f(sums.m - m) / l : 0.f;
     sums.scale(f);
-    if constexpr (F32) sums.shift(ev - 141);
+    if constexpr (F32) sums.shift(sums.e - 141);
     float* all = reinterpret_cast<float*>(sh.lds);
 #pragma unroll
     for (int d = 0; d < HD / 32; ++d)
@@ -493,7 +522,6 @@ __device__ __forceinline__ void attend_wide(const PrefixAttnArgs& a, const Span<
     const bool any = first < s.n * a.group;
     const Queries<HD> q(a, s, kvh, first + li);
     Sums<HD> sums;
-    int ev = 20;
     Raw8<T> kr[PIECES], vr[PIECES];
     // this thread's piece of the first 256; the others are whole rows of keys on
     const int key = tid / (HD / 8), col = 8 * (tid % (HD / 8));
@@ -518,7 +546,8 @@ __device__ __forceinline__ void attend_wide(const PrefixAttnArgs& a, const Span<
     };
     load(s.k0);
     for (int k = s.k0; k < s.k1; k += 64) {
-        float c = q.factor(1.f), fk = 1.f;
+        float c = q.factor(1.f), fk = 1.f, fv = 1.f;
+        int low = 0;
         if constexpr (F32) {
             uint32_t mk = 0, mv = 0;
 #pragma unroll
@@ -533,18 +562,16 @@ __device__ __forceinline__ void attend_wide(const PrefixAttnArgs& a, const Span<
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) mk = umax(mk, sh.largest[w][0]), mv = umax(mv, sh.largest[w][1]);
             mv = __builtin_amdgcn_readfirstlane(mv);
-            const int e = exponent_of(__builtin_amdgcn_readfirstlane(mk)), en = mv ? exponent_of(mv) : ev;   // all zero: as narrow
+            const int e = exponent_of(__builtin_amdgcn_readfirstlane(mk));
             c = q.factor(up(e));
             fk = down(e);
-            if (en > ev) {
-                sums.scale(__builtin_ldexpf(1.f, ev - en));
-                ev = en;
-            }
+            fv = down(exponent_of(mv));
+            low = sums.follow(mv ? exponent_of(mv) : 0);
         }
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             TileRows<T, HD, 64, false>::put(sh.k, tid + 256 * i, kr[i], fk);
-            TileRows<T, HD, 64, true>::put(sh.v, tid + 256 * i, vr[i], down(ev));
+            TileRows<T, HD, 64, true>::put(sh.v, tid + 256 * i, vr[i], fv);
         }
         __syncthreads();
         if (k + 64 < s.k1) load(k + 64);
@@ -552,14 +579,14 @@ __device__ __forceinline__ void attend_wide(const PrefixAttnArgs& a, const Span<
             floatx16 sc[2];
             half8 ph[4], pl[4];
             scores<T, HD, 2>(sh.k, q, sc);
-            sums.weigh(sc, c, k, q.limit, ph, pl);
+            sums.weigh(sc, c, k, q.limit, low, ph, pl);
             values<T, HD, 2>(sh.v, ph, pl, sums);
         }
     }
     const float l = pair_sum(sums.l);
     if (!q.mine) return;
     sums.scale(l == 0.f ? 0.f : 1.f / l);
-    if constexpr (F32) sums.shift(ev - 141);
+    if constexpr (F32) sums.shift(sums.e - 141);
     float* to;
     if (part < 0) {
         to = a.out + q.row * a.ldo + q.head * HD;

@@ -299,6 +299,39 @@ def test_many_small_weights_behind_a_large_one(samhip, gpu_ctx, dtype, rows, pre
     assert err <= 2.0 ** -19 + prefix * 2.0 ** -36 + (prefix / 16 + 48) * 2.0 ** -24, err
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", range(len(FORMS)))
+@pytest.mark.parametrize("large,key", [(2.0 ** 33, -5.0), (2.0 ** 40, -5.0), (3e38, -24.0)])
+@pytest.mark.parametrize("place", [0, 70, 199])
+def test_large_values_without_weight(samhip, gpu_ctx, form, large, key, place):
+    """One value row of the prefix and one of the first request's own are far
+    larger than all others, at a weight (a score 44 or 210 below the others, at
+    least) that leaves little or nothing of them.  The rest of their 64 rows are
+    zero; the rows of other tiles keep their digits."""
+    b = Batch(*FORMS[form], 4, 4, 64, "f32", seed=21)
+    b.q.abs_().add_(0.5)
+    for k, v, n in ((b.pk, b.pv, b.prefix), (b.ok, b.ov, b.own_len[0])):
+        if place < n:
+            v[place // 64 * 64:min(place // 64 * 64 + 64, n)] = 0.0
+            v[place] = large
+            k[place] = key
+    b.check(samhip, gpu_ctx)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", range(len(FORMS)))
+@pytest.mark.parametrize("large", [2.0 ** 40, 1e30])
+def test_a_large_dimension_leaves_the_others(samhip, gpu_ctx, form, large):
+    """Dimension 5 of one value row is far larger, at an ordinary weight: so are
+    that dimension's results, and the others keep their digits in the rows of
+    other tiles (its own 64 are zero), smaller ones among them."""
+    b = Batch(*FORMS[form], 4, 2, 64, "f32", seed=22)
+    b.pv[64:128] = 0.0
+    b.pv[70, 5] = large
+    b.pv[130:190].mul_(2.0 ** -30)
+    b.check(samhip, gpu_ctx)
+
+
 def test_refusals(samhip):
     L = samhip.lib()
 
