@@ -359,8 +359,8 @@ int samhip_flash_attn(samhip_context* ctx, const float* q, const float* k, const
  * of a request's n sees its first own_len - n + i + 1 own keys (and all of the
  * prefix).  A query without any key gets zeros; rows of out outside
  * [q_start[0], q_start[requests]) are left as they were.  Rows behind own_len
- * are not read, and a row that is not finite reaches only the queries that see
- * it.  Digits begin to be lost of F32 keys, and values, 2^18 times below the
+ * are not read; a key that is not finite reaches only the queries that see it,
+ * such a value only that dimension of theirs.  Digits begin to be lost of F32 keys, and values, 2^18 times below the
  * largest of 64 neighbouring rows, which share a scale; of weights 2^12 times
  * below the largest of their query (2^-34 of it at most); and of a row of
  * values 2^75 times below what others have come to.

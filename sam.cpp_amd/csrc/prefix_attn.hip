@@ -72,6 +72,8 @@ __device__ __forceinline__ void split_pair(float2_t x, half8& hi, half8& lo, int
 #endif
 }
 
+constexpr uint32_t INF_BITS = 0x7f800000u;
+
 // Eight neighbouring values as loaded.
 template <class T>
 struct Raw8;
@@ -79,15 +81,18 @@ template <>
 struct Raw8<_Float16> {
     half8 v;
     __device__ __forceinline__ void load(const _Float16* p) { v = *reinterpret_cast<const half8_at*>(p); }
-    // zeros for values of which one is not finite; whether that was so
-    __device__ __forceinline__ bool clear_non_finite() {
+    __device__ __forceinline__ bool finite() const {
+        typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
         typedef uint16_t ushort8 __attribute__((ext_vector_type(8)));
-        const ushort8 bits = __builtin_bit_cast(ushort8, v);
-        bool bad = false;
+        const ushort8 bits = __builtin_bit_cast(ushort8, v) & (uint16_t)0x7fff;
+        ushort2_t m{bits[0], bits[1]};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) bad = bad || (bits[j] & 0x7c00) == 0x7c00;
-        if (bad) v = half8{};
-        return bad;
+        for (int j = 2; j < 8; j += 2) m = __builtin_elementwise_max(m, ushort2_t{bits[j], bits[j + 1]});
+        return m[0] < 0x7c00 && m[1] < 0x7c00;
+    }
+    __device__ __forceinline__ void clear_non_finite() {   // zeros instead
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __builtin_fabsf16(v[j]) < (_Float16)__builtin_inff16() ? v[j] : (_Float16)0;
     }
 };
 template <>
@@ -106,10 +111,13 @@ struct Raw8<float> {
         }
         return m;
     }
-    __device__ __forceinline__ bool clear_non_finite() {
-        const bool bad = magnitude() >= 0x7f800000u;
-        if (bad) a = b = floatx4{};
-        return bad;
+    __device__ __forceinline__ bool finite() const { return magnitude() < INF_BITS; }
+    __device__ __forceinline__ void clear_non_finite() {   // zeros instead
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            a[j] = __builtin_fabsf(a[j]) < __builtin_inff() ? a[j] : 0.f;
+            b[j] = __builtin_fabsf(b[j]) < __builtin_inff() ? b[j] : 0.f;
+        }
     }
     // values * factor as hi + lo
     __device__ __forceinline__ void split(float factor, half8& hi, half8& lo) const {
@@ -130,6 +138,28 @@ __device__ __forceinline__ float down(int e) { return __uint_as_float(uint32_t(2
 __device__ __forceinline__ float up(int e) { return __uint_as_float(uint32_t(e - 14) << 23); }      // 2^(e - 141)
 
 __device__ __forceinline__ uint32_t wave_umax(uint32_t v) { return umax_xor32(umax_xor16(umax_row(umax_quad(v)))); }
+
+// The largest magnitude of a wave's keys or values.  An infinity or a NaN, which
+// stays in its key's scores or its value's dimension, does not set the others'
+// scale.
+template <int N>
+__device__ __forceinline__ uint32_t largest_finite(const Raw8<float> (&v)[N]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = umax(m, v[i].magnitude());
+    m = __builtin_amdgcn_readfirstlane(wave_umax(m));
+    if (m >= INF_BITS) {
+        m = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            Raw8<float> finite = v[i];
+            finite.clear_non_finite();
+            m = umax(m, finite.magnitude());
+        }
+        m = __builtin_amdgcn_readfirstlane(wave_umax(m));
+    }
+    return m;
+}
 
 // What a workgroup reads: keys [k0, k1) of one kv head, for query rows
 // [q0, q0 + n) in flattened (row, head in group) places.
@@ -203,6 +233,20 @@ struct Sums {
             for (int r = 0; r < 16; ++r) o[d][r] = __builtin_ldexpf(o[d][r], by);
     }
 
+    // Those of a row of values that are not finite
+    template <class T>
+    __device__ __forceinline__ void add_non_finite(const T* row) {
+        const int hh = (threadIdx.x & 63) >> 5;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float v = float(row[32 * d + 8 * (r >> 2) + 4 * hh + (r & 3)]);
+                if ((__float_as_uint(v) & 0x7fffffffu) >= INF_BITS) o[d][r] += v;
+                asm volatile("" ::: "memory");   // one at a time, for the registers
+            }
+    }
+
     // F32 values of one tile, whose largest has exponent `to` (0: all zero), come
     // in units of 2^(to - 141).  The sums follow it, down where they leave room:
     // values 2^75 apart keep their digits beside each other.  Returns how many
@@ -221,7 +265,7 @@ struct Sums {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const uint32_t b = __float_as_uint(o[d][r]) & 0x7fffffffu;
-                    most = umax(most, b < 0x7f800000u ? b : 0u);
+                    most = umax(most, b < INF_BITS ? b : 0u);
                 }
             const int room = 251 - int(__builtin_amdgcn_readfirstlane(wave_umax(most)) >> 23);   // they stay below 2^125
             const int by = min(e - to, max(room, 0));
@@ -401,23 +445,21 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
         }
     };
     // Keys below this one are seen by every place.  In a tile that reaches
-    // further a weight of zero keeps no infinity or NaN out, so such keys and
-    // values are replaced by zeros and the places that see them get a NaN sum.
+    // further a weight of zero keeps no infinity or NaN out: such values are
+    // zeros in it, and are added behind the last tile for those that see them.
     const int seen_by_all = s.causal ? s.limit0 + s.first / a.group : s.k1 + TILE;
+    bool non_finite_values = false;
     if (AHEAD && kw < s.k1) load(kw);
     for (int k = kw; k < s.k1; k += step) {
         if (!AHEAD) load(k);
-        uint32_t bad = 0;   // keys k + n of the tile
         if (k + TILE > seen_by_all) {
+            bool finite = true;
 #pragma unroll
-            for (int t = 0; t < STEPS; ++t) {
-                bad |= kr[t].clear_non_finite() ? 1u << li : 0u;
-                bad |= vr[t].clear_non_finite() ? 1u << (key + t * (512 / HD)) : 0u;
-            }
-            if (__any(bad != 0)) {
-                uint32_t all = 0;
-                for (int n = 0; n < TILE; ++n) all |= __any(bad >> n & 1) ? 1u << n : 0u;
-                bad = all;
+            for (int t = 0; t < STEPS; ++t) finite = finite && vr[t].finite();
+            if (!__all(finite)) {
+                non_finite_values = true;
+#pragma unroll
+                for (int t = 0; t < STEPS; ++t) vr[t].clear_non_finite();
             }
         }
         floatx16 sc[1];
@@ -426,11 +468,8 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
         float c = q.factor(1.f), fv = 1.f;
         int low = 0;
         if constexpr (F32) {
-            uint32_t m = 0, mv = 0;
-#pragma unroll
-            for (int t = 0; t < STEPS; ++t) m = umax(m, kr[t].magnitude()), mv = umax(mv, vr[t].magnitude());
-            const int e = exponent_of(__builtin_amdgcn_readfirstlane(wave_umax(m)));
-            mv = __builtin_amdgcn_readfirstlane(wave_umax(mv));
+            const int e = exponent_of(largest_finite(kr));
+            const uint32_t mv = largest_finite(vr);
             fv = down(exponent_of(mv));
             c = q.factor(up(e));
 #pragma unroll
@@ -456,9 +495,12 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
         if (AHEAD && k + step < s.k1) load(k + step);
         half8 ph[2], pl[2];
         sums.weigh(sc, c, k, q.limit, low, ph, pl);
-        if (bad && q.limit > k && bad << max(k + TILE - q.limit, 0)) sums.l = __builtin_nanf("");
         values<T, HD, 1>(vt, ph, pl, sums);
     }
+    if (non_finite_values)
+        for (int k = kw; k < s.k1; k += step)
+            for (int n = k + TILE > seen_by_all ? 0 : TILE; n < TILE; ++n)
+                if (k + n < q.limit) sums.add_non_finite(s.v + int64_t(k + n) * s.ldv);
     // the four waves' sums, joined through LDS
     sums.l = pair_sum(sums.l);
     if (hh == 0) {
@@ -549,11 +591,11 @@ __device__ __forceinline__ void attend_wide(const PrefixAttnArgs& a, const Span<
         float c = q.factor(1.f), fk = 1.f, fv = 1.f;
         int low = 0;
         if constexpr (F32) {
-            uint32_t mk = 0, mv = 0;
+            uint32_t mk = 0;
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i) mk = umax(mk, kr[i].magnitude()), mv = umax(mv, vr[i].magnitude());
+            for (int i = 0; i < PIECES; ++i) mk = umax(mk, kr[i].magnitude());
             mk = wave_umax(mk);
-            mv = wave_umax(mv);
+            const uint32_t mv = largest_finite(vr);
             if (lane == 0) sh.largest[wave][0] = mk, sh.largest[wave][1] = mv;
         }
         __syncthreads();   // the last tile is read, the largest magnitudes are written

@@ -332,6 +332,34 @@ def test_a_large_dimension_leaves_the_others(samhip, gpu_ctx, form, large):
     b.check(samhip, gpu_ctx)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", range(len(FORMS)))
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_non_finite_values_reach_only_their_dimension(samhip, gpu_ctx, dtype, causal, form):
+    """Value 70 of the prefix holds an infinity in dimension 5 of kv head 0, the
+    first request's own value 30 a NaN in dimension 9 and own value 33 a -inf in
+    dimension 40 of kv head 1 (of 64)."""
+    b = Batch(*FORMS[form], 4, 2, 64, dtype, causal=causal, seed=23)
+    ref, bound = b.reference()
+    b.pv[70, 5] = float("inf")
+    reached = torch.zeros(b.q.shape[0], 4, 64, dtype=torch.bool, device="cuda")
+    reached[:, :2, 5] = True
+    if b.own_len[0]:
+        b.ov[30, 64 + 9] = float("nan")
+        b.ov[33, 64 + 40] = float("-inf")
+        for key, d in ((30, 9), (33, 40)):
+            n = b.q_len[0]
+            reached[max(0, key - (b.own_len[0] - n)) if causal else 0:n, 2:, d] = True
+    torch.cuda.synchronize()
+    gpu_ctx.prefix_attn(b.desc(samhip))
+    gpu_ctx.synchronize()
+    out = b.out.view(-1, 4, 64)
+    assert torch.equal(~out.isfinite(), reached)
+    err, most = (out.double() - ref.view(-1, 4, 64)).abs(), bound.view(-1, 4, 64)
+    assert (err[~reached] <= most[~reached]).all(), (err[~reached] / most[~reached]).max().item()
+
+
 def test_refusals(samhip):
     L = samhip.lib()
 
