@@ -403,8 +403,8 @@ enum samhip_activation {
  * leave rows and images apart;
  * mean and biased variance over the channels / groups neighbouring channels
  * of a group in every pixel of one image (F32 runs of up to 512 values'
- * differences from one of them, joined in F64; deviations within 1e-18 ..
- * 1e18).  w, b: device F32
+ * differences from the mean of the first of them, joined in F64; deviations
+ * within 1e-18 .. 1e18).  w, b: device F32
  * [channels], each may be NULL.  channels a multiple of groups, at most 4096;
  * images at most 65535.  y may be x itself (same type and strides), and
  * overlaps nothing else.  A non-finite value makes its group's outputs

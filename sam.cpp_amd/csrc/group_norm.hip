@@ -3,9 +3,9 @@
 //   y = act((x - mean) / sqrt(var + eps) * w + b)
 // with mean and var (biased) over a group's channels of every pixel of one
 // image.  Runs of up to 512 values sum x - shift and its square in F32, the
-// shift a value of the run, and are joined in F64, where neither a group of
-// millions of values nor a mean far above the deviation costs digits; the
-// mean is subtracted as two floats (hi, then lo).  So one pass over the data
+// shift the mean of the run's first values, and are joined in F64, where
+// neither a group of millions of values nor a mean far above the deviation
+// costs digits; the mean is subtracted as two floats (hi, then lo).  So one pass over the data
 // gives the statistics.
 //   group_norm_block_kernel : one workgroup per (image, group) with the
 //                             group's values in registers: x read once
@@ -110,11 +110,15 @@ __device__ __forceinline__ void store(T* p, int n, const float (&v)[VEC]) {
     if (n & 1) p[at] = (T)a;
 }
 
-// Sums of x and x^2: F32 runs of x - shift, with a value of the run itself as
-// the shift, so that a mean far above the deviation cancels exactly; what a
-// run leaves goes to F64.
+// Sums of x and x^2: F32 runs of x - shift, so that a mean far above the
+// deviation cancels; what a run leaves goes to F64.  With the mean of k of the
+// run's n values as the shift, s2 is at most 1 + n / k times the run's squared
+// deviations, wherever outliers stand (with one value, which may be the
+// outlier, 1 + n times: 4e-5 of the variance lost at n = 256).  It need not be
+// exact: `inv` is about 1 / k.
 struct Run {
-    float shift, s1 = 0.f, s2 = 0.f;
+    float shift = 0.f, s1 = 0.f, s2 = 0.f;
+    __device__ __forceinline__ void aim(float x, float inv) { shift = __builtin_fmaf(x, inv, shift); }
     __device__ __forceinline__ void add(float x) {
         const float d = x - shift;
         s1 += d;
@@ -232,7 +236,12 @@ __global__ __launch_bounds__(1024) void group_norm_block_kernel(const TI* x, TO*
     gain_and_bias<VEC>(w, b, g * size + c, g * size + size - 1, ww, bb);
     double sum = 0.0, sq = 0.0;
     {
-        Run run{(float)v[0][0]};
+        Run run;
+        const float inv = __builtin_amdgcn_rcpf((float)(count * n));
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) run.aim(i < count && e < n ? (float)v[i][e] : 0.f, inv);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -300,9 +309,16 @@ __global__ __launch_bounds__(256) void group_norm_stats_kernel(const TI* __restr
                         for (int u = 0; u < FLIGHT; ++u)
                             v[u] = load<decltype(edge)::value>(xi + min(p + u * rows, p1 - 1) * s.x_pixel, col * VEC, s.channels);
                     });
-                    if (k == 0)
+                    if (k == 0) {
+                        int pixels = 1;
 #pragma unroll
-                        for (int e = 0; e < RUNS; ++e) run[e].shift = (float)v[0][e];
+                        for (int u = 1; u < FLIGHT; ++u) pixels += p + u * rows < p1;
+                        const float inv = __builtin_amdgcn_rcpf((float)(SAME ? pixels * VEC : pixels));
+#pragma unroll
+                        for (int u = 0; u < FLIGHT; ++u)
+#pragma unroll
+                            for (int e = 0; e < VEC; ++e) run[SAME ? 0 : e].aim(p + u * rows < p1 ? (float)v[u][e] : 0.f, inv);
+                    }
 #pragma unroll
                     for (int u = 0; u < FLIGHT; ++u)
                         if (p + u * rows < p1)

@@ -148,6 +148,26 @@ def test_captured_replays(samhip, gpu_ctx):
     graph.destroy()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,dtype", [((1, 82944, 256, 8), "f32"), ((1, 82944, 256, 8), "f16"), ((1, 40000, 345, 15), "f32"), ((2, 9000, 30, 6), "f16"),
+                                         ((24, 2048, 256, 8), "f16"), ((24, 1024, 256, 8), "f32"), ((1, 900, 36, 4), "f32")])
+@pytest.mark.parametrize("where", ["first", "two", "every 81st", "last"])
+@pytest.mark.parametrize("large", [300.0, -1e4])
+def test_outliers_wherever_they_stand(samhip, gpu_ctx, shape, dtype, where, large):
+    """Values far from all others, as the first ones of a run and elsewhere.  An
+    F32 run of 512 rounds its sum of squares by sqrt(512 / 3) half steps of 2^-24.5
+    on average, 5.5e-7 of it; about the mean of the run's first batch of 32 or
+    more that sum is at most 1.25 times the squared deviations; half of it
+    reaches 1 / deviation: 3.4e-7 beside the 5e-7 of the other steps."""
+    n, p, c, groups = shape
+    x = torch.randn(n, p, c, device="cuda", generator=torch.Generator(device="cuda").manual_seed(6)).to(torch.float16 if dtype == "f16" else torch.float32)
+    x[:, {"first": slice(0, 1), "two": slice(0, 2), "every 81st": slice(0, None, 81), "last": slice(p - 1, None)}[where], ::c // groups] = large
+    y = torch.empty(n, p, c, device="cuda")
+    call(samhip, gpu_ctx, x, y, groups, None, None, 1e-5, "none")
+    ref = definition(x, groups, None, None, 1e-5, "none")
+    assert ((y.double() - ref).norm() / ref.norm()).item() < 1e-6
+
+
 def test_refusals(samhip):
     def ok(ne=(64, 10, 2), nb=None, yne=None, ynb=None, xt=0, yt=0, groups=8, eps=1e-5, act=1, data=0x10000, w=None):
         e = 2 if xt == 1 else 4
