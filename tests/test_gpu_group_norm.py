@@ -148,6 +148,26 @@ def test_captured_replays(samhip, gpu_ctx):
     graph.destroy()
 
 
+def sum_in_steps(t):
+    """Sums over the first dimension, of at most 256 terms at once: torch's one
+    sum over many blocks of F64 has lost a block's part here now and then."""
+    while t.shape[0] > 1:
+        t = torch.nn.functional.pad(t, (0, 0) * (t.dim() - 1) + (0, -t.shape[0] % 256)) if t.shape[0] > 256 else t
+        t = t.view(-1, min(t.shape[0], 256), *t.shape[1:]).sum(1)
+    return t[0]
+
+
+def relative_error(y, x, groups, eps):
+    """Of outputs without gain, bias and activation, relative L2."""
+    n, p, c = x.shape
+    v = x.double().reshape(n, p, groups, c // groups)
+    mean = (sum_in_steps(v.sum(3).transpose(0, 1).contiguous()) * groups / (p * c))[:, None, :, None]
+    var = (sum_in_steps((v - mean).square().sum(3).transpose(0, 1).contiguous()) * groups / (p * c))[:, None, :, None]
+    ref = ((v - mean) / torch.sqrt(var + eps)).reshape(n * p, c)
+    off, all = ((t.square().sum(1)) for t in (y.double().reshape(n * p, c) - ref, ref))
+    return (sum_in_steps(off) / sum_in_steps(all)).sqrt().item()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape,dtype", [((1, 82944, 256, 8), "f32"), ((1, 82944, 256, 8), "f16"), ((1, 40000, 345, 15), "f32"), ((2, 9000, 30, 6), "f16"),
                                          ((24, 2048, 256, 8), "f16"), ((24, 1024, 256, 8), "f32"), ((1, 900, 36, 4), "f32")])
@@ -164,8 +184,7 @@ def test_outliers_wherever_they_stand(samhip, gpu_ctx, shape, dtype, where, larg
     x[:, {"first": slice(0, 1), "two": slice(0, 2), "every 81st": slice(0, None, 81), "last": slice(p - 1, None)}[where], ::c // groups] = large
     y = torch.empty(n, p, c, device="cuda")
     call(samhip, gpu_ctx, x, y, groups, None, None, 1e-5, "none")
-    ref = definition(x, groups, None, None, 1e-5, "none")
-    assert ((y.double() - ref).norm() / ref.norm()).item() < 1e-6
+    assert relative_error(y, x, groups, 1e-5) < 1e-6
 
 
 def test_refusals(samhip):
