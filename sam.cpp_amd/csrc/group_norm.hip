@@ -3,10 +3,11 @@
 //   y = act((x - mean) / sqrt(var + eps) * w + b)
 // with mean and var (biased) over a group's channels of every pixel of one
 // image.  Runs of up to 512 values sum x - shift and its square in F32, the
-// shift the mean of the run's first values, and are joined in F64, where
-// neither a group of millions of values nor a mean far above the deviation
-// costs digits; the mean is subtracted as two floats (hi, then lo).  So one pass over the data
-// gives the statistics.
+// shift the mean of the run's first values, and are joined in F64 as sums of
+// x - base, the base a group's first value, so that neither a group of millions
+// of values nor a mean far above the deviation costs digits; the mean is
+// subtracted as two floats (hi, then lo).  So one pass over the data gives the
+// statistics.
 //   group_norm_block_kernel : one workgroup per (image, group) with the
 //                             group's values in registers: x read once
 //   group_norm_stats_kernel, _finish_kernel, _apply_kernel : larger groups
@@ -110,8 +111,9 @@ __device__ __forceinline__ void store(T* p, int n, const float (&v)[VEC]) {
     if (n & 1) p[at] = (T)a;
 }
 
-// Sums of x and x^2: F32 runs of x - shift, so that a mean far above the
-// deviation cancels; what a run leaves goes to F64.  With the mean of k of the
+// Sums of x - base and its square: F32 runs of x - shift, so that a mean far
+// above the deviation cancels; what a run leaves goes to F64, about a base that
+// all runs of a group share.  With the mean of k of the
 // run's n values as the shift, s2 is at most 1 + n / k times the run's squared
 // deviations, wherever outliers stand (with one value, which may be the
 // outlier, 1 + n times: 4e-5 of the variance lost at n = 256).  It need not be
@@ -124,8 +126,8 @@ struct Run {
         s1 += d;
         s2 = __builtin_fmaf(d, d, s2);
     }
-    __device__ __forceinline__ void into(float n, double& sum, double& sq) const {
-        const double a = shift, s = s1;
+    __device__ __forceinline__ void into(float n, float base, double& sum, double& sq) const {
+        const double a = (double)shift - (double)base, s = s1;
         sum += __builtin_fma((double)n, a, s);
         sq += __builtin_fma(a, __builtin_fma((double)n, a, 2.0 * s), (double)s2);
     }
@@ -162,9 +164,12 @@ struct Moments {
 
 constexpr int kGroupNormInline = 2048;   // partial sums that every workgroup of the last launch adds up itself
 
-__device__ __forceinline__ Moments moments(double sum, double sq, double n, float eps) {
-    const double mean = sum / n;
-    double var = sq / n - mean * mean;   // F64: loses (mean / deviation)^2 of 2^-53
+// From sums of x - base and its square.  The base is one of the n values, so
+// that its distance from the mean is at most sqrt(n) deviations, and the
+// variance loses at most n 2^-53 of itself.
+__device__ __forceinline__ Moments moments(double sum, double sq, double n, double base, float eps) {
+    const double off = sum / n, mean = base + off;
+    double var = sq / n - off * off;
     var = var < 0.0 ? 0.0 : var;         // a NaN stays one
     Moments m;
     m.hi = (float)mean;
@@ -222,6 +227,7 @@ __global__ __launch_bounds__(1024) void group_norm_block_kernel(const TI* x, TO*
     const int count = row < rows && row < s.pixels ? (s.pixels - 1 - row) / rows + 1 : 0;   // at most NV
     const int64_t first = min(row, s.pixels - 1), x_step = rows * s.x_pixel, y_step = rows * s.y_pixel;
     const TI* xg = x + image * s.x_image + first * s.x_pixel;
+    const float base = (float)x[image * s.x_image + g * size];
     TO* yg = y + image * s.y_image + g * size + c + first * s.y_pixel;
     Vector<TI> v[NV];
     const auto fetch = [&](auto edge) {
@@ -246,7 +252,7 @@ __global__ __launch_bounds__(1024) void group_norm_block_kernel(const TI* x, TO*
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) run.add(i < count && e < n ? (float)v[i][e] : run.shift);
-        if (count) run.into((float)(count * n), sum, sq);
+        if (count) run.into((float)(count * n), base, sum, sq);
     }
     sum = wave_sum(sum);
     sq = wave_sum(sq);
@@ -260,7 +266,7 @@ __global__ __launch_bounds__(1024) void group_norm_block_kernel(const TI* x, TO*
         sum += part[i][0];
         sq += part[i][1];
     }
-    const Moments m = moments(sum, sq, double(s.pixels) * size, eps);
+    const Moments m = moments(sum, sq, double(s.pixels) * size, base, eps);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
         ww[e] = ww[e] * m.rstd;
@@ -292,13 +298,20 @@ __global__ __launch_bounds__(256) void group_norm_stats_kernel(const TI* __restr
     const int tid = threadIdx.x, cols = (s.channels + VEC - 1) / VEC;
     const int width = min(cols, 256), rows = 256 / width, row = tid / width, col0 = tid - row * width;
     const int p0 = blockIdx.x * chunk + row, p1 = min((blockIdx.x + 1) * chunk, s.pixels);
-    const int plane = rows * RUNS * cols;
+    const int plane = rows * RUNS * cols, size = s.channels / s.groups;
+    const TI* xi = x + blockIdx.y * s.x_image;
+    const TI early = xi[min(tid, s.groups - 1) * size];   // a group's base, under way from here
     if (row < rows) {
         for (int col = col0; col < cols; col += width) {
             double sum[RUNS], sq[RUNS];
+            TI base[RUNS];
+            int first = col * VEC / size * size, behind = first + size;   // the group's channels
 #pragma unroll
-            for (int e = 0; e < RUNS; ++e) sum[e] = sq[e] = 0.0;
-            const TI* xi = x + blockIdx.y * s.x_image;
+            for (int e = 0; e < RUNS; ++e) {
+                sum[e] = sq[e] = 0.0;
+                if (col * VEC + e == behind) first = behind, behind += size;
+                base[e] = xi[min(first, s.channels - 1)];
+            }
             for (int p = p0; p < p1;) {
                 const int q = p;
                 Run run[RUNS];
@@ -316,8 +329,9 @@ __global__ __launch_bounds__(256) void group_norm_stats_kernel(const TI* __restr
                         const float inv = __builtin_amdgcn_rcpf((float)(SAME ? pixels * VEC : pixels));
 #pragma unroll
                         for (int u = 0; u < FLIGHT; ++u)
+                            if (p + u * rows < p1)
 #pragma unroll
-                            for (int e = 0; e < VEC; ++e) run[SAME ? 0 : e].aim(p + u * rows < p1 ? (float)v[u][e] : 0.f, inv);
+                                for (int e = 0; e < VEC; ++e) run[SAME ? 0 : e].aim((float)v[u][e], inv);
                     }
 #pragma unroll
                     for (int u = 0; u < FLIGHT; ++u)
@@ -327,7 +341,13 @@ __global__ __launch_bounds__(256) void group_norm_stats_kernel(const TI* __restr
                 }
                 const float count = (float)((min(p, p1) - q + rows - 1) / rows * (SAME ? VEC : 1));
 #pragma unroll
-                for (int e = 0; e < RUNS; ++e) run[e].into(count, sum[e], sq[e]);
+                for (int e = 0; e < RUNS; ++e) {
+                    TI b = base[e];
+#if defined(__HIP_DEVICE_COMPILE__)
+                    asm("" : "+v"(b));   // not converted ahead of the loop, which would wait for it there
+#endif
+                    run[e].into(count, (float)b, sum[e], sq[e]);
+                }
             }
 #pragma unroll
             for (int e = 0; e < RUNS; ++e) {
@@ -337,7 +357,6 @@ __global__ __launch_bounds__(256) void group_norm_stats_kernel(const TI* __restr
         }
     }
     __syncthreads();
-    const int size = s.channels / s.groups;
     const int members = SAME ? size / VEC : size, all = rows * members;
     // as many lanes per group as leave a place for every group, 64 at most
     int lanes = 64;
@@ -353,20 +372,27 @@ __global__ __launch_bounds__(256) void group_norm_stats_kernel(const TI* __restr
         sum = lane_sum(sum, lanes);
         sq = lane_sum(sq, lanes);
         if ((tid & (lanes - 1)) == 0) {
-            double* out = partial + ((int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * s.groups + g) * 2;
+            double* out = partial + ((int64_t(blockIdx.y) * (gridDim.x + 1) + blockIdx.x) * s.groups + g) * 2;
             out[0] = sum;
             out[1] = sq;
         }
+    }
+    if (blockIdx.x == 0) {
+        double* bases = partial + (int64_t(blockIdx.y) * (gridDim.x + 1) + gridDim.x) * s.groups * 2;
+        for (int g = tid; g < s.groups; g += 256) bases[2 * g] = (double)(g == tid ? early : xi[g * size]);
     }
 }
 
 // An image's partial sums over its chunks, by 256 threads: thread t adds
 // every (256 / groups)-th chunk's of group t % groups, neighbours reading
-// neighbouring places.  `out` has a place for each group.
+// neighbouring places.  The groups' bases stand behind the last chunk's sums.
+// `out` has a place for each group.
 __device__ __forceinline__ void finish(const double* __restrict__ partial, int chunks, int groups, double n, float eps,
                                        double (*lds)[2], Moments* out) {
     typedef double double2_t __attribute__((ext_vector_type(2)));
     const int tid = threadIdx.x;
+    const double* bases = partial + int64_t(chunks) * groups * 2;
+    double base = bases[2 * min(tid, groups - 1)];   // here, not in the loop, which would wait for all loads at its head
     for (int g0 = 0; g0 < groups; g0 += 256) {
         const int here = min(groups - g0, 256), step = 256 / here, c0 = tid / here, g = tid - c0 * here;
         double sum = 0.0, sq = 0.0;
@@ -387,8 +413,9 @@ __device__ __forceinline__ void finish(const double* __restrict__ partial, int c
                 sum += lds[tid + i * here][0];
                 sq += lds[tid + i * here][1];
             }
-            out[g0 + tid] = moments(sum, sq, n, eps);
+            out[g0 + tid] = moments(sum, sq, n, base, eps);
         }
+        if (g0 + 256 < groups) base = bases[2 * min(g0 + 256 + tid, groups - 1)];
         __syncthreads();
     }
 }
@@ -396,7 +423,7 @@ __device__ __forceinline__ void finish(const double* __restrict__ partial, int c
 __global__ __launch_bounds__(256) void group_norm_finish_kernel(const double* __restrict__ partial, int chunks, int groups, double n,
                                                                 float eps, Moments* __restrict__ out) {
     __shared__ double lds[256][2];
-    finish(partial + int64_t(blockIdx.x) * chunks * groups * 2, chunks, groups, n, eps, lds, out + int64_t(blockIdx.x) * groups);
+    finish(partial + int64_t(blockIdx.x) * (chunks + 1) * groups * 2, chunks, groups, n, eps, lds, out + int64_t(blockIdx.x) * groups);
 }
 
 // FINISH: the workgroups add up the partial sums themselves.
@@ -431,7 +458,7 @@ __global__ __launch_bounds__(256) void group_norm_apply_kernel(const TI* x, TO* 
         gain_and_bias<VEC>(w, b, col0 * VEC, s.channels - 1, ww, bb);
     }
     if constexpr (FINISH) {
-        finish(partial + int64_t(blockIdx.y) * chunks * s.groups * 2, chunks, s.groups, double(s.pixels) * size, eps, lds, shared);
+        finish(partial + int64_t(blockIdx.y) * (chunks + 1) * s.groups * 2, chunks, s.groups, double(s.pixels) * size, eps, lds, shared);
         __syncthreads();
     }
     const auto moments_of = [&](int g) -> Moments {   // from LDS or from memory, never from either by one pointer
@@ -515,7 +542,7 @@ void launch_typed(const TI* x, TO* y, const GroupNormShape& s, const float* w, c
     else group_norm_stats_kernel<TI, false><<<grid, 256, lds * VEC, stream>>>(x, s, chunk, partial);
     Moments* stats = nullptr;
     if (int64_t(chunks) * s.groups > kGroupNormInline) {
-        stats = reinterpret_cast<Moments*>(partial + int64_t(s.images) * chunks * s.groups * 2);
+        stats = reinterpret_cast<Moments*>(partial + int64_t(s.images) * (chunks + 1) * s.groups * 2);
         group_norm_finish_kernel<<<s.images, 256, 0, stream>>>(partial, chunks, s.groups, double(s.pixels) * size, eps, stats);
     }
 #define SAMHIP_GN_APPLY(SAME, PAST) \
@@ -562,7 +589,7 @@ int group_norm_stats_chunk(const GroupNormShape& s, int vec) {
 size_t group_norm_scratch_bytes(const GroupNormShape& s, int vec) {
     if (group_norm_one_launch(s, vec)) return 0;
     const int chunk = group_norm_stats_chunk(s, vec), chunks = (s.pixels + chunk - 1) / chunk;
-    return (size_t(chunks) * 16 + sizeof(Moments)) * s.images * s.groups;
+    return ((size_t(chunks) + 1) * 16 + sizeof(Moments)) * s.images * s.groups;
 }
 
 void launch_group_norm(const void* x, int x_type, void* y, int y_type, const GroupNormShape& s, const float* w, const float* b,

@@ -187,6 +187,19 @@ def test_outliers_wherever_they_stand(samhip, gpu_ctx, shape, dtype, where, larg
     assert relative_error(y, x, groups, 1e-5) < 1e-6
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("p", [200, 40000])
+@pytest.mark.parametrize("mean", [1e5, -3e6])
+@pytest.mark.parametrize("channels", [32, 28])
+def test_mean_a_million_deviations_away(samhip, gpu_ctx, p, mean, channels):
+    """F64 sums of squares would keep four digits of the variance here.  The
+    reference takes x as rounded to F32."""
+    x = torch.randn(2, p, channels, device="cuda", generator=torch.Generator(device="cuda").manual_seed(7)) + mean
+    y = torch.empty_like(x)
+    call(samhip, gpu_ctx, x, y, 4, None, None, 1e-5, "none")
+    assert relative_error(y, x, 4, 1e-5) < 1e-6
+
+
 def test_refusals(samhip):
     def ok(ne=(64, 10, 2), nb=None, yne=None, ynb=None, xt=0, yt=0, groups=8, eps=1e-5, act=1, data=0x10000, w=None):
         e = 2 if xt == 1 else 4
