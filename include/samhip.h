@@ -125,7 +125,10 @@ int samhip_device_count(int* count);
 int samhip_context_create(const samhip_options* options, samhip_context** out);
 void samhip_context_destroy(samhip_context* ctx);
 /* Run subsequent calls on `hip_stream` (a hipStream_t); NULL restores the
- * context's own stream. */
+ * context's own stream.  The new stream waits (hipStreamWaitEvent) for what is
+ * queued on the old one, since calls share the context's scratch.  Not so where
+ * the caller is capturing either of them into a graph of its own: then the
+ * caller orders the calls, replays included. */
 int samhip_context_set_stream(samhip_context* ctx, void* hip_stream);
 int samhip_synchronize(samhip_context* ctx);
 

@@ -111,6 +111,7 @@ struct samhip_context {
     int q8_rounding = SAMHIP_Q8_ROUND_X86;
     hipStream_t own_stream = nullptr;
     hipStream_t stream = nullptr;
+    hipEvent_t switched = nullptr;   // samhip_context_set_stream's, from its first use on
     // staged fp16 activations [M][K], F32 row scales [M] and, on the tall
     // path, the call's fp16 weights [N][K]
     void* staging = nullptr;
@@ -500,6 +501,7 @@ void samhip_context_destroy(samhip_context* ctx) {
         (void)hipEventDestroy(r.stop);
     }
     for (hipEvent_t e : ctx->event_pool) (void)hipEventDestroy(e);
+    if (ctx->switched) (void)hipEventDestroy(ctx->switched);
     if (ctx->own_stream) (void)hipStreamDestroy(ctx->own_stream);
     delete ctx;
 }
@@ -507,7 +509,25 @@ void samhip_context_destroy(samhip_context* ctx) {
 int samhip_context_set_stream(samhip_context* ctx, void* hip_stream) {
     if (!ctx) return fail(SAMHIP_ERR_INVALID_ARGUMENT, "null context");
     SAMHIP_NOT_WHILE_CAPTURING(ctx, "context_set_stream");
-    ctx->stream = hip_stream ? static_cast<hipStream_t>(hip_stream) : ctx->own_stream;
+    const hipStream_t next = hip_stream ? static_cast<hipStream_t>(hip_stream) : ctx->own_stream;
+    if (next == ctx->stream) return SAMHIP_OK;
+    if (int rc = set_device(ctx)) return rc;
+    // Calls leave what their next launch reads in the context's scratch, and
+    // the next call on the other stream would write over it: that stream waits.
+    // An event cannot join a stream that the caller is capturing to one outside
+    // of that capture, and there is no work on a stream that is gone.
+    const auto ordinary = [](hipStream_t s) {
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(s, &status) == hipSuccess) return status == hipStreamCaptureStatusNone;
+        (void)hipGetLastError();
+        return false;
+    };
+    if (ordinary(ctx->stream) && ordinary(next)) {
+        if (!ctx->switched) HIP_TRY(hipEventCreateWithFlags(&ctx->switched, hipEventDisableTiming), "hipEventCreate");
+        HIP_TRY(hipEventRecord(ctx->switched, ctx->stream), "hipEventRecord");
+        HIP_TRY(hipStreamWaitEvent(next, ctx->switched, 0), "hipStreamWaitEvent");
+    }
+    ctx->stream = next;
     return SAMHIP_OK;
 }
 

@@ -172,3 +172,41 @@ def test_runs_on_the_callers_stream(samhip):
         for n in want:
             assert torch.equal(got[n], want[n]), n
         ctx.set_stream(None)
+
+
+def test_a_switch_of_streams_orders_the_calls(samhip):
+    """Calls on one stream, still waiting behind other work, share the context's
+    scratch with those made on the next: the next stream waits."""
+    with samhip.Context(0) as ctx:
+        s = Service(samhip, ctx)
+        inputs = []
+        for _ in range(3):
+            s.new_inputs()
+            inputs.append([v.clone() for v in (s.map, s.prompt, s.query)])
+        want = []
+        for given in inputs:
+            for v, k in zip((s.map, s.prompt, s.query), given):
+                v.copy_(k)
+            torch.cuda.synchronize()
+            s.run()
+            ctx.synchronize()
+            want.append({n: v.clone() for n, v in s.t.items()})
+        services = [Service(samhip, ctx) for _ in inputs]
+        streams = [torch.cuda.Stream() for _ in inputs[:2]] + [None]
+        for each, given in zip(services, inputs):
+            for v, k in zip((each.map, each.prompt, each.query), given):
+                v.copy_(k)
+        big = torch.randn(4096, 4096, device="cuda")
+        torch.cuda.synchronize()
+        for each, stream in zip(services, streams):
+            if stream:
+                with torch.cuda.stream(stream):
+                    held = big
+                    for _ in range(4):
+                        held = held @ big * 1e-3
+            ctx.set_stream(stream.cuda_stream if stream else None)
+            each.run()
+        ctx.synchronize()   # the last stream, behind both others
+        for each, expected in zip(services, want):
+            for n in expected:
+                assert torch.equal(each.t[n], expected[n]), n
