@@ -360,6 +360,25 @@ def test_non_finite_values_reach_only_their_dimension(samhip, gpu_ctx, dtype, ca
     assert (err[~reached] <= most[~reached]).all(), (err[~reached] / most[~reached]).max().item()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", range(len(FORMS)))
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("scale", [0.0, -0.125, -2.0, 1e-30])
+def test_scales_of_either_sign_and_zero(samhip, gpu_ctx, scale, dtype, form):
+    b = Batch(*FORMS[form], 4, 2, 64, dtype, causal=True, seed=26)
+    b.scale = abs(scale)
+    if scale < 0:   # as with the queries' signs turned
+        b.q.neg_()
+    ref, bound = b.reference()
+    if scale < 0:
+        b.q.neg_()
+    b.scale = scale
+    torch.cuda.synchronize()
+    gpu_ctx.prefix_attn(b.desc(samhip))
+    gpu_ctx.synchronize()
+    b.verify(ref, bound)
+
+
 def test_refusals(samhip):
     L = samhip.lib()
 
