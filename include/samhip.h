@@ -187,7 +187,7 @@ int samhip_mul_mat_noalloc(samhip_context* ctx, const samhip_tensor* w, const sa
  * with base the shared product, e.g. of samhip_mul_mat.  The adapters stand
  * in banks of equal slots, a (F32 or F16, ne = {K, R, slots, 1}) and b (the
  * same type, ne = {R, N, slots, 1}), with any row and slot strides that leave
- * rows and slots apart; at most 4096 slots. */
+ * rows and slots apart; at most 4096 slots, K to 2^24, N and M to 2^23. */
 typedef struct samhip_lora_bank {
     int32_t version;        /* SAMHIP_ABI_VERSION */
     samhip_tensor a, b;     /* R at most 256 */
@@ -370,7 +370,8 @@ int samhip_flash_attn(samhip_context* ctx, const float* q, const float* k, const
  * The three tables are read on the device (at every replay of a captured
  * call) and cut to what exists: query rows to [0, rows), lengths to
  * [0, own_max] and the rows of own_k; an own_start outside them means no
- * keys.  q_start must not decrease.  out overlaps no other operand. */
+ * keys.  q_start must not decrease.  out overlaps no other operand.  At most
+ * 4096 heads, 2^23 rows * heads, 2^20 requests, 2^30 keys. */
 typedef struct samhip_prefix_attn_desc {
     int32_t version;                  /* SAMHIP_ABI_VERSION */
     int32_t heads, kv_heads;          /* heads a multiple of kv_heads */
@@ -409,7 +410,7 @@ enum samhip_activation {
  * differences from the mean of the first of them, joined in F64; deviations
  * within 1e-18 .. 1e18).  w, b: device F32
  * [channels], each may be NULL.  channels a multiple of groups, at most 4096;
- * images at most 65535.  y may be x itself (same type and strides), and
+ * images at most 65535, pixels 2^30.  y may be x itself (same type and strides), and
  * overlaps nothing else.  A non-finite value makes its group's outputs
  * non-finite.  May be captured. */
 int samhip_supports_group_norm(const samhip_tensor* x, const samhip_tensor* y, int32_t groups, const float* w,

@@ -11,10 +11,10 @@
 //   group_norm_block_kernel : one workgroup per (image, group) with the
 //                             group's values in registers: x read once
 //   group_norm_stats_kernel, _finish_kernel, _apply_kernel : larger groups
-// Bound by HBM for large maps (288 x 288 x 256 F32 with ReLU: 43.7 us, 3.9 TB/s
-// of x once and y; 17 for the sums and 27 for the rest, whose reads find part
+// Bound by HBM for large maps (288 x 288 x 256 F32 with ReLU: 43.1 us, 3.9 TB/s
+// of x once and y; 16 for the sums and 27 for the rest, whose reads find part
 // of x in the last-level cache), by two launches' latency for small ones
-// (36 x 36 x 256: 8.2 us).
+// (36 x 36 x 256: 8.4 us).
 #include "internal.hpp"
 #include "q8stage.hpp"
 
@@ -530,7 +530,8 @@ void launch_typed(const TI* x, TO* y, const GroupNormShape& s, const float* w, c
     const int chunk = group_norm_stats_chunk(s, VEC), chunks = (s.pixels + chunk - 1) / chunk;
     const dim3 grid(chunks, s.images);
     // A map that no L2 would hold is written past the caches: 288 x 288 x 256
-    // F32 57.2 -> 45.3 us (no write-back of the L2s at the launch's end)
+    // F32 57.2 -> 45.3 us (no write-back of the L2s at the launch's end; that
+    // is 85 MB, with nothing behind it that reads the map: 32 MiB is a guess)
     const bool past_cache = int64_t(s.images) * s.pixels * s.channels * int64_t(sizeof(TO)) > (int64_t(32) << 20);
     const int apply_chunk = chunk_of(s, VEC, 1024 / s.images);
     const dim3 apply_grid((s.pixels + apply_chunk - 1) / apply_chunk, s.images);
@@ -566,7 +567,7 @@ int group_norm_vec(int x_type) { return x_type == T_F16 ? kVec<_Float16> : kVec<
 
 // Eight vectors of each of 1024 threads are what a workgroup holds; past 8192
 // channels of pixels a CU's arithmetic takes longer than another launch,
-// unless there are groups for most CUs.
+// unless there are groups for most CUs (limits from a few sizes, not swept).
 bool group_norm_one_launch(const GroupNormShape& s, int vec) {
     const int size = s.channels / s.groups, cols = (size + vec - 1) / vec, rows = 1024 / cols;
     return (s.pixels + rows - 1) / rows <= 8 && (int64_t(s.pixels) * size <= 8192 || int64_t(s.groups) * s.images >= 192);

@@ -13,10 +13,14 @@
 //   lora_down_kernel  : t = A x, the K range split over workgroups
 //   lora_up_kernel    : y = base + scale * B t
 // Products on the F32 matrix instruction: F32 products and sums throughout.
-// Bound by HBM with many rows (41472 x 1024 -> 4736, rank 32, 8 slots: 421 us,
+// Bound by HBM with many rows (41472 x 1024 -> 4736, rank 32, 8 slots: 419 us,
 // 4.1 TB/s, most of it the second launch, from base to y; a copy of the bytes
 // takes 364), by one or two launches' latency with few (16 rows 1024 -> 1024,
-// rank 16: 6.3 us; 256 rows 1024 -> 4096: 10.1).
+// rank 16: 6.3 us; 256 rows 1024 -> 4096: 10.0), by A from L2 where K is the
+// long side of a high rank (8260 x 3591 -> 273, rank 47, F32: 114 us, 28 of
+// bytes), and past rank 64 by tiles too small for the matrix instruction (41472
+// x 1024 -> 1024, 8 slots: 387 us at rank 128, 1125 at 256, where the
+// instruction takes 126 and 252).
 #include <algorithm>
 
 #include "internal.hpp"
@@ -589,7 +593,7 @@ void launch_typed(const LoraArgs& a, hipStream_t stream) {
 
 void lora_plan(LoraArgs& a, int cus) {
     a.copy_bare = a.base != a.y || a.ldbase != a.ldy;
-    a.past_cache = a.m * a.n * 4 > (int64_t(32) << 20);   // an output that no L2 would hold
+    a.past_cache = a.m * a.n * 4 > (int64_t(32) << 20);   // an output that no L2 would hold (measured at 786 MB only)
     a.part_ld = (a.rank + 15) / 16 * 16;
     const int columns = (a.n + 255) / 256;
     // tiles of a block of `rows` rows: whole ones, and one begun per slot
@@ -607,7 +611,8 @@ void lora_plan(LoraArgs& a, int cus) {
     a.block_rows = int(few);
     a.block_tiles = tiles_of(few, a.tile_rows);
     a.tile_count = int((a.m + a.block_rows - 1) / a.block_rows) * a.block_tiles;
-    // about two workgroups per CU from splits of at least 256 values of K
+    // about two workgroups per CU from splits of at least 256 values of K (and
+    // three from blocks of columns below: not swept)
     const int64_t full = (a.m + a.tile_rows - 1) / a.tile_rows;
     a.splits = int(std::max<int64_t>(1, std::min<int64_t>((2 * cus + full - 1) / full, (a.k + 255) / 256)));
     a.k_len = ((a.k + a.splits - 1) / a.splits + 127) / 128 * 128;

@@ -16,11 +16,13 @@
 // scaled by powers of two so that the largest magnitude lies in [2^14, 2^15),
 // which leaves ~22 bits to those no more than 2^18 times smaller.  F16 keys and
 // values enter as they are.
-// Bound by the vector instructions of softmax and splitting beside the matrix
+// Bound, with many queries, by vector instructions (softmax, splitting) and by
+// waits at barriers and for data with two waves a SIMD, beside the matrix
 // instructions (8 prompts of 201 queries on 5184 + 33 F32 keys, 8 heads of 32:
-// 48 us, 550 TFLOP/s of hi + lo products; 64 queries of 16 heads of 128 on
-// 65536 F16 keys: 76 us, 905 TFLOP/s, and 103 with up to 1024 own keys each),
-// by two launches' latency for few queries (8 on 5184: 9 us).
+// 49 us, 530 TFLOP/s of hi + lo products, vector instructions 25 us and matrix
+// instructions 10 us of it; 64 queries of 16 heads of 128 on 65536 F16 keys: 85
+// us, 810 TFLOP/s, and 98 with up to 1024 own keys each), by two launches'
+// latency for few queries (8 on 5184: 9.3 us).
 #include <algorithm>
 #include <type_traits>
 
@@ -819,7 +821,8 @@ void prefix_attn_plan(PrefixAttnArgs& a, int head_dim, int cus) {
     // ceil(workgroups / CUs) of them, each with its tiles of `step` keys and about
     // three tiles' time to begin and end; one alone reaches some 60 % of
     // what three together do, two 85 %.  A split costs its partial sums' way
-    // to memory and back, 3 TB/s, where a tile takes 0.5 us + 6 ns a dimension.
+    // to memory and back, 3 TB/s, where a tile takes 0.5 us + 6 ns a dimension
+    // (constants fitted to a few batches between 8 and 1608 queries, not swept).
     const auto splits = [&](int64_t groups, int64_t keys, int step) {
         const int most = int(std::max<int64_t>(1, std::min<int64_t>((keys + 255) / 256, (4 * cus + groups - 1) / groups)));
         const double tile_us = 0.5 + 0.006 * head_dim, split_us = double(a.rows) * a.heads * head_dim * 8 / 3e6;
