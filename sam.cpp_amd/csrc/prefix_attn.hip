@@ -770,12 +770,12 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(PrefixAttnArgs a) {
         }
         const float mnew = fmaxf(m, wave_max(lp != 0.f ? mp : -__builtin_inff()));
         const float old = m == mnew ? 1.f : __builtin_amdgcn_exp2f(m - mnew);
-        float f = lp != 0.f ? lp * __builtin_amdgcn_exp2f(mp - mnew) : 0.f;   // 0: no key in this part
+        float f = lp != 0.f ? lp * __builtin_amdgcn_exp2f(mp - mnew) : 0.f;
         const float before = l * old;
         m = mnew;
         l = before + wave_sum(f);
         const float inv = l == 0.f ? 0.f : 1.f / l;   // v stays a mean
-        f = f * inv;
+        f = lp != 0.f ? f * inv : -1.f;   // no key in this part
         v = v * (before * inv);
         const int here = min(a.parts - p0, 64);
         const float* parts = a.part_o + (item * a.parts + p0) * HD + d;
@@ -788,12 +788,12 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(PrefixAttnArgs a) {
                 const int p = p1 + u * AT_ONCE + slot, at = min(p, here - 1);
                 o[u] = *reinterpret_cast<const floatx4*>(parts + at * HD);
                 fp[u] = __shfl(f, at, 64);
-                if (p >= here) fp[u] = 0.f;
+                if (p >= here) fp[u] = -1.f;
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] += fp[u] != 0.f ? o[u][j] * fp[u] : 0.f;   // without keys its sums may never have been written
+                for (int j = 0; j < 4; ++j) v[j] += fp[u] < 0.f ? 0.f : o[u][j] * fp[u];   // without keys its mean may never have been written
         };
         int p1 = 0;
         for (; p1 + 3 * AT_ONCE < here; p1 += 4 * AT_ONCE) add(std::integral_constant<int, 4>{}, p1);

@@ -379,6 +379,27 @@ def test_scales_of_either_sign_and_zero(samhip, gpu_ctx, scale, dtype, form):
     b.verify(ref, bound)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", range(2))
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_non_finite_values_count_at_any_weight(samhip, gpu_ctx, dtype, form):
+    """The prefix' scores lie 100 and more below the own keys': what its values
+    weigh is nothing, but an infinity among them is not."""
+    b = Batch(*FORMS[form], 4, 4, 64, dtype, seed=27)
+    b.q.abs_().add_(0.5)
+    b.pk.fill_(-24.0)
+    ref, bound = b.reference()
+    b.pv[70, 5] = float("inf")
+    torch.cuda.synchronize()
+    gpu_ctx.prefix_attn(b.desc(samhip))
+    gpu_ctx.synchronize()
+    out, ref, bound = (t.view(-1, 4, 64) for t in (b.out, ref, bound))
+    assert not out[:, 0, 5].isfinite().any()
+    rest = torch.ones_like(out, dtype=torch.bool)
+    rest[:, 0, 5] = False
+    assert ((out.double() - ref).abs() <= bound)[rest].all()
+
+
 def test_refusals(samhip):
     L = samhip.lib()
 
