@@ -39,6 +39,7 @@ extern "C" {
 enum samhip_type {
     SAMHIP_TYPE_F32 = 0,
     SAMHIP_TYPE_F16 = 1,
+    SAMHIP_TYPE_Q4_0 = 2,   /* caches of keys and values only (samhip_kv_cache) */
     SAMHIP_TYPE_Q8_0 = 8,
     SAMHIP_TYPE_Q8_1 = 9,
     SAMHIP_TYPE_Q4_K = 12,
@@ -390,6 +391,116 @@ int samhip_supports_prefix_attn(const samhip_prefix_attn_desc* desc);
 /* May be captured. */
 int samhip_prefix_attn(samhip_context* ctx, const samhip_prefix_attn_desc* desc);
 
+/* Rotary positions with up to three axes, e.g. time, height and width (no
+ * reference counterpart as an operator of its own: the vision blocks take a
+ * table, samhip_vit_block_desc's freqs_cis, whose rotation this is with two
+ * axes, AXIAL and ADJACENT).  A head of head_dim values holds
+ * pairs[0] + pairs[1] + pairs[2] pairs, one axis' behind the other's; pair p,
+ * the j-th of axis a, is turned by
+ *   angle = position[a] * scale[a] * theta^-(j / pairs[a])       (AXIAL)
+ *   angle = position[a] * scale[a] * theta^-(p / all pairs)      (SHARED)
+ *   y0 = x0 cos - x1 sin,  y1 = x0 sin + x1 cos
+ * and values behind the pairs stay as they are.  Angles in F64; cos and sin
+ * are rounded to F32, then each product, then the sum. */
+enum samhip_rope_layout {
+    SAMHIP_ROPE_ADJACENT = 0,   /* pair p: values 2p and 2p + 1 */
+    SAMHIP_ROPE_HALVES = 1      /* pair p: values p and p + all pairs */
+};
+enum samhip_rope_spectrum {
+    SAMHIP_ROPE_AXIAL = 0,      /* every axis from frequency 1 down */
+    SAMHIP_ROPE_SHARED = 1      /* one run of frequencies over all pairs */
+};
+typedef struct samhip_rope_desc {
+    int32_t version;            /* SAMHIP_ABI_VERSION */
+    int32_t head_dim;           /* even, at most 256 */
+    int32_t axes;               /* 1 to 3 */
+    int32_t pairs[3];           /* of each axis, at least 1; together at most head_dim / 2 */
+    int32_t layout, spectrum;   /* enum samhip_rope_layout, enum samhip_rope_spectrum */
+    double theta;               /* at least 1 */
+    double scale[3];            /* within +-2^20 */
+    const int32_t* positions;   /* device I32 [rows][axes], of any sign */
+} samhip_rope_desc;
+
+/* x, y: F32 or F16 (each its own) {heads * head_dim, rows}, at most 2^23 rows
+ * of 2^20 values, any row strides that leave rows apart; y may be x itself
+ * (same type and strides) and overlaps nothing else.  Positions are read on
+ * the device, at every replay of a captured call too.  May be captured. */
+int samhip_supports_rope(const samhip_rope_desc* rope, const samhip_tensor* x, const samhip_tensor* y);
+int samhip_rope(samhip_context* ctx, const samhip_rope_desc* rope, const samhip_tensor* x, const samhip_tensor* y);
+
+/* A cache of keys and values in 8 or 4 bits, in pages (no reference
+ * counterpart; for programs that keep the rows of many requests, as
+ * samhip_prefix_attn's own rows).  k and v are Q8_0 or Q4_0 rows, ne =
+ * {kv_heads * head_dim, rows}, whose bytes are ggml's: a Q8_0 block as
+ * samhip_quantize_rows writes it, a Q4_0 block F16 d and 16 bytes, byte i
+ * with value i's code in its low and value i + 16's in its high half.
+ * Position p of request r stands in row
+ *   pages[r][p / page_rows] * page_rows + p % page_rows.
+ * Of the rows that a call has of request r, n = row_start[r + 1] -
+ * row_start[r] (rows of q, out, k or v), row i stands at position
+ * len[r] - n + i: len counts what a request has in the cache with this call's
+ * rows among it.  The three tables are read on the device, at every replay of
+ * a captured call too.  What does not exist has no place: positions below 0
+ * or from len or max_pages * page_rows on, pages outside the cache's whole
+ * ones.  row_start must not decrease. */
+typedef struct samhip_kv_cache {
+    int32_t version;            /* SAMHIP_ABI_VERSION */
+    int32_t kv_heads, head_dim; /* head_dim 32, 64 or 128; at most 4096 kv heads */
+    int32_t page_rows;          /* any number; max_pages * page_rows at most 2^30 */
+    samhip_tensor k, v;         /* of one type, the same ne (fewer than 2^31 rows); even row strides */
+    int32_t requests;           /* at most 2^20 */
+    int32_t max_pages;
+    const int32_t* pages;       /* device I32 [requests][max_pages]; not read with max_pages 0 */
+    const int32_t* row_start;   /* device I32 [requests + 1] */
+    const int32_t* len;         /* device I32 [requests] */
+} samhip_kv_cache;
+
+/* Writes rows of keys and values, F32 {kv_heads * head_dim, rows}, to their
+ * requests' places, the keys turned by `rope` on their way (NULL: as they
+ * are; its head_dim is the cache's, its positions are those of k's rows):
+ *   Q8_0: as samhip_quantize_rows in the context's q8_rounding
+ *   Q4_0: d = m / -8 with m the first value of the largest magnitude, codes
+ *         min(15, int(x * (1 / d) + 8.5)), d stored as F16
+ * A NaN is stored as a zero, a block with an infinity reads back as NaN.
+ * Rows without a place, and those outside [row_start[0],
+ * row_start[requests]), are not written.  Two rows with one place (pages that
+ * requests share) leave either's blocks there.  k, v and the cache do not
+ * overlap.  At most 2^23 rows.  May be captured. */
+int samhip_supports_cache_write(const samhip_kv_cache* cache, const samhip_rope_desc* rope, const samhip_tensor* k,
+                                const samhip_tensor* v);
+int samhip_cache_write(samhip_context* ctx, const samhip_kv_cache* cache, const samhip_rope_desc* rope,
+                       const samhip_tensor* k, const samhip_tensor* v);
+
+/* Reads the same rows back into k and v, F32 or F16 (both the same)
+ * {kv_heads * head_dim, rows}: d * code, rounded once for F16.  Rows without
+ * a place become zeros; those outside [row_start[0], row_start[requests]) are
+ * left as they were.  May be captured. */
+int samhip_supports_cache_read(const samhip_kv_cache* cache, const samhip_tensor* k, const samhip_tensor* v);
+int samhip_cache_read(samhip_context* ctx, const samhip_kv_cache* cache, const samhip_tensor* k, const samhip_tensor* v);
+
+/* Attention of a batch of requests over such a cache: for every query row and
+ * head
+ *   out = softmax(scale * q K^T) V
+ * over the request's positions that have a place, with `causal` those up to
+ * the row's own.  F32-accurate on the values the blocks stand for.  Grouped
+ * heads: head h reads kv head h / (heads / kv_heads).  A query that sees no
+ * position gets zeros; rows of out outside [row_start[0],
+ * row_start[requests]) are left as they were.  A key whose blocks' scales are
+ * not finite makes NaN of the queries that see it, such a value block of its
+ * 32 dimensions of theirs.  out overlaps no other operand.  At most 4096
+ * heads, 2^23 rows * heads.  May be captured. */
+typedef struct samhip_cache_attn_desc {
+    int32_t version;            /* SAMHIP_ABI_VERSION */
+    int32_t heads;              /* a multiple of kv_heads */
+    float scale;
+    int32_t causal;
+    int32_t max_len;            /* positions from it on are not read, whatever len says */
+    samhip_tensor q, out;       /* F32 {heads * head_dim, rows} */
+    samhip_kv_cache cache;
+} samhip_cache_attn_desc;
+int samhip_supports_cache_attn(const samhip_cache_attn_desc* desc);
+int samhip_cache_attn(samhip_context* ctx, const samhip_cache_attn_desc* desc);
+
 /* Activation after a normalization. */
 enum samhip_activation {
     SAMHIP_ACT_NONE = 0,
@@ -450,7 +561,8 @@ int samhip_trace_pause(samhip_context* ctx, int paused);
  * into a HIP graph instead of running, and graph_launch replays them on the
  * context's stream with one host call.  Only samhip_mul_mat,
  * samhip_quantize_rows, samhip_dequantize_rows, samhip_lora_add,
- * samhip_prefix_attn and samhip_group_norm may be captured; every other entry
+ * samhip_prefix_attn, samhip_group_norm, samhip_rope, samhip_cache_write,
+ * samhip_cache_read and samhip_cache_attn may be captured; every other entry
  * point fails with INVALID_ARGUMENT while a capture is open.  A
  * captured call must fit the context's current staging (run the same
  * product once before capturing); staging that has to grow later is

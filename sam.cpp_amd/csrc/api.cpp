@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "internal.hpp"
+#include "kv_cache.hpp"
 
 using namespace samhip;
 
@@ -388,6 +389,138 @@ const char* prefix_attn_problem(const samhip_prefix_attn_desc* d) {
     if (rows * d->heads > (int64_t(1) << 23) || d->prefix_k.ne[1] > (int64_t(1) << 30) || d->own_max > (1 << 30) ||
         d->requests > (1 << 20))
         return "dimension too large";
+    return nullptr;
+}
+
+const char* rope_problem(const samhip_rope_desc* d) {
+    if (!d) return "null descriptor";
+    if (d->version != SAMHIP_ABI_VERSION) return "unsupported descriptor version";
+    if (d->head_dim < 2 || d->head_dim > 256 || d->head_dim % 2) return "head_dim must be even and at most 256";
+    if (d->axes < 1 || d->axes > 3) return "1 to 3 axes";
+    int64_t pairs = 0;
+    for (int i = 0; i < d->axes; ++i) {
+        if (d->pairs[i] < 1) return "every axis needs a pair";
+        if (!std::isfinite(d->scale[i]) || std::fabs(d->scale[i]) > 1048576.0) return "scale must lie within +-2^20";
+        pairs += d->pairs[i];
+    }
+    if (pairs > d->head_dim / 2) return "more pairs than a head has";
+    if (d->layout != SAMHIP_ROPE_ADJACENT && d->layout != SAMHIP_ROPE_HALVES) return "unknown layout";
+    if (d->spectrum != SAMHIP_ROPE_AXIAL && d->spectrum != SAMHIP_ROPE_SHARED) return "unknown spectrum";
+    if (!(d->theta >= 1.0) || std::isinf(d->theta)) return "theta must be at least 1 and finite";
+    if (!d->positions || reinterpret_cast<uintptr_t>(d->positions) % 4) return "positions must be I32";
+    return nullptr;
+}
+
+RopeArgs rope_args(const samhip_rope_desc& d) {
+    RopeArgs a{};
+    a.positions = d.positions;
+    a.axes = d.axes;
+    a.halves = d.layout == SAMHIP_ROPE_HALVES;
+    for (int i = 0; i < d.axes; ++i) a.pairs += d.pairs[i];
+    for (int i = 0, p = 0; i < d.axes; ++i)
+        for (int j = 0; j < d.pairs[i]; ++j, ++p) {
+            const double power = d.spectrum == SAMHIP_ROPE_AXIAL ? double(j) / d.pairs[i] : double(p) / a.pairs;
+            a.frequency[p] = d.scale[i] * std::exp(-power * std::log(d.theta));
+            a.axis[p] = uint8_t(i);
+        }
+    return a;
+}
+
+const char* rope_rows_problem(const samhip_rope_desc* d, const samhip_tensor* x, const samhip_tensor* y) {
+    if (const char* why = rope_problem(d)) return why;
+    if (!x || !y) return "null tensor descriptor";
+    for (const samhip_tensor* t : {x, y})
+        if (const char* why = strided_problem(*t, 2)) return why;
+    if (x->ne[0] <= 0 || x->ne[1] <= 0) return "empty operand";
+    if (x->ne[0] % d->head_dim) return "rows must be whole heads";
+    if (y->ne[0] != x->ne[0] || y->ne[1] != x->ne[1]) return "y must have the shape of x";
+    if (x->data == y->data && (x->type != y->type || x->nb[1] != y->nb[1])) return "in place, x and y must be of one type and stride";
+    if (x->ne[0] > (int64_t(1) << 20) || x->ne[1] > (int64_t(1) << 23)) return "dimension too large";
+    return nullptr;
+}
+
+const char* cache_problem(const samhip_kv_cache& c) {
+    if (c.version != SAMHIP_ABI_VERSION) return "unsupported cache version";
+    if (c.k.type != T_Q8_0 && c.k.type != T_Q4_0) return "a cache must be Q8_0 or Q4_0";
+    if (c.v.type != c.k.type) return "keys and values must be of one type";
+    if (c.head_dim != 32 && c.head_dim != 64 && c.head_dim != 128) return "head_dim must be 32, 64 or 128";
+    if (c.kv_heads < 1 || c.kv_heads > 4096) return "1 to 4096 kv heads";
+    const int64_t width = int64_t(c.kv_heads) * c.head_dim;
+    if (c.k.ne[1] != c.v.ne[1]) return "keys and values differ in rows";
+    for (const samhip_tensor* t : {&c.k, &c.v}) {
+        if (t->ne[0] != width) return "the cache must be kv_heads * head_dim wide";
+        if (t->ne[1] < 0 || t->ne[1] > INT32_MAX || t->ne[2] != 1 || t->ne[3] != 1) return "bad dimension";
+        if (t->ne[1] == 0) continue;
+        if (t->nb[0] != size_t(block_bytes(t->type))) return "cache nb[0] must equal the block size";
+        if (t->nb[1] < row_bytes(t->type, width)) return "cache rows overlap";
+        if (t->nb[1] > (size_t(1) << 30)) return "stride too large";
+        if (!t->data) return "null data pointer";
+        if (reinterpret_cast<uintptr_t>(t->data) % 2 || t->nb[1] % 2) return "cache rows must be 2-byte aligned";
+    }
+    if (c.requests < 1 || c.requests > (1 << 20)) return "1 to 2^20 requests";
+    if (c.page_rows < 1 || c.max_pages < 0) return "pages must have rows";
+    if (int64_t(c.max_pages) * c.page_rows > (int64_t(1) << 30)) return "more than 2^30 positions a request";
+    if (!c.row_start || !c.len || (c.max_pages > 0 && !c.pages)) return "null table";
+    for (const int32_t* t : {c.pages, c.row_start, c.len})
+        if (reinterpret_cast<uintptr_t>(t) % 4) return "tables must be 4-byte aligned";
+    return nullptr;
+}
+
+KvCacheArgs cache_args(const samhip_kv_cache& c) {
+    KvCacheArgs a{};
+    a.k = static_cast<uint8_t*>(c.k.data);
+    a.v = static_cast<uint8_t*>(c.v.data);
+    a.ldk = int64_t(c.k.nb[1]);
+    a.ldv = int64_t(c.v.nb[1]);
+    a.pages = c.pages;
+    a.row_start = c.row_start;
+    a.len = c.len;
+    a.kv_heads = c.kv_heads;
+    a.head_dim = c.head_dim;
+    a.requests = c.requests;
+    a.max_pages = c.max_pages;
+    a.page = Divisor::of(uint32_t(c.page_rows));
+    a.page_count = uint32_t(c.k.ne[1] / c.page_rows);
+    a.capacity = c.max_pages * c.page_rows;
+    return a;
+}
+
+// Rows of keys and values beside a cache.
+const char* cache_rows_problem(const samhip_kv_cache* c, const samhip_tensor* k, const samhip_tensor* v) {
+    if (!c) return "null cache";
+    if (const char* why = cache_problem(*c)) return why;
+    if (!k || !v) return "null tensor descriptor";
+    for (const samhip_tensor* t : {k, v}) {
+        if (const char* why = strided_problem(*t, 2)) return why;
+        if (t->ne[0] != int64_t(c->kv_heads) * c->head_dim || t->ne[1] != k->ne[1]) return "k and v must be [kv_heads * head_dim, rows]";
+    }
+    if (k->type != v->type) return "k and v must be of one type";
+    if (k->ne[1] <= 0) return "empty operand";
+    if (k->ne[1] > (int64_t(1) << 23)) return "dimension too large";
+    return nullptr;
+}
+
+const char* cache_write_problem(const samhip_kv_cache* c, const samhip_rope_desc* rope, const samhip_tensor* k, const samhip_tensor* v) {
+    if (const char* why = cache_rows_problem(c, k, v)) return why;
+    if (k->type != T_F32) return "k and v must be F32";
+    if (!rope) return nullptr;
+    if (const char* why = rope_problem(rope)) return why;
+    return rope->head_dim == c->head_dim ? nullptr : "the rotation's head_dim must be the cache's";
+}
+
+const char* cache_attn_problem(const samhip_cache_attn_desc* d) {
+    if (!d) return "null descriptor";
+    if (d->version != SAMHIP_ABI_VERSION) return "unsupported descriptor version";
+    if (const char* why = cache_problem(d->cache)) return why;
+    for (const samhip_tensor* t : {&d->q, &d->out})
+        if (const char* why = strided_problem(*t, 2)) return why;
+    if (d->q.type != T_F32 || d->out.type != T_F32) return "q and out must be F32";
+    if (d->heads < 1 || d->heads > 4096 || d->heads % d->cache.kv_heads) return "heads must be a multiple of kv_heads";
+    const int64_t width = int64_t(d->heads) * d->cache.head_dim, rows = d->q.ne[1];
+    if (d->q.ne[0] != width || d->out.ne[0] != width || d->out.ne[1] != rows) return "q and out must be [heads * head_dim, rows]";
+    if (rows <= 0 || d->max_len < 0) return "empty operand";
+    if (!std::isfinite(d->scale)) return "scale must be finite";
+    if (rows * d->heads > (int64_t(1) << 23)) return "dimension too large";
     return nullptr;
 }
 
@@ -1326,6 +1459,84 @@ int samhip_prefix_attn(samhip_context* ctx, const samhip_prefix_attn_desc* d) {
     return traced(ctx, "prefix_attn", d->prefix_k.type, a.rows, int64_t(a.heads) * d->head_dim, a.prefix, [&]() -> int {
         launch_prefix_attn(a, d->prefix_k.type, d->head_dim, ctx->staging, ctx->stream);
         HIP_TRY(hipGetLastError(), "prefix_attn launch");
+        return SAMHIP_OK;
+    });
+}
+
+int samhip_supports_rope(const samhip_rope_desc* rope, const samhip_tensor* x, const samhip_tensor* y) {
+    return rope_rows_problem(rope, x, y) == nullptr ? 1 : 0;
+}
+
+int samhip_rope(samhip_context* ctx, const samhip_rope_desc* rope, const samhip_tensor* x, const samhip_tensor* y) {
+    if (!ctx) return fail(SAMHIP_ERR_INVALID_ARGUMENT, "null context");
+    if (const char* why = rope_rows_problem(rope, x, y)) return fail(SAMHIP_ERR_INVALID_ARGUMENT, "rope: %s", why);
+    const RopeRows r{x->data, y->data, int64_t(x->nb[1] / block_bytes(x->type)), int64_t(y->nb[1] / block_bytes(y->type)),
+                     int(x->ne[1]), int(x->ne[0] / rope->head_dim), rope->head_dim};
+    if (int rc = set_device(ctx)) return rc;
+    return traced(ctx, "rope", x->type, r.rows, x->ne[0], 0, [&]() -> int {
+        launch_rope(r, x->type, y->type, rope_args(*rope), ctx->cus, ctx->stream);
+        HIP_TRY(hipGetLastError(), "rope launch");
+        return SAMHIP_OK;
+    });
+}
+
+int samhip_supports_cache_write(const samhip_kv_cache* cache, const samhip_rope_desc* rope, const samhip_tensor* k,
+                                const samhip_tensor* v) {
+    return cache_write_problem(cache, rope, k, v) == nullptr ? 1 : 0;
+}
+
+int samhip_cache_write(samhip_context* ctx, const samhip_kv_cache* cache, const samhip_rope_desc* rope,
+                       const samhip_tensor* k, const samhip_tensor* v) {
+    if (!ctx) return fail(SAMHIP_ERR_INVALID_ARGUMENT, "null context");
+    if (const char* why = cache_write_problem(cache, rope, k, v)) return fail(SAMHIP_ERR_INVALID_ARGUMENT, "cache_write: %s", why);
+    if (int rc = set_device(ctx)) return rc;
+    return traced(ctx, "cache_write", cache->k.type, k->ne[1], k->ne[0], 0, [&]() -> int {
+        launch_cache_write(cache_args(*cache), cache->k.type, ctx->q8_rounding == SAMHIP_Q8_ROUND_X86, rope ? rope_args(*rope) : RopeArgs{},
+                           static_cast<const float*>(k->data), int64_t(k->nb[1] / 4), static_cast<const float*>(v->data),
+                           int64_t(v->nb[1] / 4), int(k->ne[1]), ctx->cus, ctx->stream);
+        HIP_TRY(hipGetLastError(), "cache_write launch");
+        return SAMHIP_OK;
+    });
+}
+
+int samhip_supports_cache_read(const samhip_kv_cache* cache, const samhip_tensor* k, const samhip_tensor* v) {
+    return cache_rows_problem(cache, k, v) == nullptr ? 1 : 0;
+}
+
+int samhip_cache_read(samhip_context* ctx, const samhip_kv_cache* cache, const samhip_tensor* k, const samhip_tensor* v) {
+    if (!ctx) return fail(SAMHIP_ERR_INVALID_ARGUMENT, "null context");
+    if (const char* why = cache_rows_problem(cache, k, v)) return fail(SAMHIP_ERR_INVALID_ARGUMENT, "cache_read: %s", why);
+    const int e = block_bytes(k->type);
+    if (int rc = set_device(ctx)) return rc;
+    return traced(ctx, "cache_read", cache->k.type, k->ne[1], k->ne[0], 0, [&]() -> int {
+        launch_cache_read(cache_args(*cache), cache->k.type, k->data, int64_t(k->nb[1] / e), v->data, int64_t(v->nb[1] / e), k->type,
+                          int(k->ne[1]), ctx->cus, ctx->stream);
+        HIP_TRY(hipGetLastError(), "cache_read launch");
+        return SAMHIP_OK;
+    });
+}
+
+int samhip_supports_cache_attn(const samhip_cache_attn_desc* desc) { return cache_attn_problem(desc) == nullptr ? 1 : 0; }
+
+int samhip_cache_attn(samhip_context* ctx, const samhip_cache_attn_desc* d) {
+    if (!ctx) return fail(SAMHIP_ERR_INVALID_ARGUMENT, "null context");
+    if (const char* why = cache_attn_problem(d)) return fail(SAMHIP_ERR_INVALID_ARGUMENT, "cache_attn: %s", why);
+    CacheAttnArgs a{};
+    a.cache = cache_args(d->cache);
+    a.q = static_cast<const float*>(d->q.data);
+    a.ldq = int64_t(d->q.nb[1] / 4);
+    a.out = static_cast<float*>(d->out.data);
+    a.ldo = int64_t(d->out.nb[1] / 4);
+    a.rows = int(d->q.ne[1]);
+    a.heads = d->heads;
+    a.group = d->heads / d->cache.kv_heads;
+    a.max_len = std::min(d->max_len, a.cache.capacity);
+    a.scale = d->scale;
+    a.causal = d->causal != 0;
+    if (int rc = set_device(ctx)) return rc;
+    return traced(ctx, "cache_attn", d->cache.k.type, a.rows, d->q.ne[0], a.max_len, [&]() -> int {
+        launch_cache_attn(a, d->cache.k.type, ctx->staging, ctx->stream);
+        HIP_TRY(hipGetLastError(), "cache_attn launch");
         return SAMHIP_OK;
     });
 }

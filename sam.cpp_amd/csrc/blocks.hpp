@@ -10,6 +10,7 @@
 //   Q5_K : Q4_K header, u8 qh[32] @16, u8 qs[128] @48            176 B / 256
 //   Q6_K : u8 ql[128] @0, u8 qh[64] @128, i8 sc[16] @192, f16 d @208  210 B / 256
 //   Q8_1 : f16 d @0, f16 s @2, i8 q[32] @4                       36 B / 32
+//   Q4_0 : f16 d @0, u8 qs[16] @2 (caches of keys and values)    18 B / 32
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -17,7 +18,7 @@
 
 namespace samhip {
 
-enum : int { T_F32 = 0, T_F16 = 1, T_Q8_0 = 8, T_Q8_1 = 9, T_Q4_K = 12, T_Q5_K = 13, T_Q6_K = 14, T_Q8_K = 15,
+enum : int { T_F32 = 0, T_F16 = 1, T_Q4_0 = 2, T_Q8_0 = 8, T_Q8_1 = 9, T_Q4_K = 12, T_Q5_K = 13, T_Q6_K = 14, T_Q8_K = 15,
               T_I32 = 26 };
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -28,10 +29,10 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 __host__ __device__ constexpr int block_elems(int t) {
-    return (t == T_Q8_0 || t == T_Q8_1) ? 32 : (t == T_Q4_K || t == T_Q5_K || t == T_Q6_K || t == T_Q8_K) ? 256 : 1;
+    return (t == T_Q8_0 || t == T_Q8_1 || t == T_Q4_0) ? 32 : (t == T_Q4_K || t == T_Q5_K || t == T_Q6_K || t == T_Q8_K) ? 256 : 1;
 }
 __host__ __device__ constexpr int block_bytes(int t) {
-    return t == T_Q8_0 ? 34 : t == T_Q8_1 ? 36 : t == T_Q4_K ? 144 : t == T_Q5_K ? 176 : t == T_Q6_K ? 210
+    return t == T_Q8_0 ? 34 : t == T_Q4_0 ? 18 : t == T_Q8_1 ? 36 : t == T_Q4_K ? 144 : t == T_Q5_K ? 176 : t == T_Q6_K ? 210
          : t == T_Q8_K ? 292 : t == T_F16 ? 2 : 4;
 }
 

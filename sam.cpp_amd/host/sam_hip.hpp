@@ -264,6 +264,16 @@ public:
         check_status(samhip_group_norm(ctx_, &x, &y, groups, w, b, eps, activation));
     }
 
+    // Rotary positions, and caches of keys and values in 8 or 4 bits.
+    void rope(const samhip_rope_desc& rope, const samhip_tensor& x, const samhip_tensor& y) { check_status(samhip_rope(ctx_, &rope, &x, &y)); }
+    void cache_write(const samhip_kv_cache& cache, const samhip_rope_desc* rope, const samhip_tensor& k, const samhip_tensor& v) {
+        check_status(samhip_cache_write(ctx_, &cache, rope, &k, &v));
+    }
+    void cache_read(const samhip_kv_cache& cache, const samhip_tensor& k, const samhip_tensor& v) {
+        check_status(samhip_cache_read(ctx_, &cache, &k, &v));
+    }
+    void cache_attn(const samhip_cache_attn_desc& desc) { check_status(samhip_cache_attn(ctx_, &desc)); }
+
 private:
     HipBackend(samhip_context* ctx, int device, HipComputeMode compute) : ctx_(ctx), device_(device), compute_(compute) {}
     void reset() {

@@ -16,14 +16,16 @@ LIB_PATH = os.path.join(HERE, "libsamhip.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "samhip.h")
 
 ABI_VERSION = 1
-F32, F16, Q8_0, Q8_1, Q4_K, Q5_K, Q6_K, Q8_K, I32 = 0, 1, 8, 9, 12, 13, 14, 15, 26
+F32, F16, Q4_0, Q8_0, Q8_1, Q4_K, Q5_K, Q6_K, Q8_K, I32 = 0, 1, 2, 8, 9, 12, 13, 14, 15, 26
 COMPUTE_Q8_NATIVE, COMPUTE_F16 = 0, 1
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU_ERF = 0, 1, 2, 3
 ROUND_X86, ROUND_REF = 0, 1
+ROPE_ADJACENT, ROPE_HALVES = 0, 1
+ROPE_AXIAL, ROPE_SHARED = 0, 1
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_DEVICE, ERR_OUT_OF_MEMORY = 0, -1, -2, -3, -4
-BLOCK_ELEMS = {F32: 1, F16: 1, Q8_0: 32, Q8_1: 32, Q4_K: 256, Q5_K: 256, Q6_K: 256, Q8_K: 256, I32: 1}
-BLOCK_BYTES = {F32: 4, F16: 2, Q8_0: 34, Q8_1: 36, Q4_K: 144, Q5_K: 176, Q6_K: 210, Q8_K: 292, I32: 4}
-TYPE_NAMES = {Q8_0: "q8_0", Q8_1: "q8_1", Q4_K: "q4_K", Q5_K: "q5_K", Q6_K: "q6_K", Q8_K: "q8_K", F32: "f32",
+BLOCK_ELEMS = {F32: 1, F16: 1, Q4_0: 32, Q8_0: 32, Q8_1: 32, Q4_K: 256, Q5_K: 256, Q6_K: 256, Q8_K: 256, I32: 1}
+BLOCK_BYTES = {F32: 4, F16: 2, Q4_0: 18, Q8_0: 34, Q8_1: 36, Q4_K: 144, Q5_K: 176, Q6_K: 210, Q8_K: 292, I32: 4}
+TYPE_NAMES = {Q4_0: "q4_0", Q8_0: "q8_0", Q8_1: "q8_1", Q4_K: "q4_K", Q5_K: "q5_K", Q6_K: "q6_K", Q8_K: "q8_K", F32: "f32",
               F16: "f16"}
 
 # Every entry point the header declares, with its ctypes signature.
@@ -102,6 +104,25 @@ class PrefixAttnDesc(ctypes.Structure):
                [(n, ctypes.c_void_p) for n in ("q_start", "own_start", "own_len")]
 
 
+class RopeDesc(ctypes.Structure):
+    """samhip_rope_desc."""
+    _fields_ = [("version", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("axes", ctypes.c_int32), ("pairs", ctypes.c_int32 * 3),
+                ("layout", ctypes.c_int32), ("spectrum", ctypes.c_int32), ("theta", ctypes.c_double), ("scale", ctypes.c_double * 3),
+                ("positions", ctypes.c_void_p)]
+
+
+class KvCache(ctypes.Structure):
+    """samhip_kv_cache."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("version", "kv_heads", "head_dim", "page_rows")] + [("k", Tensor), ("v", Tensor)] + \
+               [("requests", ctypes.c_int32), ("max_pages", ctypes.c_int32)] + [(n, ctypes.c_void_p) for n in ("pages", "row_start", "len")]
+
+
+class CacheAttnDesc(ctypes.Structure):
+    """samhip_cache_attn_desc."""
+    _fields_ = [("version", ctypes.c_int32), ("heads", ctypes.c_int32), ("scale", ctypes.c_float), ("causal", ctypes.c_int32),
+                ("max_len", ctypes.c_int32), ("q", Tensor), ("out", Tensor), ("cache", KvCache)]
+
+
 SIGNATURES = {
     "samhip_abi_version": ([], _I),
     "samhip_device_count": ([_P], _I),
@@ -141,6 +162,14 @@ SIGNATURES = {
     "samhip_lora_add": ([_P, ctypes.POINTER(LoraBank)] + [ctypes.POINTER(Tensor)] * 4, _I),
     "samhip_supports_prefix_attn": ([ctypes.POINTER(PrefixAttnDesc)], _I),
     "samhip_prefix_attn": ([_P, ctypes.POINTER(PrefixAttnDesc)], _I),
+    "samhip_supports_rope": ([ctypes.POINTER(RopeDesc)] + [ctypes.POINTER(Tensor)] * 2, _I),
+    "samhip_rope": ([_P, ctypes.POINTER(RopeDesc)] + [ctypes.POINTER(Tensor)] * 2, _I),
+    "samhip_supports_cache_write": ([ctypes.POINTER(KvCache), ctypes.POINTER(RopeDesc)] + [ctypes.POINTER(Tensor)] * 2, _I),
+    "samhip_cache_write": ([_P, ctypes.POINTER(KvCache), ctypes.POINTER(RopeDesc)] + [ctypes.POINTER(Tensor)] * 2, _I),
+    "samhip_supports_cache_read": ([ctypes.POINTER(KvCache)] + [ctypes.POINTER(Tensor)] * 2, _I),
+    "samhip_cache_read": ([_P, ctypes.POINTER(KvCache)] + [ctypes.POINTER(Tensor)] * 2, _I),
+    "samhip_supports_cache_attn": ([ctypes.POINTER(CacheAttnDesc)], _I),
+    "samhip_cache_attn": ([_P, ctypes.POINTER(CacheAttnDesc)], _I),
     "samhip_supports_group_norm": ([ctypes.POINTER(Tensor), ctypes.POINTER(Tensor), _I32, _P, _P, ctypes.c_float, _I32], _I),
     "samhip_group_norm": ([_P, ctypes.POINTER(Tensor), ctypes.POINTER(Tensor), _I32, _P, _P, ctypes.c_float, _I32], _I),
 }
@@ -234,6 +263,22 @@ def prefix_attn_desc(heads, kv_heads, head_dim, scale, q, out, prefix_k, prefix_
     """A samhip_prefix_attn_desc; the tables are device addresses of I32."""
     return PrefixAttnDesc(ABI_VERSION, heads, kv_heads, head_dim, scale, 1 if causal else 0, requests, own_max, q, out,
                           prefix_k, prefix_v, own_k, own_v, q_start_ptr, own_start_ptr, own_len_ptr)
+
+
+def rope_desc(head_dim, pairs, positions_ptr, layout=ROPE_ADJACENT, spectrum=ROPE_AXIAL, theta=10000.0, scale=None):
+    """A samhip_rope_desc; pairs and scale (1 where None) one to an axis, positions the device address of I32 [rows][axes]."""
+    three = lambda v: (*v, *[0] * (3 - len(v)))  # noqa: E731
+    return RopeDesc(ABI_VERSION, head_dim, len(pairs), three(pairs), layout, spectrum, theta, three(scale or [1.0] * len(pairs)), positions_ptr)
+
+
+def kv_cache(kv_heads, head_dim, page_rows, k, v, requests, max_pages, pages_ptr, row_start_ptr, len_ptr):
+    """A samhip_kv_cache over Q8_0 or Q4_0 descriptors k and v; the tables are device addresses of I32."""
+    return KvCache(ABI_VERSION, kv_heads, head_dim, page_rows, k, v, requests, max_pages, pages_ptr, row_start_ptr, len_ptr)
+
+
+def cache_attn_desc(heads, scale, cache, q, out, max_len, causal=False):
+    """A samhip_cache_attn_desc."""
+    return CacheAttnDesc(ABI_VERSION, heads, scale, 1 if causal else 0, max_len, q, out, cache)
 
 
 def validate_quantized_payload(qtype, ne0, rows, payload):
@@ -338,6 +383,23 @@ class Context:
     def prefix_attn(self, desc):
         """samhip_prefix_attn."""
         check(lib().samhip_prefix_attn(self.handle, ctypes.byref(desc)))
+
+    def rope(self, rope, x, y):
+        """samhip_rope."""
+        check(lib().samhip_rope(self.handle, ctypes.byref(rope), ctypes.byref(x), ctypes.byref(y)))
+
+    def cache_write(self, cache, rope, k, v):
+        """samhip_cache_write; rope is a descriptor or None."""
+        check(lib().samhip_cache_write(self.handle, ctypes.byref(cache), None if rope is None else ctypes.byref(rope), ctypes.byref(k),
+                                       ctypes.byref(v)))
+
+    def cache_read(self, cache, k, v):
+        """samhip_cache_read."""
+        check(lib().samhip_cache_read(self.handle, ctypes.byref(cache), ctypes.byref(k), ctypes.byref(v)))
+
+    def cache_attn(self, desc):
+        """samhip_cache_attn."""
+        check(lib().samhip_cache_attn(self.handle, ctypes.byref(desc)))
 
     def group_norm(self, x, y, groups, w_ptr, b_ptr, eps, activation=ACT_NONE):
         """samhip_group_norm on channels-last descriptors {channels, pixels, images}."""

@@ -1,0 +1,707 @@
+"""Rotary positions (samhip_rope), rows to and from caches of keys and values
+in Q8_0 or Q4_0 pages (samhip_cache_write, samhip_cache_read) and attention over
+them (samhip_cache_attn), against their definitions in F64.
+
+Rotation.  cos and sin are F32 numbers (2^-24 each), each product and the sum
+are rounded (2^-24): |error| <= 4 * 2^-24 (|x0| + |x1|), and the output's own
+rounding for F16, 2^-11 |y| + 2^-25 (subnormals).  Angles: the F64 product of
+position, scale and frequency, whose own roundings (4 * 2^-53 of the angle)
+come on top.
+
+Stored rows are compared with codes and scales computed in the definition's F32
+steps, byte by byte; rotated ones are rotated by samhip_rope first, whose bits
+the rotation on the way has.
+
+Attention, as for samhip_prefix_attn: with keys and values as the blocks stand
+for, operands of 22 bits and F32 sums, a score is off by at most
+  ds = scale sum|q||k| (head_dim 2^-24 + 5 * 2^-22),
+and |error| <= sum w|v| (2 ds + 2^-19 + (n / 16 + 48) 2^-24).  Weights times
+value scales below 2^-16 of their query's largest are off by 2^-39 of it at
+most (fp16's smallest step), on codes up to 128: + n 2^-32 max(w |d|)."""
+
+import math
+
+import numpy as np
+import pytest
+
+try:
+    import torch
+except ImportError:   # pragma: no cover
+    torch = None
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"f32": "float32", "f16": "float16"}
+
+
+def dtype_of(name):
+    return getattr(torch, DTYPES[name])
+
+
+def describe(samhip, t):
+    return samhip.tensor_nd(samhip.F16 if t.dtype == torch.float16 else samhip.F32, t.shape[::-1],
+                            [v * t.element_size() for v in t.stride()[::-1]], t.data_ptr())
+
+
+def strided(t, pad, dtype=None):
+    held = torch.full((t.shape[0], t.shape[1] + pad), float("nan"), device=t.device, dtype=dtype or t.dtype)
+    held[:, :t.shape[1]] = t
+    return held[:, :t.shape[1]]
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+# --- rotation -----------------------------------------------------------------
+
+
+class Turn:
+    """A rotation and its definition."""
+
+    def __init__(self, hd, pairs, positions, halves=False, shared=False, theta=10000.0, scale=None):
+        self.hd, self.pairs, self.positions, self.halves, self.shared, self.theta = hd, pairs, positions, halves, shared, theta
+        self.scale = scale or [1.0] * len(pairs)
+
+    def desc(self, samhip):
+        return samhip.rope_desc(self.hd, self.pairs, self.positions.data_ptr(), samhip.ROPE_HALVES if self.halves else samhip.ROPE_ADJACENT,
+                                samhip.ROPE_SHARED if self.shared else samhip.ROPE_AXIAL, self.theta, self.scale)
+
+    def reference(self, x):
+        """The rotation in F64, what F32 steps may be off by, and what angles may."""
+        total = sum(self.pairs)
+        x = x.double().view(x.shape[0], -1, self.hd)
+        y, off = x.clone(), torch.zeros_like(x)
+        p = 0
+        for a, n in enumerate(self.pairs):
+            for j in range(n):
+                freq = self.theta ** (-p / total if self.shared else -j / n)
+                angle = self.positions[:, a].double() * (self.scale[a] * freq)
+                c, s = torch.cos(angle)[:, None], torch.sin(angle)[:, None]
+                u, v = (p, p + total) if self.halves else (2 * p, 2 * p + 1)
+                y[..., u], y[..., v] = x[..., u] * c - x[..., v] * s, x[..., u] * s + x[..., v] * c
+                off[..., u] = off[..., v] = (x[..., u].abs() + x[..., v].abs()) * (4 * 2.0 ** -24 + 16 * 2.0 ** -53 * angle.abs()[:, None])
+                p += 1
+        return y.flatten(1), off.flatten(1)
+
+
+ROPES = [
+    # rows, heads, head_dim, pairs, halves, shared
+    (1, 1, 2, [1], False, False),
+    (1, 1, 64, [32], True, True),
+    (7, 3, 6, [1, 1, 1], False, False),
+    (33, 5, 32, [4, 6, 6], True, False),
+    (201, 8, 32, [8, 8], False, False),
+    (300, 2, 128, [16, 24, 24], True, True),
+    (65, 3, 50, [3, 5], True, True),
+    (19, 1, 256, [128], True, True),
+    (40, 7, 96, [5, 1, 9], False, True),
+    (1025, 4, 64, [7], True, False),
+]
+
+
+@pytest.mark.parametrize("case", range(len(ROPES)))
+@pytest.mark.parametrize("types", ["f32 f32", "f32 f16", "f16 f32", "f16 f16"])
+def test_rope(samhip, gpu_ctx, case, types):
+    rows, heads, hd, pairs, halves, shared = ROPES[case]
+    print("rope", ROPES[case], types, flush=True)
+    xt, yt = types.split()
+    for pad in (0, 3):
+        g = torch.Generator(device="cuda").manual_seed(case)
+        positions = torch.randint(-50, 5184, (rows, len(pairs)), device="cuda", generator=g, dtype=torch.int32)
+        t = Turn(hd, pairs, positions, halves, shared)
+        x = strided(torch.randn(rows, heads * hd, device="cuda", generator=g), pad, dtype_of(xt))
+        held = torch.full((rows, heads * hd + pad), 7.0, device="cuda", dtype=dtype_of(yt))
+        y = held[:, :heads * hd]
+        want, off = t.reference(x)
+        torch.cuda.synchronize()
+        gpu_ctx.rope(t.desc(samhip), describe(samhip, x), describe(samhip, y))
+        gpu_ctx.synchronize()
+        if yt == "f16":
+            off = off + want.abs() * 2.0 ** -11 + 2.0 ** -25
+        assert ((y.double() - want).abs() <= off).all()
+        assert (held[:, heads * hd:] == 7.0).all()
+        if sum(pairs) * 2 < hd:   # values behind the pairs as they are
+            tail = slice(2 * sum(pairs), hd)
+            assert torch.equal(y.reshape(rows, heads, hd)[..., tail], x.reshape(rows, heads, hd)[..., tail].to(y.dtype))
+
+
+@pytest.mark.parametrize("halves", [False, True])
+def test_rope_in_place_far_positions_and_scales(samhip, gpu_ctx, halves):
+    """Positions of the whole range, on a scale of a third: F64 angles to 2^30."""
+    far = [2 ** 31 - 1, -2 ** 31, 123456789, -7, 0, 1]
+    positions = ints([[far[i % 6], far[(i + 2) % 6]] for i in range(24)])
+    t = Turn(64, [16, 16], positions, halves, theta=500000.0, scale=[1 / 3, -2.0])
+    x = torch.randn(24, 3 * 64, device="cuda")
+    want, off = t.reference(x)
+    torch.cuda.synchronize()
+    gpu_ctx.rope(t.desc(samhip), describe(samhip, x), describe(samhip, x))
+    gpu_ctx.synchronize()
+    assert ((x.double() - want).abs() <= off).all()
+
+
+def test_rope_of_position_zero_and_non_finite_values(samhip, gpu_ctx):
+    """Position 0 leaves every bit; an infinity or a NaN reaches its pair alone."""
+    x = torch.randn(9, 4 * 32, device="cuda")
+    t = Turn(32, [5, 11], ints([[0, 0]] * 9))
+    y = torch.empty_like(x)
+    torch.cuda.synchronize()
+    gpu_ctx.rope(t.desc(samhip), describe(samhip, x), describe(samhip, y))
+    gpu_ctx.synchronize()
+    assert torch.equal(x, y)
+    for halves in (False, True):
+        t = Turn(32, [4, 8], ints([[3, 5]] * 9), halves)
+        x[2, 32 + 6], x[5, 64 + 30] = float("inf"), float("nan")   # a pair's, and one behind the pairs
+        want, off = t.reference(torch.where(x.isfinite(), x, 0.0))
+        torch.cuda.synchronize()
+        gpu_ctx.rope(t.desc(samhip), describe(samhip, x), describe(samhip, y))
+        gpu_ctx.synchronize()
+        hit = torch.zeros_like(x, dtype=torch.bool)
+        hit[2, 32 + 6] = hit[2, 32 + (18 if halves else 7)] = hit[5, 64 + 30] = True
+        assert torch.equal(~y.isfinite(), hit)
+        assert ((y.double() - want).abs() <= off)[~hit].all()
+
+
+# --- what a block holds --------------------------------------------------------
+
+
+def q8_0_blocks(x, x86):
+    """d and codes of blocks x [..., 32] (numpy F32) in the definition's F32 steps."""
+    amax = np.abs(x).max(-1, keepdims=True)
+    d = (amax / np.float32(127)).astype(np.float32)
+    with np.errstate(divide="ignore"):
+        inv = np.where(amax > 0, np.float32(127) / amax if x86 else np.float32(1) / d, np.float32(0)).astype(np.float32)
+    s = (x * inv).astype(np.float32)
+    codes = np.rint(s) if x86 else np.trunc(s + np.copysign(np.float32(0.5), s).astype(np.float64))
+    return d.astype(np.float16), codes.astype(np.int8)
+
+
+def q4_0_blocks(x):
+    first = np.abs(x).argmax(-1)[..., None]   # argmax: the first of equals
+    d = (np.take_along_axis(x, first, -1) / np.float32(-8)).astype(np.float32)
+    with np.errstate(divide="ignore"):
+        inv = np.where(d != 0, np.float32(1) / d, np.float32(0)).astype(np.float32)
+    s = ((x * inv).astype(np.float32) + np.float32(8.5)).astype(np.float32)
+    return d.astype(np.float16), np.minimum(np.trunc(s), 15).astype(np.uint8)
+
+
+def packed(x, q4, x86=True):
+    """Rows (F32 tensor) as cache bytes, a uint8 array [rows, row bytes]."""
+    b = x.cpu().numpy().reshape(x.shape[0], -1, 32)
+    d, c = q4_0_blocks(b) if q4 else q8_0_blocks(b, x86)
+    if q4:
+        c = c[..., :16] | (c[..., 16:] << 4)
+    return np.concatenate([d.view(np.uint8), c.view(np.uint8)], -1).reshape(x.shape[0], -1)
+
+
+def values(rows, q4):
+    """Cache bytes (uint8 tensor [n, row bytes]) as F64 values [n, width]."""
+    b = rows.reshape(rows.shape[0], rows.shape[1] // (18 if q4 else 34), -1)
+    d = b[..., :2].contiguous().view(torch.float16).double()
+    c = b[..., 2:]
+    codes = torch.cat([c & 15, c >> 4], -1).double() - 8 if q4 else c.contiguous().view(torch.int8).double()
+    return (d * codes).flatten(1)
+
+
+class Pages:
+    """Requests with n rows in the call and len positions, in pages dealt in no
+    order; every cache byte nobody has is 0xff (NaN scales)."""
+
+    def __init__(self, n, lens, kv_heads, hd, q4, page, seed=0, first=0, behind=0, byte_pad=0):
+        self.n, self.lens, self.kv_heads, self.hd, self.q4, self.page = n, lens, kv_heads, hd, q4, page
+        self.first, self.rows, self.width = first, first + sum(n) + behind, kv_heads * hd
+        self.row_bytes = self.width // 32 * (18 if q4 else 34)
+        counts = [-(-m // page) for m in lens]
+        self.max_pages, self.total = max(1, max(counts)) + 1, sum(counts) + 2
+        rng = np.random.default_rng(seed)
+        order = rng.permutation(self.total)
+        table = np.full((len(n), self.max_pages), -1, np.int32)
+        for r, c in enumerate(counts):
+            table[r, :c] = order[sum(counts[:r]):sum(counts[:r]) + c]
+        self.table = table
+        self.pages, self.len = ints(table.tolist()), ints(lens)
+        self.starts = [first + sum(n[:r]) for r in range(len(n) + 1)]
+        self.row_start = ints(self.starts)
+        self.caches = [torch.full((self.total * page, self.row_bytes + byte_pad), 255, dtype=torch.uint8, device="cuda") for _ in "kv"]
+        self.max_len = max(lens)
+
+    def at(self, r, positions):
+        p = np.asarray(positions)
+        return torch.as_tensor(self.table[r][p // self.page].astype(np.int64) * self.page + p % self.page, device="cuda")
+
+    def fill(self, seed=0, amp=1.0):
+        """Positions 0 .. len - 1 of every request from N(0, 1) rows."""
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        for r, m in enumerate(self.lens):
+            if m:
+                for i, c in enumerate(self.caches):
+                    x = torch.randn(m, self.width, device="cuda", generator=g) * (amp if i == 0 else 1.0)
+                    c[self.at(r, range(m)), :self.row_bytes] = torch.as_tensor(packed(x, self.q4), device="cuda")
+        return self
+
+    def desc(self, samhip):
+        t = samhip.Q4_0 if self.q4 else samhip.Q8_0
+        k, v = (samhip.tensor(t, self.width, c.shape[0], c.data_ptr(), nb1=c.stride(0)) for c in self.caches)
+        return samhip.kv_cache(self.kv_heads, self.hd, self.page, k, v, len(self.n), self.max_pages, self.pages.data_ptr(), self.row_start.data_ptr(),
+                               self.len.data_ptr())
+
+
+# --- rows to and from a cache ---------------------------------------------------
+
+STORES = [
+    # rows, lengths, kv heads, head_dim, page
+    ([1], [1], 1, 32, 1),
+    ([1] * 9, [1, 2, 64, 65, 300, 7, 31, 32, 33], 4, 128, 16),
+    ([5, 0, 33, 150, 1], [5, 9, 40, 150, 77], 3, 64, 41),
+    ([700], [1000], 8, 32, 333),
+    ([2, 3], [1, 2], 2, 32, 8),          # fewer positions than rows: the first have no place
+    ([40], [200], 1, 64, 4096),
+]
+
+
+@pytest.mark.parametrize("case", range(len(STORES)))
+@pytest.mark.parametrize("q4", [False, True])
+@pytest.mark.parametrize("turned", [None, "halves", "adjacent", "odd halves"])
+def test_write_and_read(samhip, gpu_ctx, case, q4, turned):
+    n, lens, kv_heads, hd, page = STORES[case]
+    print("write", STORES[case], "q4" if q4 else "q8", turned, flush=True)
+    for pad in (0, 3):
+        p = Pages(n, lens, kv_heads, hd, q4, page, seed=case, first=pad, behind=pad, byte_pad=2 * pad)
+        g = torch.Generator(device="cuda").manual_seed(case)
+        k, v = (strided(torch.randn(p.rows, p.width, device="cuda", generator=g), pad) for _ in "kv")
+        rope, kt = None, k
+        if turned:
+            pairs = {"halves": [hd // 4, hd // 4], "adjacent": [hd // 8, hd // 8, hd // 8], "odd halves": [3, 7]}[turned]
+            positions = torch.randint(0, 100000, (p.rows, len(pairs)), device="cuda", generator=g, dtype=torch.int32)
+            turn = Turn(hd, pairs, positions, turned != "adjacent", turned == "halves")
+            rope, kt = turn.desc(samhip), torch.empty(p.rows, p.width, device="cuda")
+            torch.cuda.synchronize()
+            gpu_ctx.rope(rope, describe(samhip, k), describe(samhip, kt))
+        torch.cuda.synchronize()
+        gpu_ctx.cache_write(p.desc(samhip), rope, describe(samhip, k), describe(samhip, v))
+        gpu_ctx.synchronize()
+        want = [torch.full_like(c, 255) for c in p.caches]
+        read = [torch.full((p.rows, p.width), 7.0, device="cuda", dtype=torch.float64) for _ in "kv"]
+        for i, x in enumerate((kt, v)):
+            bytes_ = torch.as_tensor(packed(x, q4), device="cuda")
+            for r, (rows, m) in enumerate(zip(n, lens)):
+                s0, lost = p.starts[r], max(0, rows - m)
+                read[i][s0:s0 + lost] = 0.0
+                if rows > lost:
+                    want[i][p.at(r, range(m - rows + lost, m)), :p.row_bytes] = bytes_[s0 + lost:s0 + rows]
+                    read[i][s0 + lost:s0 + rows] = values(bytes_[s0 + lost:s0 + rows], q4)
+        for i in range(2):
+            assert torch.equal(p.caches[i], want[i])
+        for out in ("f32", "f16"):
+            held = [torch.full((p.rows, p.width + pad), 7.0, device="cuda", dtype=dtype_of(out)) for _ in "kv"]
+            torch.cuda.synchronize()
+            gpu_ctx.cache_read(p.desc(samhip), *(describe(samhip, h[:, :p.width]) for h in held))
+            gpu_ctx.synchronize()
+            for i in range(2):
+                assert torch.equal(held[i][:, :p.width], read[i].to(dtype_of(out)))
+                assert (held[i][:, p.width:] == 7.0).all()
+
+
+@pytest.mark.parametrize("x86", [True, False])
+def test_q8_0_rows_are_those_of_quantize_rows(samhip, x86):
+    """Blocks of zeros, subnormals, one magnitude of both signs, ties and values
+    whose scale overflows fp16, with a NaN and with an infinity."""
+    rounding = samhip.ROUND_X86 if x86 else samhip.ROUND_REF
+    with samhip.Context(0, samhip.COMPUTE_Q8_NATIVE, rounding) as ctx:
+        rng = np.random.default_rng(5)
+        x = rng.standard_normal((64, 64)).astype(np.float32)
+        x[1] = 0
+        x[2] *= 1e-42
+        x[3, :32] = np.where(np.arange(32) % 2, -1.5, 1.5)
+        x[4] = (np.arange(64) - 31.5) * 2
+        x[4, 0] = -127
+        x[5] *= 3e7
+        x[6, 3] = np.nan
+        x[7, 40] = np.inf
+        x[8] *= 1e-30
+        want = ctx.quantize(samhip.Q8_0, x, rounding)
+        p = Pages([64], [64], 1, 64, False, 7)
+        k = torch.as_tensor(x, device="cuda")
+        torch.cuda.synchronize()
+        ctx.cache_write(p.desc(samhip), None, describe(samhip, k), describe(samhip, k))
+        ctx.synchronize()
+        at = p.at(0, range(64))
+        for c in p.caches:
+            assert np.array_equal(c[at].cpu().numpy(), want)
+        out = [torch.empty_like(k) for _ in "kv"]
+        ctx.cache_read(p.desc(samhip), *(describe(samhip, o) for o in out))
+        ctx.synchronize()
+        assert out[0][7, 32:].isnan().all() and out[0][7, :32].isfinite().all() and out[0][6].isfinite().all() and out[0][6, 3] == 0
+
+
+def test_q4_0_edges(samhip, gpu_ctx):
+    """Zeros, one magnitude of both signs (the first decides the scale's sign),
+    a NaN (a zero), an infinity (its block reads NaN), scales that overflow."""
+    rng = np.random.default_rng(6)
+    x = rng.standard_normal((10, 32)).astype(np.float32)
+    x[1] = 0
+    x[2] = np.where(np.arange(32) % 2, 2.0, -2.0)
+    x[3] = -x[2]
+    x[4, 5] = np.nan
+    x[5, 6] = -np.inf
+    x[6] *= 1e-42
+    x[7] *= 3e6
+    clean = np.where(np.isnan(x), 0, x).astype(np.float32)
+    p = Pages([10], [10], 1, 32, True, 3)
+    k = torch.as_tensor(x, device="cuda")
+    torch.cuda.synchronize()
+    gpu_ctx.cache_write(p.desc(samhip), None, describe(samhip, k), describe(samhip, k))
+    out = [torch.empty_like(k) for _ in "kv"]
+    gpu_ctx.cache_read(p.desc(samhip), *(describe(samhip, o) for o in out))
+    gpu_ctx.synchronize()
+    keep = [0, 1, 2, 3, 4, 8, 9]
+    with np.errstate(over="ignore", invalid="ignore"):
+        want = packed(torch.as_tensor(clean[keep]), True)
+    assert np.array_equal(p.caches[0][p.at(0, keep)].cpu().numpy(), want)
+    assert out[1][5].isnan().all() and (out[0][6] == 0).all() and not out[0][7].isfinite().all()
+    # the first value's sign has code 0, -8 steps; the other's 15, 7 of them
+    assert out[0][2].tolist() == [-2.0, 1.75] * 16 and out[0][3].tolist() == [2.0, -1.75] * 16 and out[0][4, 5] == 0
+
+
+def test_rows_and_pages_that_do_not_exist(samhip, gpu_ctx):
+    """Page numbers outside the cache, lengths beyond the table and row tables
+    beyond the rows: nothing outside is touched, what is there is served."""
+    p = Pages([4, 4, 4], [8, 8, 8], 1, 32, True, 4)
+    table = p.table.copy()
+    free = [i for i in range(p.total) if i != table[0, 0]]   # no page has two owners
+    table[0, 1], table[1, 0], table[1, 1], table[2, :] = p.total, -5, 2 ** 31 - 1, [free[0], free[1], 2 ** 30]
+    p.pages.copy_(ints(table.tolist()))
+    p.len.copy_(ints([8, 8, 2 ** 31 - 1]))
+    p.row_start.copy_(ints([-9, 4, 8, 2 ** 31 - 1]))
+    k = torch.randn(12, 32, device="cuda")
+    torch.cuda.synchronize()
+    gpu_ctx.cache_write(p.desc(samhip), None, describe(samhip, k), describe(samhip, k))
+    out = [torch.full_like(k, 7.0) for _ in "kv"]
+    gpu_ctx.cache_read(p.desc(samhip), *(describe(samhip, o) for o in out))
+    gpu_ctx.synchronize()
+    assert all((c == 255).all() for c in p.caches) and all((o == 0).all() for o in out)
+    p.len.copy_(ints([4, -1, 6]))
+    torch.cuda.synchronize()
+    gpu_ctx.cache_write(p.desc(samhip), None, describe(samhip, k), describe(samhip, k))
+    gpu_ctx.cache_read(p.desc(samhip), *(describe(samhip, o) for o in out))
+    gpu_ctx.synchronize()
+    want = values(torch.as_tensor(packed(k, True), device="cuda"), True)
+    want[4:8] = 0
+    for o in out:
+        assert torch.equal(o.double(), want)
+
+
+# --- attention ------------------------------------------------------------------
+
+
+class Attend:
+    def __init__(self, pages, heads, causal=False, pad=0, seed=0, amp=1.0, scale=None):
+        self.p, self.heads, self.causal = pages, heads, causal
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        self.q = strided(torch.randn(pages.rows, heads * pages.hd, device="cuda", generator=g) * amp, pad)
+        self.scale = pages.hd ** -0.5 if scale is None else scale
+        self.held = torch.full((pages.rows, heads * pages.hd + pad), 7.0, device="cuda")
+        self.out = self.held[:, :heads * pages.hd]
+        self.max_len = pages.max_len
+
+    def desc(self, samhip):
+        return samhip.cache_attn_desc(self.heads, self.scale, self.p.desc(samhip), describe(samhip, self.q), describe(samhip, self.out), self.max_len,
+                                      self.causal)
+
+    def reference(self, lens=None, n=None, starts=None):
+        p, h, hd, group = self.p, self.heads, self.p.hd, self.heads // self.p.kv_heads
+        lens, n, starts = lens or p.lens, n or p.n, starts or p.starts
+        ref = torch.full((p.rows, h * hd), 7.0, device="cuda", dtype=torch.float64)
+        bound = torch.zeros_like(ref)
+        for r, rows in enumerate(n):
+            if not rows:
+                continue
+            m, s0 = min(lens[r], self.max_len), starts[r]
+            q = self.q[s0:s0 + rows].double().view(rows, h, hd)
+            if not m:
+                ref[s0:s0 + rows] = 0.0
+                continue
+            at = p.at(r, range(m))
+            k, v = (values(c[at][:, :p.row_bytes], p.q4).view(m, p.kv_heads, hd) for c in p.caches)
+            seen = torch.ones(rows, m, dtype=torch.bool, device="cuda")
+            if self.causal:
+                seen = torch.arange(m, device="cuda")[None, :] <= torch.arange(rows, device="cuda")[:, None] + (lens[r] - rows)
+            most_d = v.view(m, -1, 32).abs().amax(-1).view(m, p.kv_heads, -1).amax(-1) / (8 if p.q4 else 127)
+            for head in range(h):
+                kk, vv = k[:, head // group], v[:, head // group]
+                s = (q[:, head] @ kk.t()) * self.scale
+                mag = (q[:, head].abs() @ kk.abs().t()) * abs(self.scale)
+                some = seen.any(1, keepdim=True)
+                top = s.masked_fill(~seen, -torch.inf).amax(1, keepdim=True)
+                w = torch.where(seen, torch.exp(s - torch.where(some, top, 0.0)), 0.0)
+                w = w / torch.where(some, w.sum(1, keepdim=True), 1.0)
+                cols = slice(head * hd, (head + 1) * hd)
+                ref[s0:s0 + rows, cols] = w @ vv
+                ds = mag.masked_fill(~seen, 0.0).amax(1, keepdim=True) * (hd * 2.0 ** -24 + 5 * 2.0 ** -22)
+                bound[s0:s0 + rows, cols] = (w @ vv.abs()) * (2 * ds + 2.0 ** -19 + (m / 16 + 48) * 2.0 ** -24) + \
+                    m * 2.0 ** -32 * (w * most_d[:, head // group]).amax(1, keepdim=True)
+        return ref, bound
+
+    def run(self, samhip, ctx):
+        torch.cuda.synchronize()
+        ctx.cache_attn(self.desc(samhip))
+        ctx.synchronize()
+
+    def check(self, samhip, ctx):
+        ref, bound = self.reference()
+        self.run(samhip, ctx)
+        self.verify(ref, bound)
+
+    def verify(self, ref, bound):
+        err = (self.out.double() - ref).abs()
+        assert (err <= bound).all(), (err / bound.clamp(min=1e-30)).max().item()
+        assert (self.held[:, self.heads * self.p.hd:] == 7.0).all()
+
+
+ATTENDS = [
+    # rows, lengths, heads, kv heads, page
+    ([1], [0], 1, 1, 16),
+    ([1], [1], 2, 1, 16),
+    ([1] * 8, [5184, 64, 1, 33, 2, 0, 31, 32], 8, 8, 64),
+    ([1] * 70, [(37 * i) % 700 for i in range(70)], 8, 2, 41),
+    ([5, 0, 150, 31, 0, 1, 64], [9, 3, 300, 1031, 0, 77, 64], 12, 4, 41),
+    ([3, 40], [0, 50], 4, 4, 7),
+    ([2, 3], [700, 20], 16, 1, 1),
+    ([9] * 5, [700, 1, 256, 257, 0], 3, 3, 256),
+    ([4, 1], [3000, 129], 24, 2, 333),
+    ([300], [300], 2, 2, 128),
+]
+
+
+@pytest.mark.parametrize("case", range(len(ATTENDS)))
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("q4", [False, True])
+def test_cache_attn(samhip, gpu_ctx, case, hd, q4):
+    n, lens, heads, kv_heads, page = ATTENDS[case]
+    print("cache_attn", ATTENDS[case], hd, "q4" if q4 else "q8", flush=True)
+    for causal in (False, True):
+        p = Pages(n, lens, kv_heads, hd, q4, page, seed=case, first=(0, 2)[causal], behind=(0, 3)[causal], byte_pad=(0, 6)[causal]).fill(case)
+        Attend(p, heads, causal, pad=(0, 3)[causal], seed=case).check(samhip, gpu_ctx)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("q4", [False, True])
+def test_peaked_scores(samhip, gpu_ctx, q4, rows):
+    """Scores of hundreds: one key takes all the weight, the largest so far moves."""
+    p = Pages([rows, rows], [2000, 265], 2, 64, q4, 64, seed=3).fill(3, amp=6.0)
+    Attend(p, 4, True, amp=6.0, seed=3).check(samhip, gpu_ctx)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("scale", [0.0, -0.125, -2.0, 1e-30])
+def test_scales_of_either_sign_and_zero(samhip, gpu_ctx, scale, rows):
+    p = Pages([rows, rows], [700, 65], 2, 64, True, 64, seed=4).fill(4)
+    Attend(p, 4, True, seed=4, scale=scale).check(samhip, gpu_ctx)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("exponent", [-100, -40, 40, 100])
+def test_queries_of_any_magnitude(samhip, gpu_ctx, exponent, rows):
+    p = Pages([rows], [700], 2, 64, False, 64, seed=5).fill(5)
+    a = Attend(p, 4, seed=5, scale=0.125 * 2.0 ** -exponent if abs(exponent) < 100 else 2.0 ** -math.copysign(100, exponent))
+    a.q.mul_(2.0 ** exponent)
+    a.q[0, :64] = 0.0
+    a.check(samhip, gpu_ctx)
+
+
+def scale_blocks(p, r, which, positions, factor, block=None):
+    """Multiplies the scales of a request's blocks (which: 0 keys, 1 values)."""
+    c, at = p.caches[which], p.at(r, positions)
+    rows = c[at]
+    b = rows[:, :p.row_bytes].reshape(len(at), -1, 18 if p.q4 else 34)
+    d = b[..., :2].contiguous().view(torch.float16).float() * factor
+    new = d.half().view(torch.uint8)
+    if block is None:
+        b[..., :2] = new
+    else:
+        b[:, block, :2] = new[:, block]
+    rows[:, :p.row_bytes] = b.reshape(len(at), -1)
+    c[at] = rows
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("q4", [False, True])
+def test_values_of_many_magnitudes(samhip, gpu_ctx, q4, rows):
+    """Value rows of zeros, of 2^-12 and 2^14 times the others, in runs and alone."""
+    p = Pages([rows, rows], [900, 700], 2, 64, q4, 64, seed=6).fill(6)
+    scale_blocks(p, 0, 1, range(0, 128), 0.0)
+    scale_blocks(p, 0, 1, range(200, 300), 2.0 ** -12)
+    scale_blocks(p, 0, 1, range(400, 432), 2.0 ** 14)
+    scale_blocks(p, 1, 1, [5, 77, 300], 2.0 ** 14)
+    scale_blocks(p, 1, 1, range(600, 700), 2.0 ** -13)
+    Attend(p, 4, True, seed=6).check(samhip, gpu_ctx)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("below", [10.0, 18.5])
+def test_large_values_of_little_weight(samhip, gpu_ctx, below, rows):
+    """The second half's values are 2^20 times the first's, at scores `below`
+    nats under them: both count."""
+    p = Pages([rows], [512], 1, 32, True, 64, seed=7).fill(7)
+    a = Attend(p, 1, seed=7, scale=1.0)
+    a.q.fill_(1.0)
+    k = torch.zeros(512, 32, device="cuda")
+    k[256:] = -below / 32
+    p.caches[0][p.at(0, range(512))] = torch.as_tensor(packed(k, True), device="cuda")
+    scale_blocks(p, 0, 1, range(0, 256), 2.0 ** -9)
+    scale_blocks(p, 0, 1, range(256, 512), 2.0 ** 11)
+    a.check(samhip, gpu_ctx)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("q4", [False, True])
+def test_non_finite_blocks_reach_only_queries_that_see_them(samhip, gpu_ctx, q4, rows):
+    """Key 690 of request 0 has a NaN scale in kv head 0; value 695 an infinite
+    one in kv head 1's second block."""
+    p = Pages([rows, 3], [700, 40], 2, 64, q4, 41, seed=8).fill(8)
+    a = Attend(p, 4, True, seed=8)
+    ref, bound = a.reference()
+    scale_blocks(p, 0, 0, [690], float("nan"), 1)
+    scale_blocks(p, 0, 1, [695], float("inf"), 3)
+    a.run(samhip, gpu_ctx)
+    hit = torch.zeros(rows + 3, 4, 64, dtype=torch.bool, device="cuda")
+    for i in range(rows):
+        position = 700 - rows + i
+        hit[i, :2] |= position >= 690
+        hit[i, 2:, 32:] |= position >= 695
+    out = a.out.view(-1, 4, 64)
+    assert torch.equal(~out.isfinite(), hit)
+    err, most = (out.double() - ref.view(-1, 4, 64)).abs(), bound.view(-1, 4, 64)
+    assert (err[~hit] <= most[~hit]).all()
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_pages_and_lengths_that_do_not_exist(samhip, gpu_ctx, rows):
+    """A page outside the cache hides its positions; lengths are cut to max_len,
+    the table and zero; rows outside the row table are left alone."""
+    p = Pages([rows] * 3, [300, 300, 300], 2, 64, True, 41, seed=9).fill(9)
+    a = Attend(p, 4, seed=9)
+    table = p.table.copy()
+    table[1, 2] = p.total
+    table[2, 0] = -7
+    p.pages.copy_(ints(table.tolist()))
+    p.len.copy_(ints([2 ** 31 - 1, 300, 200]))
+    p.row_start.copy_(ints([-3, rows, 2 * rows, 2 ** 31 - 1]))
+    a.max_len = 290
+    a.run(samhip, gpu_ctx)
+    keys = [range(290), [i for i in range(290) if i // 41 != 2], range(41, 200)]
+    q = a.q.double().view(-1, 4, 64)
+    for r in range(3):
+        at = p.at(r, keys[r])
+        k, v = (values(c[at][:, :p.row_bytes], True).view(-1, 2, 64) for c in p.caches)
+        for h in range(4):
+            w = torch.softmax(q[r * rows:(r + 1) * rows, h] @ k[:, h // 2].t() * a.scale, -1)
+            got = a.out.view(-1, 4, 64)[r * rows:(r + 1) * rows, h].double()
+            assert ((got - w @ v[:, h // 2]).abs() <= 1e-5).all()
+    p.len.copy_(ints([0, -4, 0]))
+    a.run(samhip, gpu_ctx)
+    assert (a.out == 0).all()
+
+
+def test_captured_replays_follow_the_tables(samhip, gpu_ctx):
+    """One graph of a step (rotated queries, rows written, attention), replayed
+    as the requests' caches grow; each replay gives the eager step's bits."""
+    n, steps = 6, 4
+    p = Pages([1] * n, [20 + 40 * i + steps for i in range(n)], 2, 64, True, 16, seed=11).fill(11)
+    a = Attend(p, 4, True, seed=11)
+    k, v, q = (torch.zeros(n, w, device="cuda") for w in (128, 128, 256))
+    positions = torch.zeros(n, 1, device="cuda", dtype=torch.int32)
+    turn = Turn(64, [32], positions, True, True)
+
+    def step():
+        gpu_ctx.rope(turn.desc(samhip), describe(samhip, q), describe(samhip, a.q))
+        gpu_ctx.cache_write(p.desc(samhip), turn.desc(samhip), describe(samhip, k), describe(samhip, v))
+        gpu_ctx.cache_attn(a.desc(samhip))
+
+    torch.cuda.synchronize()
+    step()   # staging
+    gpu_ctx.capture_begin()
+    step()
+    graph = gpu_ctx.capture_end()
+    fresh = [c.clone() for c in p.caches]
+    rolls = []
+    for replayed in (False, True):
+        g = torch.Generator(device="cuda").manual_seed(1)
+        for c, f in zip(p.caches, fresh):
+            c.copy_(f)
+        outs = []
+        for t in range(steps):
+            for x in (k, v, q):
+                x.normal_(generator=g)
+            lens = [20 + 40 * i + t + 1 for i in range(n)]
+            p.len.copy_(ints(lens))
+            positions.copy_(ints([[m - 1] for m in lens]))
+            a.held.fill_(7.0)
+            torch.cuda.synchronize()
+            if replayed:
+                graph.launch()
+            else:
+                step()
+            gpu_ctx.synchronize()
+            outs.append((a.out.clone(), *[c.clone() for c in p.caches]))
+            ref, bound = a.reference(lens)
+            a.verify(ref, bound)
+            torch.randn(512, 256, device="cuda") @ torch.randn(256, 64, device="cuda")
+        rolls.append(outs)
+    graph.destroy()
+    for e, r in zip(*rolls):
+        for x, y in zip(e, r):
+            assert torch.equal(x, y)
+
+
+def test_a_service_on_its_own_stream(samhip):
+    """Prompts and then single tokens, all on a caller's stream and with other
+    work queued before: rows stored step by step serve as those stored at once."""
+    with samhip.Context(0) as ctx:
+        lens, hd, kv, heads = [40, 7, 129], 32, 4, 8
+        g = torch.Generator(device="cuda").manual_seed(12)
+        total = sum(lens)
+        rows = {n: torch.randn(total, w * hd, device="cuda", generator=g) for n, w in (("q", heads), ("k", kv), ("v", kv))}
+        grid = torch.stack([torch.arange(total, device="cuda") // 9, torch.arange(total, device="cuda") % 9], 1).int()
+        turn = lambda positions: Turn(hd, [8, 8], positions)  # noqa: E731
+        stream = torch.cuda.Stream()
+        ctx.set_stream(stream.cuda_stream)
+        with torch.cuda.stream(stream):
+            def serve(p, picks):
+                """The call of rows `picks` (of all), p.n to a request."""
+                x = {n: t[picks].contiguous() for n, t in rows.items()}
+                at = grid[picks].contiguous()
+                ctx.rope(turn(at).desc(samhip), describe(samhip, x["q"]), describe(samhip, x["q"]))
+                ctx.cache_write(p.desc(samhip), turn(at).desc(samhip), describe(samhip, x["k"]), describe(samhip, x["v"]))
+                out = torch.empty_like(x["q"])
+                ctx.cache_attn(samhip.cache_attn_desc(heads, hd ** -0.5, p.desc(samhip), describe(samhip, x["q"]), describe(samhip, out), max(lens), True))
+                keep.append((x, at, p))
+                return out
+
+            keep, starts = [], [sum(lens[:r]) for r in range(3)]
+            big = torch.randn(2048, 2048, device="cuda")
+            for _ in range(4):
+                big = big @ big * 1e-3
+            p = Pages(lens, lens, kv, hd, True, 16, seed=12)
+            once = serve(p, list(range(total)))
+            bytes_once = [c.clone() for c in p.caches]
+            for c in p.caches:
+                c.fill_(255)
+            # all but the last 3 of each as prompts, then one by one
+            split = Pages([m - 3 for m in lens], [m - 3 for m in lens], kv, hd, True, 16, seed=12)
+            split.pages, split.caches, split.max_pages = p.pages, p.caches, p.max_pages
+            picks = [s + i for s, m in zip(starts, lens) for i in range(m - 3)]
+            got = torch.empty_like(once)
+            got[picks] = serve(split, picks)
+            for t in (3, 2, 1):
+                one = Pages([1] * 3, [m - t + 1 for m in lens], kv, hd, True, 16, seed=12)
+                one.pages, one.caches, one.max_pages = p.pages, p.caches, p.max_pages
+                picks = [s + m - t for s, m in zip(starts, lens)]
+                got[picks] = serve(one, picks)
+                keep.append(one)
+        stream.synchronize()
+        for c, b in zip(p.caches, bytes_once):
+            assert torch.equal(c, b)
+        # weights and sums in another order: the tolerance of two results of one definition
+        assert ((got - once).abs() <= 2 * 2.0 ** -17 * once.abs().amax()).all()
+        ctx.set_stream(None)
