@@ -1530,10 +1530,12 @@ int samhip_cache_attn(samhip_context* ctx, const samhip_cache_attn_desc* d) {
     a.rows = int(d->q.ne[1]);
     a.heads = d->heads;
     a.group = d->heads / d->cache.kv_heads;
-    a.max_len = std::min(d->max_len, a.cache.capacity);
+    a.max_len = a.cache.page_count ? std::min(d->max_len, a.cache.capacity) : 0;
     a.scale = d->scale;
     a.causal = d->causal != 0;
     if (int rc = set_device(ctx)) return rc;
+    cache_attn_plan(a, ctx->cus);
+    if (int rc = ensure_staging(ctx, cache_attn_scratch_bytes(a))) return rc;
     return traced(ctx, "cache_attn", d->cache.k.type, a.rows, d->q.ne[0], a.max_len, [&]() -> int {
         launch_cache_attn(a, d->cache.k.type, ctx->staging, ctx->stream);
         HIP_TRY(hipGetLastError(), "cache_attn launch");

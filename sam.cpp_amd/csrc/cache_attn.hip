@@ -1,12 +1,32 @@
 // Attention of a batch of requests over keys and values held in Q8_0 or Q4_0
 // pages:
 //   out = softmax(scale * q K^T) V
-// A workgroup takes a query row and head, a thread every 256th key, each with a
-// running maximum, sum of weights and weighted sum of values of its own.
+// Grouped heads: the queries that share a kv head are neighbouring places of a
+// tile (place = query row * group + head in group).  A tile's keys may be split
+// over workgroups; each part leaves a base b, the sum l of its weights
+// 2^(score - b) (scores in units of log 2) and its weighted mean of values,
+// which a second launch joins.
+//
+// F32-accurate on fp16 matrix instructions: a block's codes are exact in fp16
+// and queries enter as hi + lo halves, scaled by a power of two per query.
+// Weights are held against the largest contribution, weight times value scale,
+// and not against the largest weight: of one query the products 2^(score - b) *
+// scale stay below 2^15, the largest of a tile that moved b at 2^13, so that
+// as hi + lo they keep 22 bits down to 2^-16 of the largest contribution so
+// far, wherever its weight or its scale comes from.  A scale of zero counts as
+// 2^-40 in this, for its weight has its place in the sum.
+//
+// Few places (8 or 16): a wave takes 32 keys at a time, its codes through LDS
+// that no other wave touches, read transposed for values.  A query's hi and lo
+// are two columns of one operand (8 queries make 16), scores leave with a key's
+// scale block by block, and the weights take the value scales block by block,
+// since these differ from key to key.
+// Many places: 128 to a workgroup, 64 keys at a time, decoded once into hi + lo
+// halves in LDS for its four waves.
 #include <algorithm>
 
+#include "attn_tiles.hpp"
 #include "kv_cache.hpp"
-#include "q8stage.hpp"
 
 #pragma clang fp contract(off)
 
@@ -14,98 +34,737 @@ namespace samhip {
 
 namespace {
 
-constexpr float LOG2E = 1.44269504088896340736f;
-constexpr int THREADS = 256;
+constexpr int WAVES = 4;
+constexpr float NO_BASE = -1e30f;         // below every score, and finite
+constexpr int ZERO_SCALE = -40;           // log 2 of what a zero scale counts as
+
+typedef uint32_t u32x2_at __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32x4_at __attribute__((ext_vector_type(4), aligned(2)));
+typedef int int2_t __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ bool finite_half(uint32_t bits) { return (bits & 0x7c00u) != 0x7c00u; }
+
+__device__ __forceinline__ float max_xor16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_xor32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_xor16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Two codes in the low bytes of a dword's halves, less `bias`: 1024 + code is
+// an fp16 number whose low bits are the code.
+__device__ __forceinline__ half2_t less(uint32_t codes, float bias) {
+    return __builtin_bit_cast(half2_t, codes | 0x64006400u) - half2_t{(_Float16)(1024.f + bias), (_Float16)(1024.f + bias)};
+}
+// ... in bits 4 to 7 of the halves: 1024 + 16 code
+__device__ __forceinline__ half2_t less_high(uint32_t codes) {
+    const half2_t sixteenth{(_Float16)0.0625f, (_Float16)0.0625f}, bias{(_Float16)-72.f, (_Float16)-72.f};
+    return __builtin_elementwise_fma(__builtin_bit_cast(half2_t, codes | 0x64006400u), sixteenth, bias);
+}
+__device__ __forceinline__ half8 joined(half2_t a, half2_t b, half2_t c, half2_t d) {
+    return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// Bytes 0, 2, 1, 3 of each dword as fp16: Q8_0 codes, and the low and the high
+// halves of Q4_0 bytes.
+__device__ __forceinline__ half8 codes_q8(uint32_t w0, uint32_t w1) {
+    w0 ^= 0x80808080u;
+    w1 ^= 0x80808080u;
+    return joined(less(w0 & 0x00ff00ffu, 128.f), less(w0 >> 8 & 0x00ff00ffu, 128.f), less(w1 & 0x00ff00ffu, 128.f),
+                  less(w1 >> 8 & 0x00ff00ffu, 128.f));
+}
+[[maybe_unused]] __device__ __forceinline__ half8 codes_low(uint32_t w0, uint32_t w1) {
+    return joined(less(w0 & 0x000f000fu, 8.f), less(w0 >> 8 & 0x000f000fu, 8.f), less(w1 & 0x000f000fu, 8.f),
+                  less(w1 >> 8 & 0x000f000fu, 8.f));
+}
+[[maybe_unused]] __device__ __forceinline__ half8 codes_high(uint32_t w0, uint32_t w1) {
+    return joined(less_high(w0 & 0x00f000f0u), less_high(w0 >> 8 & 0x00f000f0u), less_high(w1 & 0x00f000f0u),
+                  less_high(w1 >> 8 & 0x00f000f0u));
+}
+constexpr int ORDER[8] = {0, 2, 1, 3, 4, 6, 5, 7};   // the bytes of an operand's elements
+
+// What a workgroup has: places [first, ..) of request `request`, whose n query
+// rows begin at q0, and its positions [k0, k1).
+struct Span {
+    int request, q0, n, first;
+    int k0, k1;
+    int end, limit0;      // a query row i sees positions below min(end, limit0 + i)
+    __device__ __forceinline__ int limit(bool causal, int i) const { return causal ? min(end, limit0 + i) : end; }
+};
+
+// The t-th tile of `places` places of all requests; false past the last.
+__device__ __forceinline__ bool find_tile(const CacheAttnArgs& a, int places, int t, int& request, int& tile) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int r0 = 0; r0 < a.cache.requests; r0 += 64) {
+        int tiles = 0;
+        if (r0 + lane < a.cache.requests) {
+            int from;
+            tiles = (max(request_rows(a.cache, a.rows, r0 + lane, from), 0) * a.group + places - 1) / places;
+        }
+        int sum = tiles;
+        for (int off = 1; off < 64; off <<= 1) {
+            const int x = __shfl_up(sum, off, 64);
+            if (lane >= off) sum += x;
+        }
+        const uint64_t past = __ballot(before + sum > t);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            request = r0 + at;
+            tile = t - before - (__shfl(sum, at, 64) - __shfl(tiles, at, 64));
+            return true;
+        }
+        before += __shfl(sum, 63, 64);
+    }
+    return false;
+}
+
+// Workgroups are dispatched round-robin over the 8 XCDs: the kv heads of the
+// same keys, whose blocks share cache lines, follow each other on one of them.
+__device__ __forceinline__ bool find_span(const CacheAttnArgs& a, int places, int step, Span& s, int& kvh, int& split) {
+    const int order = blockIdx.x >> 3, set = (blockIdx.x & 7) + 8 * (order / a.cache.kv_heads);
+    kvh = order % a.cache.kv_heads;
+    if (set >= a.tiles * a.splits) return false;
+    split = set / a.tiles;
+    int tile;
+    if (!find_tile(a, places, set - split * a.tiles, s.request, tile)) return false;
+    s.n = request_rows(a.cache, a.rows, s.request, s.q0);
+    s.first = tile * places;
+    const int len = request_len(a.cache, s.request);
+    s.end = min(len, a.max_len);
+    s.limit0 = len - s.n + 1;
+    const int tile_end = max(s.limit(a.causal, min(s.n - 1, (s.first + places - 1) / a.group)), 0);
+    const int chunk = ((tile_end + a.splits - 1) / a.splits + step - 1) / step * step;
+    s.k0 = min(split * chunk, tile_end);
+    s.k1 = min(s.k0 + chunk, tile_end);
+    return true;
+}
+
+// Where a part's results go: the output itself when it is the only one.
+__device__ __forceinline__ float* part_of(const CacheAttnArgs& a, int row, int head, int hd, int split) {
+    return a.splits == 1 ? a.out + row * a.ldo + head * hd : a.part_o + ((int64_t(row) * a.heads + head) * a.splits + split) * hd;
+}
+__device__ __forceinline__ void leave_part(const CacheAttnArgs& a, int row, int head, int split, float base, float sum) {
+    if (a.splits == 1) return;
+    float* ml = a.part_ml + ((int64_t(row) * a.heads + head) * a.splits + split) * 2;
+    ml[0] = base;
+    ml[1] = sum;
+}
+
+// --- few places -------------------------------------------------------------
+
+template <int TYPE, int HD>
+struct KeyTile {
+    static constexpr int KEYS = 32, BB = block_bytes(TYPE), BLOCKS = HD / 32, HALVES = TYPE == T_Q8_0 ? 2 : 1;
+    static constexpr int CHUNKS = BLOCKS * HALVES;      // 16 bytes of codes of each key
+    // A chunk's 32 keys follow each other, so that reads of 16 keys fill the
+    // banks; the padding spreads the blocks that a row's lanes write.
+    static constexpr int STRIDE = KEYS * 16 + (TYPE == T_Q8_0 ? 32 : 64);
+    static constexpr int VALUES = CHUNKS * STRIDE, SCALES = 2 * VALUES, LOGS = SCALES + 2 * BLOCKS * KEYS * 2, BYTES = LOGS + KEYS * 4;
+    static constexpr int PIECES = HD / 32;              // blocks of a lane
+};
 
 template <int TYPE>
-__device__ __forceinline__ float block_value(const uint8_t* block, int i) {
-    float d = half_bits_to_float(*reinterpret_cast<const uint16_t*>(block));
-    d = d - d == 0.f ? d : __builtin_nanf("");
-    if (TYPE == T_Q8_0) return d * float(int8_t(block[2 + i]));
-    const int byte = block[2 + (i & 15)];
-    return d * float((i < 16 ? byte & 15 : byte >> 4) - 8);
+struct Block {
+    uint32_t d;
+    u32x4 w[TYPE == T_Q8_0 ? 2 : 1];
+    __device__ __forceinline__ void load(const uint8_t* p) {
+        d = *reinterpret_cast<const uint16_t*>(p);
+        w[0] = *reinterpret_cast<const u32x4_at*>(p + 2);
+        if constexpr (TYPE == T_Q8_0) w[1] = *reinterpret_cast<const u32x4_at*>(p + 18);
+    }
+};
+
+template <int TYPE, int HD, int NT>
+struct NarrowShared {
+    static constexpr int PLACES = 8 * NT, TILES = WAVES * KeyTile<TYPE, HD>::BYTES, SUMS = WAVES * PLACES * (HD + 4) * 4;
+    uint8_t __attribute__((aligned(16))) lds[TILES > SUMS ? TILES : SUMS];
+    float b[WAVES][PLACES], l[WAVES][PLACES];
+};
+
+template <int TYPE, int HD, int NT>
+__global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : NT == 1 ? 2 : 1) void cache_attn_narrow_kernel(CacheAttnArgs a) {
+    typedef KeyTile<TYPE, HD> T;
+    typedef NarrowShared<TYPE, HD, NT> Shared;
+    __shared__ Shared sh;
+    Span s;
+    int kvh, split;
+    if (!find_span(a, Shared::PLACES, T::KEYS * WAVES, s, kvh, split)) return;
+    const KvCacheArgs& c = a.cache;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quarter = lane >> 4;
+    const float low = float(lane & 1);   // 1: this lane's column is a query's lo
+    // queries: column 2g + part of tile t, dimensions in the order of the keys' operand
+    half8 q[NT][T::BLOCKS];
+    float cq[NT];
+    int limit[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int place = s.first + 8 * t + (col >> 1), i = place / a.group, head = kvh * a.group + place - i * a.group;
+        const bool mine = i < s.n;
+        limit[t] = mine ? s.limit(a.causal, i) : 0;
+        const float* from = a.q + (s.q0 + (mine ? i : 0)) * a.ldq + head * HD;
+        float x[T::BLOCKS][8];
+        uint32_t m = 0;
+#pragma unroll
+        for (int blk = 0; blk < T::BLOCKS; ++blk)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                // Q8_0: 8 neighbours; Q4_0: 4 and the 4 that stand 16 behind them
+                const float4_at v = *reinterpret_cast<const float4_at*>(from + 32 * blk + (TYPE == T_Q8_0 ? 8 * quarter + 4 * h : 4 * quarter + 16 * h));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    x[blk][4 * h + j] = v[j];
+                    m = umax(m, __float_as_uint(v[j]) & 0x7fffffffu);
+                }
+            }
+        const int e = exponent_of(umax_xor32(umax_xor16(m)));
+        const float f = a.scale < 0.f ? -down(e) : down(e);
+        cq[t] = fmaxf(fabsf(a.scale) * LOG2E * up(e), 0x1p-120f);   // a product with a masked one is -inf
+#pragma unroll
+        for (int blk = 0; blk < T::BLOCKS; ++blk)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float y = x[blk][ORDER[j]] * f, hi = float((_Float16)y);
+                q[t][blk][j] = (_Float16)(low != 0.f ? y - hi : y);
+            }
+    }
+    uint8_t* tile = sh.lds + wave * T::BYTES;
+    _Float16* scales = reinterpret_cast<_Float16*>(tile + T::SCALES);   // [keys, values][block][key]
+    float* logs = reinterpret_cast<float*>(tile + T::LOGS);
+    floatx4 o[NT][2 * T::BLOCKS];
+    float base[NT], l[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        base[t] = NO_BASE;
+        l[t] = 0.f;
+#pragma unroll
+        for (int d = 0; d < 2 * T::BLOCKS; ++d) o[t][d] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const int step = T::KEYS * WAVES, kw = s.k0 + T::KEYS * wave;
+    // block f = lane + 64 i of a tile: keys' first, a key's blocks side by side
+    const auto key_of = [&](int i) { return (lane + 64 * i) % HD / T::BLOCKS; };
+    const auto of_values = [&](int i) { return lane + 64 * i >= HD; };
+    const int blk_of = lane % T::BLOCKS;
+    const uint8_t* k_at = c.k + (kvh * T::BLOCKS + blk_of) * T::BB;
+    const uint8_t* v_at = c.v + (kvh * T::BLOCKS + blk_of) * T::BB;
+    Block<TYPE> raw[T::PIECES];
+    // the cache row of position k + lane (lanes 0 to 31), -1: none
+    const auto row_of = [&](int k) { return lane < T::KEYS && k + lane < s.k1 ? cache_row(c, s.request, k + lane) : -1; };
+    const auto load = [&](int row) {
+#pragma unroll
+        for (int i = 0; i < T::PIECES; ++i) {
+            const int64_t r = max(__shfl(row, key_of(i), 64), 0);   // where there is none, row 0's blocks with scales of zero
+            raw[i].load(of_values(i) ? v_at + r * c.ldv : k_at + r * c.ldk);
+        }
+    };
+    bool odd_values = false;
+    int row = -1;
+    uint32_t here = 0, next_here = 0;
+    if (kw < s.k1) {
+        row = row_of(kw);
+        next_here = uint32_t(__ballot(row >= 0));
+        load(row);
+        row = row_of(kw + step);
+    }
+    for (int k = kw; k < s.k1; k += step) {
+        here = next_here;
+        wave_lds_handoff();   // the last tile's reads came first
+#pragma unroll
+        for (int i = 0; i < T::PIECES; ++i) {
+            const int key = key_of(i);
+            const bool there = here >> key & 1, v = of_values(i);
+            uint32_t d = raw[i].d;
+            if (!finite_half(d)) {
+                odd_values = odd_values || (v && there);   // added behind the last tile, for those that see them
+                d = v ? 0u : 0x7e00u;
+            }
+            d = there ? d : 0u;
+            uint8_t* to = tile + (v ? T::VALUES : 0) + blk_of * T::HALVES * T::STRIDE + key * 16;
+            *reinterpret_cast<u32x4*>(to) = raw[i].w[0];
+            if constexpr (TYPE == T_Q8_0) *reinterpret_cast<u32x4*>(to + T::STRIDE) = raw[i].w[1];
+            reinterpret_cast<uint16_t*>(scales)[((v ? T::BLOCKS : 0) + blk_of) * T::KEYS + key] = uint16_t(d);
+            if (T::BLOCKS == 1 || 64 * i >= HD) {   // values: the largest scale of a key's blocks
+                uint32_t most = d & 0x7fffu;
+                if (T::BLOCKS == 2) most = umax_dpp<DPP_XOR1>(most);
+                if (T::BLOCKS == 4) most = umax_quad(most);
+                if (v && blk_of == 0) logs[key] = fmaxf(__builtin_amdgcn_logf(half_bits_to_float(most)), float(ZERO_SCALE));
+            }
+        }
+        wave_lds_handoff();
+        if (k + step < s.k1) {
+            next_here = uint32_t(__ballot(row >= 0));
+            load(row);
+            row = row_of(k + 2 * step);
+        }
+        // scores of keys 16n + 4 quarter + i
+        floatx4 sc[NT][2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) sc[t][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int blk = 0; blk < T::BLOCKS; ++blk) {
+                half8 keys;
+                if constexpr (TYPE == T_Q8_0) {
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(tile + (2 * blk + (quarter >> 1)) * T::STRIDE + (16 * n + col) * 16 + 8 * (quarter & 1));
+                    keys = codes_q8(w[0], w[1]);
+                } else {
+                    const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + blk * T::STRIDE + (16 * n + col) * 16 + 4 * quarter);
+                    keys = joined(less(w & 0x000f000fu, 8.f), less(w >> 8 & 0x000f000fu, 8.f), less_high(w & 0x00f000f0u), less_high(w >> 8 & 0x00f000f0u));
+                }
+                const half4 d = *reinterpret_cast<const half4*>(scales + blk * T::KEYS + 16 * n + 4 * quarter);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const floatx4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, q[t][blk], floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[t][n][i] = __builtin_fmaf(float(d[i]), p[i], sc[t][n][i]);
+                }
+            }
+        }
+        float log_d[8];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const floatx4 v = *reinterpret_cast<const floatx4*>(logs + 16 * n + 4 * quarter);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) log_d[4 * n + i] = v[i];
+        }
+        float w[NT][8];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[t][j] = sc[t][j >> 2][j & 3] + dpp<DPP_XOR1>(sc[t][j >> 2][j & 3]);   // hi's and lo's
+            if (here != 0xffffffffu || __any(k + T::KEYS > limit[t])) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int key = 16 * (j >> 2) + 4 * quarter + (j & 3);
+                    if (!(here >> key & 1) || k + key >= limit[t]) w[t][j] = -__builtin_inff();
+                }
+            }
+            float top = __builtin_fmaf(w[t][0], cq[t], log_d[0]);
+#pragma unroll
+            for (int j = 1; j < 8; ++j) top = fmaxf(top, __builtin_fmaf(w[t][j], cq[t], log_d[j]));
+            top = max_xor32(max_xor16(top));
+            if (__any(top > base[t] + 15.f)) {
+                const float moved = top > base[t] + 15.f ? top - 13.f : base[t], f = __builtin_amdgcn_exp2f(base[t] - moved);
+                base[t] = moved;
+                l[t] *= f;
+                const float f0 = __shfl(f, 4 * quarter, 64), f1 = __shfl(f, 4 * quarter + 2, 64);   // of the queries of this lane's rows
+#pragma unroll
+                for (int d = 0; d < 2 * T::BLOCKS; ++d) {
+                    o[t][d][0] *= f0;
+                    o[t][d][1] *= f0;
+                    o[t][d][2] *= f1;
+                    o[t][d][3] *= f1;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                w[t][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[t][j], cq[t], -base[t]));
+                l[t] += w[t][j];
+            }
+        }
+        // O += P V, P the weights with a block's scales, of key 4 quarter + j and 16 + 4 quarter + j - 4
+        [[maybe_unused]] const uint8_t* values = tile + T::VALUES + (4 * quarter + (col >> 1 & 3) + (col >> 3) * 16) * 16 + 8 * (col & 1);
+#pragma unroll
+        for (int blk = 0; blk < T::BLOCKS; ++blk) {
+            half8 p[NT];
+            const _Float16* dv = scales + (T::BLOCKS + blk) * T::KEYS + 4 * quarter;
+            const half4 d0 = *reinterpret_cast<const half4*>(dv), d1 = *reinterpret_cast<const half4*>(dv + 16);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const int j0 = ORDER[j], j1 = ORDER[j + 1];
+                    const float x0 = w[t][j0] * float(j0 < 4 ? d0[j0 & 3] : d1[j0 & 3]), x1 = w[t][j1] * float(j1 < 4 ? d0[j1 & 3] : d1[j1 & 3]);
+                    const half2_t h = __builtin_convertvector(float2_t{x0, x1}, half2_t);
+                    const half2_t y = __builtin_convertvector(float2_t{__builtin_fmaf(-float(h[0]), low, x0), __builtin_fmaf(-float(h[1]), low, x1)}, half2_t);
+                    p[t][j] = y[0];
+                    p[t][j + 1] = y[1];
+                }
+            half8 v[2];
+#if defined(__HIP_DEVICE_COMPILE__)
+            // lane i of 16 gets byte i of the 8 keys that the lanes address, two lanes to a key
+            const auto read = [&](const uint8_t* at) {
+                return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) int2_t*)(at)));
+            };
+            if constexpr (TYPE == T_Q8_0) {
+                const u32x2 w0 = read(values + 2 * blk * T::STRIDE), w1 = read(values + (2 * blk + 1) * T::STRIDE);
+                v[0] = codes_q8(w0[0], w0[1]);
+                v[1] = codes_q8(w1[0], w1[1]);
+            } else {
+                const u32x2 w0 = read(values + blk * T::STRIDE);
+                v[0] = codes_low(w0[0], w0[1]);
+                v[1] = codes_high(w0[0], w0[1]);
+            }
+#endif
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) o[t][2 * blk + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[t], v[h], o[t][2 * blk + h], 0, 0, 0);
+        }
+    }
+    if (__any(odd_values)) {
+        // values whose scale is no number were zeros: NaN for the queries that see them
+        for (int k = kw; k < s.k1; k += step)
+            for (int n = 0; n < min(T::KEYS, s.k1 - k); ++n) {
+                const int r = cache_row(c, s.request, k + n);
+                if (r < 0) continue;
+#pragma unroll
+                for (int blk = 0; blk < T::BLOCKS; ++blk) {
+                    if (finite_half(*reinterpret_cast<const uint16_t*>(c.v + r * c.ldv + (kvh * T::BLOCKS + blk) * T::BB))) continue;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (k + n < __shfl(limit[t], 4 * quarter + (i & 2), 64)) o[t][2 * blk][i] = o[t][2 * blk + 1][i] = __builtin_nanf("");
+                }
+            }
+    }
+    // the four waves' sums, joined through LDS
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        l[t] = pair_sum(sum_xor16(l[t]));
+        if (quarter == 0 && low == 0.f) {
+            sh.b[wave][8 * t + (col >> 1)] = base[t];
+            sh.l[wave][8 * t + (col >> 1)] = l[t];
+        }
+    }
+    __syncthreads();   // also: every wave is past its tiles
+    float* all = reinterpret_cast<float*>(sh.lds);
+    const auto joined_sum = [&](int p, float& most) {
+        most = NO_BASE;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) most = fmaxf(most, sh.l[w][p] != 0.f ? sh.b[w][p] : NO_BASE);
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) sum += sh.l[w][p] != 0.f ? sh.l[w][p] * __builtin_amdgcn_exp2f(sh.b[w][p] - most) : 0.f;
+        return sum;
+    };
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const int p = 8 * t + 2 * quarter + g;
+            float most;
+            const float sum = joined_sum(p, most);
+            const float f = sh.l[wave][p] != 0.f ? __builtin_amdgcn_exp2f(sh.b[wave][p] - most) / sum : 0.f;
+#pragma unroll
+            for (int d = 0; d < 2 * T::BLOCKS; ++d) all[(wave * Shared::PLACES + p) * (HD + 4) + 16 * d + col] = (o[t][d][2 * g] + o[t][d][2 * g + 1]) * f;
+        }
+    if (tid < Shared::PLACES) {
+        const int place = s.first + tid, i = place / a.group;
+        float most;
+        const float sum = joined_sum(tid, most);
+        if (i < s.n) leave_part(a, s.q0 + i, kvh * a.group + place - i * a.group, split, most, sum);
+    }
+    __syncthreads();
+    constexpr int QUADS = HD / 4;
+    for (int t = tid; t < Shared::PLACES * QUADS; t += 64 * WAVES) {
+        const int p = t / QUADS, d = 4 * (t % QUADS), place = s.first + p, i = place / a.group;
+        if (i >= s.n) continue;
+        floatx4 v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) v += *reinterpret_cast<const floatx4*>(all + (w * Shared::PLACES + p) * (HD + 4) + d);
+        *reinterpret_cast<float4_at*>(part_of(a, s.q0 + i, kvh * a.group + place - i * a.group, HD, split) + d) = v;
+    }
+}
+
+// --- many places --------------------------------------------------------------
+
+constexpr int TILE = 32;                  // query places of a wave
+constexpr int WIDE_KEYS = 64;
+
+// Eight neighbouring values of a row.
+template <int TYPE>
+struct Octet {
+    static constexpr int SHIFT = TYPE == T_Q8_0 ? 7 : 3;   // no code's magnitude passes 2^SHIFT
+    uint32_t d, w0, w1;
+    __device__ __forceinline__ void load(const uint8_t* head_row, int octet) {
+        const uint8_t* block = head_row + (octet >> 2) * block_bytes(TYPE);
+        d = *reinterpret_cast<const uint16_t*>(block);
+        const u32x2_at w = *reinterpret_cast<const u32x2_at*>(block + 2 + 8 * (octet & (TYPE == T_Q8_0 ? 3 : 1)));
+        w0 = w[0];
+        w1 = w[1];
+    }
+    // values * factor as hi + lo; a code less its bias is one fma, exact
+    __device__ __forceinline__ void split(int octet, float factor, half8& hi, half8& lo) const {
+        const float df = half_bits_to_float(d) * factor, bias = df * (TYPE == T_Q8_0 ? -128.f : -8.f);
+        const uint32_t c0 = TYPE == T_Q8_0 ? w0 ^ 0x80808080u : w0 >> (2 * (octet & 2)) & 0x0f0f0f0fu;
+        const uint32_t c1 = TYPE == T_Q8_0 ? w1 ^ 0x80808080u : w1 >> (2 * (octet & 2)) & 0x0f0f0f0fu;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const uint32_t c = j < 4 ? c0 : c1;
+            const float x0 = __builtin_fmaf(float(c >> (8 * (j & 3)) & 0xffu), df, bias), x1 = __builtin_fmaf(float(c >> (8 * (j & 3) + 8) & 0xffu), df, bias);
+            split_pair(float2_t{x0, x1}, hi, lo, j);
+        }
+    }
+};
+
+template <int HD>
+struct WideShared {
+    typedef TileShape<2, HD, WIDE_KEYS, false> K;
+    typedef TileShape<2, HD, WIDE_KEYS, true> V;
+    uint8_t __attribute__((aligned(16))) k[K::BYTES];
+    uint8_t __attribute__((aligned(16))) v[V::BYTES];
+    uint32_t largest[WAVES][2];
+    int rows[2][WIDE_KEYS];
+    uint64_t here[4];
+};
+
+// Biased exponent of 2^SHIFT times the largest scale, zeros as 2^ZERO_SCALE.
+template <int TYPE>
+__device__ __forceinline__ int scale_exponent(uint32_t half_bits) {
+    return max(int(__float_as_uint(half_bits_to_float(half_bits)) >> 23), 127 + ZERO_SCALE) + Octet<TYPE>::SHIFT;
 }
 
 template <int TYPE, int HD>
-__global__ __launch_bounds__(THREADS) void cache_attn_kernel(CacheAttnArgs a) {
-    __shared__ float q[HD], m_of[THREADS], part[THREADS], total;
-    const int row = blockIdx.x / a.heads, head = blockIdx.x - row * a.heads, kvh = head / a.group, tid = threadIdx.x;
+__global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_kernel(CacheAttnArgs a) {
+    typedef WideShared<HD> Shared;
+    constexpr int PIECES = HD / 32, BB = block_bytes(TYPE);   // of 8 values, a thread's part of a tile
+    __shared__ Shared sh;
+    Span s;
+    int kvh, split;
+    if (!find_span(a, TILE * WAVES, WIDE_KEYS, s, kvh, split)) return;
     const KvCacheArgs& c = a.cache;
-    int lo = 0, hi = c.requests;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (c.row_start[mid + 1] <= row) lo = mid + 1;
-        else hi = mid;
-    }
-    if (lo == c.requests) return;
-    int from;
-    const int n = request_rows(c, a.rows, lo, from), i = row - from;
-    if (i < 0 || i >= n) return;
-    const int len = request_len(c, lo);
-    int end = min(len, a.max_len);
-    if (a.causal) end = min(end, len - n + i + 1);
-    for (int d = tid; d < HD; d += THREADS) q[d] = a.q[row * a.ldq + head * HD + d];
-    __syncthreads();
-    float o[HD], m = -__builtin_inff(), l = 0.f;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hh = lane >> 5;
+    const int place = s.first + TILE * wave + li, i_row = place / a.group, head = kvh * a.group + place - i_row * a.group;
+    const bool mine = i_row < s.n;
+    const int row = s.q0 + (mine ? i_row : 0), limit = mine ? min(s.limit(a.causal, i_row), s.k1) : 0;
+    // queries: lane (li, hh) has place li's values 16t + 8hh .. + 7
+    half8 q_hi[HD / 16], q_lo[HD / 16];
+    float cq;
+    {
+        floatx8 x[HD / 16];
+        uint32_t m = 0;
 #pragma unroll
-    for (int d = 0; d < HD; ++d) o[d] = 0.f;
-    for (int p = tid; p < end; p += THREADS) {
-        const int64_t at = cache_row(c, lo, p);   // times a stride: 64 bits
-        if (at < 0) continue;
-        const uint8_t* k = c.k + at * c.ldk + kvh * (HD / 32) * block_bytes(TYPE);
-        const uint8_t* v = c.v + at * c.ldv + kvh * (HD / 32) * block_bytes(TYPE);
-        float s = 0.f;
-        for (int b = 0; b < HD / 32; ++b)
-            for (int d = 0; d < 32; ++d) s += q[32 * b + d] * block_value<TYPE>(k + b * block_bytes(TYPE), d);
-        s = s * a.scale * LOG2E;
-        const float mnew = fmaxf(m, s), f = m == mnew ? 1.f : __builtin_amdgcn_exp2f(m - mnew), w = __builtin_amdgcn_exp2f(s - mnew);
-        m = mnew;
-        l = l * f + w;
+        for (int t = 0; t < HD / 16; ++t) {
+            const float* from = a.q + row * a.ldq + head * HD + 16 * t + 8 * hh;
+            const float4_at u = *reinterpret_cast<const float4_at*>(from), v = *reinterpret_cast<const float4_at*>(from + 4);
+            x[t] = floatx8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
 #pragma unroll
-        for (int d = 0; d < HD; ++d) o[d] = o[d] * f + w * block_value<TYPE>(v + d / 32 * block_bytes(TYPE), d & 31);
-    }
-    m_of[tid] = m;
-    __syncthreads();
-    float most = -__builtin_inff();
-    for (int t = 0; t < THREADS; ++t) most = fmaxf(most, m_of[t]);
-    const float f = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - most);
-    part[tid] = l * f;
-    __syncthreads();
-    if (tid == 0) {
-        float sum = 0.f;
-        for (int t = 0; t < THREADS; ++t) sum += part[t];
-        total = sum;
-    }
-    __syncthreads();
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    for (int d = 0; d < HD; ++d) {
-        float v = 0.f;
-#pragma unroll
-        for (int e = 0; e < HD; ++e) v = e == d ? o[e] : v;
-        __syncthreads();
-        part[tid] = l == 0.f ? 0.f : v * f;
-        __syncthreads();
-        for (int half = THREADS / 2; half > 0; half >>= 1) {
-            if (tid < half) part[tid] += part[tid + half];
-            __syncthreads();
+            for (int j = 0; j < 8; ++j) m = umax(m, __float_as_uint(x[t][j]) & 0x7fffffffu);
         }
-        if (tid == 0) a.out[row * a.ldo + head * HD + d] = part[0] * inv;
+        const int e = exponent_of(umax_xor32(m));
+        const float f = a.scale < 0.f ? -down(e) : down(e);
+        cq = fabsf(a.scale) * LOG2E * up(e);
+#pragma unroll
+        for (int t = 0; t < HD / 16; ++t)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) split_pair(float2_t{x[t][j] * f, x[t][j + 1] * f}, q_hi[t], q_lo[t], j);
     }
+    // o[d] holds, transposed, dimensions 32d + 8 (r / 4) + 4hh + r % 4 of place li
+    floatx16 o[HD / 32];
+    float base = NO_BASE, l = 0.f;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+
+    // this thread's piece of the first 256; the others are whole rows of keys on
+    constexpr int EACH = 2048 / HD;
+    const int key = tid / (HD / 8), octet = tid % (HD / 8);
+    const uint8_t *k_at = c.k + kvh * (HD / 32) * BB, *v_at = c.v + kvh * (HD / 32) * BB;
+    Octet<TYPE> kr[PIECES], vr[PIECES];
+    uint32_t there = 0;   // of the pieces, whether their key has a row
+    const auto load = [&](const int* rows) {
+        there = 0;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int r = rows[key + i * EACH];
+            there |= uint32_t(r >= 0) << i;
+            const int64_t at = max(r, 0);   // where there is none, row 0's blocks with scales of zero
+            kr[i].load(k_at + at * c.ldk, octet);
+            vr[i].load(v_at + at * c.ldv, octet);
+        }
+    };
+    // Cache rows of a tile, looked up by the first wave two tiles ahead.
+    const auto row_at = [&](int k) { return k + lane < s.k1 ? cache_row(c, s.request, k + lane) : -1; };
+    const auto put_rows = [&](int t, int r) {
+        const uint64_t here = __ballot(r >= 0);
+        sh.rows[t & 1][lane] = r;
+        if (lane == 0) sh.here[t & 3] = here;
+    };
+    int ahead = -1;
+    if (wave == 0 && s.k0 < s.k1) {
+        put_rows(0, row_at(s.k0));
+        put_rows(1, row_at(s.k0 + WIDE_KEYS));
+        ahead = row_at(s.k0 + 2 * WIDE_KEYS);
+    }
+    __syncthreads();
+    if (s.k0 < s.k1) load(sh.rows[0]);
+    bool odd_values = false;
+    int t_now = 0;
+    const int wave_end = [&] {   // no place of this wave sees a key behind it
+        int v = limit;
+        for (int off = 1; off < 32; off <<= 1) v = max(v, __shfl_xor(v, off, 64));
+        return __builtin_amdgcn_readfirstlane(v);
+    }();
+    for (int k = s.k0; k < s.k1; k += WIDE_KEYS, ++t_now) {
+        uint32_t mk = 0, mv = 0;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const bool is = there >> i & 1;
+            if (!finite_half(kr[i].d)) kr[i].d = 0x7e00u;
+            if (!finite_half(vr[i].d)) {
+                odd_values = odd_values || is;   // added behind the last tile, for those that see them
+                vr[i].d = 0;
+            }
+            kr[i].d = is ? kr[i].d : 0u;
+            vr[i].d = is ? vr[i].d : 0u;
+            const uint32_t dk = kr[i].d & 0x7fffu;
+            mk = umax(mk, dk < 0x7c00u ? dk : 0u);
+            mv = umax(mv, vr[i].d & 0x7fffu);
+        }
+        mk = wave_umax(mk);
+        mv = wave_umax(mv);
+        if (lane == 0) sh.largest[wave][0] = mk, sh.largest[wave][1] = mv;
+        __syncthreads();   // the last tile is read, the largest scales are written
+        mk = mv = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) mk = umax(mk, sh.largest[w][0]), mv = umax(mv, sh.largest[w][1]);
+        const int ek = scale_exponent<TYPE>(__builtin_amdgcn_readfirstlane(mk)), ev = scale_exponent<TYPE>(__builtin_amdgcn_readfirstlane(mv));
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            half8 hi, lo;
+            kr[i].split(octet, down(ek), hi, lo);
+            half8* to = Shared::K::piece(sh.k, tid + 256 * i);
+            *to = hi;
+            to[WIDE_KEYS * Shared::K::STRIDE / 16] = lo;
+            vr[i].split(octet, down(ev), hi, lo);
+            to = Shared::V::piece(sh.v, tid + 256 * i);
+            *to = hi;
+            to[WIDE_KEYS * Shared::V::STRIDE / 16] = lo;
+        }
+        if (wave == 0) put_rows(t_now + 2, ahead);
+        __syncthreads();
+        if (k + WIDE_KEYS < s.k1) {
+            load(sh.rows[(t_now + 1) & 1]);
+            if (wave == 0) ahead = row_at(k + 3 * WIDE_KEYS);
+        }
+        if (k >= wave_end) continue;
+        floatx16 sc[2];
+        scores<2, HD, 2>(sh.k, q_hi, q_lo, sc);
+        const uint64_t here = sh.here[t_now & 3];
+        if (here != ~uint64_t(0) || __any(k + WIDE_KEYS > limit)) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int at = 32 * n + 8 * (r >> 2) + 4 * hh + (r & 3);
+                    if (!(here >> at & 1) || k + at >= limit) sc[n][r] = -__builtin_inff();
+                }
+        }
+        const float f = fmaxf(cq * up(ek), 0x1p-120f), unit = float(ev - 141);   // values are in units of 2^unit
+        float top = sc[0][0];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = __builtin_elementwise_maximum(top, sc[n][r]);
+        const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        top = __builtin_fmaf(__builtin_elementwise_maximum(__uint_as_float(other[0]), __uint_as_float(other[1])), f, unit);
+        if (__any(top > base + 15.f)) {
+            const float moved = top > base + 15.f ? top - 13.f : base, by = __builtin_amdgcn_exp2f(base - moved);
+            base = moved;
+            l *= by;
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= by;
+        }
+        const float shift = unit - base;
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                sc[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][r], f, shift));
+                sum += sc[n][r];
+            }
+        l += sum * __builtin_ldexpf(1.f, 141 - ev);
+        half8 p_hi[4], p_lo[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) split_pair(float2_t{sc[u / 2][8 * (u % 2) + j], sc[u / 2][8 * (u % 2) + j + 1]}, p_hi[u], p_lo[u], j);
+        values<2, HD, 2>(sh.v, p_hi, p_lo, o);
+    }
+    if (__syncthreads_or(odd_values)) {
+        // values whose scale is no number were zeros: NaN for the queries that see them
+        for (int k = s.k0; k < s.k1; ++k) {
+            const int r = cache_row(c, s.request, k);
+            if (r < 0) continue;
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+                if (!finite_half(*reinterpret_cast<const uint16_t*>(v_at + r * c.ldv + d * BB)) && k < limit)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[d][e] = __builtin_nanf("");
+        }
+    }
+    l = pair_sum(l);
+    if (!mine) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (hh == 0) leave_part(a, row, head, split, base, l);
+    float* to = part_of(a, row, head, HD, split);
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+            *reinterpret_cast<float4_at*>(to + 32 * d + 2 * r + 4 * hh) = floatx4{o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv};
+}
+
+template <int HD>
+__global__ __launch_bounds__(256) void cache_attn_merge_kernel(CacheAttnArgs a) {
+    const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6), items = int64_t(a.rows) * a.heads;   // a wave per (row, head)
+    if (item >= items) return;
+    const int64_t row = item / a.heads, h = item - row * a.heads;
+    if (row < min(max(a.cache.row_start[0], 0), a.rows) || row >= min(max(a.cache.row_start[a.cache.requests], 0), a.rows)) return;
+    merge_parts<HD>(a.part_ml + item * a.splits * 2, a.part_o + item * a.splits * HD, a.splits, a.out + row * a.ldo + h * HD);
+}
+
+template <int TYPE, int HD>
+void launch_typed(const CacheAttnArgs& a, hipStream_t stream) {
+    const unsigned groups = unsigned((int64_t(a.tiles) * a.splits + 7) / 8 * 8 * a.cache.kv_heads);
+    if (a.query_tiles == 0) cache_attn_wide_kernel<TYPE, HD><<<groups, 64 * WAVES, 0, stream>>>(a);
+    else if (a.query_tiles == 1) cache_attn_narrow_kernel<TYPE, HD, 1><<<groups, 64 * WAVES, 0, stream>>>(a);
+    else cache_attn_narrow_kernel<TYPE, HD, 2><<<groups, 64 * WAVES, 0, stream>>>(a);
+    if (a.splits > 1) cache_attn_merge_kernel<HD><<<unsigned((int64_t(a.rows) * a.heads + 3) / 4), 256, 0, stream>>>(a);
 }
 
 template <int TYPE>
-void launch_typed(const CacheAttnArgs& a, hipStream_t stream) {
-    const unsigned groups = unsigned(a.rows) * a.heads;
-    if (a.cache.head_dim == 32) cache_attn_kernel<TYPE, 32><<<groups, THREADS, 0, stream>>>(a);
-    else if (a.cache.head_dim == 64) cache_attn_kernel<TYPE, 64><<<groups, THREADS, 0, stream>>>(a);
-    else cache_attn_kernel<TYPE, 128><<<groups, THREADS, 0, stream>>>(a);
+void launch_of_type(const CacheAttnArgs& a, hipStream_t stream) {
+    if (a.cache.head_dim == 32) launch_typed<TYPE, 32>(a, stream);
+    else if (a.cache.head_dim == 64) launch_typed<TYPE, 64>(a, stream);
+    else launch_typed<TYPE, 128>(a, stream);
 }
 
 }  // namespace
 
-void launch_cache_attn(const CacheAttnArgs& a, int type, void*, hipStream_t stream) {
-    if (type == T_Q4_0) launch_typed<T_Q4_0>(a, stream);
-    else launch_typed<T_Q8_0>(a, stream);
+void cache_attn_plan(CacheAttnArgs& a, int cus) {
+    const int64_t places = int64_t(a.rows) * a.group, requests = std::min(a.cache.requests, a.rows);
+    const int64_t each = (places + requests - 1) / requests;   // of a request with its share of the rows
+    a.query_tiles = each <= 8 ? 1 : each <= 16 ? 2 : 0;
+    const int tile = a.query_tiles ? 8 * a.query_tiles : TILE * WAVES, step = a.query_tiles ? 32 * WAVES : WIDE_KEYS;
+    a.tiles = int(places / tile + requests);
+    const int64_t groups = ((each + tile - 1) / tile) * requests * a.cache.kv_heads;
+    const int64_t most = std::max<int64_t>(1, a.max_len / (4 * step));
+    a.splits = int(std::max<int64_t>(1, std::min<int64_t>((4 * cus + groups - 1) / groups, most)));
+}
+
+size_t cache_attn_scratch_bytes(const CacheAttnArgs& a) {
+    return a.splits > 1 ? size_t(a.splits) * a.rows * a.heads * (a.cache.head_dim + 2) * 4 : 0;
+}
+
+void launch_cache_attn(CacheAttnArgs a, int type, void* scratch, hipStream_t stream) {
+    a.part_o = static_cast<float*>(scratch);
+    a.part_ml = a.part_o + size_t(a.splits) * a.rows * a.heads * a.cache.head_dim;
+    if (type == T_Q4_0) launch_of_type<T_Q4_0>(a, stream);
+    else launch_of_type<T_Q8_0>(a, stream);
 }
 
 }  // namespace samhip

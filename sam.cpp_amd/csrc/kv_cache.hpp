@@ -96,16 +96,23 @@ void launch_cache_write(const KvCacheArgs& c, int type, bool x86, const RopeArgs
 void launch_cache_read(const KvCacheArgs& c, int type, void* k, int64_t ldk, void* v, int64_t ldv, int out_type, int rows,
                        int cus, hipStream_t stream);
 
+// cache_attn_plan sets the fields behind `causal` but the two scratch
+// pointers, which launch_cache_attn sets.
 struct CacheAttnArgs {
     KvCacheArgs cache;
     const float* q;
     float* out;
     int64_t ldq, ldo;
     int rows, heads, group;
-    int max_len;                           // at most the capacity
+    int max_len;                           // at most the capacity; 0 where the cache has no page
     float scale;
     bool causal;
+    int query_tiles;                       // of 8 places; 0: 128 places to a workgroup
+    int tiles, splits;                     // tiles of all requests (at most), and parts of their keys
+    float *part_o, *part_ml;
 };
-void launch_cache_attn(const CacheAttnArgs& a, int type, void* scratch, hipStream_t stream);
+void cache_attn_plan(CacheAttnArgs& a, int cus);
+size_t cache_attn_scratch_bytes(const CacheAttnArgs& a);
+void launch_cache_attn(CacheAttnArgs a, int type, void* scratch, hipStream_t stream);
 
 }  // namespace samhip
