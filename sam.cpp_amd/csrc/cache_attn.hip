@@ -16,11 +16,14 @@
 // far, wherever its weight or its scale comes from.  A scale of zero counts as
 // 2^-40 in this, for its weight has its place in the sum.
 //
-// Few places (8 or 16): a wave takes 32 keys at a time, its codes through LDS
-// that no other wave touches, read transposed for values.  A query's hi and lo
-// are two columns of one operand (8 queries make 16), scores leave with a key's
-// scale block by block, and the weights take the value scales block by block,
-// since these differ from key to key.
+// Few places: a wave takes 32 keys at a time, their codes through LDS that no
+// other wave touches, read transposed for values.  An operand's 16 columns are
+// places times blocks: column (place, block) has the query's part of that block
+// and zeros for the others, so that the products of all blocks run on into one
+// accumulator and a lane scales them by its own block's key scale, and weights
+// take one block's value scale in each lane instead of all blocks' in every
+// one.  (With hi and lo as columns, and a lane's scores and weights block by
+// block, 64 queries of 16 heads of 128 on up to 8192 keys took 84 us.)
 // Many places: 128 to a workgroup, 64 keys at a time, decoded once into hi + lo
 // halves in LDS for its four waves.
 #include <algorithm>
@@ -57,35 +60,37 @@ __device__ __forceinline__ float sum_xor16(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Two codes in the low bytes of a dword's halves, less `bias`: 1024 + code is
-// an fp16 number whose low bits are the code.
-__device__ __forceinline__ half2_t less(uint32_t codes, float bias) {
-    return __builtin_bit_cast(half2_t, codes | 0x64006400u) - half2_t{(_Float16)(1024.f + bias), (_Float16)(1024.f + bias)};
-}
-// ... in bits 4 to 7 of the halves: 1024 + 16 code
-__device__ __forceinline__ half2_t less_high(uint32_t codes) {
-    const half2_t sixteenth{(_Float16)0.0625f, (_Float16)0.0625f}, bias{(_Float16)-72.f, (_Float16)-72.f};
-    return __builtin_elementwise_fma(__builtin_bit_cast(half2_t, codes | 0x64006400u), sixteenth, bias);
-}
-__device__ __forceinline__ half8 joined(half2_t a, half2_t b, half2_t c, half2_t d) {
-    return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-// Bytes 0, 2, 1, 3 of each dword as fp16: Q8_0 codes, and the low and the high
-// halves of Q4_0 bytes.
-__device__ __forceinline__ half8 codes_q8(uint32_t w0, uint32_t w1) {
-    w0 ^= 0x80808080u;
-    w1 ^= 0x80808080u;
-    return joined(less(w0 & 0x00ff00ffu, 128.f), less(w0 >> 8 & 0x00ff00ffu, 128.f), less(w1 & 0x00ff00ffu, 128.f),
-                  less(w1 >> 8 & 0x00ff00ffu, 128.f));
-}
-[[maybe_unused]] __device__ __forceinline__ half8 codes_low(uint32_t w0, uint32_t w1) {
-    return joined(less(w0 & 0x000f000fu, 8.f), less(w0 >> 8 & 0x000f000fu, 8.f), less(w1 & 0x000f000fu, 8.f),
-                  less(w1 >> 8 & 0x000f000fu, 8.f));
-}
-[[maybe_unused]] __device__ __forceinline__ half8 codes_high(uint32_t w0, uint32_t w1) {
-    return joined(less_high(w0 & 0x00f000f0u), less_high(w0 >> 8 & 0x00f000f0u), less_high(w1 & 0x00f000f0u),
-                  less_high(w1 >> 8 & 0x00f000f0u));
-}
+__device__ __forceinline__ half8 joined(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __builtin_bit_cast(half8, u32x4{a, b, c, d}); }
+
+// Bytes 0, 2, 1, 3 of two dwords as fp16 operands: Q8_0 codes, or the low or
+// the high halves of Q4_0 bytes less 8.  1024 + u is an fp16 number whose low
+// bits are u (with the sign of a Q8_0 code turned, u = code + 128; of a high
+// half, 16 code); the rest is taken off again, exactly.  The constants stay in
+// registers, for v_and_or_b32 and v_pk_add_f16.
+struct Unpack {
+    uint32_t bytes = 0x00ff00ffu, low = 0x000f000fu, high = 0x00f000f0u, magic = 0x64006400u;
+    half2_t bias8{(_Float16)-1152.f, (_Float16)-1152.f}, bias4{(_Float16)-1032.f, (_Float16)-1032.f};
+    half2_t sixteenth{(_Float16)0.0625f, (_Float16)0.0625f}, bias16{(_Float16)-72.f, (_Float16)-72.f};
+    __device__ __forceinline__ Unpack() {
+#if defined(__HIP_DEVICE_COMPILE__)
+        asm("" : "+s"(bytes), "+s"(low), "+s"(high), "+v"(magic));
+        asm("" : "+s"(bias8), "+s"(bias4), "+s"(sixteenth), "+v"(bias16));
+#endif
+    }
+    static __device__ __forceinline__ uint32_t bits(half2_t v) { return __builtin_bit_cast(uint32_t, v); }
+    __device__ __forceinline__ half2_t number(uint32_t w, uint32_t mask) const { return __builtin_bit_cast(half2_t, (w & mask) | magic); }
+    __device__ __forceinline__ uint32_t q8_two(uint32_t w) const { return bits(number(w, bytes) + bias8); }
+    __device__ __forceinline__ uint32_t low_two(uint32_t w) const { return bits(number(w, low) + bias4); }
+    __device__ __forceinline__ uint32_t high_two(uint32_t w) const { return bits(__builtin_elementwise_fma(number(w, high), sixteenth, bias16)); }
+    __device__ __forceinline__ half8 q8(uint32_t w0, uint32_t w1) const {
+        w0 ^= 0x80808080u;
+        w1 ^= 0x80808080u;
+        return joined(q8_two(w0), q8_two(w0 >> 8), q8_two(w1), q8_two(w1 >> 8));
+    }
+    __device__ __forceinline__ half8 q4_low(uint32_t w0, uint32_t w1) const { return joined(low_two(w0), low_two(w0 >> 8), low_two(w1), low_two(w1 >> 8)); }
+    __device__ __forceinline__ half8 q4_high(uint32_t w0, uint32_t w1) const { return joined(high_two(w0), high_two(w0 >> 8), high_two(w1), high_two(w1 >> 8)); }
+    __device__ __forceinline__ half8 q4_keys(uint32_t w) const { return joined(low_two(w), low_two(w >> 8), high_two(w), high_two(w >> 8)); }
+};
 constexpr int ORDER[8] = {0, 2, 1, 3, 4, 6, 5, 7};   // the bytes of an operand's elements
 
 // What a workgroup has: places [first, ..) of request `request`, whose n query
@@ -97,16 +102,25 @@ struct Span {
     __device__ __forceinline__ int limit(bool causal, int i) const { return causal ? min(end, limit0 + i) : end; }
 };
 
-// The t-th tile of `places` places of all requests; false past the last.
-__device__ __forceinline__ bool find_tile(const CacheAttnArgs& a, int places, int t, int& request, int& tile) {
-    const int lane = threadIdx.x & 63;
+// Workgroups are dispatched round-robin over the 8 XCDs: the kv heads of the
+// same keys, whose blocks share cache lines, follow each other on one of them.
+// The tile is found among 64 requests at a time, each lane with the rows and
+// the length of one, so that one load's latency is all the tables cost.
+__device__ __forceinline__ bool find_span(const CacheAttnArgs& a, int places, int step, Span& s, int& kvh, int& split) {
+    const int lane = threadIdx.x & 63, order = blockIdx.x >> 3;
+    const int sets = int(a.by_kv_heads.quotient(order)), set = (blockIdx.x & 7) + 8 * sets;
+    kvh = order - sets * a.cache.kv_heads;
+    if (set >= a.tiles * a.splits) return false;
+    split = int(a.by_tiles.quotient(set));
+    const int t = set - split * a.tiles;
     int before = 0;
     for (int r0 = 0; r0 < a.cache.requests; r0 += 64) {
-        int tiles = 0;
+        int from = 0, n = 0, len = 0;
         if (r0 + lane < a.cache.requests) {
-            int from;
-            tiles = (max(request_rows(a.cache, a.rows, r0 + lane, from), 0) * a.group + places - 1) / places;
+            n = max(request_rows(a.cache, a.rows, r0 + lane, from), 0);
+            len = request_len(a.cache, r0 + lane);
         }
+        const int tiles = (n * a.group + places - 1) / places;
         int sum = tiles;
         for (int off = 1; off < 64; off <<= 1) {
             const int x = __shfl_up(sum, off, 64);
@@ -115,34 +129,22 @@ __device__ __forceinline__ bool find_tile(const CacheAttnArgs& a, int places, in
         const uint64_t past = __ballot(before + sum > t);
         if (past) {
             const int at = __builtin_ctzll(past);
-            request = r0 + at;
-            tile = t - before - (__shfl(sum, at, 64) - __shfl(tiles, at, 64));
+            s.request = r0 + at;
+            s.q0 = __builtin_amdgcn_readlane(from, at);
+            s.n = __builtin_amdgcn_readlane(n, at);
+            len = __builtin_amdgcn_readlane(len, at);
+            s.first = (t - before - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(tiles, at))) * places;
+            s.end = min(len, a.max_len);
+            s.limit0 = len - s.n + 1;
+            const int tile_end = max(s.limit(a.causal, min(s.n - 1, a.row_of_place(s.first + places - 1))), 0);
+            const int chunk = (tile_end + a.splits * step - 1) / (a.splits * step) * step;
+            s.k0 = min(split * chunk, tile_end);
+            s.k1 = min(s.k0 + chunk, tile_end);
             return true;
         }
-        before += __shfl(sum, 63, 64);
+        before += __builtin_amdgcn_readlane(sum, 63);
     }
     return false;
-}
-
-// Workgroups are dispatched round-robin over the 8 XCDs: the kv heads of the
-// same keys, whose blocks share cache lines, follow each other on one of them.
-__device__ __forceinline__ bool find_span(const CacheAttnArgs& a, int places, int step, Span& s, int& kvh, int& split) {
-    const int order = blockIdx.x >> 3, set = (blockIdx.x & 7) + 8 * (order / a.cache.kv_heads);
-    kvh = order % a.cache.kv_heads;
-    if (set >= a.tiles * a.splits) return false;
-    split = set / a.tiles;
-    int tile;
-    if (!find_tile(a, places, set - split * a.tiles, s.request, tile)) return false;
-    s.n = request_rows(a.cache, a.rows, s.request, s.q0);
-    s.first = tile * places;
-    const int len = request_len(a.cache, s.request);
-    s.end = min(len, a.max_len);
-    s.limit0 = len - s.n + 1;
-    const int tile_end = max(s.limit(a.causal, min(s.n - 1, (s.first + places - 1) / a.group)), 0);
-    const int chunk = ((tile_end + a.splits - 1) / a.splits + step - 1) / step * step;
-    s.k0 = min(split * chunk, tile_end);
-    s.k1 = min(s.k0 + chunk, tile_end);
-    return true;
 }
 
 // Where a part's results go: the output itself when it is the only one.
@@ -182,13 +184,14 @@ struct Block {
 
 template <int TYPE, int HD, int NT>
 struct NarrowShared {
-    static constexpr int PLACES = 8 * NT, TILES = WAVES * KeyTile<TYPE, HD>::BYTES, SUMS = WAVES * PLACES * (HD + 4) * 4;
+    static constexpr int EACH = 512 / HD, PLACES = EACH * NT;   // places of an operand, of a workgroup
+    static constexpr int TILES = WAVES * KeyTile<TYPE, HD>::BYTES, SUMS = WAVES * PLACES * (HD + 4) * 4;
     uint8_t __attribute__((aligned(16))) lds[TILES > SUMS ? TILES : SUMS];
     float b[WAVES][PLACES], l[WAVES][PLACES];
 };
 
 template <int TYPE, int HD, int NT>
-__global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : NT == 1 ? 2 : 1) void cache_attn_narrow_kernel(CacheAttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow_kernel(CacheAttnArgs a) {
     typedef KeyTile<TYPE, HD> T;
     typedef NarrowShared<TYPE, HD, NT> Shared;
     __shared__ Shared sh;
@@ -197,41 +200,39 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : NT == 1 ? 2 : 1) void ca
     if (!find_span(a, Shared::PLACES, T::KEYS * WAVES, s, kvh, split)) return;
     const KvCacheArgs& c = a.cache;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quarter = lane >> 4;
-    const float low = float(lane & 1);   // 1: this lane's column is a query's lo
-    // queries: column 2g + part of tile t, dimensions in the order of the keys' operand
-    half8 q[NT][T::BLOCKS];
+    const int g = col / T::BLOCKS, my_blk = col % T::BLOCKS;   // this lane's column
+    // row 4 quarter + i of the products with values: its place, and whether it is of block `blk`
+    const auto place_of = [&](int i) { return (4 * quarter + i) / T::BLOCKS; };
+    const auto is_of = [](int i, int blk) { return i % T::BLOCKS == blk; };
+    const Unpack unpack;
+    half8 q_hi[NT][T::BLOCKS], q_lo[NT][T::BLOCKS];
     float cq[NT];
     int limit[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int place = s.first + 8 * t + (col >> 1), i = place / a.group, head = kvh * a.group + place - i * a.group;
+        const int place = s.first + Shared::EACH * t + g, i = a.row_of_place(place), head = kvh * a.group + place - i * a.group;
         const bool mine = i < s.n;
         limit[t] = mine ? s.limit(a.causal, i) : 0;
-        const float* from = a.q + (s.q0 + (mine ? i : 0)) * a.ldq + head * HD;
-        float x[T::BLOCKS][8];
+        // Q8_0: 8 neighbours; Q4_0: 4 and the 4 that stand 16 behind them
+        const float* from = a.q + (s.q0 + (mine ? i : 0)) * a.ldq + head * HD + 32 * my_blk + (TYPE == T_Q8_0 ? 8 : 4) * quarter;
+        const float4_at u = *reinterpret_cast<const float4_at*>(from), v = *reinterpret_cast<const float4_at*>(from + (TYPE == T_Q8_0 ? 4 : 16));
+        const float x[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
         uint32_t m = 0;
 #pragma unroll
-        for (int blk = 0; blk < T::BLOCKS; ++blk)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                // Q8_0: 8 neighbours; Q4_0: 4 and the 4 that stand 16 behind them
-                const float4_at v = *reinterpret_cast<const float4_at*>(from + 32 * blk + (TYPE == T_Q8_0 ? 8 * quarter + 4 * h : 4 * quarter + 16 * h));
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    x[blk][4 * h + j] = v[j];
-                    m = umax(m, __float_as_uint(v[j]) & 0x7fffffffu);
-                }
-            }
+        for (int j = 0; j < 8; ++j) m = umax(m, __float_as_uint(x[j]) & 0x7fffffffu);
+        if (T::BLOCKS >= 2) m = umax_dpp<DPP_XOR1>(m);
+        if (T::BLOCKS == 4) m = umax_dpp<DPP_XOR2>(m);
         const int e = exponent_of(umax_xor32(umax_xor16(m)));
         const float f = a.scale < 0.f ? -down(e) : down(e);
-        cq[t] = fmaxf(fabsf(a.scale) * LOG2E * up(e), 0x1p-120f);   // a product with a masked one is -inf
+        cq[t] = fmaxf(fabsf(a.scale) * LOG2E * up(e), 0x1p-120f);   // a masked score times it is -inf
+        half8 hi, lo;
 #pragma unroll
-        for (int blk = 0; blk < T::BLOCKS; ++blk)
+        for (int j = 0; j < 8; j += 2) split_pair(float2_t{x[ORDER[j]] * f, x[ORDER[j + 1]] * f}, hi, lo, j);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float y = x[blk][ORDER[j]] * f, hi = float((_Float16)y);
-                q[t][blk][j] = (_Float16)(low != 0.f ? y - hi : y);
-            }
+        for (int blk = 0; blk < T::BLOCKS; ++blk) {
+            q_hi[t][blk] = my_blk == blk ? hi : half8{};
+            q_lo[t][blk] = my_blk == blk ? lo : half8{};
+        }
     }
     uint8_t* tile = sh.lds + wave * T::BYTES;
     _Float16* scales = reinterpret_cast<_Float16*>(tile + T::SCALES);   // [keys, values][block][key]
@@ -246,6 +247,10 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : NT == 1 ? 2 : 1) void ca
         for (int d = 0; d < 2 * T::BLOCKS; ++d) o[t][d] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
 
+    float zero = 0.f;   // kept from the compiler, which would make a product with a conversion of the mixed fma
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm("" : "+s"(zero));
+#endif
     const int step = T::KEYS * WAVES, kw = s.k0 + T::KEYS * wave;
     // block f = lane + 64 i of a tile: keys' first, a key's blocks side by side
     const auto key_of = [&](int i) { return (lane + 64 * i) % HD / T::BLOCKS; };
@@ -256,41 +261,64 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : NT == 1 ? 2 : 1) void ca
     Block<TYPE> raw[T::PIECES];
     // the cache row of position k + lane (lanes 0 to 31), -1: none
     const auto row_of = [&](int k) { return lane < T::KEYS && k + lane < s.k1 ? cache_row(c, s.request, k + lane) : -1; };
+    // 32 rows on end, as pages of many rows have them, are a scalar base and
+    // offsets that never change.
+    const uint32_t k_off = uint32_t(lane / T::BLOCKS) * uint32_t(c.ldk) + blk_of * T::BB, v_off = uint32_t(lane / T::BLOCKS) * uint32_t(c.ldv) + blk_of * T::BB;
+    uint32_t there = 0;   // the keys of the tile in `raw` that have a row
     const auto load = [&](int row) {
+        const int first = __builtin_amdgcn_readfirstlane(row);
+        there = uint32_t(__ballot(row >= 0));
+        if (HD > 32 && a.short_rows && there == 0xffffffffu && __all(lane >= T::KEYS || row == first + lane)) {
+            const uint8_t *kb = c.k + int64_t(first) * c.ldk + kvh * (T::BLOCKS * T::BB), *vb = c.v + int64_t(first) * c.ldv + kvh * (T::BLOCKS * T::BB);
 #pragma unroll
-        for (int i = 0; i < T::PIECES; ++i) {
-            const int64_t r = max(__shfl(row, key_of(i), 64), 0);   // where there is none, row 0's blocks with scales of zero
-            raw[i].load(of_values(i) ? v_at + r * c.ldv : k_at + r * c.ldk);
+            for (int i = 0; i < T::PIECES; ++i) {
+                constexpr int ROWS = 64 / T::BLOCKS;   // of a piece
+                const int before = 64 * i % HD / T::BLOCKS / ROWS * ROWS;
+                if (of_values(i)) raw[i].load(vb + before * c.ldv + v_off);
+                else raw[i].load(kb + before * c.ldk + k_off);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < T::PIECES; ++i) {
+                const int64_t r = max(__shfl(row, key_of(i), 64), 0);   // where there is none, row 0's blocks with scales of zero
+                raw[i].load(of_values(i) ? v_at + r * c.ldv : k_at + r * c.ldk);
+            }
         }
     };
     bool odd_values = false;
     int row = -1;
-    uint32_t here = 0, next_here = 0;
     if (kw < s.k1) {
         row = row_of(kw);
-        next_here = uint32_t(__ballot(row >= 0));
         load(row);
         row = row_of(kw + step);
     }
     for (int k = kw; k < s.k1; k += step) {
-        here = next_here;
+        const uint32_t here = there;
         wave_lds_handoff();   // the last tile's reads came first
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < T::PIECES; ++i) odd = odd || !finite_half(raw[i].d);
+        if (here != 0xffffffffu || __any(odd)) {
+#pragma unroll
+            for (int i = 0; i < T::PIECES; ++i) {
+                const bool is = here >> key_of(i) & 1, v = of_values(i);
+                if (!finite_half(raw[i].d)) {
+                    odd_values = odd_values || (v && is);   // added behind the last tile, for those that see them
+                    raw[i].d = v ? 0u : 0x7e00u;
+                }
+                raw[i].d = is ? raw[i].d : 0u;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < T::PIECES; ++i) {
             const int key = key_of(i);
-            const bool there = here >> key & 1, v = of_values(i);
-            uint32_t d = raw[i].d;
-            if (!finite_half(d)) {
-                odd_values = odd_values || (v && there);   // added behind the last tile, for those that see them
-                d = v ? 0u : 0x7e00u;
-            }
-            d = there ? d : 0u;
+            const bool v = of_values(i);
             uint8_t* to = tile + (v ? T::VALUES : 0) + blk_of * T::HALVES * T::STRIDE + key * 16;
             *reinterpret_cast<u32x4*>(to) = raw[i].w[0];
             if constexpr (TYPE == T_Q8_0) *reinterpret_cast<u32x4*>(to + T::STRIDE) = raw[i].w[1];
-            reinterpret_cast<uint16_t*>(scales)[((v ? T::BLOCKS : 0) + blk_of) * T::KEYS + key] = uint16_t(d);
+            reinterpret_cast<uint16_t*>(scales)[((v ? T::BLOCKS : 0) + blk_of) * T::KEYS + key] = uint16_t(raw[i].d);
             if (T::BLOCKS == 1 || 64 * i >= HD) {   // values: the largest scale of a key's blocks
-                uint32_t most = d & 0x7fffu;
+                uint32_t most = raw[i].d & 0x7fffu;
                 if (T::BLOCKS == 2) most = umax_dpp<DPP_XOR1>(most);
                 if (T::BLOCKS == 4) most = umax_quad(most);
                 if (v && blk_of == 0) logs[key] = fmaxf(__builtin_amdgcn_logf(half_bits_to_float(most)), float(ZERO_SCALE));
@@ -298,47 +326,45 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : NT == 1 ? 2 : 1) void ca
         }
         wave_lds_handoff();
         if (k + step < s.k1) {
-            next_here = uint32_t(__ballot(row >= 0));
             load(row);
             row = row_of(k + 2 * step);
         }
-        // scores of keys 16n + 4 quarter + i
-        floatx4 sc[NT][2];
+        // scores of keys 16n + 4 quarter + i: the block's of this column, then the sum over its place's columns
+        float w[NT][8];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
+            floatx4 sc[NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) sc[t][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; t < NT; ++t) sc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int blk = 0; blk < T::BLOCKS; ++blk) {
                 half8 keys;
                 if constexpr (TYPE == T_Q8_0) {
-                    const u32x2 w = *reinterpret_cast<const u32x2*>(tile + (2 * blk + (quarter >> 1)) * T::STRIDE + (16 * n + col) * 16 + 8 * (quarter & 1));
-                    keys = codes_q8(w[0], w[1]);
+                    const u32x2 code = *reinterpret_cast<const u32x2*>(tile + (2 * blk + (quarter >> 1)) * T::STRIDE + (16 * n + col) * 16 + 8 * (quarter & 1));
+                    keys = unpack.q8(code[0], code[1]);
                 } else {
-                    const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + blk * T::STRIDE + (16 * n + col) * 16 + 4 * quarter);
-                    keys = joined(less(w & 0x000f000fu, 8.f), less(w >> 8 & 0x000f000fu, 8.f), less_high(w & 0x00f000f0u), less_high(w >> 8 & 0x00f000f0u));
+                    keys = unpack.q4_keys(*reinterpret_cast<const uint32_t*>(tile + blk * T::STRIDE + (16 * n + col) * 16 + 4 * quarter));
                 }
-                const half4 d = *reinterpret_cast<const half4*>(scales + blk * T::KEYS + 16 * n + 4 * quarter);
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const floatx4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, q[t][blk], floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sc[t][n][i] = __builtin_fmaf(float(d[i]), p[i], sc[t][n][i]);
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, q_hi[t][blk], sc[t], 0, 0, 0);
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, q_lo[t][blk], sc[t], 0, 0, 0);
                 }
             }
-        }
-        float log_d[8];
+            const half4 d = *reinterpret_cast<const half4*>(scales + my_blk * T::KEYS + 16 * n + 4 * quarter);
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const floatx4 v = *reinterpret_cast<const floatx4*>(logs + 16 * n + 4 * quarter);
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) log_d[4 * n + i] = v[i];
+                for (int i = 0; i < 4; ++i) {
+                    float x = __builtin_fmaf(float(d[i]), sc[t][i], zero);
+                    if (T::BLOCKS >= 2) x += dpp<DPP_XOR1>(x);
+                    if (T::BLOCKS == 4) x += dpp<DPP_XOR2>(x);
+                    w[t][4 * n + i] = x;
+                }
         }
-        float w[NT][8];
+        const floatx4 log_d[2] = {*reinterpret_cast<const floatx4*>(logs + 4 * quarter), *reinterpret_cast<const floatx4*>(logs + 16 + 4 * quarter)};
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[t][j] = sc[t][j >> 2][j & 3] + dpp<DPP_XOR1>(sc[t][j >> 2][j & 3]);   // hi's and lo's
             if (here != 0xffffffffu || __any(k + T::KEYS > limit[t])) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -346,21 +372,20 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : NT == 1 ? 2 : 1) void ca
                     if (!(here >> key & 1) || k + key >= limit[t]) w[t][j] = -__builtin_inff();
                 }
             }
-            float top = __builtin_fmaf(w[t][0], cq[t], log_d[0]);
+            float top = __builtin_fmaf(w[t][0], cq[t], log_d[0][0]);
 #pragma unroll
-            for (int j = 1; j < 8; ++j) top = fmaxf(top, __builtin_fmaf(w[t][j], cq[t], log_d[j]));
+            for (int j = 1; j < 8; ++j) top = fmaxf(top, __builtin_fmaf(w[t][j], cq[t], log_d[j >> 2][j & 3]));
             top = max_xor32(max_xor16(top));
             if (__any(top > base[t] + 15.f)) {
                 const float moved = top > base[t] + 15.f ? top - 13.f : base[t], f = __builtin_amdgcn_exp2f(base[t] - moved);
                 base[t] = moved;
                 l[t] *= f;
-                const float f0 = __shfl(f, 4 * quarter, 64), f1 = __shfl(f, 4 * quarter + 2, 64);   // of the queries of this lane's rows
 #pragma unroll
-                for (int d = 0; d < 2 * T::BLOCKS; ++d) {
-                    o[t][d][0] *= f0;
-                    o[t][d][1] *= f0;
-                    o[t][d][2] *= f1;
-                    o[t][d][3] *= f1;
+                for (int i = 0; i < 4; ++i) {
+                    const float f_i = __shfl(f, place_of(i) * T::BLOCKS, 64);   // of the query of row i
+#pragma unroll
+                    for (int d = 0; d < 2 * T::BLOCKS; ++d)
+                        if (is_of(i, d >> 1)) o[t][d][i] *= f_i;
                 }
             }
 #pragma unroll
@@ -369,44 +394,49 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : NT == 1 ? 2 : 1) void ca
                 l[t] += w[t][j];
             }
         }
-        // O += P V, P the weights with a block's scales, of key 4 quarter + j and 16 + 4 quarter + j - 4
+        // O += P V, P the weights with this column's block's scales; element j is key
+        // 4 quarter + j or 16 + 4 quarter + j - 4 in either operand.  Of a block's
+        // products only the rows of that block count.
         [[maybe_unused]] const uint8_t* values = tile + T::VALUES + (4 * quarter + (col >> 1 & 3) + (col >> 3) * 16) * 16 + 8 * (col & 1);
-#pragma unroll
-        for (int blk = 0; blk < T::BLOCKS; ++blk) {
-            half8 p[NT];
-            const _Float16* dv = scales + (T::BLOCKS + blk) * T::KEYS + 4 * quarter;
+        half8 p_hi[NT], p_lo[NT];
+        {
+            const _Float16* dv = scales + (T::BLOCKS + my_blk) * T::KEYS + 4 * quarter;
             const half4 d0 = *reinterpret_cast<const half4*>(dv), d1 = *reinterpret_cast<const half4*>(dv + 16);
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     const int j0 = ORDER[j], j1 = ORDER[j + 1];
-                    const float x0 = w[t][j0] * float(j0 < 4 ? d0[j0 & 3] : d1[j0 & 3]), x1 = w[t][j1] * float(j1 < 4 ? d0[j1 & 3] : d1[j1 & 3]);
-                    const half2_t h = __builtin_convertvector(float2_t{x0, x1}, half2_t);
-                    const half2_t y = __builtin_convertvector(float2_t{__builtin_fmaf(-float(h[0]), low, x0), __builtin_fmaf(-float(h[1]), low, x1)}, half2_t);
-                    p[t][j] = y[0];
-                    p[t][j + 1] = y[1];
+                    const float x0 = __builtin_fmaf(w[t][j0], float(j0 < 4 ? d0[j0 & 3] : d1[j0 & 3]), zero);
+                    const float x1 = __builtin_fmaf(w[t][j1], float(j1 < 4 ? d0[j1 & 3] : d1[j1 & 3]), zero);
+                    split_pair(float2_t{x0, x1}, p_hi[t], p_lo[t], j);
                 }
+        }
+#pragma unroll
+        for (int blk = 0; blk < T::BLOCKS; ++blk) {
             half8 v[2];
 #if defined(__HIP_DEVICE_COMPILE__)
             // lane i of 16 gets byte i of the 8 keys that the lanes address, two lanes to a key
-            const auto read = [&](const uint8_t* at) {
-                return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) int2_t*)(at)));
+            const auto read = [&](int chunk) {
+                return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) int2_t*)(values + chunk * T::STRIDE)));
             };
             if constexpr (TYPE == T_Q8_0) {
-                const u32x2 w0 = read(values + 2 * blk * T::STRIDE), w1 = read(values + (2 * blk + 1) * T::STRIDE);
-                v[0] = codes_q8(w0[0], w0[1]);
-                v[1] = codes_q8(w1[0], w1[1]);
+                const u32x2 w0 = read(2 * blk), w1 = read(2 * blk + 1);
+                v[0] = unpack.q8(w0[0], w0[1]);
+                v[1] = unpack.q8(w1[0], w1[1]);
             } else {
-                const u32x2 w0 = read(values + blk * T::STRIDE);
-                v[0] = codes_low(w0[0], w0[1]);
-                v[1] = codes_high(w0[0], w0[1]);
+                const u32x2 w0 = read(blk);
+                v[0] = unpack.q4_low(w0[0], w0[1]);
+                v[1] = unpack.q4_high(w0[0], w0[1]);
             }
 #endif
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) o[t][2 * blk + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[t], v[h], o[t][2 * blk + h], 0, 0, 0);
+                for (int h = 0; h < 2; ++h) {
+                    o[t][2 * blk + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p_hi[t], v[h], o[t][2 * blk + h], 0, 0, 0);
+                    o[t][2 * blk + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p_lo[t], v[h], o[t][2 * blk + h], 0, 0, 0);
+                }
         }
     }
     if (__any(odd_values)) {
@@ -422,7 +452,7 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : NT == 1 ? 2 : 1) void ca
                     for (int t = 0; t < NT; ++t)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (k + n < __shfl(limit[t], 4 * quarter + (i & 2), 64)) o[t][2 * blk][i] = o[t][2 * blk + 1][i] = __builtin_nanf("");
+                            if (k + n < __shfl(limit[t], place_of(i) * T::BLOCKS, 64)) o[t][2 * blk][i] = o[t][2 * blk + 1][i] = __builtin_nanf("");
                 }
             }
     }
@@ -430,9 +460,9 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : NT == 1 ? 2 : 1) void ca
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         l[t] = pair_sum(sum_xor16(l[t]));
-        if (quarter == 0 && low == 0.f) {
-            sh.b[wave][8 * t + (col >> 1)] = base[t];
-            sh.l[wave][8 * t + (col >> 1)] = l[t];
+        if (quarter == 0 && my_blk == 0) {
+            sh.b[wave][Shared::EACH * t + g] = base[t];
+            sh.l[wave][Shared::EACH * t + g] = l[t];
         }
     }
     __syncthreads();   // also: every wave is past its tiles
@@ -449,16 +479,17 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : NT == 1 ? 2 : 1) void ca
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            const int p = 8 * t + 2 * quarter + g;
+        for (int i = 0; i < 4; ++i) {
+            const int p = Shared::EACH * t + place_of(i);
             float most;
             const float sum = joined_sum(p, most);
             const float f = sh.l[wave][p] != 0.f ? __builtin_amdgcn_exp2f(sh.b[wave][p] - most) / sum : 0.f;
 #pragma unroll
-            for (int d = 0; d < 2 * T::BLOCKS; ++d) all[(wave * Shared::PLACES + p) * (HD + 4) + 16 * d + col] = (o[t][d][2 * g] + o[t][d][2 * g + 1]) * f;
+            for (int d = 0; d < 2 * T::BLOCKS; ++d)
+                if (is_of(i, d >> 1)) all[(wave * Shared::PLACES + p) * (HD + 4) + 16 * d + col] = o[t][d][i] * f;
         }
     if (tid < Shared::PLACES) {
-        const int place = s.first + tid, i = place / a.group;
+        const int place = s.first + tid, i = a.row_of_place(place);
         float most;
         const float sum = joined_sum(tid, most);
         if (i < s.n) leave_part(a, s.q0 + i, kvh * a.group + place - i * a.group, split, most, sum);
@@ -466,7 +497,7 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : NT == 1 ? 2 : 1) void ca
     __syncthreads();
     constexpr int QUADS = HD / 4;
     for (int t = tid; t < Shared::PLACES * QUADS; t += 64 * WAVES) {
-        const int p = t / QUADS, d = 4 * (t % QUADS), place = s.first + p, i = place / a.group;
+        const int p = t / QUADS, d = 4 * (t % QUADS), place = s.first + p, i = a.row_of_place(place);
         if (i >= s.n) continue;
         floatx4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -533,7 +564,7 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
     if (!find_span(a, TILE * WAVES, WIDE_KEYS, s, kvh, split)) return;
     const KvCacheArgs& c = a.cache;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hh = lane >> 5;
-    const int place = s.first + TILE * wave + li, i_row = place / a.group, head = kvh * a.group + place - i_row * a.group;
+    const int place = s.first + TILE * wave + li, i_row = a.row_of_place(place), head = kvh * a.group + place - i_row * a.group;
     const bool mine = i_row < s.n;
     const int row = s.q0 + (mine ? i_row : 0), limit = mine ? min(s.limit(a.causal, i_row), s.k1) : 0;
     // queries: lane (li, hh) has place li's values 16t + 8hh .. + 7
@@ -748,12 +779,21 @@ void launch_of_type(const CacheAttnArgs& a, hipStream_t stream) {
 void cache_attn_plan(CacheAttnArgs& a, int cus) {
     const int64_t places = int64_t(a.rows) * a.group, requests = std::min(a.cache.requests, a.rows);
     const int64_t each = (places + requests - 1) / requests;   // of a request with its share of the rows
-    a.query_tiles = each <= 8 ? 1 : each <= 16 ? 2 : 0;
-    const int tile = a.query_tiles ? 8 * a.query_tiles : TILE * WAVES, step = a.query_tiles ? 32 * WAVES : WIDE_KEYS;
+    const int of_operand = 512 / a.cache.head_dim;
+    a.query_tiles = each <= of_operand ? 1 : each <= 2 * of_operand ? 2 : 0;
+    const int tile = a.query_tiles ? of_operand * a.query_tiles : TILE * WAVES, step = a.query_tiles ? 32 * WAVES : WIDE_KEYS;
     a.tiles = int(places / tile + requests);
     const int64_t groups = ((each + tile - 1) / tile) * requests * a.cache.kv_heads;
+    a.by_group = Divisor::of(a.group);
+    a.by_kv_heads = Divisor::of(a.cache.kv_heads);
+    a.by_tiles = Divisor::of(a.tiles);
+    a.short_rows = std::max(a.cache.ldk, a.cache.ldv) < (int64_t(1) << 26);
+    // Three workgroups a CU, as many as are there at once: one round (64 single
+    // queries of 16 heads of 128 on up to 8192 keys, for 2, 3, 4, 6, 8 a CU: 79,
+    // 72, 80, 74, 78 us; 8 of 8 heads of 32 on 5217: 16.4, 15.9, 15.9, 15.9, 15.9),
+    // but no part below four tiles of every wave.
     const int64_t most = std::max<int64_t>(1, a.max_len / (4 * step));
-    a.splits = int(std::max<int64_t>(1, std::min<int64_t>((4 * cus + groups - 1) / groups, most)));
+    a.splits = int(std::max<int64_t>(1, std::min<int64_t>((3 * cus + groups - 1) / groups, most)));
 }
 
 size_t cache_attn_scratch_bytes(const CacheAttnArgs& a) {

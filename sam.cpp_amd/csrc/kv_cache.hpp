@@ -107,7 +107,10 @@ struct CacheAttnArgs {
     int max_len;                           // at most the capacity; 0 where the cache has no page
     float scale;
     bool causal;
+    bool short_rows;                       // the bytes of 32 rows fit 31 bits
     int query_tiles;                       // of 8 places; 0: 128 places to a workgroup
+    Divisor by_group, by_kv_heads, by_tiles;
+    __host__ __device__ int row_of_place(int place) const { return int(by_group.quotient(place)); }   // of a request's
     int tiles, splits;                     // tiles of all requests (at most), and parts of their keys
     float *part_o, *part_ml;
 };
