@@ -130,10 +130,11 @@ __device__ __forceinline__ float pair_sum(float l) {
     return __uint_as_float(other[0]) + __uint_as_float(other[1]);
 }
 
-// A wave joins the parts of one row and head: their maxima and sums one to a
-// lane, then HD / 4 lanes to a part's mean.
+// A wave joins the parts of one row and head (ml_apart and o_apart floats from
+// one to the next): their maxima and sums one to a lane, then HD / 4 lanes to a
+// part's mean.
 template <int HD>
-__device__ __forceinline__ void merge_parts(const float* part_ml, const float* part_o, int count, float* out) {
+__device__ __forceinline__ void merge_parts(const float* part_ml, int64_t ml_apart, const float* part_o, int64_t o_apart, int count, float* out) {
     constexpr int QUADS = HD / 4, AT_ONCE = 64 / QUADS;
     const int lane = threadIdx.x & 63;
     const int d = 4 * (lane % QUADS), slot = lane / QUADS;
@@ -142,7 +143,7 @@ __device__ __forceinline__ void merge_parts(const float* part_ml, const float* p
     for (int p0 = 0; p0 < count; p0 += 64) {
         float mp = -__builtin_inff(), lp = 0.f;
         if (p0 + lane < count) {
-            const float* ml = part_ml + (p0 + lane) * 2;
+            const float* ml = part_ml + (p0 + lane) * ml_apart;
             mp = ml[0];
             lp = ml[1];
         }
@@ -156,7 +157,7 @@ __device__ __forceinline__ void merge_parts(const float* part_ml, const float* p
         f = lp != 0.f ? f * inv : -1.f;   // no key in this part
         v = v * (before * inv);
         const int here = min(count - p0, 64);
-        const float* parts = part_o + p0 * HD + d;
+        const float* parts = part_o + p0 * o_apart + d;
         const auto add = [&](auto at_once, int p1) {   // parts p1 + slot, p1 + slot + AT_ONCE, ..
             constexpr int U = decltype(at_once)::value;
             floatx4 o[U];
@@ -164,7 +165,7 @@ __device__ __forceinline__ void merge_parts(const float* part_ml, const float* p
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int p = p1 + u * AT_ONCE + slot, at = min(p, here - 1);
-                o[u] = *reinterpret_cast<const floatx4*>(parts + at * HD);
+                o[u] = *reinterpret_cast<const floatx4*>(parts + at * o_apart);
                 fp[u] = __shfl(f, at, 64);
                 if (p >= here) fp[u] = -1.f;
             }

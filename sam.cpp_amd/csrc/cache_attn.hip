@@ -38,6 +38,7 @@ namespace samhip {
 namespace {
 
 constexpr int WAVES = 4;
+constexpr int kCacheAttnMaxShared = 4096; // requests beyond which each is one part: a workgroup would spend its time on the tables
 constexpr float NO_BASE = -1e30f;         // below every score, and finite
 constexpr int ZERO_SCALE = -40;           // log 2 of what a zero scale counts as
 
@@ -93,67 +94,126 @@ struct Unpack {
 };
 constexpr int ORDER[8] = {0, 2, 1, 3, 4, 6, 5, 7};   // the bytes of an operand's elements
 
-// What a workgroup has: places [first, ..) of request `request`, whose n query
-// rows begin at q0, and its positions [k0, k1).
+// Sum over the lanes up to and with this one (row shifts, then the last lanes of
+// rows 0 and 2, and of row 1, to what lies behind them).
+__device__ __forceinline__ int running_sum(int v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+#endif
+    return v;
+}
+
+// A request's share of the grid: tiles of its places, and parts of its keys.
+// Parts are even in work over the whole call: with W the tiles' steps of keys
+// of all requests, a part has about W / slots steps, so that a long request has
+// more of them and no workgroup much more to do than another (64 requests of
+// 4096 to 8192 keys in three parts each: 72 us; so: 68).  The parts of requests
+// that have several number at most 2 * slots.
+struct Share {
+    int request, q0, n, len, tiles, parts;
+    int before, kept;   // items (tile, part) of the requests before, and those of them that are kept for the join
+};
+
+// The request for which match(first row, rows, items to its end) holds first; the
+// requests are read 64 at a time, a lane to each.
+template <class Match>
+__device__ __forceinline__ bool find_request(const CacheAttnArgs& a, Match match, Share& s) {
+    const int lane = threadIdx.x & 63;
+    int from, n, len, tiles, steps;
+    const auto read = [&](int r0) {
+        from = n = len = 0;
+        if (r0 + lane < a.cache.requests) {
+            n = max(request_rows(a.cache, a.rows, r0 + lane, from), 0);
+            len = request_len(a.cache, r0 + lane);
+        }
+        tiles = int(a.by_places.quotient(n * a.group + a.by_places.d - 1));
+        steps = int(a.by_step.quotient(min(len, a.max_len) + a.by_step.d - 1));
+    };
+    read(0);
+    float of_part = 0.f;   // 1 / steps of a part
+    if (a.slots) {
+        float work = float(tiles) * float(steps), all = float(tiles);
+        for (int r0 = 64; r0 < a.cache.requests; r0 += 64) {
+            read(r0);
+            work += float(tiles) * float(steps);
+            all += float(tiles);
+        }
+        if (a.cache.requests > 64) read(0);
+        // every tile's last part is a half too much, on average; a thousandth more, for the sums' roundings
+        const float slots = fmaxf(float(a.slots) - 0.5f * wave_sum(all), 0.5f * float(a.slots));
+        of_part = 1.f / fmaxf(float(a.least_steps), fminf(__builtin_ceilf(wave_sum(work) * 1.001f / slots), 1e9f));
+    }
+    int before = 0, kept = 0;
+    for (int r0 = 0; r0 < a.cache.requests; r0 += 64) {
+        if (r0) read(r0);
+        const int parts = max(1, int(__builtin_ceilf(float(steps) * of_part))), items = tiles * parts, to_keep = parts > 1 ? items : 0;
+        const int sum = running_sum(items), kept_sum = running_sum(to_keep);
+        const uint64_t hit = __ballot(match(from, n, before + sum));
+        if (hit) {
+            const int at = __builtin_ctzll(hit);
+            s.request = r0 + at;
+            s.q0 = __builtin_amdgcn_readlane(from, at);
+            s.n = __builtin_amdgcn_readlane(n, at);
+            s.len = __builtin_amdgcn_readlane(len, at);
+            s.tiles = __builtin_amdgcn_readlane(tiles, at);
+            s.parts = __builtin_amdgcn_readlane(parts, at);
+            s.before = before + __builtin_amdgcn_readlane(sum - items, at);
+            s.kept = kept + __builtin_amdgcn_readlane(kept_sum - to_keep, at);
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
+        kept += __builtin_amdgcn_readlane(kept_sum, 63);
+    }
+    return false;
+}
+
+// What a workgroup has: places [first, ..) of a request whose n query rows begin
+// at q0, and its positions [k0, k1).
 struct Span {
-    int request, q0, n, first;
+    int request, q0, n, first, kvh;
     int k0, k1;
     int end, limit0;      // a query row i sees positions below min(end, limit0 + i)
+    int kept;             // the place of its results among those to be joined, -1: the output itself
     __device__ __forceinline__ int limit(bool causal, int i) const { return causal ? min(end, limit0 + i) : end; }
 };
 
 // Workgroups are dispatched round-robin over the 8 XCDs: the kv heads of the
 // same keys, whose blocks share cache lines, follow each other on one of them.
-// The tile is found among 64 requests at a time, each lane with the rows and
-// the length of one, so that one load's latency is all the tables cost.
-__device__ __forceinline__ bool find_span(const CacheAttnArgs& a, int places, int step, Span& s, int& kvh, int& split) {
-    const int lane = threadIdx.x & 63, order = blockIdx.x >> 3;
-    const int sets = int(a.by_kv_heads.quotient(order)), set = (blockIdx.x & 7) + 8 * sets;
-    kvh = order - sets * a.cache.kv_heads;
-    if (set >= a.tiles * a.splits) return false;
-    split = int(a.by_tiles.quotient(set));
-    const int t = set - split * a.tiles;
-    int before = 0;
-    for (int r0 = 0; r0 < a.cache.requests; r0 += 64) {
-        int from = 0, n = 0, len = 0;
-        if (r0 + lane < a.cache.requests) {
-            n = max(request_rows(a.cache, a.rows, r0 + lane, from), 0);
-            len = request_len(a.cache, r0 + lane);
-        }
-        const int tiles = (n * a.group + places - 1) / places;
-        int sum = tiles;
-        for (int off = 1; off < 64; off <<= 1) {
-            const int x = __shfl_up(sum, off, 64);
-            if (lane >= off) sum += x;
-        }
-        const uint64_t past = __ballot(before + sum > t);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            s.request = r0 + at;
-            s.q0 = __builtin_amdgcn_readlane(from, at);
-            s.n = __builtin_amdgcn_readlane(n, at);
-            len = __builtin_amdgcn_readlane(len, at);
-            s.first = (t - before - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(tiles, at))) * places;
-            s.end = min(len, a.max_len);
-            s.limit0 = len - s.n + 1;
-            const int tile_end = max(s.limit(a.causal, min(s.n - 1, a.row_of_place(s.first + places - 1))), 0);
-            const int chunk = (tile_end + a.splits * step - 1) / (a.splits * step) * step;
-            s.k0 = min(split * chunk, tile_end);
-            s.k1 = min(s.k0 + chunk, tile_end);
-            return true;
-        }
-        before += __builtin_amdgcn_readlane(sum, 63);
-    }
-    return false;
+__device__ __forceinline__ bool find_span(const CacheAttnArgs& a, Span& s) {
+    const int order = blockIdx.x >> 3, sets = int(a.by_kv_heads.quotient(order)), item = (blockIdx.x & 7) + 8 * sets;
+    s.kvh = order - sets * a.cache.kv_heads;
+    Share share;
+    if (!find_request(a, [&](int, int, int to) { return to > item; }, share)) return false;
+    const int local = item - share.before, part = local / share.tiles, places = int(a.by_places.d), step = int(a.by_step.d);
+    s.request = share.request;
+    s.q0 = share.q0;
+    s.n = share.n;
+    s.first = (local - part * share.tiles) * places;
+    s.kept = share.parts > 1 ? share.kept + local : -1;
+    s.end = min(share.len, a.max_len);
+    s.limit0 = share.len - s.n + 1;
+    const int tile_end = max(s.limit(a.causal, min(s.n - 1, a.row_of_place(s.first + places - 1))), 0);
+    const int chunk = (int(a.by_step.quotient(tile_end + step - 1)) + share.parts - 1) / share.parts * step;
+    s.k0 = min(part * chunk, tile_end);
+    s.k1 = min(s.k0 + chunk, tile_end);
+    return true;
 }
 
-// Where a part's results go: the output itself when it is the only one.
-__device__ __forceinline__ float* part_of(const CacheAttnArgs& a, int row, int head, int hd, int split) {
-    return a.splits == 1 ? a.out + row * a.ldo + head * hd : a.part_o + ((int64_t(row) * a.heads + head) * a.splits + split) * hd;
+// Where the results of a tile's p-th place go.
+__device__ __forceinline__ int64_t kept_place(const CacheAttnArgs& a, int kvh, int kept, int p) {
+    return (int64_t(kvh) * 2 * a.slots + kept) * a.by_places.d + p;
 }
-__device__ __forceinline__ void leave_part(const CacheAttnArgs& a, int row, int head, int split, float base, float sum) {
-    if (a.splits == 1) return;
-    float* ml = a.part_ml + ((int64_t(row) * a.heads + head) * a.splits + split) * 2;
+__device__ __forceinline__ float* result_of(const CacheAttnArgs& a, const Span& s, int p, int row, int head, int hd) {
+    return s.kept < 0 ? a.out + row * a.ldo + head * hd : a.part_o + kept_place(a, s.kvh, s.kept, p) * hd;
+}
+__device__ __forceinline__ void leave_sum(const CacheAttnArgs& a, const Span& s, int p, float base, float sum) {
+    if (s.kept < 0) return;
+    float* ml = a.part_ml + kept_place(a, s.kvh, s.kept, p) * 2;
     ml[0] = base;
     ml[1] = sum;
 }
@@ -196,44 +256,52 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
     typedef NarrowShared<TYPE, HD, NT> Shared;
     __shared__ Shared sh;
     Span s;
-    int kvh, split;
-    if (!find_span(a, Shared::PLACES, T::KEYS * WAVES, s, kvh, split)) return;
+    if (!find_span(a, s)) return;
+    const int kvh = s.kvh;
     const KvCacheArgs& c = a.cache;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quarter = lane >> 4;
     const int g = col / T::BLOCKS, my_blk = col % T::BLOCKS;   // this lane's column
     // row 4 quarter + i of the products with values: its place, and whether it is of block `blk`
     const auto place_of = [&](int i) { return (4 * quarter + i) / T::BLOCKS; };
     const auto is_of = [](int i, int blk) { return i % T::BLOCKS == blk; };
+    int limit[NT];
+    floatx8 x[NT];   // this column's and quarter's part of the queries
+    const auto load_queries = [&] {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int place = s.first + Shared::EACH * t + g, i = a.row_of_place(place), head = kvh * a.group + place - i * a.group;
+            const bool mine = i < s.n;
+            limit[t] = mine ? s.limit(a.causal, i) : 0;
+            // Q8_0: 8 neighbours; Q4_0: 4 and the 4 that stand 16 behind them
+            const float* from = a.q + (s.q0 + (mine ? i : 0)) * a.ldq + head * HD + 32 * my_blk + (TYPE == T_Q8_0 ? 8 : 4) * quarter;
+            const float4_at u = *reinterpret_cast<const float4_at*>(from), v = *reinterpret_cast<const float4_at*>(from + (TYPE == T_Q8_0 ? 4 : 16));
+            x[t] = floatx8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+        }
+    };
     const Unpack unpack;
     half8 q_hi[NT][T::BLOCKS], q_lo[NT][T::BLOCKS];
     float cq[NT];
-    int limit[NT];
+    const auto split_queries = [&] {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int place = s.first + Shared::EACH * t + g, i = a.row_of_place(place), head = kvh * a.group + place - i * a.group;
-        const bool mine = i < s.n;
-        limit[t] = mine ? s.limit(a.causal, i) : 0;
-        // Q8_0: 8 neighbours; Q4_0: 4 and the 4 that stand 16 behind them
-        const float* from = a.q + (s.q0 + (mine ? i : 0)) * a.ldq + head * HD + 32 * my_blk + (TYPE == T_Q8_0 ? 8 : 4) * quarter;
-        const float4_at u = *reinterpret_cast<const float4_at*>(from), v = *reinterpret_cast<const float4_at*>(from + (TYPE == T_Q8_0 ? 4 : 16));
-        const float x[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
-        uint32_t m = 0;
+        for (int t = 0; t < NT; ++t) {
+            uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = umax(m, __float_as_uint(x[j]) & 0x7fffffffu);
-        if (T::BLOCKS >= 2) m = umax_dpp<DPP_XOR1>(m);
-        if (T::BLOCKS == 4) m = umax_dpp<DPP_XOR2>(m);
-        const int e = exponent_of(umax_xor32(umax_xor16(m)));
-        const float f = a.scale < 0.f ? -down(e) : down(e);
-        cq[t] = fmaxf(fabsf(a.scale) * LOG2E * up(e), 0x1p-120f);   // a masked score times it is -inf
-        half8 hi, lo;
+            for (int j = 0; j < 8; ++j) m = umax(m, __float_as_uint(x[t][j]) & 0x7fffffffu);
+            if (T::BLOCKS >= 2) m = umax_dpp<DPP_XOR1>(m);
+            if (T::BLOCKS == 4) m = umax_dpp<DPP_XOR2>(m);
+            const int e = exponent_of(umax_xor32(umax_xor16(m)));
+            const float f = a.scale < 0.f ? -down(e) : down(e);
+            cq[t] = fmaxf(fabsf(a.scale) * LOG2E * up(e), 0x1p-120f);   // a masked score times it is -inf
+            half8 hi, lo;
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) split_pair(float2_t{x[ORDER[j]] * f, x[ORDER[j + 1]] * f}, hi, lo, j);
+            for (int j = 0; j < 8; j += 2) split_pair(float2_t{x[t][ORDER[j]] * f, x[t][ORDER[j + 1]] * f}, hi, lo, j);
 #pragma unroll
-        for (int blk = 0; blk < T::BLOCKS; ++blk) {
-            q_hi[t][blk] = my_blk == blk ? hi : half8{};
-            q_lo[t][blk] = my_blk == blk ? lo : half8{};
+            for (int blk = 0; blk < T::BLOCKS; ++blk) {
+                q_hi[t][blk] = my_blk == blk ? hi : half8{};
+                q_lo[t][blk] = my_blk == blk ? lo : half8{};
+            }
         }
-    }
+    };
     uint8_t* tile = sh.lds + wave * T::BYTES;
     _Float16* scales = reinterpret_cast<_Float16*>(tile + T::SCALES);   // [keys, values][block][key]
     float* logs = reinterpret_cast<float*>(tile + T::LOGS);
@@ -258,13 +326,13 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
     const int blk_of = lane % T::BLOCKS;
     const uint8_t* k_at = c.k + (kvh * T::BLOCKS + blk_of) * T::BB;
     const uint8_t* v_at = c.v + (kvh * T::BLOCKS + blk_of) * T::BB;
-    Block<TYPE> raw[T::PIECES];
+    Block<TYPE> raw[T::PIECES];   // the next tile
     // the cache row of position k + lane (lanes 0 to 31), -1: none
     const auto row_of = [&](int k) { return lane < T::KEYS && k + lane < s.k1 ? cache_row(c, s.request, k + lane) : -1; };
     // 32 rows on end, as pages of many rows have them, are a scalar base and
     // offsets that never change.
     const uint32_t k_off = uint32_t(lane / T::BLOCKS) * uint32_t(c.ldk) + blk_of * T::BB, v_off = uint32_t(lane / T::BLOCKS) * uint32_t(c.ldv) + blk_of * T::BB;
-    uint32_t there = 0;   // the keys of the tile in `raw` that have a row
+    uint32_t there = 0;           // its keys that have a row
     const auto load = [&](int row) {
         const int first = __builtin_amdgcn_readfirstlane(row);
         there = uint32_t(__ballot(row >= 0));
@@ -286,12 +354,11 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
         }
     };
     bool odd_values = false;
-    int row = -1;
-    if (kw < s.k1) {
-        row = row_of(kw);
-        load(row);
-        row = row_of(kw + step);
-    }
+    int row = row_of(kw);
+    load_queries();   // behind the table's load, before what waits for it
+    if (kw < s.k1) load(row);
+    row = row_of(kw + step);
+    split_queries();
     for (int k = kw; k < s.k1; k += step) {
         const uint32_t here = there;
         wave_lds_handoff();   // the last tile's reads came first
@@ -492,7 +559,7 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
         const int place = s.first + tid, i = a.row_of_place(place);
         float most;
         const float sum = joined_sum(tid, most);
-        if (i < s.n) leave_part(a, s.q0 + i, kvh * a.group + place - i * a.group, split, most, sum);
+        if (i < s.n) leave_sum(a, s, tid, most, sum);
     }
     __syncthreads();
     constexpr int QUADS = HD / 4;
@@ -502,7 +569,7 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
         floatx4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) v += *reinterpret_cast<const floatx4*>(all + (w * Shared::PLACES + p) * (HD + 4) + d);
-        *reinterpret_cast<float4_at*>(part_of(a, s.q0 + i, kvh * a.group + place - i * a.group, HD, split) + d) = v;
+        *reinterpret_cast<float4_at*>(result_of(a, s, p, s.q0 + i, kvh * a.group + place - i * a.group, HD) + d) = v;
     }
 }
 
@@ -560,8 +627,8 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
     constexpr int PIECES = HD / 32, BB = block_bytes(TYPE);   // of 8 values, a thread's part of a tile
     __shared__ Shared sh;
     Span s;
-    int kvh, split;
-    if (!find_span(a, TILE * WAVES, WIDE_KEYS, s, kvh, split)) return;
+    if (!find_span(a, s)) return;
+    const int kvh = s.kvh;
     const KvCacheArgs& c = a.cache;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hh = lane >> 5;
     const int place = s.first + TILE * wave + li, i_row = a.row_of_place(place), head = kvh * a.group + place - i_row * a.group;
@@ -740,8 +807,8 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
     l = pair_sum(l);
     if (!mine) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (hh == 0) leave_part(a, row, head, split, base, l);
-    float* to = part_of(a, row, head, HD, split);
+    if (hh == 0) leave_sum(a, s, TILE * wave + li, base, l);
+    float* to = result_of(a, s, TILE * wave + li, row, head, HD);
 #pragma unroll
     for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
@@ -749,22 +816,27 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
             *reinterpret_cast<float4_at*>(to + 32 * d + 2 * r + 4 * hh) = floatx4{o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv};
 }
 
+// A wave per (row, head): joins its parts where there are several.
 template <int HD>
 __global__ __launch_bounds__(256) void cache_attn_merge_kernel(CacheAttnArgs a) {
-    const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6), items = int64_t(a.rows) * a.heads;   // a wave per (row, head)
+    const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6), items = int64_t(a.rows) * a.heads;
     if (item >= items) return;
-    const int64_t row = item / a.heads, h = item - row * a.heads;
-    if (row < min(max(a.cache.row_start[0], 0), a.rows) || row >= min(max(a.cache.row_start[a.cache.requests], 0), a.rows)) return;
-    merge_parts<HD>(a.part_ml + item * a.splits * 2, a.part_o + item * a.splits * HD, a.splits, a.out + row * a.ldo + h * HD);
+    const int row = int(item / a.heads), h = int(item - int64_t(row) * a.heads);
+    Share s;
+    if (!find_request(a, [&](int from, int n, int) { return row >= from && row < from + n; }, s) || s.parts == 1) return;
+    const int kvh = a.row_of_place(h), place = (row - s.q0) * a.group + h - kvh * a.group;   // (heads of a kv head are a group too)
+    const int tile = int(a.by_places.quotient(place)), p = place - tile * int(a.by_places.d);
+    const int64_t first = kept_place(a, kvh, s.kept + tile, p), apart = int64_t(s.tiles) * a.by_places.d;
+    merge_parts<HD>(a.part_ml + first * 2, apart * 2, a.part_o + first * HD, apart * HD, s.parts, a.out + row * a.ldo + h * HD);
 }
 
 template <int TYPE, int HD>
 void launch_typed(const CacheAttnArgs& a, hipStream_t stream) {
-    const unsigned groups = unsigned((int64_t(a.tiles) * a.splits + 7) / 8 * 8 * a.cache.kv_heads);
+    const unsigned groups = unsigned((a.slots + a.tiles + 7) / 8 * 8 * a.cache.kv_heads);
     if (a.query_tiles == 0) cache_attn_wide_kernel<TYPE, HD><<<groups, 64 * WAVES, 0, stream>>>(a);
     else if (a.query_tiles == 1) cache_attn_narrow_kernel<TYPE, HD, 1><<<groups, 64 * WAVES, 0, stream>>>(a);
     else cache_attn_narrow_kernel<TYPE, HD, 2><<<groups, 64 * WAVES, 0, stream>>>(a);
-    if (a.splits > 1) cache_attn_merge_kernel<HD><<<unsigned((int64_t(a.rows) * a.heads + 3) / 4), 256, 0, stream>>>(a);
+    if (a.slots) cache_attn_merge_kernel<HD><<<unsigned((int64_t(a.rows) * a.heads + 3) / 4), 256, 0, stream>>>(a);
 }
 
 template <int TYPE>
@@ -783,26 +855,28 @@ void cache_attn_plan(CacheAttnArgs& a, int cus) {
     a.query_tiles = each <= of_operand ? 1 : each <= 2 * of_operand ? 2 : 0;
     const int tile = a.query_tiles ? of_operand * a.query_tiles : TILE * WAVES, step = a.query_tiles ? 32 * WAVES : WIDE_KEYS;
     a.tiles = int(places / tile + requests);
-    const int64_t groups = ((each + tile - 1) / tile) * requests * a.cache.kv_heads;
     a.by_group = Divisor::of(a.group);
     a.by_kv_heads = Divisor::of(a.cache.kv_heads);
-    a.by_tiles = Divisor::of(a.tiles);
+    a.by_places = Divisor::of(tile);
+    a.by_step = Divisor::of(step);
     a.short_rows = std::max(a.cache.ldk, a.cache.ldv) < (int64_t(1) << 26);
-    // Three workgroups a CU, as many as are there at once: one round (64 single
-    // queries of 16 heads of 128 on up to 8192 keys, for 2, 3, 4, 6, 8 a CU: 79,
-    // 72, 80, 74, 78 us; 8 of 8 heads of 32 on 5217: 16.4, 15.9, 15.9, 15.9, 15.9),
-    // but no part below four tiles of every wave.
-    const int64_t most = std::max<int64_t>(1, a.max_len / (4 * step));
-    a.splits = int(std::max<int64_t>(1, std::min<int64_t>((3 * cus + groups - 1) / groups, most)));
+    // About as many parts as run at once (us for 2, 3, 4, 5, 6 workgroups a CU: 64
+    // queries of 16 heads of 128 on up to 8192 Q4_0 keys 78, 68, 74, 71, 67; 16
+    // heads of 64 on 32768 248, 212, 224, 250, 222; 8 of 8 heads of 32 378, 377,
+    // 278, 278, 338; 8 prompts of 201 queries 61, 69, 63, 65, 65).
+    a.least_steps = 2;
+    const int at_once = !a.query_tiles ? 2 : a.cache.head_dim == 32 ? 4 : 3;
+    a.slots = std::max(1, at_once * cus / a.cache.kv_heads);
+    if (a.max_len <= a.least_steps * step || a.cache.requests > kCacheAttnMaxShared) a.slots = 0;
 }
 
 size_t cache_attn_scratch_bytes(const CacheAttnArgs& a) {
-    return a.splits > 1 ? size_t(a.splits) * a.rows * a.heads * (a.cache.head_dim + 2) * 4 : 0;
+    return size_t(2) * a.slots * a.cache.kv_heads * a.by_places.d * (a.cache.head_dim + 2) * 4;
 }
 
 void launch_cache_attn(CacheAttnArgs a, int type, void* scratch, hipStream_t stream) {
     a.part_o = static_cast<float*>(scratch);
-    a.part_ml = a.part_o + size_t(a.splits) * a.rows * a.heads * a.cache.head_dim;
+    a.part_ml = a.part_o + size_t(2) * a.slots * a.cache.kv_heads * a.by_places.d * a.cache.head_dim;
     if (type == T_Q4_0) launch_of_type<T_Q4_0>(a, stream);
     else launch_of_type<T_Q8_0>(a, stream);
 }

@@ -108,10 +108,11 @@ struct CacheAttnArgs {
     float scale;
     bool causal;
     bool short_rows;                       // the bytes of 32 rows fit 31 bits
-    int query_tiles;                       // of 8 places; 0: 128 places to a workgroup
-    Divisor by_group, by_kv_heads, by_tiles;
+    int query_tiles;                       // of 512 / head_dim places; 0: 128 places to a workgroup
+    Divisor by_group, by_kv_heads, by_places, by_step;   // by_places, by_step: a workgroup's places, and its keys at a time
+    int tiles;                             // of all requests, at most
+    int slots, least_steps;                // parts of keys of a kv head in all, and the steps of the smallest; 0 slots: one part each
     __host__ __device__ int row_of_place(int place) const { return int(by_group.quotient(place)); }   // of a request's
-    int tiles, splits;                     // tiles of all requests (at most), and parts of their keys
     float *part_o, *part_ml;
 };
 void cache_attn_plan(CacheAttnArgs& a, int cus);

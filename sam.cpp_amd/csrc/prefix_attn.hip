@@ -644,7 +644,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(PrefixAttnArgs a) {
     if (item >= items) return;
     const int64_t row = item / a.heads, h = item - row * a.heads;
     if (row < min(max(a.q_start[0], 0), a.rows) || row >= min(max(a.q_start[a.requests], 0), a.rows)) return;
-    merge_parts<HD>(a.part_ml + item * a.parts * 2, a.part_o + item * a.parts * HD, a.parts, a.out + row * a.ldo + h * HD);
+    merge_parts<HD>(a.part_ml + item * a.parts * 2, 2, a.part_o + item * a.parts * HD, HD, a.parts, a.out + row * a.ldo + h * HD);
 }
 
 template <class T, int HD>
