@@ -24,8 +24,9 @@
 // take one block's value scale in each lane instead of all blocks' in every
 // one.  (With hi and lo as columns, and a lane's scores and weights block by
 // block, 64 queries of 16 heads of 128 on up to 8192 keys took 84 us.)
-// Many places: 128 to a workgroup, 64 keys at a time, decoded once into hi + lo
-// halves in LDS for its four waves.
+// Many places: 128 to a workgroup, 64 keys at a time as fp16 codes in LDS for its
+// four waves, the next ones written beside them.  Key scales multiply a block's
+// products, value scales the weights.
 #include <algorithm>
 
 #include "attn_tiles.hpp"
@@ -578,10 +579,9 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
 constexpr int TILE = 32;                  // query places of a wave
 constexpr int WIDE_KEYS = 64;
 
-// Eight neighbouring values of a row.
+// Eight neighbouring codes of a row, and their block's scale.
 template <int TYPE>
 struct Octet {
-    static constexpr int SHIFT = TYPE == T_Q8_0 ? 7 : 3;   // no code's magnitude passes 2^SHIFT
     uint32_t d, w0, w1;
     __device__ __forceinline__ void load(const uint8_t* head_row, int octet) {
         const uint8_t* block = head_row + (octet >> 2) * block_bytes(TYPE);
@@ -590,41 +590,35 @@ struct Octet {
         w0 = w[0];
         w1 = w[1];
     }
-    // values * factor as hi + lo; a code less its bias is one fma, exact
-    __device__ __forceinline__ void split(int octet, float factor, half8& hi, half8& lo) const {
-        const float df = half_bits_to_float(d) * factor, bias = df * (TYPE == T_Q8_0 ? -128.f : -8.f);
+    // as fp16, in order
+    __device__ __forceinline__ half8 codes(const Unpack& unpack, int octet) const {
         const uint32_t c0 = TYPE == T_Q8_0 ? w0 ^ 0x80808080u : w0 >> (2 * (octet & 2)) & 0x0f0f0f0fu;
         const uint32_t c1 = TYPE == T_Q8_0 ? w1 ^ 0x80808080u : w1 >> (2 * (octet & 2)) & 0x0f0f0f0fu;
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            const uint32_t c = j < 4 ? c0 : c1;
-            const float x0 = __builtin_fmaf(float(c >> (8 * (j & 3)) & 0xffu), df, bias), x1 = __builtin_fmaf(float(c >> (8 * (j & 3) + 8) & 0xffu), df, bias);
-            split_pair(float2_t{x0, x1}, hi, lo, j);
-        }
+        const half2_t bias = TYPE == T_Q8_0 ? unpack.bias8 : unpack.bias4;
+        // bytes 0 and 1, or 2 and 3, each below a 0x64
+        const auto two = [&](uint32_t c, uint32_t select) { return Unpack::bits(__builtin_bit_cast(half2_t, __builtin_amdgcn_perm(unpack.magic, c, select)) + bias); };
+        return joined(two(c0, 0x07010700u), two(c0, 0x07030702u), two(c1, 0x07010700u), two(c1, 0x07030702u));
     }
 };
 
 template <int HD>
 struct WideShared {
-    typedef TileShape<2, HD, WIDE_KEYS, false> K;
-    typedef TileShape<2, HD, WIDE_KEYS, true> V;
-    uint8_t __attribute__((aligned(16))) k[K::BYTES];
-    uint8_t __attribute__((aligned(16))) v[V::BYTES];
-    uint32_t largest[WAVES][2];
-    int rows[2][WIDE_KEYS];
+    typedef TileShape<1, HD, WIDE_KEYS, false> K;
+    typedef TileShape<1, HD, WIDE_KEYS, true> V;
+    struct Tile {
+        uint8_t __attribute__((aligned(16))) k[K::BYTES];
+        uint8_t __attribute__((aligned(16))) v[V::BYTES];
+        _Float16 __attribute__((aligned(16))) scales[2][HD / 32][WIDE_KEYS];   // of keys, of values
+        uint32_t most[WAVES];                                                  // the largest of the values'
+    } tile[2];
+    int rows[4][WIDE_KEYS];
     uint64_t here[4];
 };
-
-// Biased exponent of 2^SHIFT times the largest scale, zeros as 2^ZERO_SCALE.
-template <int TYPE>
-__device__ __forceinline__ int scale_exponent(uint32_t half_bits) {
-    return max(int(__float_as_uint(half_bits_to_float(half_bits)) >> 23), 127 + ZERO_SCALE) + Octet<TYPE>::SHIFT;
-}
 
 template <int TYPE, int HD>
 __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_kernel(CacheAttnArgs a) {
     typedef WideShared<HD> Shared;
-    constexpr int PIECES = HD / 32, BB = block_bytes(TYPE);   // of 8 values, a thread's part of a tile
+    constexpr int PIECES = HD / 32, BLOCKS = HD / 32, BB = block_bytes(TYPE);   // of 8 values, a thread's part of a tile
     __shared__ Shared sh;
     Span s;
     if (!find_span(a, s)) return;
@@ -634,6 +628,23 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
     const int place = s.first + TILE * wave + li, i_row = a.row_of_place(place), head = kvh * a.group + place - i_row * a.group;
     const bool mine = i_row < s.n;
     const int row = s.q0 + (mine ? i_row : 0), limit = mine ? min(s.limit(a.causal, i_row), s.k1) : 0;
+
+    // Cache rows of a tile, looked up by the first wave three tiles ahead.
+    const auto row_at = [&](int k) { return k + lane < s.k1 ? cache_row(c, s.request, k + lane) : -1; };
+    const auto put_rows = [&](int t, int r) {
+        const uint64_t here = __ballot(r >= 0);
+        sh.rows[t & 3][lane] = r;
+        if (lane == 0) sh.here[t & 3] = here;
+    };
+    int ahead = -1;
+    if (wave == 0) {
+        const int r0 = row_at(s.k0), r1 = row_at(s.k0 + WIDE_KEYS), r2 = row_at(s.k0 + 2 * WIDE_KEYS);
+        put_rows(0, r0);
+        put_rows(1, r1);
+        put_rows(2, r2);
+        ahead = row_at(s.k0 + 3 * WIDE_KEYS);
+    }
+
     // queries: lane (li, hh) has place li's values 16t + 8hh .. + 7
     half8 q_hi[HD / 16], q_lo[HD / 16];
     float cq;
@@ -650,24 +661,28 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
         }
         const int e = exponent_of(umax_xor32(m));
         const float f = a.scale < 0.f ? -down(e) : down(e);
-        cq = fabsf(a.scale) * LOG2E * up(e);
+        cq = fmaxf(fabsf(a.scale) * LOG2E * up(e), 0x1p-120f);   // a masked score times it is -inf
 #pragma unroll
         for (int t = 0; t < HD / 16; ++t)
 #pragma unroll
             for (int j = 0; j < 8; j += 2) split_pair(float2_t{x[t][j] * f, x[t][j + 1] * f}, q_hi[t], q_lo[t], j);
     }
     // o[d] holds, transposed, dimensions 32d + 8 (r / 4) + 4hh + r % 4 of place li
-    floatx16 o[HD / 32];
-    float base = NO_BASE, l = 0.f;
+    floatx16 o[BLOCKS];
+    float base = NO_BASE, l = 0.f, zero = 0.f;   // (zero: kept from the compiler, for the mixed fma)
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm("" : "+s"(zero));
+#endif
 #pragma unroll
-    for (int d = 0; d < HD / 32; ++d)
+    for (int d = 0; d < BLOCKS; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
 
     // this thread's piece of the first 256; the others are whole rows of keys on
     constexpr int EACH = 2048 / HD;
     const int key = tid / (HD / 8), octet = tid % (HD / 8);
-    const uint8_t *k_at = c.k + kvh * (HD / 32) * BB, *v_at = c.v + kvh * (HD / 32) * BB;
+    const uint8_t *k_at = c.k + kvh * BLOCKS * BB, *v_at = c.v + kvh * BLOCKS * BB;
+    const Unpack unpack;
     Octet<TYPE> kr[PIECES], vr[PIECES];
     uint32_t there = 0;   // of the pieces, whether their key has a row
     const auto load = [&](const int* rows) {
@@ -681,116 +696,132 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
             vr[i].load(v_at + at * c.ldv, octet);
         }
     };
-    // Cache rows of a tile, looked up by the first wave two tiles ahead.
-    const auto row_at = [&](int k) { return k + lane < s.k1 ? cache_row(c, s.request, k + lane) : -1; };
-    const auto put_rows = [&](int t, int r) {
-        const uint64_t here = __ballot(r >= 0);
-        sh.rows[t & 1][lane] = r;
-        if (lane == 0) sh.here[t & 3] = here;
+    bool odd_values = false;
+    const auto put = [&](typename Shared::Tile& tile) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const bool is = there >> i & 1;
+            uint32_t dk = is ? kr[i].d : 0u, dv = is ? vr[i].d : 0u;
+            if (!finite_half(dk)) dk = 0x7e00u;
+            if (!finite_half(dv)) {
+                odd_values = true;   // added behind the last tile, for those that see them
+                dv = 0;
+            }
+            most = umax(most, dv & 0x7fffu);
+            const int f = tid + 256 * i;
+            *Shared::K::piece(tile.k, f) = kr[i].codes(unpack, octet);
+            *Shared::V::piece(tile.v, f) = vr[i].codes(unpack, octet);
+            if (octet % 4 == 0) {
+                reinterpret_cast<uint16_t*>(tile.scales[0][octet / 4])[key + i * EACH] = uint16_t(dk);
+                reinterpret_cast<uint16_t*>(tile.scales[1][octet / 4])[key + i * EACH] = uint16_t(dv);
+            }
+        }
+        most = wave_umax(most);
+        if (lane == 0) tile.most[wave] = most;
     };
-    int ahead = -1;
-    if (wave == 0 && s.k0 < s.k1) {
-        put_rows(0, row_at(s.k0));
-        put_rows(1, row_at(s.k0 + WIDE_KEYS));
-        ahead = row_at(s.k0 + 2 * WIDE_KEYS);
+    __syncthreads();
+    if (s.k0 < s.k1) {
+        load(sh.rows[0]);
+        put(sh.tile[0]);
+        if (s.k0 + WIDE_KEYS < s.k1) load(sh.rows[1]);
     }
     __syncthreads();
-    if (s.k0 < s.k1) load(sh.rows[0]);
-    bool odd_values = false;
-    int t_now = 0;
-    const int wave_end = [&] {   // no place of this wave sees a key behind it
+    const int wave_end = [&] {   // no place of this wave sees a key from it on
         int v = limit;
         for (int off = 1; off < 32; off <<= 1) v = max(v, __shfl_xor(v, off, 64));
         return __builtin_amdgcn_readfirstlane(v);
     }();
+    int t_now = 0;
     for (int k = s.k0; k < s.k1; k += WIDE_KEYS, ++t_now) {
-        uint32_t mk = 0, mv = 0;
+        const typename Shared::Tile& tile = sh.tile[t_now & 1];
+        if (k < wave_end) {
+            uint32_t most = 0;
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const bool is = there >> i & 1;
-            if (!finite_half(kr[i].d)) kr[i].d = 0x7e00u;
-            if (!finite_half(vr[i].d)) {
-                odd_values = odd_values || is;   // added behind the last tile, for those that see them
-                vr[i].d = 0;
-            }
-            kr[i].d = is ? kr[i].d : 0u;
-            vr[i].d = is ? vr[i].d : 0u;
-            const uint32_t dk = kr[i].d & 0x7fffu;
-            mk = umax(mk, dk < 0x7c00u ? dk : 0u);
-            mv = umax(mv, vr[i].d & 0x7fffu);
-        }
-        mk = wave_umax(mk);
-        mv = wave_umax(mv);
-        if (lane == 0) sh.largest[wave][0] = mk, sh.largest[wave][1] = mv;
-        __syncthreads();   // the last tile is read, the largest scales are written
-        mk = mv = 0;
+            for (int w = 0; w < WAVES; ++w) most = umax(most, tile.most[w]);
+            const float log_d = fmaxf(__builtin_amdgcn_logf(half_bits_to_float(most)), float(ZERO_SCALE));
+            const uint64_t here = sh.here[t_now & 3];
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) mk = umax(mk, sh.largest[w][0]), mv = umax(mv, sh.largest[w][1]);
-        const int ek = scale_exponent<TYPE>(__builtin_amdgcn_readfirstlane(mk)), ev = scale_exponent<TYPE>(__builtin_amdgcn_readfirstlane(mv));
+            for (int n = 0; n < WIDE_KEYS / 32; ++n) {
+                // scores of keys 32n + 8 (r / 4) + 4hh + r % 4, block by block
+                const uint8_t* kt = tile.k + (32 * n + li) * Shared::K::STRIDE + 16 * hh;
+                floatx16 sc;
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            half8 hi, lo;
-            kr[i].split(octet, down(ek), hi, lo);
-            half8* to = Shared::K::piece(sh.k, tid + 256 * i);
-            *to = hi;
-            to[WIDE_KEYS * Shared::K::STRIDE / 16] = lo;
-            vr[i].split(octet, down(ev), hi, lo);
-            to = Shared::V::piece(sh.v, tid + 256 * i);
-            *to = hi;
-            to[WIDE_KEYS * Shared::V::STRIDE / 16] = lo;
-        }
-        if (wave == 0) put_rows(t_now + 2, ahead);
-        __syncthreads();
-        if (k + WIDE_KEYS < s.k1) {
-            load(sh.rows[(t_now + 1) & 1]);
-            if (wave == 0) ahead = row_at(k + 3 * WIDE_KEYS);
-        }
-        if (k >= wave_end) continue;
-        floatx16 sc[2];
-        scores<2, HD, 2>(sh.k, q_hi, q_lo, sc);
-        const uint64_t here = sh.here[t_now & 3];
-        if (here != ~uint64_t(0) || __any(k + WIDE_KEYS > limit)) {
+                for (int blk = 0; blk < BLOCKS; ++blk) {
+                    floatx16 p;
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+                    for (int r = 0; r < 16; ++r) p[r] = 0.f;
+#pragma unroll
+                    for (int u = 2 * blk; u < 2 * blk + 2; ++u) {
+                        const half8 keys = *reinterpret_cast<const half8*>(kt + 32 * u);
+                        p = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys, q_hi[u], p, 0, 0, 0);
+                        p = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys, q_lo[u], p, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4) {
+                        const half4 d = *reinterpret_cast<const half4*>(tile.scales[0][blk] + 32 * n + 2 * r + 4 * hh);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) sc[r + j] = __builtin_fmaf(float(d[j]), p[r + j], blk ? sc[r + j] : zero);
+                    }
+                }
+                const uint32_t here_n = uint32_t(here >> (32 * n));
+                if (here_n != 0xffffffffu || __any(k + 32 * n + 32 > limit)) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int at = 8 * (r >> 2) + 4 * hh + (r & 3);
+                        if (!(here_n >> at & 1) || k + 32 * n + at >= limit) sc[r] = -__builtin_inff();
+                    }
+                }
+                float top = sc[0];
+#pragma unroll
+                for (int r = 1; r < 16; ++r) top = __builtin_elementwise_maximum(top, sc[r]);
+                const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                top = __builtin_fmaf(__builtin_elementwise_maximum(__uint_as_float(other[0]), __uint_as_float(other[1])), cq, log_d);
+                if (__any(top > base + 15.f)) {
+                    const float moved = top > base + 15.f ? top - 13.f : base, by = __builtin_amdgcn_exp2f(base - moved);
+                    base = moved;
+                    l *= by;
+#pragma unroll
+                    for (int d = 0; d < BLOCKS; ++d)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[d][r] *= by;
+                }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int at = 32 * n + 8 * (r >> 2) + 4 * hh + (r & 3);
-                    if (!(here >> at & 1) || k + at >= limit) sc[n][r] = -__builtin_inff();
+                    sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], cq, -base));
+                    l += sc[r];
                 }
-        }
-        const float f = fmaxf(cq * up(ek), 0x1p-120f), unit = float(ev - 141);   // values are in units of 2^unit
-        float top = sc[0][0];
+                // O^T += V^T P^T, P the weights with a block's scales: of 16 keys, lane
+                // (li, hh) has keys 4hh .. + 3 and 8 + 4hh .. + 3 of both operands
+                const uint8_t* vt = tile.v + (32 * n + 4 * hh + ((lane & 15) >> 2)) * Shared::V::STRIDE + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+                for (int d = 0; d < BLOCKS; ++d) {
+                    half8 p_hi[2], p_lo[2];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) top = __builtin_elementwise_maximum(top, sc[n][r]);
-        const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-        top = __builtin_fmaf(__builtin_elementwise_maximum(__uint_as_float(other[0]), __uint_as_float(other[1])), f, unit);
-        if (__any(top > base + 15.f)) {
-            const float moved = top > base + 15.f ? top - 13.f : base, by = __builtin_amdgcn_exp2f(base - moved);
-            base = moved;
-            l *= by;
+                    for (int r = 0; r < 16; r += 4) {
+                        const half4 dv = *reinterpret_cast<const half4*>(tile.scales[1][d] + 32 * n + 2 * r + 4 * hh);
 #pragma unroll
-            for (int d = 0; d < HD / 32; ++d)
+                        for (int j = 0; j < 4; j += 2)
+                            split_pair(float2_t{__builtin_fmaf(sc[r + j], float(dv[j]), zero), __builtin_fmaf(sc[r + j + 1], float(dv[j + 1]), zero)}, p_hi[r >> 3],
+                                       p_lo[r >> 3], (r & 7) + j);
+                    }
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[d][r] *= by;
-        }
-        const float shift = unit - base;
-        float sum = 0.f;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                sc[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][r], f, shift));
-                sum += sc[n][r];
+                    for (int u = 0; u < 2; ++u) {
+                        const uint8_t* at = vt + 16 * u * Shared::V::STRIDE + 64 * d;
+                        const half8 v = __builtin_shufflevector(ds_read_tr(at), ds_read_tr(at + 8 * Shared::V::STRIDE), 0, 1, 2, 3, 4, 5, 6, 7);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p_hi[u], o[d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p_lo[u], o[d], 0, 0, 0);
+                    }
+                }
             }
-        l += sum * __builtin_ldexpf(1.f, 141 - ev);
-        half8 p_hi[4], p_lo[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) split_pair(float2_t{sc[u / 2][8 * (u % 2) + j], sc[u / 2][8 * (u % 2) + j + 1]}, p_hi[u], p_lo[u], j);
-        values<2, HD, 2>(sh.v, p_hi, p_lo, o);
+        }
+        if (k + WIDE_KEYS < s.k1) put(sh.tile[(t_now + 1) & 1]);
+        if (k + 2 * WIDE_KEYS < s.k1) load(sh.rows[(t_now + 2) & 3]);
+        if (wave == 0) {
+            put_rows(t_now + 3, ahead);
+            ahead = row_at(k + 4 * WIDE_KEYS);
+        }
+        __syncthreads();   // the next tile is written, this one read
     }
     if (__syncthreads_or(odd_values)) {
         // values whose scale is no number were zeros: NaN for the queries that see them
@@ -798,7 +829,7 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
             const int r = cache_row(c, s.request, k);
             if (r < 0) continue;
 #pragma unroll
-            for (int d = 0; d < HD / 32; ++d)
+            for (int d = 0; d < BLOCKS; ++d)
                 if (!finite_half(*reinterpret_cast<const uint16_t*>(v_at + r * c.ldv + d * BB)) && k < limit)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[d][e] = __builtin_nanf("");
@@ -810,24 +841,82 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
     if (hh == 0) leave_sum(a, s, TILE * wave + li, base, l);
     float* to = result_of(a, s, TILE * wave + li, row, head, HD);
 #pragma unroll
-    for (int d = 0; d < HD / 32; ++d)
+    for (int d = 0; d < BLOCKS; ++d)
 #pragma unroll
         for (int r = 0; r < 16; r += 4)
             *reinterpret_cast<float4_at*>(to + 32 * d + 2 * r + 4 * hh) = floatx4{o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv};
 }
 
-// A wave per (row, head): joins its parts where there are several.
-template <int HD>
-__global__ __launch_bounds__(256) void cache_attn_merge_kernel(CacheAttnArgs a) {
-    const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6), items = int64_t(a.rows) * a.heads;
-    if (item >= items) return;
-    const int row = int(item / a.heads), h = int(item - int64_t(row) * a.heads);
+// Joins the parts of a row's heads.  HD / 4 lanes have a part's mean, SLOTS such
+// groups every SLOTS-th part of a head, and a wave 256 / HD / SLOTS heads of a
+// row, for finding the row's request costs it more than a join of few parts
+// (1608 rows of 8 heads of 32 in three parts: 4.6 us, a wave to each head 8.0).
+template <int HD, int SLOTS>
+__global__ __launch_bounds__(256) void cache_attn_merge_kernel(CacheAttnArgs a, Divisor by_sets) {
+    constexpr int QUADS = HD / 4, HEADS = 64 / (QUADS * SLOTS), AT_ONCE = 4;
+    const uint32_t unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int row = int(by_sets.quotient(unit)), lane = threadIdx.x & 63, slot = lane / QUADS % SLOTS, d = 4 * (lane % QUADS);
+    if (row >= a.rows) return;
     Share s;
     if (!find_request(a, [&](int from, int n, int) { return row >= from && row < from + n; }, s) || s.parts == 1) return;
+    const int head = int(unit - row * by_sets.d) * HEADS + lane / (QUADS * SLOTS), h = min(head, a.heads - 1);
     const int kvh = a.row_of_place(h), place = (row - s.q0) * a.group + h - kvh * a.group;   // (heads of a kv head are a group too)
     const int tile = int(a.by_places.quotient(place)), p = place - tile * int(a.by_places.d);
     const int64_t first = kept_place(a, kvh, s.kept + tile, p), apart = int64_t(s.tiles) * a.by_places.d;
-    merge_parts<HD>(a.part_ml + first * 2, apart * 2, a.part_o + first * HD, apart * HD, s.parts, a.out + row * a.ldo + h * HD);
+    const float *ml = a.part_ml + first * 2, *o = a.part_o + first * HD + d;
+    float m = -__builtin_inff(), l = 0.f;
+    floatx4 v{0.f, 0.f, 0.f, 0.f};   // a mean
+    for (int part = slot; part < s.parts; part += AT_ONCE * SLOTS) {
+        float m_of[AT_ONCE], l_of[AT_ONCE];
+        floatx4 o_of[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int64_t at = min(part + u * SLOTS, s.parts - 1) * apart;
+            m_of[u] = ml[2 * at];
+            l_of[u] = part + u * SLOTS < s.parts ? ml[2 * at + 1] : 0.f;
+            o_of[u] = *reinterpret_cast<const floatx4*>(o + at * HD);
+        }
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) top = fmaxf(top, l_of[u] != 0.f ? m_of[u] : -__builtin_inff());
+        const float before = m == top ? l : l * __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        l = before;
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            m_of[u] = l_of[u] != 0.f ? l_of[u] * __builtin_amdgcn_exp2f(m_of[u] - top) : 0.f;
+            l += m_of[u];
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        v = v * (before * inv);
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += l_of[u] != 0.f ? o_of[u][j] * (m_of[u] * inv) : 0.f;   // without keys its mean may never have been written
+    }
+    if constexpr (SLOTS > 1) {
+        float top = m;
+#pragma unroll
+        for (int off = QUADS; off < QUADS * SLOTS; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+        float mine = m == top ? l : l * __builtin_amdgcn_exp2f(m - top), sum = mine;
+#pragma unroll
+        for (int off = QUADS; off < QUADS * SLOTS; off <<= 1) sum += __shfl_xor(sum, off, 64);
+        mine = sum == 0.f ? 0.f : mine / sum;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j] = v[j] * mine;
+#pragma unroll
+            for (int off = QUADS; off < QUADS * SLOTS; off <<= 1) v[j] += __shfl_xor(v[j], off, 64);
+        }
+    }
+    if (head < a.heads && slot == 0) *reinterpret_cast<float4_at*>(a.out + row * a.ldo + h * HD + d) = v;
+}
+
+template <int HD, int SLOTS>
+void launch_merge(const CacheAttnArgs& a, hipStream_t stream) {
+    constexpr int HEADS = 256 / (HD * SLOTS);
+    const int sets = (a.heads + HEADS - 1) / HEADS;
+    cache_attn_merge_kernel<HD, SLOTS><<<unsigned((int64_t(a.rows) * sets + 3) / 4), 256, 0, stream>>>(a, Divisor::of(sets));
 }
 
 template <int TYPE, int HD>
@@ -836,7 +925,9 @@ void launch_typed(const CacheAttnArgs& a, hipStream_t stream) {
     if (a.query_tiles == 0) cache_attn_wide_kernel<TYPE, HD><<<groups, 64 * WAVES, 0, stream>>>(a);
     else if (a.query_tiles == 1) cache_attn_narrow_kernel<TYPE, HD, 1><<<groups, 64 * WAVES, 0, stream>>>(a);
     else cache_attn_narrow_kernel<TYPE, HD, 2><<<groups, 64 * WAVES, 0, stream>>>(a);
-    if (a.slots) cache_attn_merge_kernel<HD><<<unsigned((int64_t(a.rows) * a.heads + 3) / 4), 256, 0, stream>>>(a);
+    // few places: few rows, of many parts
+    if (a.slots && a.query_tiles) launch_merge<HD, 256 / HD>(a, stream);
+    else if (a.slots) launch_merge<HD, 1>(a, stream);
 }
 
 template <int TYPE>
@@ -863,9 +954,12 @@ void cache_attn_plan(CacheAttnArgs& a, int cus) {
     // About as many parts as run at once (us for 2, 3, 4, 5, 6 workgroups a CU: 64
     // queries of 16 heads of 128 on up to 8192 Q4_0 keys 78, 68, 74, 71, 67; 16
     // heads of 64 on 32768 248, 212, 224, 250, 222; 8 of 8 heads of 32 378, 377,
-    // 278, 278, 338; 8 prompts of 201 queries 61, 69, 63, 65, 65).
+    // 278, 278, 338; many places, 8 prompts of 201 queries of 8 heads of 32 on up to
+    // 5217 Q8_0 keys 54, 51, 53, -, 53; 13 requests of up to 150 queries of 12 heads
+    // of 64 on up to 1300 34, 42, 40, -, 44: registers hold two of these in a CU, and
+    // three of head_dim 32).
     a.least_steps = 2;
-    const int at_once = !a.query_tiles ? 2 : a.cache.head_dim == 32 ? 4 : 3;
+    const int at_once = !a.query_tiles ? (a.cache.head_dim == 32 ? 3 : 2) : a.cache.head_dim == 32 ? 4 : 3;
     a.slots = std::max(1, at_once * cus / a.cache.kv_heads);
     if (a.max_len <= a.least_steps * step || a.cache.requests > kCacheAttnMaxShared) a.slots = 0;
 }
