@@ -732,8 +732,17 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
         for (int off = 1; off < 32; off <<= 1) v = max(v, __shfl_xor(v, off, 64));
         return __builtin_amdgcn_readfirstlane(v);
     }();
+    // What shares a SIMD is served oldest first: the last of three workgroups would
+    // run alone in the end, and slowly (48.0 us for 8 prompts of 201 queries of 8
+    // heads of 32; so that who is behind comes first: 42.6).
+    const int quarter = (s.k1 - s.k0) / 4;
+    __builtin_amdgcn_s_setprio(3);
     int t_now = 0;
     for (int k = s.k0; k < s.k1; k += WIDE_KEYS, ++t_now) {
+        const int done = k - s.k0;
+        if (done >= 3 * quarter) __builtin_amdgcn_s_setprio(0);
+        else if (done >= 2 * quarter) __builtin_amdgcn_s_setprio(1);
+        else if (done >= quarter) __builtin_amdgcn_s_setprio(2);
         const typename Shared::Tile& tile = sh.tile[t_now & 1];
         if (k < wave_end) {
             uint32_t most = 0;
@@ -955,8 +964,8 @@ void cache_attn_plan(CacheAttnArgs& a, int cus) {
     // queries of 16 heads of 128 on up to 8192 Q4_0 keys 78, 68, 74, 71, 67; 16
     // heads of 64 on 32768 248, 212, 224, 250, 222; 8 of 8 heads of 32 378, 377,
     // 278, 278, 338; many places, 8 prompts of 201 queries of 8 heads of 32 on up to
-    // 5217 Q8_0 keys 54, 51, 53, -, 53; 13 requests of up to 150 queries of 12 heads
-    // of 64 on up to 1300 34, 42, 40, -, 44: registers hold two of these in a CU, and
+    // 5217 Q8_0 keys 49, 43, 57, 50, 47; 13 requests of up to 150 queries of 12 heads
+    // of 64 on up to 1300 30, 40, 37, 43, 43: registers hold two of these in a CU, and
     // three of head_dim 32).
     a.least_steps = 2;
     const int at_once = !a.query_tiles ? (a.cache.head_dim == 32 ? 3 : 2) : a.cache.head_dim == 32 ? 4 : 3;
