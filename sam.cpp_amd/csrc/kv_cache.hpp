@@ -63,16 +63,40 @@ __device__ __forceinline__ int cache_row(const KvCacheArgs& c, int r, int positi
     return page < c.page_count ? int(page * c.page.d + (uint32_t(position) - p * c.page.d)) : -1;
 }
 
+// The first request that ends behind `row`, c.requests where none does: 64 probes
+// at a time, for a wave that asks for one row.
+__device__ __forceinline__ int first_request(const KvCacheArgs& c, int row) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, hi = c.requests;
+    while (lo < hi) {
+        const int stride = (hi - lo + 63) >> 6, at = int(min(int64_t(lo) + int64_t(stride) * (lane + 1) - 1, int64_t(hi) - 1));
+        const uint64_t hit = __ballot(c.row_start[at + 1] > row);
+        if (!hit) {
+            lo = hi;
+        } else {
+            const int f = __builtin_ctzll(hit);
+            hi = __builtin_amdgcn_readlane(at, f);
+            lo += stride * f;
+        }
+    }
+    return lo;
+}
+
 // The cache row where row `row` of `rows` in the call stands, -1 where it has
-// no place, -2 where no request has it.
-__device__ __forceinline__ int place_of_row(const KvCacheArgs& c, int rows, int row) {
-    int lo = 0, hi = c.requests;   // the first request that ends behind the row
+// no place, -2 where no request has it; its request is `lo` or, where rows of
+// others lie between, not far behind.
+__device__ __forceinline__ int place_of_row(const KvCacheArgs& c, int rows, int row, int lo) {
+    int hi = lo;
+    for (uint32_t step = 1; hi < c.requests && c.row_start[hi + 1] <= row; step *= 2) {
+        lo = hi + 1;
+        hi = int(min(int64_t(hi) + step, int64_t(c.requests)));
+    }
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (c.row_start[mid + 1] <= row) lo = mid + 1;
         else hi = mid;
     }
-    if (lo == c.requests) return -2;
+    if (lo >= c.requests) return -2;
     int from;
     const int n = request_rows(c, rows, lo, from), i = row - from;
     if (i < 0 || i >= n) return -2;
