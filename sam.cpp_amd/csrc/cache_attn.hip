@@ -205,6 +205,21 @@ __device__ __forceinline__ bool find_span(const CacheAttnArgs& a, Span& s) {
     return true;
 }
 
+// What shares a SIMD is served oldest first, so that the last workgroup would run
+// alone in the end, and slowly; with this, who is behind goes first (8 prompts of
+// 201 queries of 8 heads of 32: 48.0 us without, 42.6 with it; 64 queries of 16
+// heads of 128 on up to 8192 keys: 66.5, 64.5).
+struct Progress {
+    int k0, quarter;
+    __device__ __forceinline__ explicit Progress(const Span& s) : k0(s.k0), quarter((s.k1 - s.k0) / 4) { __builtin_amdgcn_s_setprio(3); }
+    __device__ __forceinline__ void at(int k) const {
+        const int done = k - k0;
+        if (done >= 3 * quarter) __builtin_amdgcn_s_setprio(0);
+        else if (done >= 2 * quarter) __builtin_amdgcn_s_setprio(1);
+        else if (done >= quarter) __builtin_amdgcn_s_setprio(2);
+    }
+};
+
 // Where the results of a tile's p-th place go.
 __device__ __forceinline__ int64_t kept_place(const CacheAttnArgs& a, int kvh, int kept, int p) {
     return (int64_t(kvh) * 2 * a.slots + kept) * a.by_places.d + p;
@@ -360,7 +375,9 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
     if (kw < s.k1) load(row);
     row = row_of(kw + step);
     split_queries();
+    const Progress progress(s);
     for (int k = kw; k < s.k1; k += step) {
+        progress.at(k);
         const uint32_t here = there;
         wave_lds_handoff();   // the last tile's reads came first
         bool odd = false;
@@ -732,17 +749,10 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
         for (int off = 1; off < 32; off <<= 1) v = max(v, __shfl_xor(v, off, 64));
         return __builtin_amdgcn_readfirstlane(v);
     }();
-    // What shares a SIMD is served oldest first: the last of three workgroups would
-    // run alone in the end, and slowly (48.0 us for 8 prompts of 201 queries of 8
-    // heads of 32; so that who is behind comes first: 42.6).
-    const int quarter = (s.k1 - s.k0) / 4;
-    __builtin_amdgcn_s_setprio(3);
+    const Progress progress(s);
     int t_now = 0;
     for (int k = s.k0; k < s.k1; k += WIDE_KEYS, ++t_now) {
-        const int done = k - s.k0;
-        if (done >= 3 * quarter) __builtin_amdgcn_s_setprio(0);
-        else if (done >= 2 * quarter) __builtin_amdgcn_s_setprio(1);
-        else if (done >= quarter) __builtin_amdgcn_s_setprio(2);
+        progress.at(k);
         const typename Shared::Tile& tile = sh.tile[t_now & 1];
         if (k < wave_end) {
             uint32_t most = 0;
