@@ -208,7 +208,7 @@ __device__ __forceinline__ bool find_span(const CacheAttnArgs& a, Span& s) {
 // What shares a SIMD is served oldest first, so that the last workgroup would run
 // alone in the end, and slowly; with this, who is behind goes first (8 prompts of
 // 201 queries of 8 heads of 32: 48.0 us without, 42.6 with it; 64 queries of 16
-// heads of 128 on up to 8192 keys: 66.5, 64.5).
+// heads of 128 on up to 8192 keys: 66.5, 64.5 then).
 struct Progress {
     int k0, quarter;
     __device__ __forceinline__ explicit Progress(const Span& s) : k0(s.k0), quarter((s.k1 - s.k0) / 4) { __builtin_amdgcn_s_setprio(3); }
@@ -275,7 +275,7 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
     if (!find_span(a, s)) return;
     const int kvh = s.kvh;
     const KvCacheArgs& c = a.cache;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quarter = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quarter = lane >> 4;
     const int g = col / T::BLOCKS, my_blk = col % T::BLOCKS;   // this lane's column
     // row 4 quarter + i of the products with values: its place, and whether it is of block `blk`
     const auto place_of = [&](int i) { return (4 * quarter + i) / T::BLOCKS; };
@@ -641,7 +641,7 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
     if (!find_span(a, s)) return;
     const int kvh = s.kvh;
     const KvCacheArgs& c = a.cache;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hh = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, hh = lane >> 5;
     const int place = s.first + TILE * wave + li, i_row = a.row_of_place(place), head = kvh * a.group + place - i_row * a.group;
     const bool mine = i_row < s.n;
     const int row = s.q0 + (mine ? i_row : 0), limit = mine ? min(s.limit(a.causal, i_row), s.k1) : 0;
