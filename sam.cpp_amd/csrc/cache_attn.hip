@@ -39,7 +39,6 @@ namespace samhip {
 namespace {
 
 constexpr int WAVES = 4;
-constexpr int kCacheAttnMaxShared = 4096; // requests beyond which each is one part: a workgroup would spend its time on the tables
 constexpr float NO_BASE = -1e30f;         // below every score, and finite
 constexpr int ZERO_SCALE = -40;           // log 2 of what a zero scale counts as
 
@@ -120,57 +119,107 @@ struct Share {
     int before, kept;   // items (tile, part) of the requests before, and those of them that are kept for the join
 };
 
-// The request for which match(first row, rows, items to its end) holds first; the
-// requests are read 64 at a time, a lane to each.
-template <class Match>
-__device__ __forceinline__ bool find_request(const CacheAttnArgs& a, Match match, Share& s) {
-    const int lane = threadIdx.x & 63;
-    int from, n, len, tiles, steps;
-    const auto read = [&](int r0) {
-        from = n = len = 0;
-        if (r0 + lane < a.cache.requests) {
-            n = max(request_rows(a.cache, a.rows, r0 + lane, from), 0);
-            len = request_len(a.cache, r0 + lane);
+// Rows, length, tiles and steps of request r.
+struct Request {
+    int from = 0, n = 0, len = 0, tiles = 0, steps = 0;
+    __device__ __forceinline__ Request(const CacheAttnArgs& a, int r) {
+        if (r < a.cache.requests) {
+            n = max(request_rows(a.cache, a.rows, r, from), 0);
+            len = request_len(a.cache, r);
         }
         tiles = int(a.by_places.quotient(n * a.group + a.by_places.d - 1));
         steps = int(a.by_step.quotient(min(len, a.max_len) + a.by_step.d - 1));
-    };
-    read(0);
-    float of_part = 0.f;   // 1 / steps of a part
+    }
+    __device__ __forceinline__ int parts(float of_part) const { return max(1, int(__builtin_ceilf(float(steps) * of_part))); }
+};
+
+// 1 / steps of a part, from the sums over the requests.
+__device__ __forceinline__ float part_of(const CacheAttnArgs& a, float work, float tiles) {
+    // every tile's last part is a half too much, on average; a thousandth more, for the sums' roundings
+    const float slots = fmaxf(float(a.slots) - 0.5f * tiles, 0.5f * float(a.slots));
+    return 1.f / fmaxf(float(a.least_steps), fminf(__builtin_ceilf(work * 1.001f / slots), 1e9f));
+}
+
+// The request of an item, or of a row: up to 64 are read at once, a lane to each;
+// of more, a launch before has left the sums to be searched (1024 requests of one
+// query of 16 heads of 128 on up to 512 keys: every workgroup summing up for itself
+// 188 us, so 100).
+__device__ __forceinline__ bool find_request(const CacheAttnArgs& a, bool of_row, int value, Share& s) {
+    if (a.ends) {
+        s.request = first_above(of_row ? a.cache.row_start + 1 : a.ends, a.cache.requests, value);
+        if (s.request >= a.cache.requests) return false;
+        const Request r(a, s.request);
+        s.q0 = r.from;
+        s.n = r.n;
+        s.len = r.len;
+        s.tiles = r.tiles;
+        s.parts = r.parts(*a.of_part);
+        s.before = a.ends[s.request] - s.tiles * s.parts;
+        s.kept = a.kept[s.request];
+    } else {
+        const Request r(a, threadIdx.x & 63);
+        const float of_part = a.slots ? part_of(a, wave_sum(float(r.tiles) * float(r.steps)), wave_sum(float(r.tiles))) : 0.f;
+        const int parts = r.parts(of_part), items = r.tiles * parts, to_keep = parts > 1 ? items : 0;
+        const int sum = running_sum(items), kept = running_sum(to_keep);
+        const uint64_t hit = __ballot((of_row ? r.from + r.n : sum) > value);
+        if (!hit) return false;
+        const int at = __builtin_ctzll(hit);
+        s.request = at;
+        s.q0 = __builtin_amdgcn_readlane(r.from, at);
+        s.n = __builtin_amdgcn_readlane(r.n, at);
+        s.len = __builtin_amdgcn_readlane(r.len, at);
+        s.tiles = __builtin_amdgcn_readlane(r.tiles, at);
+        s.parts = __builtin_amdgcn_readlane(parts, at);
+        s.before = __builtin_amdgcn_readlane(sum - items, at);
+        s.kept = __builtin_amdgcn_readlane(kept - to_keep, at);
+    }
+    // (tables that are not in order have none of these)
+    const int first = of_row ? s.q0 : s.before, count = of_row ? s.n : s.tiles * s.parts;
+    return value >= first && value - first < count && (s.parts == 1 || (s.kept >= 0 && s.kept + s.tiles * s.parts <= 2 * a.slots));
+}
+
+// The sums over more than 64 requests, by one workgroup.
+constexpr int SUMS_THREADS = 1024;
+__global__ __launch_bounds__(SUMS_THREADS) void cache_attn_sums_kernel(CacheAttnArgs a) {
+    __shared__ float works[SUMS_THREADS / 64], counts[SUMS_THREADS / 64];
+    __shared__ int items_of[SUMS_THREADS / 64], kept_of[SUMS_THREADS / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    float of_part = 0.f;
     if (a.slots) {
-        float work = float(tiles) * float(steps), all = float(tiles);
-        for (int r0 = 64; r0 < a.cache.requests; r0 += 64) {
-            read(r0);
-            work += float(tiles) * float(steps);
-            all += float(tiles);
+        float work = 0.f, tiles = 0.f;
+        for (int r0 = 0; r0 < a.cache.requests; r0 += SUMS_THREADS) {
+            const Request r(a, r0 + tid);
+            work += float(r.tiles) * float(r.steps);
+            tiles += float(r.tiles);
         }
-        if (a.cache.requests > 64) read(0);
-        // every tile's last part is a half too much, on average; a thousandth more, for the sums' roundings
-        const float slots = fmaxf(float(a.slots) - 0.5f * wave_sum(all), 0.5f * float(a.slots));
-        of_part = 1.f / fmaxf(float(a.least_steps), fminf(__builtin_ceilf(wave_sum(work) * 1.001f / slots), 1e9f));
+        works[wave] = wave_sum(work);
+        counts[wave] = wave_sum(tiles);
+        __syncthreads();
+        const int w = lane % (SUMS_THREADS / 64);
+        of_part = part_of(a, wave_sum(lane == w ? works[w] : 0.f), wave_sum(lane == w ? counts[w] : 0.f));
     }
-    int before = 0, kept = 0;
-    for (int r0 = 0; r0 < a.cache.requests; r0 += 64) {
-        if (r0) read(r0);
-        const int parts = max(1, int(__builtin_ceilf(float(steps) * of_part))), items = tiles * parts, to_keep = parts > 1 ? items : 0;
-        const int sum = running_sum(items), kept_sum = running_sum(to_keep);
-        const uint64_t hit = __ballot(match(from, n, before + sum));
-        if (hit) {
-            const int at = __builtin_ctzll(hit);
-            s.request = r0 + at;
-            s.q0 = __builtin_amdgcn_readlane(from, at);
-            s.n = __builtin_amdgcn_readlane(n, at);
-            s.len = __builtin_amdgcn_readlane(len, at);
-            s.tiles = __builtin_amdgcn_readlane(tiles, at);
-            s.parts = __builtin_amdgcn_readlane(parts, at);
-            s.before = before + __builtin_amdgcn_readlane(sum - items, at);
-            s.kept = kept + __builtin_amdgcn_readlane(kept_sum - to_keep, at);
-            return true;
+    int before = 0, kept_before = 0;
+    for (int r0 = 0; r0 < a.cache.requests; r0 += SUMS_THREADS) {
+        const Request r(a, r0 + tid);
+        const int parts = r.parts(of_part), items = r.tiles * parts, to_keep = parts > 1 ? items : 0;
+        int sum = running_sum(items), kept = running_sum(to_keep);
+        if (lane == 63) items_of[wave] = sum, kept_of[wave] = kept;
+        __syncthreads();
+        int all = 0, all_kept = 0;
+        for (int w = 0; w < SUMS_THREADS / 64; ++w) {
+            if (w == wave) sum += before + all, kept += kept_before + all_kept;
+            all += items_of[w];
+            all_kept += kept_of[w];
         }
-        before += __builtin_amdgcn_readlane(sum, 63);
-        kept += __builtin_amdgcn_readlane(kept_sum, 63);
+        before += all;
+        kept_before += all_kept;
+        if (r0 + tid < a.cache.requests) {
+            a.ends[r0 + tid] = sum;
+            a.kept[r0 + tid] = kept - to_keep;
+        }
+        __syncthreads();
     }
-    return false;
+    if (tid == 0) *a.of_part = of_part;
 }
 
 // What a workgroup has: places [first, ..) of a request whose n query rows begin
@@ -189,7 +238,7 @@ __device__ __forceinline__ bool find_span(const CacheAttnArgs& a, Span& s) {
     const int order = blockIdx.x >> 3, sets = int(a.by_kv_heads.quotient(order)), item = (blockIdx.x & 7) + 8 * sets;
     s.kvh = order - sets * a.cache.kv_heads;
     Share share;
-    if (!find_request(a, [&](int, int, int to) { return to > item; }, share)) return false;
+    if (!find_request(a, false, item, share)) return false;
     const int local = item - share.before, part = local / share.tiles, places = int(a.by_places.d), step = int(a.by_step.d);
     s.request = share.request;
     s.q0 = share.q0;
@@ -877,7 +926,7 @@ __global__ __launch_bounds__(256) void cache_attn_merge_kernel(CacheAttnArgs a, 
     const int row = int(by_sets.quotient(unit)), lane = threadIdx.x & 63, slot = lane / QUADS % SLOTS, d = 4 * (lane % QUADS);
     if (row >= a.rows) return;
     Share s;
-    if (!find_request(a, [&](int from, int n, int) { return row >= from && row < from + n; }, s) || s.parts == 1) return;
+    if (!find_request(a, true, row, s) || s.parts == 1) return;
     const int head = int(unit - row * by_sets.d) * HEADS + lane / (QUADS * SLOTS), h = min(head, a.heads - 1);
     const int kvh = a.row_of_place(h), place = (row - s.q0) * a.group + h - kvh * a.group;   // (heads of a kv head are a group too)
     const int tile = int(a.by_places.quotient(place)), p = place - tile * int(a.by_places.d);
@@ -940,6 +989,7 @@ void launch_merge(const CacheAttnArgs& a, hipStream_t stream) {
 
 template <int TYPE, int HD>
 void launch_typed(const CacheAttnArgs& a, hipStream_t stream) {
+    if (a.ends) cache_attn_sums_kernel<<<1, SUMS_THREADS, 0, stream>>>(a);
     const unsigned groups = unsigned((a.slots + a.tiles + 7) / 8 * 8 * a.cache.kv_heads);
     if (a.query_tiles == 0) cache_attn_wide_kernel<TYPE, HD><<<groups, 64 * WAVES, 0, stream>>>(a);
     else if (a.query_tiles == 1) cache_attn_narrow_kernel<TYPE, HD, 1><<<groups, 64 * WAVES, 0, stream>>>(a);
@@ -980,16 +1030,25 @@ void cache_attn_plan(CacheAttnArgs& a, int cus) {
     a.least_steps = 2;
     const int at_once = !a.query_tiles ? (a.cache.head_dim == 32 ? 3 : 2) : a.cache.head_dim == 32 ? 4 : 3;
     a.slots = std::max(1, at_once * cus / a.cache.kv_heads);
-    if (a.max_len <= a.least_steps * step || a.cache.requests > kCacheAttnMaxShared) a.slots = 0;
+    if (a.max_len <= a.least_steps * step) a.slots = 0;
 }
 
+namespace {
+size_t kept_places(const CacheAttnArgs& a) { return size_t(2) * a.slots * a.cache.kv_heads * a.by_places.d; }
+}  // namespace
+
 size_t cache_attn_scratch_bytes(const CacheAttnArgs& a) {
-    return size_t(2) * a.slots * a.cache.kv_heads * a.by_places.d * (a.cache.head_dim + 2) * 4;
+    return kept_places(a) * (a.cache.head_dim + 2) * 4 + (a.cache.requests > 64 ? 8 * size_t(a.cache.requests) + 4 : 0);
 }
 
 void launch_cache_attn(CacheAttnArgs a, int type, void* scratch, hipStream_t stream) {
     a.part_o = static_cast<float*>(scratch);
-    a.part_ml = a.part_o + size_t(2) * a.slots * a.cache.kv_heads * a.by_places.d * a.cache.head_dim;
+    a.part_ml = a.part_o + kept_places(a) * a.cache.head_dim;
+    if (a.cache.requests > 64) {
+        a.ends = reinterpret_cast<int32_t*>(a.part_ml + kept_places(a) * 2);
+        a.kept = a.ends + a.cache.requests;
+        a.of_part = reinterpret_cast<float*>(a.kept + a.cache.requests);
+    }
     if (type == T_Q4_0) launch_of_type<T_Q4_0>(a, stream);
     else launch_of_type<T_Q8_0>(a, stream);
 }

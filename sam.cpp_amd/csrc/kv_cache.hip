@@ -222,7 +222,7 @@ struct CacheRowShape {
 __device__ __forceinline__ void find_places(const KvCacheArgs& c, int rows, int row0, int n, int* place) {
     const int first = threadIdx.x & ~63;   // of the wave's rows
     if (first >= n) return;
-    const int r = first_request(c, row0 + first);
+    const int r = first_above(c.row_start + 1, c.requests, row0 + first);
     if (int(threadIdx.x) < n) place[threadIdx.x] = place_of_row(c, rows, row0 + threadIdx.x, r);
 }
 

@@ -63,14 +63,14 @@ __device__ __forceinline__ int cache_row(const KvCacheArgs& c, int r, int positi
     return page < c.page_count ? int(page * c.page.d + (uint32_t(position) - p * c.page.d)) : -1;
 }
 
-// The first request that ends behind `row`, c.requests where none does: 64 probes
-// at a time, for a wave that asks for one row.
-__device__ __forceinline__ int first_request(const KvCacheArgs& c, int row) {
+// The first of `count` ascending ends that is above `value`, count where none is:
+// 64 probes at a time, for a wave that asks for one value.
+__device__ __forceinline__ int first_above(const int32_t* ends, int count, int value) {
     const int lane = threadIdx.x & 63;
-    int lo = 0, hi = c.requests;
+    int lo = 0, hi = count;
     while (lo < hi) {
         const int stride = (hi - lo + 63) >> 6, at = int(min(int64_t(lo) + int64_t(stride) * (lane + 1) - 1, int64_t(hi) - 1));
-        const uint64_t hit = __ballot(c.row_start[at + 1] > row);
+        const uint64_t hit = __ballot(ends[at] > value);
         if (!hit) {
             lo = hi;
         } else {
@@ -120,8 +120,8 @@ void launch_cache_write(const KvCacheArgs& c, int type, bool x86, const RopeArgs
 void launch_cache_read(const KvCacheArgs& c, int type, void* k, int64_t ldk, void* v, int64_t ldv, int out_type, int rows,
                        int cus, hipStream_t stream);
 
-// cache_attn_plan sets the fields behind `causal` but the two scratch
-// pointers, which launch_cache_attn sets.
+// cache_attn_plan sets the fields behind `causal` but the scratch pointers, which
+// launch_cache_attn sets.
 struct CacheAttnArgs {
     KvCacheArgs cache;
     const float* q;
@@ -138,6 +138,8 @@ struct CacheAttnArgs {
     int slots, least_steps;                // parts of keys of a kv head in all, and the steps of the smallest; 0 slots: one part each
     __host__ __device__ int row_of_place(int place) const { return int(by_group.quotient(place)); }   // of a request's
     float *part_o, *part_ml;
+    int32_t *ends, *kept;                  // null: at most 64 requests; else items to a request's end, and kept ones before it
+    float* of_part;                        // 1 / steps of a part
 };
 void cache_attn_plan(CacheAttnArgs& a, int cus);
 size_t cache_attn_scratch_bytes(const CacheAttnArgs& a);
