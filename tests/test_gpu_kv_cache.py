@@ -705,3 +705,169 @@ def test_a_service_on_its_own_stream(samhip):
         # weights and sums in another order: the tolerance of two results of one definition
         assert ((got - once).abs() <= 2 * 2.0 ** -17 * once.abs().amax()).all()
         ctx.set_stream(None)
+
+
+# --- large, many, at once ----------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,requests,longest", [([1, 0, 2], 300, 400), ([1], 5000, 300), ([1], 1500, 60), ([40], 80, 300)])
+def test_many_requests(samhip, gpu_ctx, rows, requests, longest):
+    """More requests than a wave's lanes, rows of some and of none; lengths that
+    leave one part of keys, and several."""
+    print("many", rows, requests, longest, flush=True)
+    n = [rows[i % len(rows)] for i in range(requests)]
+    lens = [max(n[i], 137 * i % longest) for i in range(requests)]
+    lens[-3] = 8 * longest   # one of many parts
+    p = Pages(n, lens, 2, 32, True, 16, seed=13, first=2, behind=3)
+    for i, c in enumerate(p.caches):   # all positions at once
+        at = torch.cat([p.at(r, range(m)) for r, m in enumerate(lens)])
+        g = torch.Generator(device="cuda").manual_seed(i)
+        c[at, :p.row_bytes] = torch.as_tensor(packed(torch.randn(len(at), 64, device="cuda", generator=g), True), device="cuda")
+    Attend(p, 4, True, seed=13).check(samhip, gpu_ctx)
+    # the same tables for rows to and from the cache
+    k = torch.randn(p.rows, 64, device="cuda")
+    out = [torch.full_like(k, 7.0) for _ in "kv"]
+    torch.cuda.synchronize()
+    gpu_ctx.cache_write(p.desc(samhip), None, describe(samhip, k), describe(samhip, k))
+    gpu_ctx.cache_read(p.desc(samhip), *(describe(samhip, o) for o in out))
+    gpu_ctx.synchronize()
+    want = torch.full_like(k, 7.0)
+    here = slice(p.starts[0], p.starts[-1])
+    want[here] = values(torch.as_tensor(packed(k[here], True), device="cuda"), True).float()
+    for i in range(2):
+        assert torch.equal(out[i], want)
+        at = torch.cat([p.at(r, range(m - a, m)) for r, (a, m) in enumerate(zip(n, lens)) if a])
+        assert torch.equal(values(p.caches[i][at][:, :p.row_bytes], True).float(), want[here])
+
+
+@pytest.mark.parametrize("q4", [False, True])
+@pytest.mark.parametrize("hd,group", [(32, 24), (64, 12), (128, 6), (128, 8), (64, 3)])
+def test_places_of_two_operands_and_fewer(samhip, gpu_ctx, q4, hd, group):
+    """Single rows of groups of heads between a whole operand's places and two's."""
+    p = Pages([1, 1, 0, 1], [3001, 40, 5, 700], 2, hd, q4, 32, seed=14).fill(14)
+    Attend(p, 2 * group, True, seed=14).check(samhip, gpu_ctx)
+
+
+def test_as_many_kv_heads_as_there_may_be(samhip, gpu_ctx):
+    p = Pages([1, 1], [3, 600], 1024, 32, True, 64, seed=15).fill(15)
+    Attend(p, 1024, seed=15).check(samhip, gpu_ctx)
+    p = Pages([1], [5], 4096, 32, False, 4, seed=16).fill(16)
+    Attend(p, 4096, seed=16).check(samhip, gpu_ctx)
+
+
+@pytest.mark.parametrize("stride,rows,lens", [(2 ** 26 + 2, 1, [33, 40]), (2 ** 26 + 4, 20, [33, 40]), (2 ** 23, 1, [600])])
+def test_offsets_past_32_bits(samhip, gpu_ctx, stride, rows, lens):
+    """Caches of more than 4 GiB: rows a long way from each other."""
+    print("offsets", stride, rows, lens, flush=True)
+    row_bytes = 4 * 64 // 32 * 18
+    p = Pages([rows] * len(lens), lens, 4, 64, True, 16, seed=17, byte_pad=stride - row_bytes)
+    assert p.caches[0].numel() > 2 ** 32
+
+    def rows_of(c, at):
+        return c[:, :p.row_bytes][at]
+
+    k, v = (torch.randn(p.rows, 256, device="cuda") for _ in "kv")
+    for i, c in enumerate(p.caches):
+        narrow = c[:, :p.row_bytes]
+        for r, m in enumerate(lens):
+            g = torch.Generator(device="cuda").manual_seed(10 * r + i)
+            narrow[p.at(r, range(m))] = torch.as_tensor(packed(torch.randn(m, 256, device="cuda", generator=g), True), device="cuda")
+    torch.cuda.synchronize()
+    gpu_ctx.cache_write(p.desc(samhip), None, describe(samhip, k), describe(samhip, v))
+    out = [torch.empty_like(k) for _ in "kv"]
+    gpu_ctx.cache_read(p.desc(samhip), *(describe(samhip, o) for o in out))
+    gpu_ctx.synchronize()
+    for x, o, c in zip((k, v), out, p.caches):
+        bytes_ = torch.as_tensor(packed(x, True), device="cuda")
+        assert torch.equal(o.double(), values(bytes_, True))
+        for r, m in enumerate(lens):
+            assert torch.equal(rows_of(c, p.at(r, range(m - rows, m))), bytes_[r * rows:(r + 1) * rows])
+    a = Attend(p, 4, True, seed=17)
+    near = Pages([rows] * len(lens), lens, 4, 64, True, 16, seed=17)   # the same rows next to each other, for the reference
+    for c, f in zip(near.caches, p.caches):
+        for r, m in enumerate(lens):
+            c[near.at(r, range(m))] = rows_of(f, p.at(r, range(m)))
+    b = Attend(near, 4, True, seed=17)
+    ref, bound = b.reference()
+    a.run(samhip, gpu_ctx)
+    a.verify(ref, bound)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_caches_without_pages(samhip, gpu_ctx, rows):
+    """Pages larger than the cache, and requests without any: zeros, and nothing
+    written."""
+    for page, max_pages in ((1 << 20, 3), (16, 0)):
+        p = Pages([rows] * 2, [50, 40], 2, 32, False, 16, seed=18).fill(18)
+        p.page, p.max_pages = page, max_pages
+        before = [c.clone() for c in p.caches]
+        k = torch.randn(p.rows, 64, device="cuda")
+        out = [torch.full_like(k, 7.0) for _ in "kv"]
+        a = Attend(p, 2, seed=18)
+        torch.cuda.synchronize()
+        gpu_ctx.cache_write(p.desc(samhip), None, describe(samhip, k), describe(samhip, k))
+        gpu_ctx.cache_read(p.desc(samhip), *(describe(samhip, o) for o in out))
+        a.run(samhip, gpu_ctx)
+        assert (a.out == 0).all() and all((o == 0).all() for o in out)
+        assert all(torch.equal(c, b) for c, b in zip(p.caches, before))
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_queries_that_are_not_finite_spoil_their_head_alone(samhip, gpu_ctx, rows, bad):
+    p = Pages([rows, rows], [700, 33], 2, 64, True, 64, seed=19).fill(19)
+    a = Attend(p, 4, seed=19)
+    ref, bound = a.reference()
+    a.q[0, 64 + 5] = bad
+    a.q[rows, 3 * 64 + 40] = -bad
+    a.run(samhip, gpu_ctx)
+    hit = torch.zeros(2 * rows, 4, 64, dtype=torch.bool, device="cuda")
+    hit[0, 1] = hit[rows, 3] = True
+    out = a.out.view(-1, 4, 64)
+    assert torch.equal(~out.isfinite(), hit)
+    assert ((out.double() - ref.view(-1, 4, 64)).abs() <= bound.view(-1, 4, 64))[~hit].all()
+
+
+def test_two_contexts_at_once(samhip):
+    """Calls of two contexts, neither waiting for the other: scratch is each one's own."""
+    with samhip.Context(0) as one, samhip.Context(0) as two:
+        work = []
+        for i, ctx in enumerate((one, two)):
+            p = Pages([1] * (5 + 70 * i), [900 - 11 * j for j in range(5 + 70 * i)], 2, 64, True, 16, seed=20 + i).fill(20 + i)
+            a = Attend(p, 4, True, seed=20 + i)
+            work.append((ctx, a, a.reference()))
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for ctx, a, _ in work:
+                ctx.cache_attn(a.desc(samhip))
+        for ctx, a, (ref, bound) in work:
+            ctx.synchronize()
+            a.verify(ref, bound)
+
+
+def test_two_graphs_that_share_scratch(samhip, gpu_ctx):
+    """Graphs of few and of many requests, replayed in turn with eager work between."""
+    work = []
+    for i, (n, lens) in enumerate((([1] * 3, [2000, 5, 800]), ([1] * 90, [700 - 7 * j for j in range(90)]), ([40] * 3, [900, 41, 300]))):
+        p = Pages(n, lens, 2, 64, i == 1, 16, seed=30 + i).fill(30 + i)
+        a = Attend(p, 4, True, seed=30 + i)
+        ref, bound = a.reference()
+        a.run(samhip, gpu_ctx)   # scratch
+        a.verify(ref, bound)
+        work.append([a, ref, bound, a.out.clone()])
+    graphs = []
+    for a, *_ in work:
+        gpu_ctx.capture_begin()
+        gpu_ctx.cache_attn(a.desc(samhip))
+        graphs.append(gpu_ctx.capture_end())
+    for turn in range(4):
+        for (a, ref, bound, eager), graph in zip(work, graphs):
+            a.held.fill_(7.0)
+            torch.cuda.synchronize()
+            graph.launch()
+            gpu_ctx.synchronize()
+            assert torch.equal(a.out, eager)
+            torch.randn(256, 256, device="cuda") @ torch.randn(256, 64, device="cuda")
+        work[turn % 3][0].run(samhip, gpu_ctx)
+    for graph in graphs:
+        graph.destroy()
