@@ -39,6 +39,7 @@ namespace samhip {
 namespace {
 
 constexpr int WAVES = 4;
+constexpr int MOST_PARTS = 32;             // of a tile's keys where waves have heads of their own
 constexpr float NO_BASE = -1e30f;         // below every score, and finite
 constexpr int ZERO_SCALE = -40;           // log 2 of what a zero scale counts as
 
@@ -235,8 +236,8 @@ struct Span {
 // Workgroups are dispatched round-robin over the 8 XCDs: the kv heads of the
 // same keys, whose blocks share cache lines, follow each other on one of them.
 __device__ __forceinline__ bool find_span(const CacheAttnArgs& a, Span& s) {
-    const int order = blockIdx.x >> 3, sets = int(a.by_kv_heads.quotient(order)), item = (blockIdx.x & 7) + 8 * sets;
-    s.kvh = order - sets * a.cache.kv_heads;
+    const int order = blockIdx.x >> 3, sets = int(a.by_head_sets.quotient(order)), item = (blockIdx.x & 7) + 8 * sets;
+    s.kvh = (order - sets * int(a.by_head_sets.d)) * a.wave_heads;
     Share share;
     if (!find_request(a, false, item, share)) return false;
     const int local = item - share.before, part = local / share.tiles, places = int(a.by_places.d), step = int(a.by_step.d);
@@ -273,12 +274,12 @@ struct Progress {
 __device__ __forceinline__ int64_t kept_place(const CacheAttnArgs& a, int kvh, int kept, int p) {
     return (int64_t(kvh) * 2 * a.slots + kept) * a.by_places.d + p;
 }
-__device__ __forceinline__ float* result_of(const CacheAttnArgs& a, const Span& s, int p, int row, int head, int hd) {
-    return s.kept < 0 ? a.out + row * a.ldo + head * hd : a.part_o + kept_place(a, s.kvh, s.kept, p) * hd;
+__device__ __forceinline__ float* result_of(const CacheAttnArgs& a, const Span& s, int kvh, int p, int row, int head, int hd) {
+    return s.kept < 0 ? a.out + row * a.ldo + head * hd : a.part_o + kept_place(a, kvh, s.kept, p) * hd;
 }
-__device__ __forceinline__ void leave_sum(const CacheAttnArgs& a, const Span& s, int p, float base, float sum) {
+__device__ __forceinline__ void leave_sum(const CacheAttnArgs& a, const Span& s, int kvh, int p, float base, float sum) {
     if (s.kept < 0) return;
-    float* ml = a.part_ml + kept_place(a, s.kvh, s.kept, p) * 2;
+    float* ml = a.part_ml + kept_place(a, kvh, s.kept, p) * 2;
     ml[0] = base;
     ml[1] = sum;
 }
@@ -322,9 +323,9 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
     __shared__ Shared sh;
     Span s;
     if (!find_span(a, s)) return;
-    const int kvh = s.kvh;
     const KvCacheArgs& c = a.cache;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quarter = lane >> 4;
+    const int wave_head = wave & (a.wave_heads - 1), kvh = s.kvh + wave_head;
     const int g = col / T::BLOCKS, my_blk = col % T::BLOCKS;   // this lane's column
     // row 4 quarter + i of the products with values: its place, and whether it is of block `blk`
     const auto place_of = [&](int i) { return (4 * quarter + i) / T::BLOCKS; };
@@ -384,7 +385,7 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
 #if defined(__HIP_DEVICE_COMPILE__)
     asm("" : "+s"(zero));
 #endif
-    const int step = T::KEYS * WAVES, kw = s.k0 + T::KEYS * wave;
+    const int step = int(a.by_step.d), kw = s.k0 + T::KEYS * (wave >> __builtin_ctz(a.wave_heads));
     // block f = lane + 64 i of a tile: keys' first, a key's blocks side by side
     const auto key_of = [&](int i) { return (lane + 64 * i) % HD / T::BLOCKS; };
     const auto of_values = [&](int i) { return lane + 64 * i >= HD; };
@@ -590,7 +591,7 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
                 }
             }
     }
-    // the four waves' sums, joined through LDS
+    // the sums of the waves of a head, joined through LDS
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         l[t] = pair_sum(sum_xor16(l[t]));
@@ -601,13 +602,11 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
     }
     __syncthreads();   // also: every wave is past its tiles
     float* all = reinterpret_cast<float*>(sh.lds);
-    const auto joined_sum = [&](int p, float& most) {
+    const auto joined_sum = [&](int of_head, int p, float& most) {
         most = NO_BASE;
         float sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) most = fmaxf(most, sh.l[w][p] != 0.f ? sh.b[w][p] : NO_BASE);
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) sum += sh.l[w][p] != 0.f ? sh.l[w][p] * __builtin_amdgcn_exp2f(sh.b[w][p] - most) : 0.f;
+        for (int w = of_head; w < WAVES; w += a.wave_heads) most = fmaxf(most, sh.l[w][p] != 0.f ? sh.b[w][p] : NO_BASE);
+        for (int w = of_head; w < WAVES; w += a.wave_heads) sum += sh.l[w][p] != 0.f ? sh.l[w][p] * __builtin_amdgcn_exp2f(sh.b[w][p] - most) : 0.f;
         return sum;
     };
 #pragma unroll
@@ -616,27 +615,27 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
         for (int i = 0; i < 4; ++i) {
             const int p = Shared::EACH * t + place_of(i);
             float most;
-            const float sum = joined_sum(p, most);
+            const float sum = joined_sum(wave_head, p, most);
             const float f = sh.l[wave][p] != 0.f ? __builtin_amdgcn_exp2f(sh.b[wave][p] - most) / sum : 0.f;
 #pragma unroll
             for (int d = 0; d < 2 * T::BLOCKS; ++d)
                 if (is_of(i, d >> 1)) all[(wave * Shared::PLACES + p) * (HD + 4) + 16 * d + col] = o[t][d][i] * f;
         }
-    if (tid < Shared::PLACES) {
-        const int place = s.first + tid, i = a.row_of_place(place);
+    if (tid < Shared::PLACES * a.wave_heads) {
+        const int p = tid % Shared::PLACES, of_head = tid / Shared::PLACES;
         float most;
-        const float sum = joined_sum(tid, most);
-        if (i < s.n) leave_sum(a, s, tid, most, sum);
+        const float sum = joined_sum(of_head, p, most);
+        if (a.row_of_place(s.first + p) < s.n) leave_sum(a, s, s.kvh + of_head, p, most, sum);
     }
     __syncthreads();
     constexpr int QUADS = HD / 4;
-    for (int t = tid; t < Shared::PLACES * QUADS; t += 64 * WAVES) {
-        const int p = t / QUADS, d = 4 * (t % QUADS), place = s.first + p, i = a.row_of_place(place);
+    for (int t = tid; t < Shared::PLACES * QUADS * a.wave_heads; t += 64 * WAVES) {
+        const int of_head = t / (Shared::PLACES * QUADS), p = t / QUADS % Shared::PLACES, d = 4 * (t % QUADS);
+        const int place = s.first + p, i = a.row_of_place(place), out_kvh = s.kvh + of_head;
         if (i >= s.n) continue;
         floatx4 v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) v += *reinterpret_cast<const floatx4*>(all + (w * Shared::PLACES + p) * (HD + 4) + d);
-        *reinterpret_cast<float4_at*>(result_of(a, s, p, s.q0 + i, kvh * a.group + place - i * a.group, HD) + d) = v;
+        for (int w = of_head; w < WAVES; w += a.wave_heads) v += *reinterpret_cast<const floatx4*>(all + (w * Shared::PLACES + p) * (HD + 4) + d);
+        *reinterpret_cast<float4_at*>(result_of(a, s, out_kvh, p, s.q0 + i, out_kvh * a.group + place - i * a.group, HD) + d) = v;
     }
 }
 
@@ -906,8 +905,8 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
     l = pair_sum(l);
     if (!mine) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (hh == 0) leave_sum(a, s, TILE * wave + li, base, l);
-    float* to = result_of(a, s, TILE * wave + li, row, head, HD);
+    if (hh == 0) leave_sum(a, s, kvh, TILE * wave + li, base, l);
+    float* to = result_of(a, s, kvh, TILE * wave + li, row, head, HD);
 #pragma unroll
     for (int d = 0; d < BLOCKS; ++d)
 #pragma unroll
@@ -990,7 +989,7 @@ void launch_merge(const CacheAttnArgs& a, hipStream_t stream) {
 template <int TYPE, int HD>
 void launch_typed(const CacheAttnArgs& a, hipStream_t stream) {
     if (a.ends) cache_attn_sums_kernel<<<1, SUMS_THREADS, 0, stream>>>(a);
-    const unsigned groups = unsigned((a.slots + a.tiles + 7) / 8 * 8 * a.cache.kv_heads);
+    const unsigned groups = unsigned((a.slots + a.tiles + 7) / 8 * 8 * int(a.by_head_sets.d));
     if (a.query_tiles == 0) cache_attn_wide_kernel<TYPE, HD><<<groups, 64 * WAVES, 0, stream>>>(a);
     else if (a.query_tiles == 1) cache_attn_narrow_kernel<TYPE, HD, 1><<<groups, 64 * WAVES, 0, stream>>>(a);
     else cache_attn_narrow_kernel<TYPE, HD, 2><<<groups, 64 * WAVES, 0, stream>>>(a);
@@ -1013,24 +1012,34 @@ void cache_attn_plan(CacheAttnArgs& a, int cus) {
     const int64_t each = (places + requests - 1) / requests;   // of a request with its share of the rows
     const int of_operand = 512 / a.cache.head_dim;
     a.query_tiles = each <= of_operand ? 1 : each <= 2 * of_operand ? 2 : 0;
-    const int tile = a.query_tiles ? of_operand * a.query_tiles : TILE * WAVES, step = a.query_tiles ? 32 * WAVES : WIDE_KEYS;
+    const int tile = a.query_tiles ? of_operand * a.query_tiles : TILE * WAVES, keys = a.query_tiles ? 32 * WAVES : WIDE_KEYS;
     a.tiles = int(places / tile + requests);
-    a.by_group = Divisor::of(a.group);
-    a.by_kv_heads = Divisor::of(a.cache.kv_heads);
-    a.by_places = Divisor::of(tile);
-    a.by_step = Divisor::of(step);
     a.short_rows = std::max(a.cache.ldk, a.cache.ldv) < (int64_t(1) << 26);
-    // About as many parts as run at once (us for 2, 3, 4, 5, 6 workgroups a CU: 64
-    // queries of 16 heads of 128 on up to 8192 Q4_0 keys 78, 68, 74, 71, 67; 16
-    // heads of 64 on 32768 248, 212, 224, 250, 222; 8 of 8 heads of 32 378, 377,
-    // 278, 278, 338; many places, 8 prompts of 201 queries of 8 heads of 32 on up to
-    // 5217 Q8_0 keys 49, 43, 57, 50, 47; 13 requests of up to 150 queries of 12 heads
-    // of 64 on up to 1300 30, 40, 37, 43, 43: registers hold two of these in a CU, and
-    // three of head_dim 32).
+    // About as many parts as run at once, which registers decide (us for 2, 3, 4, 5,
+    // 6 workgroups a CU: 64 queries on up to 8192 Q4_0 keys, 16 heads of 128 in groups
+    // of 4: 69, 62, 83, 74, 71; 8 heads of 64: 99, 79, 73, 92, 87; 8 of 32: 78, 63,
+    // 56, 55, 66; many places, 8 prompts of 201 queries of 8 heads of 32 on up to 5217
+    // Q8_0 keys: 49, 43, 57, 50, 47; 13 requests of up to 150 queries of 12 heads of
+    // 64 on up to 1300: 30, 40, 37, 43, 43).
     a.least_steps = 2;
-    const int at_once = !a.query_tiles ? (a.cache.head_dim == 32 ? 3 : 2) : a.cache.head_dim == 32 ? 4 : 3;
-    a.slots = std::max(1, at_once * cus / a.cache.kv_heads);
-    if (a.max_len <= a.least_steps * step) a.slots = 0;
+    const int at_once = !a.query_tiles ? (a.cache.head_dim == 32 ? 3 : 2) : a.cache.head_dim == 128 ? 3 : 4;
+    const bool split = a.max_len > a.least_steps * keys;
+    const auto slots = [&](int wave_heads) { return split ? std::max(1, at_once * cus / (a.cache.kv_heads / wave_heads)) : 0; };
+    // Few places: waves of one workgroup read the kv heads of the same keys, for heads
+    // share cache lines, and lines that come one by one come slowly from memory that
+    // no cache holds (64 queries of 8 kv heads of 64 on up to 8192 Q4_0 keys: 110
+    // us with four waves for a head, 90 with four heads); not where a tile would
+    // leave more parts to the join (four queries of 4 kv heads of 128 on 30000: 31.8
+    // and 45; 8 of 8 heads of 32 on up to 5217: 16.0, 14.7 with two and 15.0 with four).
+    a.wave_heads = 1;
+    if (split && a.query_tiles)
+        for (int heads : {2, 4})
+            if (a.cache.kv_heads % heads == 0 && slots(heads) <= MOST_PARTS * int64_t(a.tiles)) a.wave_heads = heads;
+    a.slots = slots(a.wave_heads);
+    a.by_group = Divisor::of(a.group);
+    a.by_head_sets = Divisor::of(a.cache.kv_heads / a.wave_heads);
+    a.by_places = Divisor::of(tile);
+    a.by_step = Divisor::of(keys / a.wave_heads);
 }
 
 namespace {

@@ -133,7 +133,8 @@ struct CacheAttnArgs {
     bool causal;
     bool short_rows;                       // the bytes of 32 rows fit 31 bits
     int query_tiles;                       // of 512 / head_dim places; 0: 128 places to a workgroup
-    Divisor by_group, by_kv_heads, by_places, by_step;   // by_places, by_step: a workgroup's places, and its keys at a time
+    int wave_heads;                        // kv heads of a workgroup, each some of its waves': 1, 2 or 4
+    Divisor by_group, by_head_sets, by_places, by_step;   // by_places, by_step: a workgroup's places of a head, and its keys at a time
     int tiles;                             // of all requests, at most
     int slots, least_steps;                // parts of keys of a kv head in all, and the steps of the smallest; 0 slots: one part each
     __host__ __device__ int row_of_place(int place) const { return int(by_group.quotient(place)); }   // of a request's

@@ -871,3 +871,20 @@ def test_two_graphs_that_share_scratch(samhip, gpu_ctx):
         work[turn % 3][0].run(samhip, gpu_ctx)
     for graph in graphs:
         graph.destroy()
+
+
+@pytest.mark.parametrize("q4", [False, True])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("kv_heads", [2, 4, 6, 8])
+def test_waves_with_heads_of_their_own(samhip, gpu_ctx, kv_heads, hd, q4):
+    """Enough requests of single rows that a workgroup takes two or four kv heads;
+    lengths that leave waves without keys."""
+    lens = [(53 * i + 1) % 977 for i in range(48)]
+    p = Pages([1] * 48, lens, kv_heads, hd, q4, 41, seed=40, behind=2).fill(40)
+    Attend(p, 2 * kv_heads, True, seed=40).check(samhip, gpu_ctx)
+    scale_blocks(p, 20, 1, [lens[20] - 1], float("inf"), kv_heads * hd // 32 - 1)   # of the last kv head's last block
+    a = Attend(p, 2 * kv_heads, seed=40)
+    a.run(samhip, gpu_ctx)
+    hit = torch.zeros(48, 2 * kv_heads, hd, dtype=torch.bool, device="cuda")
+    hit[20, -2:, -32:] = True
+    assert torch.equal(~a.out[:48].view(48, 2 * kv_heads, hd).isfinite(), hit)
