@@ -6,7 +6,12 @@
 // The angle is an F64 number (in F32 one of 10^5 would be off by 2^-8), cos and
 // sin come from their series on an eighth of a turn, in F64, and are rounded
 // once.  A workgroup makes them once for its rows and all of a row's heads.
-// All of it is bound by memory: one pass, 16-byte loads and stores.
+// All of it is bound by memory: one pass, 16-byte loads and stores.  5184 rows of
+// 32 heads of 64, F32: 16.2 us (5.2 TB/s, partly from the MALL); 41472 rows of 16
+// heads, F16: 34.0 (5.0).  Rows to a cache: 41472 of 512 F32 values of keys and
+// values, keys rotated, Q4_0: 51 us from HBM (3.8 TB/s; 41 from the MALL); back as
+// F16: 24.  A call of few rows is one launch of 4 to 6 us, a chain of loads: tables,
+// page, block.
 #include <algorithm>
 
 #include "kv_cache.hpp"
