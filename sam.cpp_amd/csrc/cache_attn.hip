@@ -364,7 +364,7 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
             if (T::BLOCKS == 4) m = umax_dpp<DPP_XOR2>(m);
             const int e = exponent_of(umax_xor32(umax_xor16(m)));
             const float f = a.scale < 0.f ? -down(e) : down(e);
-            cq[t] = fmaxf(fabsf(a.scale) * LOG2E * up(e), 0x1p-120f);   // a masked score times it is -inf
+            cq[t] = fmaxf(fabsf(a.scale) * (LOG2E * up(e)), 0x1p-120f);   // a masked score times it is -inf
             half8 hi, lo;
 #pragma unroll
             for (int j = 0; j < 8; j += 2) split_pair(float2_t{x[t][ORDER[j]] * f, x[t][ORDER[j + 1]] * f}, hi, lo, j);
@@ -733,7 +733,7 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
         }
         const int e = exponent_of(umax_xor32(m));
         const float f = a.scale < 0.f ? -down(e) : down(e);
-        cq = fmaxf(fabsf(a.scale) * LOG2E * up(e), 0x1p-120f);   // a masked score times it is -inf
+        cq = fmaxf(fabsf(a.scale) * (LOG2E * up(e)), 0x1p-120f);   // a masked score times it is -inf
 #pragma unroll
         for (int t = 0; t < HD / 16; ++t)
 #pragma unroll

@@ -280,10 +280,11 @@ struct Sums {
     }
 };
 
-// A tile of keys or values in LDS (TileShape), F32 ones as hi and lo.
+// A tile of keys or values in LDS, F32 ones as hi and lo.
 template <class T, int HD, int KEYS, bool V>
 struct TileRows : TileShape<sizeof(T) == 4 ? 2 : 1, HD, KEYS, V> {
     typedef TileShape<sizeof(T) == 4 ? 2 : 1, HD, KEYS, V> Shape;
+    static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
     // piece f (8 values) of the tile
     static __device__ __forceinline__ void put(uint8_t* tile, int f, const Raw8<T>& raw, float factor) {
         half8* to = Shape::piece(tile, f);
@@ -297,6 +298,58 @@ struct TileRows : TileShape<sizeof(T) == 4 ? 2 : 1, HD, KEYS, V> {
         }
     }
 };
+
+// sc[n] += K Q^T of keys 32n .. + 31 of a tile of keys in LDS
+template <class T, int HD, int N>
+__device__ __forceinline__ void scores(const uint8_t* kt, const Queries<HD>& q, floatx16 (&sc)[N]) {
+    typedef TileRows<T, HD, 32 * N, false> R;
+    const int lane = threadIdx.x & 63, li = lane & 31, hh = lane >> 5;
+    const uint8_t* at = kt + li * R::STRIDE + 16 * hh;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[n][r] = 0.f;
+#pragma unroll
+    for (int t = 0; t < HD / 16; ++t)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const half8 kh = *reinterpret_cast<const half8*>(at + 32 * n * R::STRIDE + 32 * t);
+            sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.hi[t], sc[n], 0, 0, 0);
+            sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, q.lo[t], sc[n], 0, 0, 0);
+            if constexpr (R::PARTS == 2) {
+                const half8 kl = *reinterpret_cast<const half8*>(at + (32 * N + 32 * n) * R::STRIDE + 32 * t);
+                sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, q.hi[t], sc[n], 0, 0, 0);
+            }
+        }
+}
+
+// O^T += V^T P^T with a tile of values in LDS: of 16 keys, lane (li, hh) holds
+// keys 4hh .. + 3 and 8 + 4hh .. + 3 of both operands, V^T read transposed.
+template <class T, int HD, int N>
+__device__ __forceinline__ void values(const uint8_t* vt, const half8 (&hi)[2 * N], const half8 (&lo)[2 * N], Sums<HD>& sums) {
+    typedef TileRows<T, HD, 32 * N, true> R;
+    const int lane = threadIdx.x & 63, hh = lane >> 5;
+    const uint8_t* at = vt + (4 * hh + ((lane & 15) >> 2)) * R::STRIDE + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    constexpr int DB = HD / 32, COUNT = 2 * N * DB, AHEAD = HD < 128 ? 1 : 0;   // 128: no registers left
+    half8 v[2][R::PARTS];   // the next one is under way during a product
+    const auto fetch = [&](int i) {
+        const uint8_t* p = at + 16 * (i / DB) * R::STRIDE + 64 * (i % DB);
+#pragma unroll
+        for (int part = 0; part < R::PARTS; ++part) {
+            const uint8_t* q = p + part * 32 * N * R::STRIDE;
+            v[i & 1][part] = __builtin_shufflevector(ds_read_tr(q), ds_read_tr(q + 8 * R::STRIDE), 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    };
+    if (AHEAD) fetch(0);
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+        const int u = i / DB, d = i % DB;
+        if (i + AHEAD < COUNT) fetch(i + AHEAD);
+        sums.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 1][0], hi[u], sums.o[d], 0, 0, 0);
+        sums.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 1][0], lo[u], sums.o[d], 0, 0, 0);
+        if constexpr (R::PARTS == 2) sums.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i & 1][R::PARTS - 1], hi[u], sums.o[d], 0, 0, 0);
+    }
+}
 
 // Few query places: all four waves have the same 32, and each takes tiles of
 // 32 keys of its own, keys straight from memory, values through LDS that no
@@ -387,7 +440,7 @@ __device__ __forceinline__ void attend_narrow(const PrefixAttnArgs& a, const Spa
         if (AHEAD && k + step < s.k1) load(k + step);
         half8 ph[2], pl[2];
         sums.weigh(sc, c, k, q.limit, low, ph, pl);
-        values<sizeof(T) == 4 ? 2 : 1, HD, 1>(vt, ph, pl, sums.o);
+        values<T, HD, 1>(vt, ph, pl, sums);
     }
     if (non_finite_values)
         for (int k = kw; k < s.k1; k += step)
@@ -512,9 +565,9 @@ __device__ __forceinline__ void attend_wide(const PrefixAttnArgs& a, const Span<
         if (any) {
             floatx16 sc[2];
             half8 ph[4], pl[4];
-            scores<sizeof(T) == 4 ? 2 : 1, HD, 2>(sh.k, q.hi, q.lo, sc);
+            scores<T, HD, 2>(sh.k, q, sc);
             sums.weigh(sc, c, k, q.limit, low, ph, pl);
-            values<sizeof(T) == 4 ? 2 : 1, HD, 2>(sh.v, ph, pl, sums.o);
+            values<T, HD, 2>(sh.v, ph, pl, sums);
         }
     }
     const float l = pair_sum(sums.l);
@@ -638,13 +691,62 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prefix_attn_kernel(PrefixAttnAr
     else attend_narrow<T, HD>(a, s, kvh, part, sh);
 }
 
+// A wave per (row, head): the parts' maxima and sums one to a lane, then
+// HD / 4 lanes to a part's mean.
 template <int HD>
 __global__ __launch_bounds__(256) void attn_merge_kernel(PrefixAttnArgs a) {
-    const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6), items = int64_t(a.rows) * a.heads;   // a wave per (row, head)
+    constexpr int QUADS = HD / 4, AT_ONCE = 64 / QUADS;
+    const int lane = threadIdx.x & 63;
+    const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6), items = int64_t(a.rows) * a.heads;
     if (item >= items) return;
     const int64_t row = item / a.heads, h = item - row * a.heads;
     if (row < min(max(a.q_start[0], 0), a.rows) || row >= min(max(a.q_start[a.requests], 0), a.rows)) return;
-    merge_parts<HD>(a.part_ml + item * a.parts * 2, 2, a.part_o + item * a.parts * HD, HD, a.parts, a.out + row * a.ldo + h * HD);
+    const int d = 4 * (lane % QUADS), slot = lane / QUADS;
+    float m = -__builtin_inff(), l = 0.f;
+    floatx4 v{0.f, 0.f, 0.f, 0.f};
+    for (int p0 = 0; p0 < a.parts; p0 += 64) {
+        float mp = -__builtin_inff(), lp = 0.f;
+        if (p0 + lane < a.parts) {
+            const float* ml = a.part_ml + (item * a.parts + p0 + lane) * 2;
+            mp = ml[0];
+            lp = ml[1];
+        }
+        const float mnew = fmaxf(m, wave_max(lp != 0.f ? mp : -__builtin_inff()));
+        const float old = m == mnew ? 1.f : __builtin_amdgcn_exp2f(m - mnew);
+        float f = lp != 0.f ? lp * __builtin_amdgcn_exp2f(mp - mnew) : 0.f;
+        const float before = l * old;
+        m = mnew;
+        l = before + wave_sum(f);
+        const float inv = l == 0.f ? 0.f : 1.f / l;   // v stays a mean
+        f = lp != 0.f ? f * inv : -1.f;   // no key in this part
+        v = v * (before * inv);
+        const int here = min(a.parts - p0, 64);
+        const float* parts = a.part_o + (item * a.parts + p0) * HD + d;
+        const auto add = [&](auto count, int p1) {   // parts p1 + slot, p1 + slot + AT_ONCE, ..
+            constexpr int U = decltype(count)::value;
+            floatx4 o[U];
+            float fp[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int p = p1 + u * AT_ONCE + slot, at = min(p, here - 1);
+                o[u] = *reinterpret_cast<const floatx4*>(parts + at * HD);
+                fp[u] = __shfl(f, at, 64);
+                if (p >= here) fp[u] = -1.f;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += fp[u] < 0.f ? 0.f : o[u][j] * fp[u];   // without keys its mean may never have been written
+        };
+        int p1 = 0;
+        for (; p1 + 3 * AT_ONCE < here; p1 += 4 * AT_ONCE) add(std::integral_constant<int, 4>{}, p1);
+        for (; p1 < here; p1 += AT_ONCE) add(std::integral_constant<int, 1>{}, p1);
+    }
+#pragma unroll
+    for (int off = QUADS; off < 64; off <<= 1)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += __shfl_xor(v[j], off, 64);
+    if (slot == 0) *reinterpret_cast<float4_at*>(a.out + row * a.ldo + h * HD + d) = v;
 }
 
 template <class T, int HD>

@@ -888,3 +888,12 @@ def test_waves_with_heads_of_their_own(samhip, gpu_ctx, kv_heads, hd, q4):
     hit = torch.zeros(48, 2 * kv_heads, hd, dtype=torch.bool, device="cuda")
     hit[20, -2:, -32:] = True
     assert torch.equal(~a.out[:48].view(48, 2 * kv_heads, hd).isfinite(), hit)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_scales_near_the_largest_number(samhip, gpu_ctx, rows):
+    """Scores of ordinary size from subnormal queries: no product on the way overflows."""
+    p = Pages([rows, rows], [700, 65], 2, 64, False, 64, seed=41).fill(41)
+    a = Attend(p, 4, seed=41, scale=3.3e38)
+    a.q.mul_(2.0 ** -128)
+    a.check(samhip, gpu_ctx)
