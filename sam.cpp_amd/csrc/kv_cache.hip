@@ -223,12 +223,13 @@ struct CacheRowShape {
     Divisor per_row, per_tensor, pairs;   // items of a row of both tensors, of one
 };
 
-// Where a workgroup's rows stand.
+// Where a workgroup's rows stand: the last wave's work, for the first has the
+// rotations of a few rows.
 __device__ __forceinline__ void find_places(const KvCacheArgs& c, int rows, int row0, int n, int* place) {
-    const int first = threadIdx.x & ~63;   // of the wave's rows
-    if (first >= n) return;
-    const int r = first_above(c.row_start + 1, c.requests, row0 + first);
-    if (int(threadIdx.x) < n) place[threadIdx.x] = place_of_row(c, rows, row0 + threadIdx.x, r);
+    static_assert(kMaxRows <= 64, "one wave finds them");
+    if (threadIdx.x < THREADS - 64) return;
+    const int r = first_above(c.row_start + 1, c.requests, row0), i = threadIdx.x & 63;
+    if (i < n) place[i] = place_of_row(c, rows, row0 + i, r);
 }
 
 // Eight values to a lane, four lanes to a block.
@@ -239,28 +240,40 @@ __global__ __launch_bounds__(THREADS) void cache_write_kernel(KvCacheArgs c, Rop
     __shared__ float2 table[kMaxTable];
     __shared__ int place[kMaxRows];
     const int row0 = blockIdx.x * s.rows_each, n = min(s.rows_each, rows - row0), lane = threadIdx.x & 63;
+    const int items = n * int(s.per_row.d);
+    struct Item {
+        int i = 0, octet = 0;
+        bool is = false, of_k = false;
+        const float* row = nullptr;
+        F4 a{0.f, 0.f, 0.f, 0.f}, b{0.f, 0.f, 0.f, 0.f};
+    };
+    const auto fetch = [&](int t) {
+        Item item;
+        item.is = t < items;
+        if (!item.is) return item;
+        item.i = int(s.per_row.quotient(t));
+        const int in_row = t - item.i * int(s.per_row.d);
+        item.of_k = in_row < int(s.per_tensor.d);
+        item.octet = item.of_k ? in_row : in_row - int(s.per_tensor.d);
+        item.row = item.of_k ? k + (row0 + item.i) * ldk : v + (row0 + item.i) * ldv;
+        item.a = *reinterpret_cast<const F4*>(item.row + 8 * item.octet);
+        item.b = *reinterpret_cast<const F4*>(item.row + 8 * item.octet + 4);
+        return item;
+    };
+    Item next = fetch(threadIdx.x);   // under way beside the tables
     find_places(c, rows, row0, n, place);
     fill_rotations(rope, s.pairs, row0, n, table);
     __syncthreads();
-    const int items = n * int(s.per_row.d);
     for (int base = 0; base < items; base += THREADS) {   // whole waves: the lanes of a block talk to each other
-        const int t = base + threadIdx.x;
-        int to = -1;
-        floatx8 x{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        int octet = 0;
-        bool of_k = false;
-        if (t < items) {
-            const int i = int(s.per_row.quotient(t)), in_row = t - i * int(s.per_row.d);
-            of_k = in_row < int(s.per_tensor.d);
-            octet = of_k ? in_row : in_row - int(s.per_tensor.d);
-            to = place[i];
-            const float* row = of_k ? k + (row0 + i) * ldk : v + (row0 + i) * ldv;
-            const F4 a = *reinterpret_cast<const F4*>(row + 8 * octet), b = *reinterpret_cast<const F4*>(row + 8 * octet + 4);
-            x = floatx8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-            if (of_k && rope.pairs) {
-                const int d0 = 8 * octet & (c.head_dim - 1);
-                turn8(x, row + (8 * octet - d0), d0, rope, table + i * rope.pairs);
-            }
+        const Item item = next;
+        if (base + THREADS < items) next = fetch(base + THREADS + threadIdx.x);
+        const int octet = item.octet;
+        const bool of_k = item.of_k;
+        const int to = item.is ? place[item.i] : -1;
+        floatx8 x{item.a[0], item.a[1], item.a[2], item.a[3], item.b[0], item.b[1], item.b[2], item.b[3]};
+        if (of_k && rope.pairs) {
+            const int d0 = 8 * octet & (c.head_dim - 1);
+            turn8(x, item.row + (8 * octet - d0), d0, rope, table + item.i * rope.pairs);
         }
         uint32_t w0 = 0, w1 = 0;
         float d, mul;
