@@ -315,18 +315,18 @@ struct Block {
     }
 };
 
-template <int TYPE, int HD, int NT>
+template <int TYPE, int HD>
 struct NarrowShared {
-    static constexpr int EACH = 512 / HD, PLACES = EACH * NT;   // places of an operand, of a workgroup
+    static constexpr int PLACES = 512 / HD;   // an operand's
     static constexpr int TILES = WAVES * KeyTile<TYPE, HD>::BYTES, SUMS = WAVES * PLACES * (HD + 4) * 4;
     uint8_t __attribute__((aligned(16))) lds[TILES > SUMS ? TILES : SUMS];
     float b[WAVES][PLACES], l[WAVES][PLACES];
 };
 
-template <int TYPE, int HD, int NT>
-__global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow_kernel(CacheAttnArgs a) {
+template <int TYPE, int HD>
+__global__ __launch_bounds__(64 * WAVES, 3) void cache_attn_narrow_kernel(CacheAttnArgs a) {
     typedef KeyTile<TYPE, HD> T;
-    typedef NarrowShared<TYPE, HD, NT> Shared;
+    typedef NarrowShared<TYPE, HD> Shared;
     __shared__ Shared sh;
     Span s;
     if (!find_span(a, s)) return;
@@ -337,56 +337,45 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
     // row 4 quarter + i of the products with values: its place, and whether it is of block `blk`
     const auto place_of = [&](int i) { return (4 * quarter + i) / T::BLOCKS; };
     const auto is_of = [](int i, int blk) { return i % T::BLOCKS == blk; };
-    int limit[NT];
-    floatx8 x[NT];   // this column's and quarter's part of the queries
+    int limit;
+    floatx8 x;   // this column's and quarter's part of the queries
     const auto load_queries = [&] {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int place = s.first + Shared::EACH * t + g, i = a.row_of_place(place), head = kvh * a.group + place - i * a.group;
-            const bool mine = i < s.n;
-            limit[t] = mine ? s.limit(a.causal, i) : 0;
-            // Q8_0: 8 neighbours; Q4_0: 4 and the 4 that stand 16 behind them
-            const float* from = a.q + (s.q0 + (mine ? i : 0)) * a.ldq + head * HD + 32 * my_blk + (TYPE == T_Q8_0 ? 8 : 4) * quarter;
-            const float4_at u = *reinterpret_cast<const float4_at*>(from), v = *reinterpret_cast<const float4_at*>(from + (TYPE == T_Q8_0 ? 4 : 16));
-            x[t] = floatx8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
-        }
+        const int place = s.first + g, i = a.row_of_place(place), head = kvh * a.group + place - i * a.group;
+        const bool mine = i < s.n;
+        limit = mine ? s.limit(a.causal, i) : 0;
+        // Q8_0: 8 neighbours; Q4_0: 4 and the 4 that stand 16 behind them
+        const float* from = a.q + (s.q0 + (mine ? i : 0)) * a.ldq + head * HD + 32 * my_blk + (TYPE == T_Q8_0 ? 8 : 4) * quarter;
+        const float4_at u = *reinterpret_cast<const float4_at*>(from), v = *reinterpret_cast<const float4_at*>(from + (TYPE == T_Q8_0 ? 4 : 16));
+        x = floatx8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
     };
     const Unpack unpack;
-    half8 q_hi[NT][T::BLOCKS], q_lo[NT][T::BLOCKS];
-    float cq[NT];
+    half8 q_hi[T::BLOCKS], q_lo[T::BLOCKS];
+    float cq;
     const auto split_queries = [&] {
+        uint32_t m = 0;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            uint32_t m = 0;
+        for (int j = 0; j < 8; ++j) m = umax(m, __float_as_uint(x[j]) & 0x7fffffffu);
+        if (T::BLOCKS >= 2) m = umax_dpp<DPP_XOR1>(m);
+        if (T::BLOCKS == 4) m = umax_dpp<DPP_XOR2>(m);
+        const int e = exponent_of(umax_xor32(umax_xor16(m)));
+        const float f = a.scale < 0.f ? -down(e) : down(e);
+        cq = fmaxf(fabsf(a.scale) * (LOG2E * up(e)), 0x1p-120f);   // a masked score times it is -inf
+        half8 hi, lo;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) m = umax(m, __float_as_uint(x[t][j]) & 0x7fffffffu);
-            if (T::BLOCKS >= 2) m = umax_dpp<DPP_XOR1>(m);
-            if (T::BLOCKS == 4) m = umax_dpp<DPP_XOR2>(m);
-            const int e = exponent_of(umax_xor32(umax_xor16(m)));
-            const float f = a.scale < 0.f ? -down(e) : down(e);
-            cq[t] = fmaxf(fabsf(a.scale) * (LOG2E * up(e)), 0x1p-120f);   // a masked score times it is -inf
-            half8 hi, lo;
+        for (int j = 0; j < 8; j += 2) split_pair(float2_t{x[ORDER[j]] * f, x[ORDER[j + 1]] * f}, hi, lo, j);
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) split_pair(float2_t{x[t][ORDER[j]] * f, x[t][ORDER[j + 1]] * f}, hi, lo, j);
-#pragma unroll
-            for (int blk = 0; blk < T::BLOCKS; ++blk) {
-                q_hi[t][blk] = my_blk == blk ? hi : half8{};
-                q_lo[t][blk] = my_blk == blk ? lo : half8{};
-            }
+        for (int blk = 0; blk < T::BLOCKS; ++blk) {
+            q_hi[blk] = my_blk == blk ? hi : half8{};
+            q_lo[blk] = my_blk == blk ? lo : half8{};
         }
     };
     uint8_t* tile = sh.lds + wave * T::BYTES;
     _Float16* scales = reinterpret_cast<_Float16*>(tile + T::SCALES);   // [keys, values][block][key]
     float* logs = reinterpret_cast<float*>(tile + T::LOGS);
-    floatx4 o[NT][2 * T::BLOCKS];
-    float base[NT], l[NT];
+    floatx4 o[2 * T::BLOCKS];
+    float base = NO_BASE, l = 0.f;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        base[t] = NO_BASE;
-        l[t] = 0.f;
-#pragma unroll
-        for (int d = 0; d < 2 * T::BLOCKS; ++d) o[t][d] = floatx4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int d = 0; d < 2 * T::BLOCKS; ++d) o[d] = floatx4{0.f, 0.f, 0.f, 0.f};
 
     float zero = 0.f;   // kept from the compiler, which would make a product with a conversion of the mixed fma
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -472,12 +461,10 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
             row = row_of(k + 2 * step);
         }
         // scores of keys 16n + 4 quarter + i: the block's of this column, then the sum over its place's columns
-        float w[NT][8];
+        float w[8];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            floatx4 sc[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) sc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+            floatx4 sc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int blk = 0; blk < T::BLOCKS; ++blk) {
                 half8 keys;
@@ -487,72 +474,62 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
                 } else {
                     keys = unpack.q4_keys(*reinterpret_cast<const uint32_t*>(tile + blk * T::STRIDE + (16 * n + col) * 16 + 4 * quarter));
                 }
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, q_hi[t][blk], sc[t], 0, 0, 0);
-                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, q_lo[t][blk], sc[t], 0, 0, 0);
-                }
+                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, q_hi[blk], sc, 0, 0, 0);
+                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, q_lo[blk], sc, 0, 0, 0);
             }
             const half4 d = *reinterpret_cast<const half4*>(scales + my_blk * T::KEYS + 16 * n + 4 * quarter);
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float x = __builtin_fmaf(float(d[i]), sc[t][i], zero);
-                    if (T::BLOCKS >= 2) x += dpp<DPP_XOR1>(x);
-                    if (T::BLOCKS == 4) x += dpp<DPP_XOR2>(x);
-                    w[t][4 * n + i] = x;
-                }
+            for (int i = 0; i < 4; ++i) {
+                float x = __builtin_fmaf(float(d[i]), sc[i], zero);
+                if (T::BLOCKS >= 2) x += dpp<DPP_XOR1>(x);
+                if (T::BLOCKS == 4) x += dpp<DPP_XOR2>(x);
+                w[4 * n + i] = x;
+            }
         }
         const floatx4 log_d[2] = {*reinterpret_cast<const floatx4*>(logs + 4 * quarter), *reinterpret_cast<const floatx4*>(logs + 16 + 4 * quarter)};
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            if (here != 0xffffffffu || __any(k + T::KEYS > limit[t])) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int key = 16 * (j >> 2) + 4 * quarter + (j & 3);
-                    if (!(here >> key & 1) || k + key >= limit[t]) w[t][j] = -__builtin_inff();
-                }
-            }
-            float top = __builtin_fmaf(w[t][0], cq[t], log_d[0][0]);
-#pragma unroll
-            for (int j = 1; j < 8; ++j) top = fmaxf(top, __builtin_fmaf(w[t][j], cq[t], log_d[j >> 2][j & 3]));
-            top = max_xor32(max_xor16(top));
-            if (__any(top > base[t] + 15.f)) {
-                const float moved = top > base[t] + 15.f ? top - 13.f : base[t], f = __builtin_amdgcn_exp2f(base[t] - moved);
-                base[t] = moved;
-                l[t] *= f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float f_i = __shfl(f, place_of(i) * T::BLOCKS, 64);   // of the query of row i
-#pragma unroll
-                    for (int d = 0; d < 2 * T::BLOCKS; ++d)
-                        if (is_of(i, d >> 1)) o[t][d][i] *= f_i;
-                }
-            }
+        if (here != 0xffffffffu || __any(k + T::KEYS > limit)) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                w[t][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[t][j], cq[t], -base[t]));
-                l[t] += w[t][j];
+                const int key = 16 * (j >> 2) + 4 * quarter + (j & 3);
+                if (!(here >> key & 1) || k + key >= limit) w[j] = -__builtin_inff();
             }
+        }
+        float top = __builtin_fmaf(w[0], cq, log_d[0][0]);
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, __builtin_fmaf(w[j], cq, log_d[j >> 2][j & 3]));
+        top = max_xor32(max_xor16(top));
+        if (__any(top > base + 15.f)) {
+            const float moved = top > base + 15.f ? top - 13.f : base, f = __builtin_amdgcn_exp2f(base - moved);
+            base = moved;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float f_i = __shfl(f, place_of(i) * T::BLOCKS, 64);   // of the query of row i
+#pragma unroll
+                for (int d = 0; d < 2 * T::BLOCKS; ++d)
+                    if (is_of(i, d >> 1)) o[d][i] *= f_i;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[j], cq, -base));
+            l += w[j];
         }
         // O += P V, P the weights with this column's block's scales; element j is key
         // 4 quarter + j or 16 + 4 quarter + j - 4 in either operand.  Of a block's
         // products only the rows of that block count.
         [[maybe_unused]] const uint8_t* values = tile + T::VALUES + (4 * quarter + (col >> 1 & 3) + (col >> 3) * 16) * 16 + 8 * (col & 1);
-        half8 p_hi[NT], p_lo[NT];
+        half8 p_hi, p_lo;
         {
             const _Float16* dv = scales + (T::BLOCKS + my_blk) * T::KEYS + 4 * quarter;
             const half4 d0 = *reinterpret_cast<const half4*>(dv), d1 = *reinterpret_cast<const half4*>(dv + 16);
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    const int j0 = ORDER[j], j1 = ORDER[j + 1];
-                    const float x0 = __builtin_fmaf(w[t][j0], float(j0 < 4 ? d0[j0 & 3] : d1[j0 & 3]), zero);
-                    const float x1 = __builtin_fmaf(w[t][j1], float(j1 < 4 ? d0[j1 & 3] : d1[j1 & 3]), zero);
-                    split_pair(float2_t{x0, x1}, p_hi[t], p_lo[t], j);
-                }
+            for (int j = 0; j < 8; j += 2) {
+                const int j0 = ORDER[j], j1 = ORDER[j + 1];
+                const float x0 = __builtin_fmaf(w[j0], float(j0 < 4 ? d0[j0 & 3] : d1[j0 & 3]), zero);
+                const float x1 = __builtin_fmaf(w[j1], float(j1 < 4 ? d0[j1 & 3] : d1[j1 & 3]), zero);
+                split_pair(float2_t{x0, x1}, p_hi, p_lo, j);
+            }
         }
 #pragma unroll
         for (int blk = 0; blk < T::BLOCKS; ++blk) {
@@ -573,12 +550,10 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
             }
 #endif
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    o[t][2 * blk + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p_hi[t], v[h], o[t][2 * blk + h], 0, 0, 0);
-                    o[t][2 * blk + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p_lo[t], v[h], o[t][2 * blk + h], 0, 0, 0);
-                }
+            for (int h = 0; h < 2; ++h) {
+                o[2 * blk + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p_hi, v[h], o[2 * blk + h], 0, 0, 0);
+                o[2 * blk + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p_lo, v[h], o[2 * blk + h], 0, 0, 0);
+            }
         }
     }
     if (__any(odd_values)) {
@@ -591,21 +566,16 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
                 for (int blk = 0; blk < T::BLOCKS; ++blk) {
                     if (finite_half(*reinterpret_cast<const uint16_t*>(c.v + r * c.ldv + (kvh * T::BLOCKS + blk) * T::BB))) continue;
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (k + n < __shfl(limit[t], place_of(i) * T::BLOCKS, 64)) o[t][2 * blk][i] = o[t][2 * blk + 1][i] = __builtin_nanf("");
+                    for (int i = 0; i < 4; ++i)
+                        if (k + n < __shfl(limit, place_of(i) * T::BLOCKS, 64)) o[2 * blk][i] = o[2 * blk + 1][i] = __builtin_nanf("");
                 }
             }
     }
     // the sums of the waves of a head, joined through LDS
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        l[t] = pair_sum(sum_xor16(l[t]));
-        if (quarter == 0 && my_blk == 0) {
-            sh.b[wave][Shared::EACH * t + g] = base[t];
-            sh.l[wave][Shared::EACH * t + g] = l[t];
-        }
+    l = pair_sum(sum_xor16(l));
+    if (quarter == 0 && my_blk == 0) {
+        sh.b[wave][g] = base;
+        sh.l[wave][g] = l;
     }
     __syncthreads();   // also: every wave is past its tiles
     float* all = reinterpret_cast<float*>(sh.lds);
@@ -617,17 +587,15 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 3 : 2) void cache_attn_narrow
         return sum;
     };
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int i = 0; i < 4; ++i) {
+        const int p = place_of(i);
+        float most;
+        const float sum = joined_sum(wave_head, p, most);
+        const float f = sh.l[wave][p] != 0.f ? __builtin_amdgcn_exp2f(sh.b[wave][p] - most) / sum : 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = Shared::EACH * t + place_of(i);
-            float most;
-            const float sum = joined_sum(wave_head, p, most);
-            const float f = sh.l[wave][p] != 0.f ? __builtin_amdgcn_exp2f(sh.b[wave][p] - most) / sum : 0.f;
-#pragma unroll
-            for (int d = 0; d < 2 * T::BLOCKS; ++d)
-                if (is_of(i, d >> 1)) all[(wave * Shared::PLACES + p) * (HD + 4) + 16 * d + col] = o[t][d][i] * f;
-        }
+        for (int d = 0; d < 2 * T::BLOCKS; ++d)
+            if (is_of(i, d >> 1)) all[(wave * Shared::PLACES + p) * (HD + 4) + 16 * d + col] = o[d][i] * f;
+    }
     if (tid < Shared::PLACES * a.wave_heads) {
         const int p = tid % Shared::PLACES, of_head = tid / Shared::PLACES;
         float most;
@@ -997,11 +965,10 @@ template <int TYPE, int HD>
 void launch_typed(const CacheAttnArgs& a, hipStream_t stream) {
     if (a.ends) cache_attn_sums_kernel<<<1, SUMS_THREADS, 0, stream>>>(a);
     const unsigned groups = unsigned((a.slots + a.tiles + 7) / 8 * 8 * int(a.by_head_sets.d));
-    if (a.query_tiles == 0) cache_attn_wide_kernel<TYPE, HD><<<groups, 64 * WAVES, 0, stream>>>(a);
-    else if (a.query_tiles == 1) cache_attn_narrow_kernel<TYPE, HD, 1><<<groups, 64 * WAVES, 0, stream>>>(a);
-    else cache_attn_narrow_kernel<TYPE, HD, 2><<<groups, 64 * WAVES, 0, stream>>>(a);
+    if (a.narrow) cache_attn_narrow_kernel<TYPE, HD><<<groups, 64 * WAVES, 0, stream>>>(a);
+    else cache_attn_wide_kernel<TYPE, HD><<<groups, 64 * WAVES, 0, stream>>>(a);
     // few places: few rows, of many parts
-    if (a.slots && a.query_tiles) launch_merge<HD, 256 / HD>(a, stream);
+    if (a.slots && a.narrow) launch_merge<HD, 256 / HD>(a, stream);
     else if (a.slots) launch_merge<HD, 1>(a, stream);
 }
 
@@ -1017,9 +984,13 @@ void launch_of_type(const CacheAttnArgs& a, hipStream_t stream) {
 void cache_attn_plan(CacheAttnArgs& a, int cus) {
     const int64_t places = int64_t(a.rows) * a.group, requests = std::min(a.cache.requests, a.rows);
     const int64_t each = (places + requests - 1) / requests;   // of a request with its share of the rows
-    const int of_operand = 512 / a.cache.head_dim;
-    a.query_tiles = each <= of_operand ? 1 : each <= 2 * of_operand ? 2 : 0;
-    const int tile = a.query_tiles ? of_operand * a.query_tiles : TILE * WAVES, keys = a.query_tiles ? 32 * WAVES : WIDE_KEYS;
+    // Up to the places of one wave of the other form (us for 16, 24, 32, 48 places of
+    // each of 48 requests on up to 3000 Q4_0 keys of 4 kv heads, few / many: head_dim 32
+    // 22 / 34, 26 / 35, 27 / 31, 34 / 39; 64: 31 / 57, 42 / 58, 50 / 50, 72 / 64; 128: 72 /
+    // 170, 102 / 171, 135 / 156, 219 / 171.  Two operands of places to a workgroup
+    // instead of two workgroups: 34, 41 and 80 at 16 places).
+    a.narrow = each <= TILE;
+    const int tile = a.narrow ? 512 / a.cache.head_dim : TILE * WAVES, keys = a.narrow ? 32 * WAVES : WIDE_KEYS;
     a.tiles = int(places / tile + requests);
     a.short_rows = std::max(a.cache.ldk, a.cache.ldv) < (int64_t(1) << 26);
     // About as many parts as run at once, which registers decide (us for 2, 3, 4, 5,
@@ -1029,7 +1000,7 @@ void cache_attn_plan(CacheAttnArgs& a, int cus) {
     // Q8_0 keys: 49, 43, 57, 50, 47; 13 requests of up to 150 queries of 12 heads of
     // 64 on up to 1300: 30, 40, 37, 43, 43).
     a.least_steps = 2;
-    const int at_once = !a.query_tiles ? (a.cache.head_dim == 32 ? 3 : 2) : a.cache.head_dim == 128 ? 3 : 4;
+    const int at_once = !a.narrow ? (a.cache.head_dim == 32 ? 3 : 2) : a.cache.head_dim == 128 ? 3 : 4;
     const bool split = a.max_len > a.least_steps * keys;
     const auto slots = [&](int wave_heads) { return split ? std::max(1, at_once * cus / (a.cache.kv_heads / wave_heads)) : 0; };
     // Few places: waves of one workgroup read the kv heads of the same keys, for heads
@@ -1039,7 +1010,7 @@ void cache_attn_plan(CacheAttnArgs& a, int cus) {
     // leave more parts to the join (four queries of 4 kv heads of 128 on 30000: 31.8
     // and 45; 8 of 8 heads of 32 on up to 5217: 16.0, 14.7 with two and 15.0 with four).
     a.wave_heads = 1;
-    if (split && a.query_tiles)
+    if (split && a.narrow)
         for (int heads : {2, 4})
             if (a.cache.kv_heads % heads == 0 && slots(heads) <= MOST_PARTS * int64_t(a.tiles)) a.wave_heads = heads;
     a.slots = slots(a.wave_heads);

@@ -132,7 +132,7 @@ struct CacheAttnArgs {
     float scale;
     bool causal;
     bool short_rows;                       // the bytes of 32 rows fit 31 bits
-    int query_tiles;                       // of 512 / head_dim places; 0: 128 places to a workgroup
+    bool narrow;                           // 512 / head_dim places to a workgroup; else 128
     int wave_heads;                        // kv heads of a workgroup, each some of its waves': 1, 2 or 4
     Divisor by_group, by_head_sets, by_places, by_step;   // by_places, by_step: a workgroup's places of a head, and its keys at a time
     int tiles;                             // of all requests, at most

@@ -897,3 +897,13 @@ def test_scales_near_the_largest_number(samhip, gpu_ctx, rows):
     a = Attend(p, 4, seed=41, scale=3.3e38)
     a.q.mul_(2.0 ** -128)
     a.check(samhip, gpu_ctx)
+
+
+@pytest.mark.parametrize("q4", [False, True])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("rows", [4, 8, 9, 16, 32, 33])
+def test_several_tiles_of_few_places(samhip, gpu_ctx, rows, hd, q4):
+    """Requests whose places fill whole tiles of the form for few, one more, and those on either side of the other form."""
+    p = Pages([rows, rows - 1, rows], [1300, rows, 333], 4, hd, q4, 16, seed=42, first=1, behind=1).fill(42)
+    for causal in (False, True):
+        Attend(p, 4, causal, pad=3, seed=42).check(samhip, gpu_ctx)
