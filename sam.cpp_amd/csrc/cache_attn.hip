@@ -28,8 +28,8 @@
 // join.  At head_dim 128 twelve waves a CU have 4.6 KB each under way, and the
 // vector instructions take 33 us, the matrix instructions 10; the rest is parts
 // that end early and HBM's lines one by one.
-// Many places: 128 to a workgroup, 64 keys at a time as fp16 codes in LDS for its
-// four waves, the next ones written beside them.  Key scales multiply a block's
+// Many places: 128 to a workgroup, 64 keys (32 of head_dim 128) at a time as fp16
+// codes in LDS for its four waves, the next ones written beside them.  Key scales multiply a block's
 // products, value scales the weights.  8 prompts of 201 queries of 8 heads of 32
 // on up to 5217 Q8_0 keys: 43.4 us, of it 4.6 the join; vector instructions (about
 // 150 for 32 keys and 32 places, 16 of them exponentials at a quarter rate) fill
@@ -617,7 +617,7 @@ __global__ __launch_bounds__(64 * WAVES, 3) void cache_attn_narrow_kernel(CacheA
 // --- many places --------------------------------------------------------------
 
 constexpr int TILE = 32;                  // query places of a wave
-constexpr int WIDE_KEYS = 64;
+constexpr int wide_keys(int head_dim) { return head_dim == 128 ? 32 : 64; }
 
 // Eight neighbouring codes of a row, and their block's scale.
 template <int TYPE>
@@ -641,8 +641,18 @@ struct Octet {
     }
 };
 
+// At head_dim 128 the queries' low halves: with them in registers, and 64 keys in
+// a tile, one wave has a SIMD (48 requests of 48 places: 170 us; so: 110).
 template <int HD>
-struct WideShared {
+struct WideLow {};
+template <>
+struct WideLow<128> {
+    half8 q_lo[WAVES][128 / 16][64];
+};
+
+template <int HD>
+struct WideShared : WideLow<HD> {
+    static constexpr int WIDE_KEYS = wide_keys(HD);
     typedef TileShape<1, HD, WIDE_KEYS, false> K;
     typedef TileShape<1, HD, WIDE_KEYS, true> V;
     struct Tile {
@@ -656,9 +666,9 @@ struct WideShared {
 };
 
 template <int TYPE, int HD>
-__global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_kernel(CacheAttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, 2) void cache_attn_wide_kernel(CacheAttnArgs a) {
     typedef WideShared<HD> Shared;
-    constexpr int PIECES = HD / 32, BLOCKS = HD / 32, BB = block_bytes(TYPE);   // of 8 values, a thread's part of a tile
+    constexpr int WIDE_KEYS = wide_keys(HD), PIECES = HD * WIDE_KEYS / 2048, BLOCKS = HD / 32, BB = block_bytes(TYPE);   // of 8 values, a thread's part of a tile
     __shared__ Shared sh;
     Span s;
     if (!find_span(a, s)) return;
@@ -670,10 +680,10 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
     const int row = s.q0 + (mine ? i_row : 0), limit = mine ? min(s.limit(a.causal, i_row), s.k1) : 0;
 
     // Cache rows of a tile, looked up by the first wave three tiles ahead.
-    const auto row_at = [&](int k) { return k + lane < s.k1 ? cache_row(c, s.request, k + lane) : -1; };
+    const auto row_at = [&](int k) { return lane < WIDE_KEYS && k + lane < s.k1 ? cache_row(c, s.request, k + lane) : -1; };
     const auto put_rows = [&](int t, int r) {
         const uint64_t here = __ballot(r >= 0);
-        sh.rows[t & 3][lane] = r;
+        if (lane < WIDE_KEYS) sh.rows[t & 3][lane] = r;
         if (lane == 0) sh.here[t & 3] = here;
     };
     int ahead = -1;
@@ -706,7 +716,15 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
         for (int t = 0; t < HD / 16; ++t)
 #pragma unroll
             for (int j = 0; j < 8; j += 2) split_pair(float2_t{x[t][j] * f, x[t][j + 1] * f}, q_hi[t], q_lo[t], j);
+        if constexpr (HD == 128) {
+#pragma unroll
+            for (int t = 0; t < HD / 16; ++t) sh.q_lo[wave][t][lane] = q_lo[t];
+        }
     }
+    const auto low = [&](int u) {
+        if constexpr (HD == 128) return sh.q_lo[wave][u][lane];
+        else return q_lo[u];
+    };
     // o[d] holds, transposed, dimensions 32d + 8 (r / 4) + 4hh + r % 4 of place li
     floatx16 o[BLOCKS];
     float base = NO_BASE, l = 0.f, zero = 0.f;   // (zero: kept from the compiler, for the mixed fma)
@@ -797,7 +815,7 @@ __global__ __launch_bounds__(64 * WAVES, HD < 128 ? 2 : 1) void cache_attn_wide_
                     for (int u = 2 * blk; u < 2 * blk + 2; ++u) {
                         const half8 keys = *reinterpret_cast<const half8*>(kt + 32 * u);
                         p = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys, q_hi[u], p, 0, 0, 0);
-                        p = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys, q_lo[u], p, 0, 0, 0);
+                        p = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys, low(u), p, 0, 0, 0);
                     }
 #pragma unroll
                     for (int r = 0; r < 16; r += 4) {
@@ -986,13 +1004,14 @@ void launch_of_type(const CacheAttnArgs& a, hipStream_t stream) {
 void cache_attn_plan(CacheAttnArgs& a, int cus) {
     const int64_t places = int64_t(a.rows) * a.group, requests = std::min(a.cache.requests, a.rows);
     const int64_t each = (places + requests - 1) / requests;   // of a request with its share of the rows
-    // Up to the places of one wave of the other form (us for 16, 24, 32, 48 places of
-    // each of 48 requests on up to 3000 Q4_0 keys of 4 kv heads, few / many: head_dim 32
-    // 22 / 34, 26 / 35, 27 / 31, 34 / 39; 64: 31 / 57, 42 / 58, 50 / 50, 72 / 64; 128: 72 /
-    // 170, 102 / 171, 135 / 156, 219 / 171.  Two operands of places to a workgroup
-    // instead of two workgroups: 34, 41 and 80 at 16 places).
-    a.narrow = each <= TILE;
-    const int tile = a.narrow ? 512 / a.cache.head_dim : TILE * WAVES, keys = a.narrow ? 32 * WAVES : WIDE_KEYS;
+    // Where the two forms meet (us for 16, 24, 32, 48 places of each of 48 requests on up
+    // to 3000 Q4_0 keys of 4 kv heads, few / many: head_dim 32 22 / 34, 26 / 35, 27 / 31,
+    // 35 / 39; 64: 31 / 57, 41 / 58, 49 / 50, 69 / 63; 128: 69 / 104, 100 / 105, 131 / 89,
+    // 215 / 107; of 8 on up to 5000, 24, 32 and 48 places: 32 16.9 / 17.7, 17.3 / 16.6, 20.3
+    // / 19.3; 64: 23 / 23, 24 / 21, 28 / 26; 128: 39 / 36, 45 / 33, 59 / 40).  Two operands
+    // of places to a workgroup instead of two workgroups: 34, 41 and 80 at 16 places.
+    a.narrow = each <= (a.cache.head_dim == 128 ? 24 : 32);
+    const int tile = a.narrow ? 512 / a.cache.head_dim : TILE * WAVES, keys = a.narrow ? 32 * WAVES : wide_keys(a.cache.head_dim);
     a.tiles = int(places / tile + requests);
     a.short_rows = std::max(a.cache.ldk, a.cache.ldv) < (int64_t(1) << 26);
     // About as many parts as run at once, which registers decide (us for 2, 3, 4, 5,

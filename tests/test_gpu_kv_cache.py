@@ -907,3 +907,13 @@ def test_several_tiles_of_few_places(samhip, gpu_ctx, rows, hd, q4):
     p = Pages([rows, rows - 1, rows], [1300, rows, 333], 4, hd, q4, 16, seed=42, first=1, behind=1).fill(42)
     for causal in (False, True):
         Attend(p, 4, causal, pad=3, seed=42).check(samhip, gpu_ctx)
+
+
+@pytest.mark.parametrize("q4", [False, True])
+@pytest.mark.parametrize("rows", [24, 25, 70, 129])
+def test_tiles_of_32_keys_of_head_dim_128(samhip, gpu_ctx, rows, q4):
+    """Lengths on either side of the many-place form's tiles and parts."""
+    for lens in ([64, 65, 33], [2000, 31, 97]):
+        p = Pages([rows, 3, rows], lens, 2, 128, q4, 41, seed=43, behind=1).fill(43)
+        for causal in (False, True):
+            Attend(p, 2, causal, seed=43).check(samhip, gpu_ctx)
