@@ -49,6 +49,7 @@ constexpr int WAVES = 4;
 constexpr int MOST_PARTS = 32;             // of a tile's keys where waves have heads of their own
 constexpr float NO_BASE = -1e30f;         // below every score, and finite
 constexpr int ZERO_SCALE = -40;           // log 2 of what a zero scale counts as
+constexpr int DPP_HALF_MIRROR = 0x141;    // lane 7 - i of its eight
 
 typedef uint32_t u32x2_at __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t u32x4_at __attribute__((ext_vector_type(4), aligned(2)));
@@ -659,7 +660,7 @@ struct WideShared : WideLow<HD> {
         uint8_t __attribute__((aligned(16))) k[K::BYTES];
         uint8_t __attribute__((aligned(16))) v[V::BYTES];
         _Float16 __attribute__((aligned(16))) scales[2][HD / 32][WIDE_KEYS];   // of keys, of values
-        uint32_t most[WAVES];                                                  // the largest of the values'
+        float __attribute__((aligned(16))) logs[WIDE_KEYS];                    // log 2 of a key's largest value scale
     } tile[2];
     int rows[4][WIDE_KEYS];
     uint64_t here[4];
@@ -756,7 +757,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attn_wide_kernel(CacheAtt
     };
     bool odd_values = false;
     const auto put = [&](typename Shared::Tile& tile) {
-        uint32_t most = 0;
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             const bool is = there >> i & 1;
@@ -766,7 +766,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attn_wide_kernel(CacheAtt
                 odd_values = true;   // added behind the last tile, for those that see them
                 dv = 0;
             }
-            most = umax(most, dv & 0x7fffu);
             const int f = tid + 256 * i;
             *Shared::K::piece(tile.k, f) = kr[i].codes(unpack, octet);
             *Shared::V::piece(tile.v, f) = vr[i].codes(unpack, octet);
@@ -774,9 +773,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attn_wide_kernel(CacheAtt
                 reinterpret_cast<uint16_t*>(tile.scales[0][octet / 4])[key + i * EACH] = uint16_t(dk);
                 reinterpret_cast<uint16_t*>(tile.scales[1][octet / 4])[key + i * EACH] = uint16_t(dv);
             }
+            uint32_t most = dv & 0x7fffu;   // of the key's blocks, a quad of lanes to each
+            if (BLOCKS == 2) most = umax_dpp<DPP_HALF_MIRROR>(most);
+            if (BLOCKS == 4) most = umax_row(most);
+            if (octet == 0) tile.logs[key + i * EACH] = fmaxf(__builtin_amdgcn_logf(half_bits_to_float(most)), float(ZERO_SCALE));
         }
-        most = wave_umax(most);
-        if (lane == 0) tile.most[wave] = most;
     };
     __syncthreads();
     if (s.k0 < s.k1) {
@@ -796,10 +797,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attn_wide_kernel(CacheAtt
         progress.at(k);
         const typename Shared::Tile& tile = sh.tile[t_now & 1];
         if (k < wave_end) {
-            uint32_t most = 0;
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) most = umax(most, tile.most[w]);
-            const float log_d = fmaxf(__builtin_amdgcn_logf(half_bits_to_float(most)), float(ZERO_SCALE));
             const uint64_t here = sh.here[t_now & 3];
 #pragma unroll
             for (int n = 0; n < WIDE_KEYS / 32; ++n) {
@@ -832,11 +829,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attn_wide_kernel(CacheAtt
                         if (!(here_n >> at & 1) || k + 32 * n + at >= limit) sc[r] = -__builtin_inff();
                     }
                 }
-                float top = sc[0];
+                // the largest contribution, of each key its own score and scale: one with a
+                // large scale may have no weight, or be hidden
+                float top = -__builtin_inff();
 #pragma unroll
-                for (int r = 1; r < 16; ++r) top = __builtin_elementwise_maximum(top, sc[r]);
+                for (int r = 0; r < 16; r += 4) {
+                    const floatx4 log_d = *reinterpret_cast<const floatx4*>(tile.logs + 32 * n + 2 * r + 4 * hh);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) top = __builtin_elementwise_maximum(top, __builtin_fmaf(sc[r + j], cq, log_d[j]));
+                }
                 const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-                top = __builtin_fmaf(__builtin_elementwise_maximum(__uint_as_float(other[0]), __uint_as_float(other[1])), cq, log_d);
+                top = __builtin_elementwise_maximum(__uint_as_float(other[0]), __uint_as_float(other[1]));
                 if (__any(top > base + 15.f)) {
                     const float moved = top > base + 15.f ? top - 13.f : base, by = __builtin_amdgcn_exp2f(base - moved);
                     base = moved;

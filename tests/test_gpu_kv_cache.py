@@ -917,3 +917,111 @@ def test_tiles_of_32_keys_of_head_dim_128(samhip, gpu_ctx, rows, q4):
         p = Pages([rows, 3, rows], lens, 2, 128, q4, 41, seed=43, behind=1).fill(43)
         for causal in (False, True):
             Attend(p, 2, causal, seed=43).check(samhip, gpu_ctx)
+
+
+# --- value scales of one tile that lie far apart ------------------------------------
+
+
+def tight(a):
+    """The definition in F64 of every row of an Attend, and what it may be off by,
+    key by key: a weight is off by its score's error ds (as above, of its own key)
+    and, through the sum of weights, by their mean; then the operands' and sums'
+    roundings, and fp16's half step 2^-25 of each product, of which the largest is
+    2^13 at least: 2^-38 of it on codes up to 128."""
+    p, hd, group = a.p, a.p.hd, a.heads // a.p.kv_heads
+    ref = torch.full((p.rows, a.heads * hd), 7.0, device="cuda", dtype=torch.float64)
+    bound = torch.zeros_like(ref)
+    for r, (n, m) in enumerate(zip(p.n, p.lens)):
+        if not n or not m:
+            continue
+        s0 = p.starts[r]
+        q = a.q[s0:s0 + n].double().view(n, a.heads, hd)
+        at = p.at(r, range(m))
+        k, v = (values(c[at][:, :p.row_bytes], p.q4).view(m, p.kv_heads, hd) for c in p.caches)
+        block = 18 if p.q4 else 34
+        d = p.caches[1][at][:, :p.row_bytes].reshape(m, -1, block)[..., :2].contiguous().view(torch.float16).double().abs()
+        d = d.view(m, p.kv_heads, -1).amax(-1)
+        hidden = torch.zeros(n, m, dtype=torch.bool, device="cuda")
+        if a.causal:
+            hidden = torch.arange(m, device="cuda")[None, :] > torch.arange(n, device="cuda")[:, None] + (m - n)
+        for h in range(a.heads):
+            kk, vv, dd = k[:, h // group], v[:, h // group], d[:, h // group]
+            w = torch.softmax(((q[:, h] @ kk.t()) * a.scale).masked_fill(hidden, -torch.inf), -1)
+            ds = (q[:, h].abs() @ kk.abs().t()) * abs(a.scale) * (hd * 2.0 ** -24 + 5 * 2.0 ** -22)
+            off = ds + (w * ds).sum(-1, keepdim=True) + 2.0 ** -19 + (m / 16 + 48) * 2.0 ** -24
+            cols = slice(h * hd, (h + 1) * hd)
+            ref[s0:s0 + n, cols] = w @ vv
+            bound[s0:s0 + n, cols] = 1.01 * (w * off) @ vv.abs() + m * 2.0 ** -31 * (w * dd).amax(1, keepdim=True)
+    return ref, bound
+
+
+def small_and_large(q4):
+    """Factors that bring value scales of N(0, 1) to about 2^-14.4, and those 2^29 times as large."""
+    return (2.0 ** -13, 2.0 ** 16) if q4 else (2.0 ** -9, 2.0 ** 20)
+
+
+@pytest.mark.parametrize("q4", [False, True])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("rows", [3, 40])
+@pytest.mark.parametrize("from_the_end", [1, 2, 20])
+def test_large_value_scales_that_some_queries_do_not_see(samhip, gpu_ctx, from_the_end, rows, hd, q4):
+    """One value row 2^29 times the others inside a tile, hidden from the first
+    rows: those have the bits that they have with an ordinary one there, and the
+    accuracy that they have without it."""
+    if from_the_end >= rows:
+        pytest.skip("seen by all")
+    print("hidden scale", from_the_end, rows, hd, q4, flush=True)
+    small, large = small_and_large(q4)
+    outs, m = [], 702
+    for factor in (small, large):
+        p = Pages([rows, rows], [m, 300], 2, hd, q4, 41, seed=50).fill(50)
+        scale_blocks(p, 0, 1, range(m), small)
+        scale_blocks(p, 0, 1, [m - from_the_end], factor / small)
+        a = Attend(p, 4, True, seed=50)
+        ref, bound = tight(a)
+        a.run(samhip, gpu_ctx)
+        a.verify(ref, bound)
+        outs.append(a.out[:rows - from_the_end].clone())
+    assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("q4", [False, True])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("place", [5, 250, 511])
+def test_large_value_scales_of_no_weight(samhip, gpu_ctx, place, rows, hd, q4):
+    """One value row 2^29 times the others, whose key is 80 nats below theirs: in
+    the first tile, inside one, and last."""
+    print("weightless scale", place, rows, hd, q4, flush=True)
+    small, large = small_and_large(q4)
+    p = Pages([rows], [512], 1, hd, q4, 64, seed=51).fill(51)
+    k = torch.zeros(512, hd, device="cuda")
+    k[place] = -80 / hd
+    p.caches[0][p.at(0, range(512))] = torch.as_tensor(packed(k, q4), device="cuda")
+    scale_blocks(p, 0, 1, range(512), small)
+    scale_blocks(p, 0, 1, [place], large / small)
+    a = Attend(p, 2, seed=51, scale=1.0)
+    a.q.fill_(1.0)
+    ref, bound = tight(a)
+    a.run(samhip, gpu_ctx)
+    a.verify(ref, bound)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("below", [10.0, 18.5, 30.0])
+@pytest.mark.parametrize("place", [250, 275])
+def test_value_scales_that_change_inside_a_tile(samhip, gpu_ctx, place, below, rows, hd):
+    """As test_large_values_of_little_weight, 2^29 apart and the change on no tile's border."""
+    p = Pages([rows], [512], 1, hd, True, 64, seed=52).fill(52)
+    k = torch.zeros(512, hd, device="cuda")
+    k[place:] = -below / hd
+    p.caches[0][p.at(0, range(512))] = torch.as_tensor(packed(k, True), device="cuda")
+    small, large = small_and_large(True)
+    scale_blocks(p, 0, 1, range(0, place), small)
+    scale_blocks(p, 0, 1, range(place, 512), large)
+    a = Attend(p, 1, seed=52, scale=1.0)
+    a.q.fill_(1.0)
+    ref, bound = tight(a)
+    a.run(samhip, gpu_ctx)
+    a.verify(ref, bound)
