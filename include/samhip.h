@@ -484,8 +484,9 @@ int samhip_cache_read(samhip_context* ctx, const samhip_kv_cache* cache, const s
  * over the request's positions that have a place, with `causal` those up to
  * the row's own.  F32-accurate on the values the blocks stand for; what a key
  * adds that is below 2^-16 of a query's largest is off by at most 2^-39 of that.
- * A query with a value that is not finite gets NaN for its head.  Grouped
- * heads: head h reads kv head h / (heads / kv_heads).  A query that sees no
+ * Scores, and scale times a query's largest value, are F32 numbers: past their
+ * range a query gets NaN, or zeros where all its scores are below it.  A query
+ * with a value that is not finite gets NaN for its head.  Grouped heads: head h reads kv head h / (heads / kv_heads).  A query that sees no
  * position gets zeros; rows of out outside [row_start[0],
  * row_start[requests]) are left as they were.  A key whose blocks' scales are
  * not finite makes NaN of the queries that see it, such a value block of its

@@ -15,6 +15,11 @@
 // as hi + lo they keep 22 bits down to 2^-16 of the largest contribution so
 // far, wherever its weight or its scale comes from.  A scale of zero counts as
 // 2^-40 in this, for its weight has its place in the sum.
+// F32 scores of 2^23 and more (FAR) are whole numbers, from which neither a
+// scale's log nor 13 can be taken: such a query's base is its largest score, as
+// rounded, and so are the others that it is taken from, so that weights are 1 at
+// most and products below 2^16.  (With the product and the difference rounded at
+// once, a score of 2^30 is 2^5 off its own base.)
 //
 // Few places: a wave takes 32 keys at a time, their codes through LDS that no
 // other wave touches, read transposed for values.  An operand's 16 columns are
@@ -47,7 +52,9 @@ namespace {
 
 constexpr int WAVES = 4;
 constexpr int MOST_PARTS = 32;             // of a tile's keys where waves have heads of their own
-constexpr float NO_BASE = -1e30f;         // below every score, and finite
+constexpr float NO_BASE = -0x1.fffffep127f;   // below every score, and finite
+constexpr float FAR = 0x1p23f;            // of scores; a base from half of it on is looked at with every tile
+constexpr float ROOM = 15.f;              // log 2 of the largest product before the base moves
 constexpr int ZERO_SCALE = -40;           // log 2 of what a zero scale counts as
 constexpr int DPP_HALF_MIRROR = 0x141;    // lane 7 - i of its eight
 
@@ -374,7 +381,7 @@ __global__ __launch_bounds__(64 * WAVES, 3) void cache_attn_narrow_kernel(CacheA
     _Float16* scales = reinterpret_cast<_Float16*>(tile + T::SCALES);   // [keys, values][block][key]
     float* logs = reinterpret_cast<float*>(tile + T::LOGS);
     floatx4 o[2 * T::BLOCKS];
-    float base = NO_BASE, l = 0.f;
+    float base = NO_BASE, l = 0.f, room = ROOM;
 #pragma unroll
     for (int d = 0; d < 2 * T::BLOCKS; ++d) o[d] = floatx4{0.f, 0.f, 0.f, 0.f};
 
@@ -498,10 +505,25 @@ __global__ __launch_bounds__(64 * WAVES, 3) void cache_attn_narrow_kernel(CacheA
         float top = __builtin_fmaf(w[0], cq, log_d[0][0]);
 #pragma unroll
         for (int j = 1; j < 8; ++j) top = fmaxf(top, __builtin_fmaf(w[j], cq, log_d[j >> 2][j & 3]));
-        top = max_xor32(max_xor16(top));
-        if (__any(top > base + 15.f)) {
-            const float moved = top > base + 15.f ? top - 13.f : base, f = __builtin_amdgcn_exp2f(base - moved);
+        float c_now = cq;
+        if (__any(top > base + room)) {
+            top = max_xor32(max_xor16(top));
+            const bool far = fabsf(top) >= FAR;
+            float moved = top > base + ROOM ? top - 13.f : base;
+            if (__any(far)) {
+                float most = base;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    w[j] = far ? w[j] * cq : w[j];
+                    most = fmaxf(most, w[j]);
+                }
+                most = max_xor32(max_xor16(most));
+                moved = far ? most : moved;
+                c_now = far ? 1.f : cq;
+            }
+            const float f = __builtin_amdgcn_exp2f(base - moved);
             base = moved;
+            room = fabsf(base) >= 0.5f * FAR ? -__builtin_inff() : ROOM;
             l *= f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -513,7 +535,7 @@ __global__ __launch_bounds__(64 * WAVES, 3) void cache_attn_narrow_kernel(CacheA
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[j], cq, -base));
+            w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[j], c_now, -base));
             l += w[j];
         }
         // O += P V, P the weights with this column's block's scales; element j is key
@@ -728,7 +750,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attn_wide_kernel(CacheAtt
     };
     // o[d] holds, transposed, dimensions 32d + 8 (r / 4) + 4hh + r % 4 of place li
     floatx16 o[BLOCKS];
-    float base = NO_BASE, l = 0.f, zero = 0.f;   // (zero: kept from the compiler, for the mixed fma)
+    float base = NO_BASE, l = 0.f, room = ROOM, zero = 0.f;   // (zero: kept from the compiler, for the mixed fma)
 #if defined(__HIP_DEVICE_COMPILE__)
     asm("" : "+s"(zero));
 #endif
@@ -838,11 +860,25 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attn_wide_kernel(CacheAtt
 #pragma unroll
                     for (int j = 0; j < 4; ++j) top = __builtin_elementwise_maximum(top, __builtin_fmaf(sc[r + j], cq, log_d[j]));
                 }
-                const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-                top = __builtin_elementwise_maximum(__uint_as_float(other[0]), __uint_as_float(other[1]));
-                if (__any(top > base + 15.f)) {
-                    const float moved = top > base + 15.f ? top - 13.f : base, by = __builtin_amdgcn_exp2f(base - moved);
+                float c_now = cq;
+                if (__any(top > base + room)) {
+                    top = max_xor32(top);
+                    const bool far = fabsf(top) >= FAR;
+                    float moved = top > base + ROOM ? top - 13.f : base;
+                    if (__any(far)) {
+                        float most = base;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            sc[r] = far ? sc[r] * cq : sc[r];
+                            most = fmaxf(most, sc[r]);
+                        }
+                        most = max_xor32(most);
+                        moved = far ? most : moved;
+                        c_now = far ? 1.f : cq;
+                    }
+                    const float by = __builtin_amdgcn_exp2f(base - moved);
                     base = moved;
+                    room = fabsf(base) >= 0.5f * FAR ? -__builtin_inff() : ROOM;
                     l *= by;
 #pragma unroll
                     for (int d = 0; d < BLOCKS; ++d)
@@ -851,7 +887,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attn_wide_kernel(CacheAtt
                 }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], cq, -base));
+                    sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], c_now, -base));
                     l += sc[r];
                 }
                 // O^T += V^T P^T, P the weights with a block's scales: of 16 keys, lane

@@ -1025,3 +1025,36 @@ def test_value_scales_that_change_inside_a_tile(samhip, gpu_ctx, place, below, r
     ref, bound = tight(a)
     a.run(samhip, gpu_ctx)
     a.verify(ref, bound)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("exponent", [4, 10, 12, 13, 14, 16, 20, 40, 90, 100])
+def test_scores_whose_f32_numbers_lie_far_apart(samhip, gpu_ctx, exponent, rows, hd):
+    """Scores up to 2^117 of either sign, a hundredth of themselves or more apart,
+    each of several keys: a query has the mean of its largest's values.  Weights
+    are then 1, products with scales below 2^16 and above 2^-10, so that fp16's
+    half step is 2^-25 on codes up to 127; hi + lo and the sums 2^-19."""
+    print("far scores", exponent, rows, hd, flush=True)
+    m, heads = 700, 2
+    for sign in (1, -1):
+        p = Pages([rows], [m], 1, hd, False, 41, seed=53).fill(53)
+        level = 1 + 37 * torch.arange(m, device="cuda") % 100
+        k = (127.0 * level)[:, None].expand(m, hd).contiguous()   # scales of whole numbers, codes of 127
+        p.caches[0][p.at(0, range(m))] = torch.as_tensor(packed(k, False), device="cuda")
+        a = Attend(p, heads, True, seed=53)
+        a.q.fill_(sign * 2.0 ** exponent)
+        a.q[:, hd:] *= -1
+        v = values(p.caches[1][p.at(0, range(m))], False)
+        ref = torch.zeros_like(a.out, dtype=torch.float64)
+        for i in range(rows):
+            seen = level[:m - rows + 1 + i]
+            for h in range(heads):
+                s = seen if (sign > 0) == (h == 0) else -seen
+                if exponent < 10:   # weights of others too
+                    w = torch.softmax(s.double() * (127 * hd * a.scale * 2.0 ** exponent), -1)
+                else:
+                    w = (s == s.max()).double() / (s == s.max()).sum()
+                ref[i, h * hd:(h + 1) * hd] = w @ v[:len(seen)]
+        a.run(samhip, gpu_ctx)
+        a.verify(ref, torch.full_like(ref, 127 * 2.0 ** -25 + 4 * 2.0 ** -19))
