@@ -14,7 +14,7 @@
 // scale stay below 2^15, the largest of a tile that moved b at 2^13, so that
 // as hi + lo they keep 22 bits down to 2^-16 of the largest contribution so
 // far, wherever its weight or its scale comes from.  A scale of zero counts as
-// 2^-40 in this, for its weight has its place in the sum.
+// 2^-80 in this, for its weight has its place in the sum.
 // F32 scores of 2^23 and more (FAR) are whole numbers, from which neither a
 // scale's log nor 13 can be taken: such a query's base is its largest score, as
 // rounded, and so are the others that it is taken from, so that weights are 1 at
@@ -55,7 +55,7 @@ constexpr int MOST_PARTS = 32;             // of a tile's keys where waves have 
 constexpr float NO_BASE = -0x1.fffffep127f;   // below every score, and finite
 constexpr float FAR = 0x1p23f;            // of scores; a base from half of it on is looked at with every tile
 constexpr float ROOM = 15.f;              // log 2 of the largest product before the base moves
-constexpr int ZERO_SCALE = -40;           // log 2 of what a zero scale counts as
+constexpr int ZERO_SCALE = -80;           // log 2 of what a zero scale counts as: 2^30 weights of 2^(15 + 80) still have an F32 sum
 constexpr int DPP_HALF_MIRROR = 0x141;    // lane 7 - i of its eight
 
 typedef uint32_t u32x2_at __attribute__((ext_vector_type(2), aligned(2)));

@@ -1058,3 +1058,21 @@ def test_scores_whose_f32_numbers_lie_far_apart(samhip, gpu_ctx, exponent, rows,
                 ref[i, h * hd:(h + 1) * hd] = w @ v[:len(seen)]
         a.run(samhip, gpu_ctx)
         a.verify(ref, torch.full_like(ref, 127 * 2.0 ** -25 + 4 * 2.0 ** -19))
+
+
+@pytest.mark.parametrize("q4", [False, True])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("above", [20.0, 45.0, 60.0])
+def test_a_key_of_nearly_all_the_weight_without_values(samhip, gpu_ctx, above, rows, hd, q4):
+    """Values of zeros at a key `above` nats over the others: what is left is theirs, to its last digits."""
+    p = Pages([rows], [300], 1, hd, q4, 64, seed=54).fill(54)
+    k = torch.zeros(300, hd, device="cuda")
+    k[100] = above / hd
+    p.caches[0][p.at(0, range(300))] = torch.as_tensor(packed(k, q4), device="cuda")
+    scale_blocks(p, 0, 1, [100], 0.0)
+    a = Attend(p, 2, seed=54, scale=1.0)
+    a.q.fill_(1.0)
+    ref, bound = tight(a)
+    a.run(samhip, gpu_ctx)
+    a.verify(ref, bound)
