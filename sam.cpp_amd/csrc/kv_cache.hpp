@@ -53,8 +53,9 @@ __device__ __forceinline__ int request_rows(const KvCacheArgs& c, int rows, int 
     return min(max(c.row_start[r + 1], 0), rows) - from;
 }
 
-// What a request has in the cache, as said.
-__device__ __forceinline__ int request_len(const KvCacheArgs& c, int r) { return min(max(c.len[r], 0), 1 << 30); }
+// What a request has in the cache, as said: more than there are positions, too,
+// for its rows stand before the end.
+__device__ __forceinline__ int request_len(const KvCacheArgs& c, int r) { return max(c.len[r], 0); }
 
 // The cache row of a position below the request's length and the capacity, or -1.
 __device__ __forceinline__ int cache_row(const KvCacheArgs& c, int r, int position) {

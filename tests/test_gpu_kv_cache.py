@@ -1076,3 +1076,47 @@ def test_a_key_of_nearly_all_the_weight_without_values(samhip, gpu_ctx, above, r
     ref, bound = tight(a)
     a.run(samhip, gpu_ctx)
     a.verify(ref, bound)
+
+
+def test_lengths_past_the_last_position_there_may_be(samhip, gpu_ctx):
+    """Tables of 2^30 positions, lengths beyond: rows stand where the length says,
+    so that some have no place, and the others' queries see up to their own."""
+    page, n = 1 << 26, 10
+    p = Pages([n], [1], 1, 32, True, 16, seed=55)
+    p.page, p.max_pages = page, 16
+    p.pages = ints([[-1] * 15 + [0]])
+    p.caches = [torch.zeros(page, 18, dtype=torch.uint8, device="cuda") for _ in "kv"]
+    k, v = (torch.randn(n, 32, device="cuda") for _ in "kv")
+    for over in (5, 9, 10, 2 ** 30 - 1):
+        lost = min(n, over)   # the last rows', from position 2^30 on
+        p.len = ints([2 ** 30 + over])
+        for c in p.caches:
+            c[-64:] = 0
+        out = [torch.full_like(k, 7.0) for _ in "kv"]
+        torch.cuda.synchronize()
+        gpu_ctx.cache_write(p.desc(samhip), None, describe(samhip, k), describe(samhip, v))
+        gpu_ctx.cache_read(p.desc(samhip), *(describe(samhip, o) for o in out))
+        gpu_ctx.synchronize()
+        for x, o, c in zip((k, v), out, p.caches):
+            bytes_ = torch.as_tensor(packed(x, True), device="cuda")
+            want = torch.zeros_like(c[-64:])
+            if lost < n:   # row i at 2^30 + over - n + i, the last page's
+                at = 64 + over - n
+                want[at:at + n - lost] = bytes_[:n - lost]
+            assert torch.equal(c[-64:], want)
+            back = values(bytes_, True)
+            back[n - lost:] = 0.0
+            assert torch.equal(o.double(), back)
+        if over != 5:
+            continue
+        # keys of zeros: a query has the mean of the values up to its position
+        p.caches[0].zero_()
+        a = Attend(p, 1, True, seed=55)
+        a.max_len = 2 ** 31 - 1
+        a.run(samhip, gpu_ctx)
+        stored = values(p.caches[1][-64:], True)
+        for i in range(n):
+            last = min(2 ** 30, 2 ** 30 + over - n + i + 1)   # positions below it are seen
+            count = last - (2 ** 30 - page)
+            want = stored[:64 - (2 ** 30 - last)].sum(0) / count
+            assert ((a.out[i].double() - want).abs() <= 1e-5 * stored.abs().sum(0) / count + 2.0 ** -40).all()
