@@ -1062,7 +1062,7 @@ void cache_attn_plan(CacheAttnArgs& a, int cus) {
     a.least_steps = 2;
     const int at_once = !a.narrow ? (a.cache.head_dim == 32 ? 3 : 2) : a.cache.head_dim == 128 ? 3 : 4;
     const bool split = a.max_len > a.least_steps * keys;
-    const auto slots = [&](int wave_heads) { return split ? std::max(1, at_once * cus / (a.cache.kv_heads / wave_heads)) : 0; };
+    const auto slots = [&](int wave_heads) { return split ? at_once * cus / (a.cache.kv_heads / wave_heads) : 0; };
     // Few places: waves of one workgroup read the kv heads of the same keys, for heads
     // share cache lines, and lines that come one by one come slowly from memory that
     // no cache holds (64 queries of 8 kv heads of 64 on up to 8192 Q4_0 keys: 110
@@ -1074,6 +1074,7 @@ void cache_attn_plan(CacheAttnArgs& a, int cus) {
         for (int heads : {2, 4})
             if (a.cache.kv_heads % heads == 0 && slots(heads) <= MOST_PARTS * int64_t(a.tiles)) a.wave_heads = heads;
     a.slots = slots(a.wave_heads);
+    if (a.slots < 2) a.slots = 0;   // as many kv heads as run at once: nothing is split
     a.by_group = Divisor::of(a.group);
     a.by_head_sets = Divisor::of(a.cache.kv_heads / a.wave_heads);
     a.by_places = Divisor::of(tile);

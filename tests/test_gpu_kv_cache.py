@@ -1120,3 +1120,22 @@ def test_lengths_past_the_last_position_there_may_be(samhip, gpu_ctx):
             count = last - (2 ** 30 - page)
             want = stored[:64 - (2 ** 30 - last)].sum(0) / count
             assert ((a.out[i].double() - want).abs() <= 1e-5 * stored.abs().sum(0) / count + 2.0 ** -40).all()
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_no_scratch_where_no_keys_are_split(samhip, rows):
+    """So many kv heads that every workgroup has all keys of its queries: nothing is kept for a join."""
+    with samhip.Context(0) as ctx:
+        p = Pages([rows], [600], 4096, 32, True, 64, seed=56)
+        x = torch.randn(600, p.width, device="cuda")
+        for c in p.caches:
+            for at in range(0, 600, 100):
+                c[p.at(0, range(at, at + 100))] = torch.as_tensor(packed(x[at:at + 100], True), device="cuda")
+        a = Attend(p, 4096, seed=56)
+        a.run(samhip, ctx)
+        assert ctx.query().activation_allocation_peak_bytes == 0
+        k = values(p.caches[0][p.at(0, range(600))], True).view(600, 4096, 32).float()
+        q = a.q.view(rows, 4096, 32)
+        w = torch.softmax(torch.bmm(q.transpose(0, 1).contiguous(), k.permute(1, 2, 0).contiguous()) * a.scale, -1)
+        want = torch.bmm(w, k.transpose(0, 1).contiguous()).transpose(0, 1).reshape(rows, -1)
+        assert ((a.out - want).abs() <= 1e-4).all()
