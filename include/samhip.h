@@ -463,9 +463,10 @@ typedef struct samhip_kv_cache {
  *         min(15, int(x * (1 / d) + 8.5)), d stored as F16
  * A NaN is stored as a zero, a block with an infinity reads back as NaN.
  * Rows without a place, and those outside [row_start[0],
- * row_start[requests]), are not written.  Two rows with one place (pages that
- * requests share) leave either's blocks there.  k, v and the cache do not
- * overlap.  At most 2^23 rows.  May be captured. */
+ * row_start[requests]), are not written.  Two rows of a call with one place
+ * (pages that requests share) leave blocks there that may mix both, a scale of
+ * one with codes of the other.  k, v and the cache do not overlap.  At most
+ * 2^23 rows.  May be captured. */
 int samhip_supports_cache_write(const samhip_kv_cache* cache, const samhip_rope_desc* rope, const samhip_tensor* k,
                                 const samhip_tensor* v);
 int samhip_cache_write(samhip_context* ctx, const samhip_kv_cache* cache, const samhip_rope_desc* rope,

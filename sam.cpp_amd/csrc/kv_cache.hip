@@ -232,7 +232,8 @@ __device__ __forceinline__ void find_places(const KvCacheArgs& c, int rows, int 
     if (i < n) place[i] = place_of_row(c, rows, row0 + i, r);
 }
 
-// Eight values to a lane, four lanes to a block.
+// Eight values to a lane, four lanes to a block, which is stored in pieces: rows
+// of two workgroups with one place may leave a mixed one.
 template <int TYPE, bool X86>
 __global__ __launch_bounds__(THREADS) void cache_write_kernel(KvCacheArgs c, RopeArgs rope, CacheRowShape s, const float* k, int64_t ldk,
                                                               const float* v, int64_t ldv, int rows) {

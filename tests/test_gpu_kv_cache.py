@@ -1139,3 +1139,26 @@ def test_no_scratch_where_no_keys_are_split(samhip, rows):
         w = torch.softmax(torch.bmm(q.transpose(0, 1).contiguous(), k.permute(1, 2, 0).contiguous()) * a.scale, -1)
         want = torch.bmm(w, k.transpose(0, 1).contiguous()).transpose(0, 1).reshape(rows, -1)
         assert ((a.out - want).abs() <= 1e-4).all()
+
+
+@pytest.mark.parametrize("q4", [False, True])
+def test_rows_with_one_place_mix_there_alone(samhip, gpu_ctx, q4):
+    """Requests whose pages are the same in one call: of what stands there each byte
+    is one of theirs, every other place holds its own row."""
+    n = 600   # several workgroups' rows
+    p = Pages([n, n, n], [n, n, n], 4, 64, q4, 16, seed=58)
+    table = p.table.copy()
+    table[2] = table[0]
+    p.pages.copy_(ints(table.tolist()))
+    k, v = (torch.randn(p.rows, p.width, device="cuda") for _ in "kv")
+    torch.cuda.synchronize()
+    gpu_ctx.cache_write(p.desc(samhip), None, describe(samhip, k), describe(samhip, v))
+    gpu_ctx.synchronize()
+    for x, c in zip((k, v), p.caches):
+        bytes_ = torch.as_tensor(packed(x, q4), device="cuda")
+        shared, own = c[p.at(0, range(n))], c[p.at(1, range(n))]
+        assert torch.equal(own, bytes_[n:2 * n])
+        assert ((shared == bytes_[:n]) | (shared == bytes_[2 * n:])).all()
+        nobody = torch.ones(len(c), dtype=torch.bool, device="cuda")
+        nobody[torch.cat([p.at(0, range(n)), p.at(1, range(n))])] = False
+        assert (c[nobody] == 255).all()
