@@ -483,16 +483,19 @@ int samhip_cache_read(samhip_context* ctx, const samhip_kv_cache* cache, const s
  * head
  *   out = softmax(scale * q K^T) V
  * over the request's positions that have a place, with `causal` those up to
- * the row's own.  F32-accurate on the values the blocks stand for; what a key
- * adds that is below 2^-16 of a query's largest is off by at most 2^-39 of that.
- * Scores, and scale times a query's largest value, are F32 numbers: past their
- * range a query gets NaN, or zeros where all its scores are below it.  A query
- * with a value that is not finite gets NaN for its head.  Grouped heads: head h reads kv head h / (heads / kv_heads).  A query that sees no
- * position gets zeros; rows of out outside [row_start[0],
- * row_start[requests]) are left as they were.  A key whose blocks' scales are
- * not finite makes NaN of the queries that see it, such a value block of its
- * 32 dimensions of theirs.  out overlaps no other operand.  At most 4096
- * heads, 2^23 rows * heads.  May be captured. */
+ * the row's own.  F32-accurate on the values the blocks stand for; of a query,
+ * keys whose weight times value scale is below 2^-16 of the largest are off by
+ * at most 2^-38 of that largest for each unit of their codes (2^-25 of the
+ * largest weight where scores pass 5 * 10^6), and its own values below 2^-16 of
+ * its largest by at most 2^-39 of that.  Scores, and scale times
+ * a query's largest value, are F32 numbers: past their range a query gets NaN,
+ * or zeros where all its scores are below it.  A query with a value that is not
+ * finite gets NaN for its head.  Grouped heads: head h reads kv head
+ * h / (heads / kv_heads).  A query that sees no position gets zeros; rows of out
+ * outside [row_start[0], row_start[requests]) are left as they were.  A key
+ * whose blocks' scales are not finite makes NaN of the queries that see it, such
+ * a value block of its 32 dimensions of theirs.  out overlaps no other operand.
+ * At most 4096 heads, 2^23 rows * heads.  May be captured. */
 typedef struct samhip_cache_attn_desc {
     int32_t version;            /* SAMHIP_ABI_VERSION */
     int32_t heads;              /* a multiple of kv_heads */
