@@ -1162,3 +1162,25 @@ def test_rows_with_one_place_mix_there_alone(samhip, gpu_ctx, q4):
         nobody = torch.ones(len(c), dtype=torch.bool, device="cuda")
         nobody[torch.cat([p.at(0, range(n)), p.at(1, range(n))])] = False
         assert (c[nobody] == 255).all()
+
+
+def test_q8_0_codes_at_ties_are_of_one_division(samhip, gpu_ctx):
+    """Values next to ties whose code follows from 127 / amax as one division, and
+    is another by a product with a rounded 1 / amax."""
+    rng = np.random.default_rng(57)
+    most = rng.uniform(0.5, 4, 1 << 16).astype(np.float32)
+    once, twice = np.float32(127) / most, np.float32(127) * (np.float32(1) / most)
+    x = ((rng.integers(0, 120, (1 << 16, 31)) + 0.5) / once[:, None]).astype(np.float32)
+    x = np.concatenate([most[:, None], x], 1)   # the largest first
+    other = np.rint(x * twice[:, None]) != np.rint(x * once[:, None])
+    x = x[other.any(1)]
+    x = x[:len(x) // 2 * 2].reshape(-1, 64)
+    assert len(x) > 1000
+    p = Pages([len(x)], [len(x)], 2, 32, False, 16, seed=57)
+    k = torch.as_tensor(x, device="cuda")
+    torch.cuda.synchronize()
+    gpu_ctx.cache_write(p.desc(samhip), None, describe(samhip, k), describe(samhip, k))
+    gpu_ctx.synchronize()
+    want = packed(k, False)
+    for c in p.caches:
+        assert np.array_equal(c[p.at(0, range(len(x)))].cpu().numpy(), want)
