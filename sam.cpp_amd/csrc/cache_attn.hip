@@ -29,16 +29,17 @@
 // take one block's value scale in each lane instead of all blocks' in every
 // one.  (With hi and lo as columns, and a lane's scores and weights block by
 // block, 64 queries of 16 heads of 128 on up to 8192 keys took 84 us.)
-// That call now: 72.7 us from HBM (3.1 TB/s), 58.6 from the MALL, of it 4.8 the
+// That call now: 72.8 us from HBM (3.1 TB/s), 57.8 from the MALL, of it 5.0 the
 // join.  At head_dim 128 twelve waves a CU have 4.6 KB each under way, and the
-// vector instructions take 33 us, the matrix instructions 10; the rest is parts
-// that end early and HBM's lines one by one.
+// vector instructions take 30 us of a SIMD, the matrix instructions 10; the rest
+// is parts that end early and HBM's lines one by one.
 // Many places: 128 to a workgroup, 64 keys (32 of head_dim 128) at a time as fp16
 // codes in LDS for its four waves, the next ones written beside them.  Key scales multiply a block's
 // products, value scales the weights.  8 prompts of 201 queries of 8 heads of 32
-// on up to 5217 Q8_0 keys: 43.4 us, of it 4.6 the join; vector instructions (about
-// 150 for 32 keys and 32 places, 16 of them exponentials at a quarter rate) fill
-// 23 us of a SIMD, matrix instructions 6.
+// on up to 5217 Q8_0 keys: 44.6 us, of it 5.2 the join; vector instructions (about
+// 160 for 32 keys and 32 places, 16 of them exponentials at a quarter rate, 16 for
+// each key's own value scale; with one scale for a tile, which is wrong where they
+// lie far apart, 43.6 us) fill 24 us of a SIMD, matrix instructions 6.
 #include <algorithm>
 
 #include "attn_tiles.hpp"
@@ -665,7 +666,7 @@ struct Octet {
 };
 
 // At head_dim 128 the queries' low halves: with them in registers, and 64 keys in
-// a tile, one wave has a SIMD (48 requests of 48 places: 170 us; so: 110).
+// a tile, one wave has a SIMD (48 requests of 48 places: 170 us; so: 111).
 template <int HD>
 struct WideLow {};
 template <>
@@ -1044,11 +1045,14 @@ void cache_attn_plan(CacheAttnArgs& a, int cus) {
     const int64_t places = int64_t(a.rows) * a.group, requests = std::min(a.cache.requests, a.rows);
     const int64_t each = (places + requests - 1) / requests;   // of a request with its share of the rows
     // Where the two forms meet (us for 16, 24, 32, 48 places of each of 48 requests on up
-    // to 3000 Q4_0 keys of 4 kv heads, few / many: head_dim 32 22 / 34, 26 / 35, 27 / 31,
-    // 35 / 39; 64: 31 / 57, 41 / 58, 49 / 50, 69 / 63; 128: 69 / 104, 100 / 105, 131 / 89,
-    // 215 / 107; of 8 on up to 5000, 24, 32 and 48 places: 32 16.9 / 17.7, 17.3 / 16.6, 20.3
-    // / 19.3; 64: 23 / 23, 24 / 21, 28 / 26; 128: 39 / 36, 45 / 33, 59 / 40).  Two operands
-    // of places to a workgroup instead of two workgroups: 34, 41 and 80 at 16 places.
+    // to 3000 Q4_0 keys of 4 kv heads, few / many: head_dim 32 21 / 34, 25 / 35, 25 / 30,
+    // 32 / 38; 64: 31 / 61, 39 / 62, 47 / 52, 67 / 66; 128: 65 / 111, 94 / 111, 123 / 91,
+    // 210 / 111; of 8 on up to 5000, 24, 32 and 48 places: 32 16.4 / 17.3, 16.9 / 17.1, 20.2
+    // / 19.1; 64: 23 / 23, 25 / 21, 29 / 26; 128: 37 / 39, 44 / 34, 57 / 41).  In Q8_0 the
+    // form for few is slower, and they meet at fewer places than this rule has: 48 requests,
+    // head_dim 64 50 / 61, 59 / 52 at 24 and 32, 128 100 / 110, 148 / 111 at 16 and 24.  Two
+    // operands of places to a workgroup instead of two workgroups, Q4_0: 34, 41 and 80 at 16
+    // places.
     a.narrow = each <= (a.cache.head_dim == 128 ? 24 : 32);
     const int tile = a.narrow ? 512 / a.cache.head_dim : TILE * WAVES, keys = a.narrow ? 32 * WAVES : wide_keys(a.cache.head_dim);
     a.tiles = int(places / tile + requests);

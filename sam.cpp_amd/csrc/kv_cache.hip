@@ -9,9 +9,9 @@
 // All of it is bound by memory: one pass, 16-byte loads and stores.  5184 rows of
 // 32 heads of 64, F32: 16.2 us (5.2 TB/s, partly from the MALL); 41472 rows of 16
 // heads, F16: 34.0 (5.0).  Rows to a cache: 41472 of 512 F32 values of keys and
-// values, keys rotated, Q4_0: 48 us from HBM (4.0 TB/s; 40 from the MALL); back as
-// F16: 23.  A call of few rows is one launch of 4 to 6 us, a chain of loads: tables,
-// page, block.
+// values, keys rotated, Q4_0: 45 us from HBM (4.3 TB/s; 41 from the MALL), Q8_0
+// 47; back as F16: 30 (21) of either, as F32 58 and 53.  A call of few rows is one
+// launch of 3 to 5 us, a chain of loads: tables, page, block.
 #include <algorithm>
 
 #include "kv_cache.hpp"
