@@ -1184,3 +1184,31 @@ def test_q8_0_codes_at_ties_are_of_one_division(samhip, gpu_ctx):
     want = packed(k, False)
     for c in p.caches:
         assert np.array_equal(c[p.at(0, range(len(x)))].cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("q4", [False, True])
+@pytest.mark.parametrize("rows,hd", [(1, 32), (3, 128), (40, 64), (40, 128), (70, 32)])
+def test_large_scores_give_means_of_values(samhip, gpu_ctx, rows, hd, q4):
+    """Random scores from 2^18 to 2^40 and past, in one part of keys and in several:
+    values between 1 and 2, so that every output lies between the smallest and the
+    largest of its dimension, but for what the bound leaves (a unit of code is at
+    most a seventh, 2^-25 of the largest weight for each key)."""
+    lens = [3000, 97]
+    for e in range(12, 36):
+        print("large scores", e, rows, hd, q4, flush=True)
+        p = Pages([rows, rows], lens, 2, hd, q4, 41, seed=59).fill(59)
+        g = torch.Generator(device="cuda").manual_seed(e)
+        for r, m in enumerate(lens):
+            x = 1 + torch.rand(m, p.width, device="cuda", generator=g)
+            p.caches[1][p.at(r, range(m))] = torch.as_tensor(packed(x, q4), device="cuda")
+        a = Attend(p, 4, True, seed=e)
+        a.q.mul_(2.0 ** e)
+        a.run(samhip, gpu_ctx)
+        for r, m in enumerate(lens):
+            v = values(p.caches[1][p.at(r, range(m))][:, :p.row_bytes], q4).view(m, 2, hd)
+            for i in range(rows):
+                seen = v[:m - rows + 1 + i]
+                lo, hi = (t.repeat_interleave(2, 0) for t in (seen.amin(0), seen.amax(0)))
+                out = a.out[p.starts[r] + i].double().view(4, hd)
+                slack = len(seen) * 16 * 2.0 ** -25 + 2.0 ** -16
+                assert ((out >= lo - slack) & (out <= hi + slack)).all(), (r, i)
